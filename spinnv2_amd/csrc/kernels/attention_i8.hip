@@ -1,0 +1,486 @@
+// Attention of new tokens to a paged int8 cache.
+//
+//   out[i] = sum_t p[i, t] v[t] / sum_t p[i, t],  p = exp(scale q[i] k[t])
+//
+// The codes are turned into 16-bit floats, exactly, and multiplied on the
+// fp16 matrix cores; a token's key scale multiplies its scores, its value
+// scale its weights.
+#include "decoder.hpp"
+
+namespace spk::dec {
+
+namespace {
+
+struct AttnArgs {
+    Spkv2KvCacheI8 c;
+    const void *q;
+    void *out;
+    const int32_t *table, *lengths, *offsets;
+    float *part, *stats;  // [row][split][head_dim] sums, [row][split][2] maximum and total; row = row of q * heads + head
+    int64_t queries, q_stride, out_stride;
+    int max_queries, max_length, table_width, heads, group, sequences;
+    int causal, window;
+    float scale;
+    int row_blocks, split_tokens, splits;
+    unsigned page_mul;  // token / page_size, by multiplication
+    int page_shift;
+};
+
+constexpr int kWaves = 4;    // of a workgroup: they deal a split's chunks out among them
+constexpr int kChunk = 32;   // tokens a wave takes at a time, as two tiles of 16
+// The running maximum of a row follows its scores only when one passes it by
+// more than 2^kSlack; weights are held as 2^kLift p in fp16, below 2^15.
+constexpr float kSlack = 8.0f;
+constexpr float kLift = 128.0f;
+
+// Two codes of a dword, picked by `sel` into the low bytes of two halves, as
+// fp16: 0x6400 + (code + 128) is 1024 + 128 + code.
+__device__ __forceinline__ half2_t codes_to_half(unsigned hi, unsigned lo, unsigned sel) {
+    const unsigned u = __builtin_amdgcn_perm(hi, lo, sel) ^ 0x64806480u;
+    constexpr half2_t kBias = {static_cast<_Float16>(1152), static_cast<_Float16>(1152)};
+    return __builtin_bit_cast(half2_t, u) - kBias;
+}
+__device__ __forceinline__ half8_t join(half2_t a, half2_t b, half2_t c, half2_t d) {
+    return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// eight codes in a row
+__device__ __forceinline__ half8_t codes8(unsigned a, unsigned b) {
+    return join(codes_to_half(0, a, 0x0c010c00u), codes_to_half(0, a, 0x0c030c02u), codes_to_half(0, b, 0x0c010c00u),
+                codes_to_half(0, b, 0x0c030c02u));
+}
+
+__device__ __forceinline__ float over_groups_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+struct Sequence {
+    int64_t row0;   // its first row of q
+    int count;      // queries computed
+    int position;   // position of its first query
+    int length;     // tokens read
+    int true_length;
+};
+__device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
+    Sequence s;
+    const int o0 = a.offsets[b], o1 = a.offsets[b + 1];
+    s.true_length = a.lengths[b];
+    s.row0 = o0;
+    s.count = min(o1 - o0, a.max_queries);
+    if (o0 < 0) s.count = 0;
+    if (o0 + static_cast<int64_t>(s.count) > a.queries) s.count = static_cast<int>(a.queries - o0);
+    s.position = s.true_length - (o1 - o0);
+    const int64_t held = static_cast<int64_t>(a.table_width) * a.c.page_size;
+    s.length = max(0, min(s.true_length, a.max_length));
+    if (s.length > held) s.length = static_cast<int>(held);
+    return s;
+}
+
+// One workgroup: RT tiles of 16 rows (query, head of the group) of one
+// sequence and kv head, and one split of its tokens.  Scores are taken
+// transposed, S^T = K q^T on 16x16 tiles: a lane then holds four tokens'
+// scores of one row, which are the weights' operand of O^T = V^T P^T as they
+// are, if V's rows are taken in the same order.  So nothing passes through LDS
+// until the waves' sums are joined.
+//
+// Lane l: column l % 16 (a row of q), group g = l / 16.
+//   K: token l % 16 of the tile, its codes g DP/4 .. + DP/4 (q in the same
+//      order of d, which the product does not see)
+//   scores, weights: tokens 4 g .. + 4 of each tile
+//   V: those tokens' codes VPL (l % 16) .. + VPL (VPL = DP / 16); product j
+//      takes d = VPL r + j as its row r
+template <typename T, int DP, int RT>
+__global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
+    constexpr bool kWide = sizeof(T) == 4;  // rows of 22 bits: two fp16 parts
+    constexpr int kParts = kWide ? 2 : 1;
+    constexpr int kPieces = DP / 64;  // 16-byte pieces of K a lane
+    constexpr int kVpl = DP / 16;     // V codes a lane
+    constexpr int kVw = kVpl / 4;
+    __shared__ __align__(16) float joined[kWaves * 64 * 4 * kVpl];
+    __shared__ float wave_max[kWaves][RT * 16], wave_sum[kWaves][RT * 16];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int head = blockIdx.y;
+    const int at_x = blockIdx.x / a.splits, split = blockIdx.x - at_x * a.splits;
+    const int b = at_x / a.row_blocks, block = at_x - b * a.row_blocks;
+    const int dim = a.c.head_dim;
+    const Sequence s = sequence(a, b);
+    const int rows = s.count * a.group, r0 = block * 16 * RT;
+    if (r0 >= rows) return;
+    const int first_q = r0 / a.group, last_q = (min(rows, r0 + 16 * RT) - 1) / a.group;
+    int low = split * a.split_tokens, high = min(s.length, low + a.split_tokens);
+    if (a.causal) {
+        high = min(high, s.position + last_q + 1);
+        if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+    }
+
+    // the rows' masks and queries, scaled by a power of two to 2^14 .. 2^15
+    half8_t qf[RT][DP / 32][kParts];
+    float factor[RT], m[RT], l[RT];
+    int last[RT], start[RT];
+    floatx4 acc[RT][kVpl];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = r0 + t * 16 + col, i = r / a.group;
+        const bool in = r < rows;
+        last[t] = a.causal ? s.position + i : s.length - 1;
+        start[t] = a.causal && a.window ? last[t] + 1 - a.window : 0;
+        const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_stride +
+                     static_cast<int64_t>(head * a.group + (r - i * a.group)) * dim;
+        float f[DP / 4];
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < DP / 4; e++) {
+            const int d = g * (DP / 4) + e;
+            f[e] = in && d < dim ? static_cast<float>(q[d]) : 0.0f;
+            top = fmaxf(top, fabsf(f[e]));
+        }
+        top = over_groups_max(top);
+        const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
+        factor[t] = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
+#pragma unroll
+        for (int x = 0; x < DP / 32; x++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = ldexpf(f[x * 8 + e], 14 - ex);
+                const _Float16 hi = static_cast<_Float16>(v);
+                qf[t][x][0][e] = hi;
+                if constexpr (kWide) qf[t][x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+            }
+        m[t] = -__builtin_inff();
+        l[t] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kVpl; j++) acc[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float unit = 0.0f, per_unit = 0.0f;  // a power of two no value scale is above, and kLift / unit
+
+    struct Chunk {
+        uintx4 k[2][kPieces];
+        unsigned v[8][kVw];
+        floatx4 ks[2], vs[2];
+        bool ok[2];
+    };
+    auto fetch = [&](Chunk &x, int at) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int t = at + 16 * h;
+            const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
+            int page = -1;
+            if (t < high) page = a.table[static_cast<int64_t>(b) * a.table_width + page_at];
+            page = __builtin_amdgcn_readfirstlane(page);
+            x.ok[h] = page >= 0 && page < a.c.pages;
+            x.ks[h] = x.vs[h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = 0; p < kPieces; p++) x.k[h][p] = uintx4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int w = 0; w < kVw; w++) x.v[4 * h + u][w] = 0;
+            if (!x.ok[h]) continue;
+            const int64_t row = (static_cast<int64_t>(page) * a.c.kv_heads + head) * a.c.page_size + (t - page_at * a.c.page_size);
+            x.ks[h] = *reinterpret_cast<const floatx4 *>(a.c.k_scale + row + 4 * g);
+            x.vs[h] = *reinterpret_cast<const floatx4 *>(a.c.v_scale + row + 4 * g);
+            const int8_t *k = a.c.k + (row + col) * dim + g * (DP / 4);
+#pragma unroll
+            for (int p = 0; p < kPieces; p++)
+                if (DP / 4 * g + 16 * p < dim) x.k[h][p] = *reinterpret_cast<const uintx4 *>(k + 16 * p);
+            const int8_t *v = a.c.v + (row + 4 * g) * dim + kVpl * col;
+            if (kVpl * col < dim) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const Vec<unsigned, kVw> y = *reinterpret_cast<const Vec<unsigned, kVw> *>(v + u * dim);
+#pragma unroll
+                    for (int w = 0; w < kVw; w++) x.v[4 * h + u][w] = y.v[w];
+                }
+            }
+        }
+    };
+    auto use = [&](const Chunk &x, int at) {
+        floatx4 sc[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; t++) sc[t][0] = sc[t][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int p = 0; p < kPieces; p++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const half8_t kf = codes8(x.k[h][p][2 * e], x.k[h][p][2 * e + 1]);
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+#pragma unroll
+                        for (int w = 0; w < kParts; w++)
+                            sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][2 * p + e][w], sc[t][h], 0, 0, 0);
+                }
+        // value scales: those of masked tokens may be anything in the cache
+        float vs[8];
+        float top = 0.0f;
+        const bool whole = at >= low && at + kChunk <= high && x.ok[0] && x.ok[1];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int token = at + 16 * (e / 4) + 4 * g + e % 4;
+            vs[e] = whole || (token >= low && token < high && x.ok[e / 4]) ? x.vs[e / 4][e % 4] : 0.0f;
+            top = fmaxf(top, vs[e]);
+        }
+        if (__any(top > unit)) {
+            const float now = __uint_as_float((__float_as_uint(fmaxf(over_groups_max(top), unit)) & kInfBits) + 0x00800000u);
+            const float ratio = unit / now;
+            unit = now;
+            per_unit = kLift / now;
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int j = 0; j < kVpl; j++) acc[t][j] *= ratio;
+        }
+        half8_t pf[RT][kParts];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float v[8], most = -__builtin_inff();
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int token = at + 16 * (e / 4) + 4 * g + e % 4;
+                v[e] = sc[t][e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor[t]);
+                const bool keep = token >= low && token < high && x.ok[e / 4] && token <= last[t] && token >= start[t];
+                v[e] = keep ? v[e] : -__builtin_inff();
+                most = fmaxf(most, v[e]);
+            }
+            if (__any(most > m[t] + kSlack)) {
+                const float now = fmaxf(m[t], over_groups_max(most));
+                const float ratio = m[t] > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[t] - now) : 0.0f;
+                m[t] = now;
+                l[t] *= ratio;
+#pragma unroll
+                for (int j = 0; j < kVpl; j++) acc[t][j] *= ratio;
+            }
+            const float from = m[t] > -__builtin_inff() ? m[t] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = __builtin_amdgcn_exp2f(v[e] - from);
+                l[t] += p;
+                const float w = p * (vs[e] * per_unit);
+                const _Float16 hi = static_cast<_Float16>(w);
+                pf[t][0][e] = hi;
+                if constexpr (kWide) pf[t][kParts - 1][e] = static_cast<_Float16>(w - static_cast<float>(hi));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kVpl; j++) {
+            const unsigned sel = 0x0c000c00u | ((4u + j % 4) << 16) | (j % 4);
+            const half8_t vf = join(codes_to_half(x.v[1][j / 4], x.v[0][j / 4], sel), codes_to_half(x.v[3][j / 4], x.v[2][j / 4], sel),
+                                    codes_to_half(x.v[5][j / 4], x.v[4][j / 4], sel), codes_to_half(x.v[7][j / 4], x.v[6][j / 4], sel));
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int w = 0; w < kParts; w++)
+                    acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t][w], acc[t][j], 0, 0, 0);
+        }
+    };
+
+    const int first = low / kChunk * kChunk;
+    Chunk now, next;
+    int at = first + wave * kChunk;
+    if (at < high) fetch(now, at);
+    while (at < high) {
+        const int then = at + kWaves * kChunk;
+        if (then < high) fetch(next, then);
+        use(now, at);
+        now = next;
+        at = then;
+    }
+
+    // the waves' sums, joined in wave order
+    const float back = unit / kLift;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        l[t] = over_groups_sum(l[t]);
+        if (g == 0) {
+            wave_max[wave][t * 16 + col] = m[t];
+            wave_sum[wave][t * 16 + col] = l[t];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        float most = wave_max[0][t * 16 + col];
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) most = fmaxf(most, wave_max[w][t * 16 + col]);
+        const bool none = !(most > -__builtin_inff());
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float r = none ? 1.0f : __builtin_amdgcn_exp2f(wave_max[w][t * 16 + col] - most);
+            total += r * wave_sum[w][t * 16 + col];
+        }
+        const float mine = (none ? 1.0f : __builtin_amdgcn_exp2f(m[t] - most)) * back;
+        if (t) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < kVpl; j += 4)
+                *reinterpret_cast<floatx4 *>(joined + (((wave * 4 + i) * kVw + j / 4) * 64 + lane) * 4) =
+                    floatx4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]} * mine;
+        __syncthreads();
+        float o[kVpl];
+#pragma unroll
+        for (int j = 0; j < kVpl; j += 4) {
+            floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++)
+                sum += *reinterpret_cast<const floatx4 *>(joined + (((w * 4 + wave) * kVw + j / 4) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[j + e] = sum[e];
+        }
+        // this wave's quarter of the columns: d = VPL (4 g + wave) + j
+        const int r = r0 + t * 16 + col, i = r / a.group, d = kVpl * (4 * g + wave);
+        if (r >= rows || d >= dim) continue;
+        const int h = head * a.group + (r - i * a.group);
+        if (a.splits > 1) {
+            const int64_t at_row = ((s.row0 + i) * a.heads + h) * a.splits + split;
+#pragma unroll
+            for (int j = 0; j < kVpl; j += 4)
+                *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d + j) = floatx4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+            if (d == 0) {
+                a.stats[2 * at_row] = most;
+                a.stats[2 * at_row + 1] = total;
+            }
+        } else {
+            T *y = static_cast<T *>(a.out) + (s.row0 + i) * a.out_stride + static_cast<int64_t>(h) * dim + d;
+            const float r_total = 1.0f / total;
+#pragma unroll
+            for (int j = 0; j < kVpl; j++) y[j] = static_cast<T>(total == 0.0f ? 0.0f : o[j] * r_total);
+        }
+    }
+}
+
+// A wave a row of q and head: its splits' sums, joined in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
+    const int head = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int b = blockIdx.x / a.max_queries, i = blockIdx.x - b * a.max_queries;
+    if (head >= a.heads) return;
+    const Sequence s = sequence(a, b);
+    if (i >= s.count) return;
+    const int64_t at = ((s.row0 + i) * a.heads + head) * a.splits;
+    float most = -__builtin_inff();
+    for (int p = 0; p < a.splits; p++) most = fmaxf(most, a.stats[2 * (at + p)]);
+    const bool none = !(most > -__builtin_inff());
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
+    for (int p = 0; p < a.splits; p++) {
+        const float sum = a.stats[2 * (at + p) + 1];
+        if (sum == 0.0f) continue;  // no token of this split is the row's
+        const float r = none ? 1.0f : __builtin_amdgcn_exp2f(a.stats[2 * (at + p)] - most);
+        total += r * sum;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (lane + 64 * e < a.c.head_dim) o[e] += r * a.part[(at + p) * a.c.head_dim + lane + 64 * e];
+    }
+    T *y = static_cast<T *>(a.out) + (s.row0 + i) * a.out_stride + static_cast<int64_t>(head) * a.c.head_dim;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (lane + 64 * e < a.c.head_dim) y[lane + 64 * e] = static_cast<T>(total == 0.0f ? 0.0f : o[e] / total);
+}
+
+struct Plan {
+    int tiles;  // of 16 rows a workgroup
+    int row_blocks, split_tokens, splits;
+    size_t part, stats;  // bytes
+};
+
+Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
+    Plan p;
+    const int64_t rows = g.max_queries * (g.heads / c.kv_heads);
+    p.tiles = rows <= 16 ? 1 : rows <= 32 || c.head_dim > 128 ? 2 : 4;
+    p.row_blocks = static_cast<int>((rows + 16 * p.tiles - 1) / (16 * p.tiles));
+    // enough workgroups for four on each CU, and no split shorter than a chunk for each wave
+    const int64_t base = static_cast<int64_t>(g.sequences) * c.kv_heads * p.row_blocks;
+    const int64_t step = kWaves * kChunk;
+    int64_t splits = std::min<int64_t>((2048 + base - 1) / base, (g.max_length + step - 1) / step);
+    splits = std::max<int64_t>(splits, 1);
+    int64_t tokens = (g.max_length + splits - 1) / splits;
+    tokens = std::max<int64_t>((tokens + step - 1) / step * step, step);
+    p.split_tokens = static_cast<int>(tokens);
+    p.splits = static_cast<int>(std::max<int64_t>((g.max_length + tokens - 1) / tokens, 1));
+    const size_t parts = p.splits > 1 ? static_cast<size_t>(g.queries) * g.heads * p.splits : 0;
+    p.part = parts * c.head_dim * sizeof(float);
+    p.stats = parts * 2 * sizeof(float);
+    return p;
+}
+
+int check(const Spkv2KvCacheI8 *c, const Spkv2AttentionI8 *g) {
+    if (int rc = check_cache(c)) return rc;
+    if (!g) return bad("attention_i8: no arguments");
+    if (!is_dtype(g->dtype)) return bad("attention_i8: unknown dtype");
+    if (g->queries < 0 || g->sequences < 0 || g->table_width < 0 || g->max_queries < 0 || g->max_length < 0)
+        return bad("attention_i8: negative size");
+    if (g->heads < 1 || g->heads % c->kv_heads) return bad("attention_i8: heads is not a multiple of kv_heads");
+    if (g->window < 0 || (g->window && !g->causal)) return bad("attention_i8: window is negative, or not causal");
+    if (g->queries > (1 << 24) || g->heads > 65535 || g->sequences > 65535 || g->max_length > (1 << 30))
+        return unsupported("attention_i8: more than 2^24 queries, 65535 heads or sequences, or 2^30 tokens");
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace spk::dec
+
+using namespace spk::dec;
+
+extern "C" int spkv2_mi355x_attention_i8_workspace(const Spkv2KvCacheI8 *c, const Spkv2AttentionI8 *g, size_t *size) {
+    return entry([&]() -> int {
+        if (!size) return bad("attention_i8: nowhere to put the size");
+        if (int rc = check(c, g)) return rc;
+        *size = 0;
+        if (g->queries == 0 || g->sequences == 0 || g->max_queries == 0) return 0;
+        const Plan p = plan(*c, *g);
+        *size = p.part + p.stats;
+        return 0;
+    });
+}
+
+extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2AttentionI8 *g, void *stream) {
+    return entry([&]() -> int {
+        if (int rc = check(c, g)) return rc;
+        if (g->queries == 0 || g->sequences == 0 || g->max_queries == 0) return 0;
+        if (!g->q || !g->out || !g->lengths || !g->offsets || (!g->table && g->table_width))
+            return bad("attention_i8: a NULL pointer");
+        const int64_t width = static_cast<int64_t>(g->heads) * c->head_dim;
+        if (g->queries > 1 && (g->q_stride < width || g->out_stride < width))
+            return bad("attention_i8: a stride is below the heads' width");
+        const Plan p = plan(*c, *g);
+        if (p.part && (!g->workspace || g->workspace_size < p.part + p.stats || !aligned(g->workspace, 16)))
+            return bad("attention_i8: the workspace is missing, too small or not 16-byte aligned");
+        if (static_cast<int64_t>(g->sequences) * p.row_blocks * p.splits > INT32_MAX ||
+            static_cast<int64_t>(g->sequences) * g->max_queries > INT32_MAX)
+            return unsupported("attention_i8: too many queries and sequences for one launch");
+        unsigned mul;
+        int shift;
+        div_magic(static_cast<unsigned>(c->page_size), &mul, &shift);
+        AttnArgs a{*c, g->q, g->out, g->table, g->lengths, g->offsets, static_cast<float *>(g->workspace),
+                   reinterpret_cast<float *>(static_cast<char *>(g->workspace) + p.part), g->queries, g->q_stride, g->out_stride,
+                   static_cast<int>(std::min<int64_t>(g->max_queries, g->queries)), static_cast<int>(g->max_length), g->table_width, g->heads,
+                   g->heads / c->kv_heads, g->sequences, g->causal, g->window, g->scale, p.row_blocks, p.split_tokens, p.splits,
+                   mul, shift};
+        const dim3 grid(g->sequences * p.row_blocks * p.splits, c->kv_heads);
+        return with_type(g->dtype, [&](auto t) {
+            using T = decltype(t);
+            auto go = [&](auto one, auto two, auto four) {
+                const char *what = "attention_i8";
+                if (int rc = p.tiles == 1 ? launch(what, one, grid, dim3(256), stream, a)
+                             : p.tiles == 2 ? launch(what, two, grid, dim3(256), stream, a)
+                                            : launch(what, four, grid, dim3(256), stream, a))
+                    return rc;
+                if (p.splits == 1) return 0;
+                const dim3 rows(static_cast<unsigned>(g->sequences * a.max_queries), (g->heads + 3) / 4);
+                return launch(what, join_splits<T>, rows, dim3(256), stream, a);
+            };
+            if (c->head_dim <= 64) return go(attend_rows<T, 64, 1>, attend_rows<T, 64, 2>, attend_rows<T, 64, 4>);
+            if (c->head_dim <= 128) return go(attend_rows<T, 128, 1>, attend_rows<T, 128, 2>, attend_rows<T, 128, 4>);
+            return go(attend_rows<T, 256, 1>, attend_rows<T, 256, 2>, attend_rows<T, 256, 2>);
+        });
+    });
+}

@@ -1,0 +1,143 @@
+// What the decoder layer's operators share: types, conversions, the checks of
+// their C entry points.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+#include <exception>
+
+#include "../runtime/context.hpp"
+#include "spkv2_decoder.h"
+
+namespace spk::dec {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWave = 64;
+
+// ---- device ----------------------------------------------------------------
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+    T v[N];
+};
+
+// N elements at p as floats: N > 1 takes a pointer aligned to the smaller of
+// 16 bytes and all N elements.
+template <int N, typename T>
+__device__ __forceinline__ void load_floats(const T *p, float (&f)[N]) {
+    constexpr int kPer = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += kPer) {
+        const Vec<T, kPer> x = *reinterpret_cast<const Vec<T, kPer> *>(p + i);
+#pragma unroll
+        for (int j = 0; j < kPer; j++) f[i + j] = static_cast<float>(x.v[j]);
+    }
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_floats(T *p, const float (&f)[N]) {
+    constexpr int kPer = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int i = 0; i < N; i += kPer) {
+        Vec<T, kPer> x;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) x.v[j] = static_cast<T>(f[i + j]);
+        *reinterpret_cast<Vec<T, kPer> *>(p + i) = x;
+    }
+}
+
+constexpr unsigned kInfBits = 0x7f800000u;
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint64_t abs_bits(double x) {
+    return static_cast<uint64_t>(__double_as_longlong(x)) & 0x7fffffffffffffffull;
+}
+
+// Codes rint(127 x / top) of N values with |x| <= top, top > 0 finite.  With
+// x, 127 / top and their product each rounded to fp32, t is within 127 * 4 *
+// 2^-24 < 2^-15 of the quotient, so it has the quotient's nearest integer
+// unless it lies within 2^-14 of the border of two.  One value in eight
+// thousand does, and where 127 / top or a wide x leaves fp32's range all do
+// (t is then infinite or NaN): those are divided in 64 bits.
+template <int N, typename P>
+__device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N]) {
+    const float inv = 127.0f / static_cast<float>(top);
+    float r[N];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float t = static_cast<float>(x[i]) * inv;
+        r[i] = rintf(t);
+        near |= !(fabsf(t - r[i]) < 0.5f - 0x1p-14f);
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            r[i] = static_cast<float>(rint(static_cast<double>(x[i]) * 127.0 / static_cast<double>(top)));
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) q[i] = static_cast<int8_t>(static_cast<int>(r[i]));
+}
+
+// ---- host ------------------------------------------------------------------
+
+inline int bad(const char *text) {
+    set_last_error_text(text);
+    return -1;
+}
+inline int unsupported(const char *text) {
+    set_last_error_text(text);
+    return SPKV2_E_UNSUPPORTED;
+}
+inline bool is_dtype(int d) { return d == SPKV2_DTYPE_FP32 || d == SPKV2_DTYPE_FP16 || d == SPKV2_DTYPE_BF16; }
+inline size_t dtype_size(int d) { return d == SPKV2_DTYPE_FP32 ? 4 : 2; }
+inline bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// (mul, shift) with n / d = n mul >> shift for 0 <= n < 2^31, d >= 1: mul =
+// ceil(2^shift / d), shift = 31 + ceil(log2 d)
+inline void div_magic(unsigned d, unsigned *mul, int *shift) {
+    int l = 0;
+    while ((uint64_t(1) << l) < d) l++;
+    *shift = 31 + l;
+    *mul = static_cast<unsigned>(((uint64_t(1) << *shift) + d - 1) / d);
+}
+
+// f(T{}) with the element type of a dtype that is_dtype() took
+template <typename F>
+inline int with_type(int dtype, F &&f) {
+    if (dtype == SPKV2_DTYPE_FP32) return f(float{});
+    if (dtype == SPKV2_DTYPE_FP16) return f(_Float16{});
+    return f(__bf16{});
+}
+
+// No exception leaves a C entry point.
+template <typename F>
+inline int entry(F &&f) noexcept {
+    try {
+        return f();
+    } catch (const std::exception &) {
+        return -1;
+    }
+}
+
+// Launches kernel(args), and returns this launch's own status, where
+// hipGetLastError would also give an earlier call's.
+template <typename A>
+inline int launch(const char *what, void (*kernel)(A), dim3 grid, dim3 block, void *stream, A args) {
+    void *ptrs[] = {&args};
+    return hip_check(hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, ptrs, 0,
+                                     static_cast<hipStream_t>(stream)),
+                     what);
+}
+
+int check_cache(const Spkv2KvCacheI8 *c);
+
+}  // namespace spk::dec

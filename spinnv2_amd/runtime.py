@@ -102,6 +102,14 @@ SIGNATURES = {
     "spkv2_mi355x_set_int8_capture": (I, [VP, I]),
     "spkv2_mi355x_conv_int8_accumulators_noalloc": (I, [VP, U32, VP, SZ]),
     "spkv2_mi355x_read_int8_tensor": (I, [VP, U32, VP, SZ]),
+    # spkv2_decoder.h
+    "spkv2_mi355x_rmsnorm_i8": (I, [VP, VP]),
+    "spkv2_mi355x_dequantize_i8": (I, [VP, VP]),
+    "spkv2_mi355x_matmul_i8": (I, [VP, VP]),
+    "spkv2_mi355x_kv_write_i8": (I, [VP, VP, VP]),
+    "spkv2_mi355x_kv_read_i8": (I, [VP, VP, VP]),
+    "spkv2_mi355x_attention_i8": (I, [VP, VP, VP]),
+    "spkv2_mi355x_attention_i8_workspace": (I, [VP, VP, ctypes.POINTER(SZ)]),
 }
 
 _LIB = None
