@@ -262,7 +262,8 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
             for (int e = 0; e < 8; e++) {
                 const float p = __builtin_amdgcn_exp2f(v[e] - from);
                 l[t] += p;
-                const float w = p * (vs[e] * per_unit);
+                // 0 where the row masks the token, whose scale may be NaN
+                const float w = v[e] == -__builtin_inff() ? 0.0f : p * (vs[e] * per_unit);
                 const _Float16 hi = static_cast<_Float16>(w);
                 pf[t][0][e] = hi;
                 if constexpr (kWide) pf[t][kParts - 1][e] = static_cast<_Float16>(w - static_cast<float>(hi));
@@ -387,15 +388,16 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
 
 struct Plan {
     int tiles;  // of 16 rows a workgroup
-    int row_blocks, split_tokens, splits;
+    int64_t row_blocks;  // up to 2^36: queries and heads are bounded
+    int split_tokens, splits;
     size_t part, stats;  // bytes
 };
 
 Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
     Plan p;
-    const int64_t rows = g.max_queries * (g.heads / c.kv_heads);
+    const int64_t rows = std::min(g.max_queries, g.queries) * (g.heads / c.kv_heads);
     p.tiles = rows <= 16 ? 1 : rows <= 32 || c.head_dim > 128 ? 2 : 4;
-    p.row_blocks = static_cast<int>((rows + 16 * p.tiles - 1) / (16 * p.tiles));
+    p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
     // enough workgroups for four on each CU, and no split shorter than a chunk for each wave
     const int64_t base = static_cast<int64_t>(g.sequences) * c.kv_heads * p.row_blocks;
     const int64_t step = kWaves * kChunk;
@@ -452,10 +454,10 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         if (g->queries > 1 && (g->q_stride < width || g->out_stride < width))
             return bad("attention_i8: a stride is below the heads' width");
         const Plan p = plan(*c, *g);
-        if (p.part && (!g->workspace || g->workspace_size < p.part + p.stats || !aligned(g->workspace, 16)))
+        if (p.splits > 1 && (!g->workspace || g->workspace_size < p.part + p.stats || !aligned(g->workspace, 16)))
             return bad("attention_i8: the workspace is missing, too small or not 16-byte aligned");
-        if (static_cast<int64_t>(g->sequences) * p.row_blocks * p.splits > INT32_MAX ||
-            static_cast<int64_t>(g->sequences) * g->max_queries > INT32_MAX)
+        if (g->sequences * p.row_blocks > INT32_MAX / p.splits ||
+            g->sequences * std::min(g->max_queries, g->queries) > INT32_MAX)
             return unsupported("attention_i8: too many queries and sequences for one launch");
         unsigned mul;
         int shift;
@@ -463,9 +465,9 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         AttnArgs a{*c, g->q, g->out, g->table, g->lengths, g->offsets, static_cast<float *>(g->workspace),
                    reinterpret_cast<float *>(static_cast<char *>(g->workspace) + p.part), g->queries, g->q_stride, g->out_stride,
                    static_cast<int>(std::min<int64_t>(g->max_queries, g->queries)), static_cast<int>(g->max_length), g->table_width, g->heads,
-                   g->heads / c->kv_heads, g->sequences, g->causal, g->window, g->scale, p.row_blocks, p.split_tokens, p.splits,
+                   g->heads / c->kv_heads, g->sequences, g->causal, g->window, g->scale, static_cast<int>(p.row_blocks), p.split_tokens, p.splits,
                    mul, shift};
-        const dim3 grid(g->sequences * p.row_blocks * p.splits, c->kv_heads);
+        const dim3 grid(static_cast<unsigned>(g->sequences * p.row_blocks * p.splits), c->kv_heads);
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             auto go = [&](auto one, auto two, auto four) {
