@@ -358,6 +358,329 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
     }
 }
 
+// ---- many rows ---------------------------------------------------------------
+
+constexpr int kTile = 64;  // tokens
+
+// One workgroup: 128 rows (query, head of the group) of one sequence and kv
+// head, 32 a wave, and one split of its tokens, 64 at a time.  The waves turn a
+// tile's codes into fp16 in LDS together, K as [token][d] and V as [d][token],
+// while they multiply the tile before.  Scores are taken transposed, S^T = K
+// q^T, on 32x32 tiles: a lane holds 16 tokens' scores of one row, and these are
+// the weights' operand of O^T = V^T P^T as they are, where V's tokens lie in
+// the same order: the 16 tokens of a product as 0-3, 8-11 (lanes 0 .. 31), 4-7,
+// 12-15 (lanes 32 .. 63).
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) attend_tiles(AttnArgs a) {
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int kParts = kWide ? 2 : 1;
+    constexpr int kK = kTile * DP * 2, kV = DP * kTile * 2;  // bytes
+    constexpr int kKItems = (DP + 63) / 64, kVItems = (DP / 2 + 63) / 64;
+    __shared__ __align__(16) int8_t lds[2 * (kK + kV)];
+    __shared__ __align__(16) float scales[2][2][kTile];
+    __shared__ __align__(16) int whole[2][4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    // the heaviest rows of a causal mask first; a sequence's and head's blocks
+    // on one XCD where their number is a multiple of eight
+    const int pairs = a.sequences * a.c.kv_heads;
+    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const int b = pair / a.c.kv_heads, head = pair - b * a.c.kv_heads;
+    const int split = rest % a.splits, block = a.row_blocks - 1 - rest / a.splits;
+    const int dim = a.c.head_dim;
+    const Sequence s = sequence(a, b);
+    const int rows = s.count * a.group, r0 = block * 128;
+    if (r0 >= rows) return;
+    const int first_q = r0 / a.group, last_q = (min(rows, r0 + 128) - 1) / a.group;
+    int low = split * a.split_tokens, high = min(s.length, low + a.split_tokens);
+    if (a.causal) {
+        high = min(high, s.position + last_q + 1);
+        if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+    }
+
+    // this wave's rows
+    const int w0 = r0 + 32 * wave, r = w0 + col, i = r / a.group, q_head = head * a.group + (r - i * a.group);
+    const bool in = r < rows;
+    const int last = a.causal ? s.position + i : s.length - 1;
+    const int start = a.causal && a.window ? last + 1 - a.window : 0;
+    const int wave_first = w0 / a.group, wave_last = (min(rows, w0 + 32) - 1) / a.group;  // queries
+    // tokens that all of the wave's rows read, and that any does
+    const int all_from = a.causal && a.window ? s.position + wave_last + 1 - a.window : 0;
+    const int all_to = a.causal ? s.position + wave_first + 1 : s.length;
+    const int any_from = a.causal && a.window ? s.position + wave_first + 1 - a.window : 0;
+    const int any_to = w0 >= rows ? 0 : a.causal ? s.position + wave_last + 1 : s.length;
+
+    half8_t qf[DP / 16][kParts];
+    float factor;
+    {
+        const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_stride + static_cast<int64_t>(q_head) * dim;
+        float f[DP / 16][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int x = 0; x < DP / 16; x++) {
+            const int d = 16 * x + 8 * h;
+            Vec<T, 8> v;
+            const bool there = in && d < dim;
+            if (there) __builtin_memcpy(v.v, q + d, sizeof(v.v));
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f[x][e] = there ? static_cast<float>(v.v[e]) : 0.0f;
+                top = fmaxf(top, fabsf(f[x][e]));
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
+        const bool negative = a.scale < 0.0f;  // q takes the sign, so that the largest score has the largest product
+        // above zero, since masked scores are -inf times it
+        factor = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, ex - 14), 0x1p-126f);
+#pragma unroll
+        for (int x = 0; x < DP / 16; x++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = ldexpf(negative ? -f[x][e] : f[x][e], 14 - ex);
+                const _Float16 hi = static_cast<_Float16>(v);
+                qf[x][0][e] = hi;
+                if constexpr (kWide) qf[x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+            }
+    }
+    floatx16 acc[DP / 32];
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[j][e] = 0.0f;
+    // Weights are held as 2^base p in fp16, base = 7 - log2(unit) with `unit` a
+    // power of two that no value scale reaches, so that a weight times its
+    // token's scale stays below 2^15; sums and totals carry the same factor.
+    float m = -__builtin_inff(), l = 0.0f, unit = 0.0f, base = 0.0f;
+
+    struct Stage {
+        uintx4 k[kKItems];
+        unsigned v[kVItems][8];
+        float scale;
+    };
+    const auto page_of = [&](int tile) {
+        const int t = tile * kTile + 16 * wave;
+        if (t >= high) return -1;
+        const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
+        const int page = a.table[static_cast<int64_t>(b) * a.table_width + page_at];
+        return page < a.c.pages ? page : -1;
+    };
+    // this wave's 16 tokens of a tile
+    const auto fetch = [&](Stage &x, int tile, int page) {
+        const int t = tile * kTile + 16 * wave;
+        const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
+        const int64_t row = (static_cast<int64_t>(page) * a.c.kv_heads + head) * a.c.page_size + (t - page_at * a.c.page_size);
+        const int8_t *k = a.c.k + row * dim, *v = a.c.v + row * dim;
+        const bool there = page >= 0;
+#pragma unroll
+        for (int n = 0; n < kKItems; n++) {
+            const int item = n * 64 + lane, at = item / (DP / 16), d = item % (DP / 16) * 16;
+            x.k[n] = uintx4{0, 0, 0, 0};
+            if (there && at < 16 && d < dim) x.k[n] = *reinterpret_cast<const uintx4 *>(k + at * dim + d);
+        }
+#pragma unroll
+        for (int n = 0; n < kVItems; n++) {
+            const int item = n * 64 + lane, d = item % (DP / 4) * 4, half = item / (DP / 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x.v[n][e] = 0;
+                if (there && half < 2 && d < dim) x.v[n][e] = *reinterpret_cast<const unsigned *>(v + (e / 4 * 8 + half * 4 + e % 4) * dim + d);
+            }
+        }
+        // lanes 0 .. 15: key scales, 16 .. 31: value scales; zeros for tokens outside the range
+        const int token = t + (lane & 15);
+        x.scale = 0.0f;
+        if (there && lane < 32 && token >= low && token < high) x.scale = (lane < 16 ? a.c.k_scale : a.c.v_scale)[row + (lane & 15)];
+    };
+    // places of 16-byte pieces that put any 16 rows' pieces of one column on different banks
+    const auto k_place = [](int row, int piece) {
+        const int turn = DP == 64 ? row / 2 & 7 : DP == 96 ? row / 4 & 3 : row & 15;
+        return row * (DP * 2) + (piece ^ turn) * 16;
+    };
+    const auto v_place = [](int row, int piece) { return row * (kTile * 2) + (piece ^ ((row / 2 ^ row / 16) & 7)) * 16; };
+    const auto put = [&](const Stage &x, int buffer, int page) {
+        int8_t *k = lds + buffer * (kK + kV), *v = k + kK;
+#pragma unroll
+        for (int n = 0; n < kKItems; n++) {
+            const int item = n * 64 + lane, at = item / (DP / 16), piece = item % (DP / 16) * 2;
+            if (DP % 64 && at >= 16) continue;
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                *reinterpret_cast<half8_t *>(k + k_place(16 * wave + at, piece + e)) = codes8(x.k[n][2 * e], x.k[n][2 * e + 1]);
+        }
+#pragma unroll
+        for (int n = 0; n < kVItems; n++) {
+            const int item = n * 64 + lane, d = item % (DP / 4) * 4, half = item / (DP / 4);
+            if (DP % 128 && half >= 2) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const unsigned sel = 0x0c000c00u | ((4u + e) << 16) | e;
+                const half8_t y = join(codes_to_half(x.v[n][1], x.v[n][0], sel), codes_to_half(x.v[n][3], x.v[n][2], sel),
+                                       codes_to_half(x.v[n][5], x.v[n][4], sel), codes_to_half(x.v[n][7], x.v[n][6], sel));
+                *reinterpret_cast<half8_t *>(v + v_place(d + e, 2 * wave + half)) = y;
+            }
+        }
+        if (lane < 32) scales[buffer][lane / 16][16 * wave + lane % 16] = x.scale;
+        if (lane == 0) whole[buffer][wave] = page >= 0;
+    };
+    const auto use = [&](int buffer, int tile) {
+        const int8_t *k = lds + buffer * (kK + kV), *v = k + kK;
+        const int at = tile * kTile;
+        if (at >= any_to || at + kTile <= any_from) return;
+        floatx16 sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[t][e] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < DP / 16; x++) {
+                const half8_t kf = *reinterpret_cast<const half8_t *>(k + k_place(32 * t + col, 2 * x + h));
+#pragma unroll
+                for (int w = 0; w < kParts; w++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][w], sc[t], 0, 0, 0);
+            }
+        }
+        const intx4 ok = *reinterpret_cast<const intx4 *>(whole[buffer]);
+        const bool clear = at >= low && at + kTile <= high && at >= all_from && at + kTile <= all_to &&
+                           __builtin_amdgcn_readfirstlane(ok[0] & ok[1] & ok[2] & ok[3]);
+        float most = -__builtin_inff();
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const floatx4 ks = *reinterpret_cast<const floatx4 *>(&scales[buffer][0][32 * t + 2 * e + 4 * h]);
+#pragma unroll
+                for (int u = 0; u < 4; u++) sc[t][e + u] *= ks[u];
+            }
+        if (!clear) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int token = at + 32 * t + 8 * (e / 4) + 4 * h + e % 4;
+                    const bool keep = token >= low && token < high && token <= last && token >= start && ok[2 * t + e / 8];
+                    sc[t][e] = keep ? sc[t][e] : -__builtin_inff();
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) most = fmaxf(most, sc[t][e]);
+        const float mine = scales[buffer][1][lane];
+        const float value = mine < __builtin_inff() ? mine : 0.0f;
+        if (__any(most * factor > m + kSlack || value > unit)) {
+            float up = value;
+#pragma unroll
+            for (int d = 32; d; d >>= 1) up = fmaxf(up, __shfl_xor(up, d));
+            const float now = fmaxf(m, fmaxf(most, __shfl_xor(most, 32)) * factor);
+            float ratio = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - now) : 0.0f;
+            m = now;
+            if (up > unit) {
+                const unsigned bits = (__float_as_uint(up) & kInfBits) + 0x00800000u;
+                const int ex = min(max(static_cast<int>(bits >> 23) - 127, -96), 127);
+                ratio *= __builtin_amdgcn_exp2f(7.0f - static_cast<float>(ex) - base);
+                unit = ldexpf(1.0f, ex);
+                base = 7.0f - static_cast<float>(ex);
+            }
+            l *= ratio;
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) acc[j] *= ratio;
+        }
+        const float from = m > -__builtin_inff() ? base - m : 0.0f;
+        half8_t pf[4][kParts];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const floatx4 vs = *reinterpret_cast<const floatx4 *>(&scales[buffer][1][32 * t + 2 * e + 4 * h]);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e + u], factor, from));
+                    l += p;
+                    // 0 where the row masks the token, whose scale may be NaN
+                    const float w = !clear && sc[t][e + u] == -__builtin_inff() ? 0.0f : p * vs[u];
+                    const _Float16 hi = static_cast<_Float16>(w);
+                    pf[2 * t + e / 8][0][e % 8 + u] = hi;
+                    if constexpr (kWide) pf[2 * t + e / 8][kParts - 1][e % 8 + u] = static_cast<_Float16>(w - static_cast<float>(hi));
+                }
+            }
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const half8_t vf = *reinterpret_cast<const half8_t *>(v + v_place(32 * j + col, 2 * g + h));
+#pragma unroll
+                for (int w = 0; w < kParts; w++) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[g][w], acc[j], 0, 0, 0);
+            }
+    };
+
+    const int first = max(low, 0) / kTile, end = high > low ? (high + kTile - 1) / kTile : 0;
+    if (first < end) {
+        Stage x;
+        int page = page_of(first);
+        fetch(x, first, page);
+        put(x, first & 1, page);
+        page = first + 1 < end ? page_of(first + 1) : -1;
+        __syncthreads();
+        for (int tile = first; tile < end; tile++) {
+            const int then = page;
+            if (tile + 1 < end) {
+                fetch(x, tile + 1, then);
+                if (tile + 2 < end) page = page_of(tile + 2);
+            }
+            use(tile & 1, tile);
+            if (tile + 1 < end) put(x, ~tile & 1, then);
+            __syncthreads();
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (a.splits > 1) {
+        if (!in) return;
+        // totals and sums without 2^base, which is this split's own
+        const float back = __builtin_amdgcn_exp2f(-base);
+        const int64_t at_row = ((s.row0 + i) * a.heads + q_head) * a.splits + split;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * j + 2 * e + 4 * h;
+                if (d < dim)
+                    *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d) = floatx4{acc[j][e], acc[j][e + 1], acc[j][e + 2], acc[j][e + 3]} * back;
+            }
+        if (h == 0) {
+            a.stats[2 * at_row] = m;
+            a.stats[2 * at_row + 1] = l * back;
+        }
+        return;
+    }
+    // through this wave's part of LDS, 32 of d at a time, to 16-byte pieces (every wave is past its last tile)
+    constexpr int kPitch = 32 + 16 / static_cast<int>(sizeof(T)), kPiece = 16 / static_cast<int>(sizeof(T));
+    T *turn = reinterpret_cast<T *>(lds + wave * ((kK + kV) / 2));
+    const float part = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float o[4] = {acc[j][e] * part, acc[j][e + 1] * part, acc[j][e + 2] * part, acc[j][e + 3] * part};
+            store_floats<4>(turn + col * kPitch + 2 * e + 4 * h, o);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        constexpr int kLanes = 32 / kPiece;
+#pragma unroll
+        for (int y = 0; y < 32; y += 64 / kLanes) {
+            const int row = y + lane / kLanes, c = lane % kLanes * kPiece, d = 32 * j + c;
+            const int rr = w0 + row, ii = rr / a.group;
+            if (rr < rows && d < dim) {
+                const Vec<T, kPiece> o = *reinterpret_cast<const Vec<T, kPiece> *>(turn + row * kPitch + c);
+                T *out = static_cast<T *>(a.out) + (s.row0 + ii) * a.out_stride + static_cast<int64_t>(head * a.group + rr - ii * a.group) * dim + d;
+                __builtin_memcpy(out, o.v, sizeof(o.v));
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
 // A wave a row of q and head: its splits' sums, joined in their order.
 template <typename T>
 __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
@@ -396,12 +719,12 @@ struct Plan {
 Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
     Plan p;
     const int64_t rows = std::min(g.max_queries, g.queries) * (g.heads / c.kv_heads);
-    p.tiles = rows <= 16 ? 1 : rows <= 32 || c.head_dim > 128 ? 2 : 4;
+    p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
     p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
     // enough workgroups for four on each CU, and no split shorter than a chunk for each wave
     const int64_t base = static_cast<int64_t>(g.sequences) * c.kv_heads * p.row_blocks;
     const int64_t step = kWaves * kChunk;
-    int64_t splits = std::min<int64_t>((2048 + base - 1) / base, (g.max_length + step - 1) / step);
+    int64_t splits = std::min<int64_t>(p.tiles == 8 ? std::max<int64_t>(512 / base, 1) : (2048 + base - 1) / base, (g.max_length + step - 1) / step);
     splits = std::max<int64_t>(splits, 1);
     int64_t tokens = (g.max_length + splits - 1) / splits;
     tokens = std::max<int64_t>((tokens + step - 1) / step * step, step);
@@ -456,7 +779,7 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         const Plan p = plan(*c, *g);
         if (p.splits > 1 && (!g->workspace || g->workspace_size < p.part + p.stats || !aligned(g->workspace, 16)))
             return bad("attention_i8: the workspace is missing, too small or not 16-byte aligned");
-        if (g->sequences * p.row_blocks > INT32_MAX / p.splits ||
+        if (g->sequences * p.row_blocks > INT32_MAX / p.splits / c->kv_heads ||
             g->sequences * std::min(g->max_queries, g->queries) > INT32_MAX)
             return unsupported("attention_i8: too many queries and sequences for one launch");
         unsigned mul;
@@ -467,22 +790,26 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
                    static_cast<int>(std::min<int64_t>(g->max_queries, g->queries)), static_cast<int>(g->max_length), g->table_width, g->heads,
                    g->heads / c->kv_heads, g->sequences, g->causal, g->window, g->scale, static_cast<int>(p.row_blocks), p.split_tokens, p.splits,
                    mul, shift};
-        const dim3 grid(static_cast<unsigned>(g->sequences * p.row_blocks * p.splits), c->kv_heads);
+        const unsigned blocks = static_cast<unsigned>(g->sequences * p.row_blocks * p.splits);
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
-            auto go = [&](auto one, auto two, auto four) {
-                const char *what = "attention_i8";
-                if (int rc = p.tiles == 1 ? launch(what, one, grid, dim3(256), stream, a)
-                             : p.tiles == 2 ? launch(what, two, grid, dim3(256), stream, a)
-                                            : launch(what, four, grid, dim3(256), stream, a))
-                    return rc;
-                if (p.splits == 1) return 0;
-                const dim3 rows(static_cast<unsigned>(g->sequences * a.max_queries), (g->heads + 3) / 4);
-                return launch(what, join_splits<T>, rows, dim3(256), stream, a);
+            const char *what = "attention_i8";
+            auto go = [&](auto one, auto two) {
+                return launch(what, p.tiles == 1 ? one : two, dim3(blocks, c->kv_heads), dim3(256), stream, a);
             };
-            if (c->head_dim <= 64) return go(attend_rows<T, 64, 1>, attend_rows<T, 64, 2>, attend_rows<T, 64, 4>);
-            if (c->head_dim <= 128) return go(attend_rows<T, 128, 1>, attend_rows<T, 128, 2>, attend_rows<T, 128, 4>);
-            return go(attend_rows<T, 256, 1>, attend_rows<T, 256, 2>, attend_rows<T, 256, 2>);
+            auto many = [&](auto kernel) { return launch(what, kernel, dim3(blocks * c->kv_heads), dim3(256), stream, a); };
+            const int dim = c->head_dim;
+            int rc;
+            if (p.tiles == 8) {
+                rc = dim <= 64 ? many(attend_tiles<T, 64>) : dim <= 96 ? many(attend_tiles<T, 96>) : dim <= 128 ? many(attend_tiles<T, 128>) : many(attend_tiles<T, 256>);
+            } else {
+                rc = dim <= 64    ? go(attend_rows<T, 64, 1>, attend_rows<T, 64, 2>)
+                     : dim <= 128 ? go(attend_rows<T, 128, 1>, attend_rows<T, 128, 2>)
+                                  : go(attend_rows<T, 256, 1>, attend_rows<T, 256, 2>);
+            }
+            if (rc || p.splits == 1) return rc;
+            const dim3 rows(static_cast<unsigned>(g->sequences * a.max_queries), (g->heads + 3) / 4);
+            return launch(what, join_splits<T>, rows, dim3(256), stream, a);
         });
     });
 }
