@@ -49,6 +49,11 @@ __device__ __forceinline__ half8_t codes8(unsigned a, unsigned b) {
                 codes_to_half(0, b, 0x0c030c02u));
 }
 
+// A value that is split into parts is rounded to fp32 first: a product fused
+// into the conversion to its high part, but not into the low part's, would give
+// parts of two values, a step of fp16 apart where one lies next to a tie.
+__device__ __forceinline__ void once(float &v) { asm("" : "+v"(v)); }
+
 __device__ __forceinline__ float over_groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -263,7 +268,8 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
                 const float p = __builtin_amdgcn_exp2f(v[e] - from);
                 l[t] += p;
                 // 0 where the row masks the token, whose scale may be NaN
-                const float w = v[e] == -__builtin_inff() ? 0.0f : p * (vs[e] * per_unit);
+                float w = v[e] == -__builtin_inff() ? 0.0f : p * (vs[e] * per_unit);
+                if constexpr (kWide) once(w);
                 const _Float16 hi = static_cast<_Float16>(w);
                 pf[t][0][e] = hi;
                 if constexpr (kWide) pf[t][kParts - 1][e] = static_cast<_Float16>(w - static_cast<float>(hi));
@@ -374,7 +380,9 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) attend_tiles(AttnArgs a) {
     constexpr bool kWide = sizeof(T) == 4;
     constexpr int kParts = kWide ? 2 : 1;
-    constexpr int kK = kTile * DP * 2, kV = DP * kTile * 2;  // bytes
+    // 16 bytes past each row: any 16 rows' pieces of one column lie on different banks
+    constexpr int kKPitch = DP * 2 + 16, kVPitch = kTile * 2 + 16;
+    constexpr int kK = kTile * kKPitch, kV = DP * kVPitch;  // bytes
     constexpr int kKItems = (DP + 63) / 64, kVItems = (DP / 2 + 63) / 64;
     __shared__ __align__(16) int8_t lds[2 * (kK + kV)];
     __shared__ __align__(16) float scales[2][2][kTile];
@@ -459,90 +467,97 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         unsigned v[kVItems][8];
         float scale;
     };
-    const auto page_of = [&](int tile) {
-        const int t = tile * kTile + 16 * wave;
-        if (t >= high) return -1;
-        const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
-        const int page = a.table[static_cast<int64_t>(b) * a.table_width + page_at];
-        return page < a.c.pages ? page : -1;
+    const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
+    const auto page_of = [&](int tile) {  // as the table has it: looked at when the tile is fetched
+        const unsigned t = min(tile * kTile + 16 * wave, high - 1);
+        return table[(static_cast<uint64_t>(t) * a.page_mul) >> a.page_shift];
     };
-    // this wave's 16 tokens of a tile
+    const auto there = [&](int page) { return page >= 0 && page < a.c.pages; };
+    // This wave's 16 tokens of a tile.  Where a page is missing (its tokens are
+    // masked) page 0 is read; codes past the head's, which meet zeros of q or
+    // give columns that are not stored, are other codes of the token.
+    unsigned k_at[kKItems], v_at[kVItems];
+#pragma unroll
+    for (int n = 0; n < kKItems; n++) {
+        const int item = n * 64 + lane;
+        k_at[n] = min(item / (DP / 16), 15) * dim + min(item % (DP / 16) * 16, dim - 16);
+    }
+#pragma unroll
+    for (int n = 0; n < kVItems; n++) {
+        const int item = n * 64 + lane;
+        v_at[n] = min(item / (DP / 4), 1) * 4 * dim + min(item % (DP / 4) * 4, dim - 4);
+    }
     const auto fetch = [&](Stage &x, int tile, int page) {
         const int t = tile * kTile + 16 * wave;
         const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
-        const int64_t row = (static_cast<int64_t>(page) * a.c.kv_heads + head) * a.c.page_size + (t - page_at * a.c.page_size);
+        const int64_t row = (static_cast<int64_t>(there(page) ? page : 0) * a.c.kv_heads + head) * a.c.page_size + (t - page_at * a.c.page_size);
         const int8_t *k = a.c.k + row * dim, *v = a.c.v + row * dim;
-        const bool there = page >= 0;
+        // the lanes' offsets are added by the loads: sums made ahead of the loop would take two registers each
 #pragma unroll
-        for (int n = 0; n < kKItems; n++) {
-            const int item = n * 64 + lane, at = item / (DP / 16), d = item % (DP / 16) * 16;
-            x.k[n] = uintx4{0, 0, 0, 0};
-            if (there && at < 16 && d < dim) x.k[n] = *reinterpret_cast<const uintx4 *>(k + at * dim + d);
-        }
+        for (int n = 0; n < kKItems; n++) asm("" : "+v"(k_at[n]));
 #pragma unroll
-        for (int n = 0; n < kVItems; n++) {
-            const int item = n * 64 + lane, d = item % (DP / 4) * 4, half = item / (DP / 4);
+        for (int n = 0; n < kVItems; n++) asm("" : "+v"(v_at[n]));
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x.v[n][e] = 0;
-                if (there && half < 2 && d < dim) x.v[n][e] = *reinterpret_cast<const unsigned *>(v + (e / 4 * 8 + half * 4 + e % 4) * dim + d);
-            }
+        for (int n = 0; n < kKItems; n++) x.k[n] = *reinterpret_cast<const uintx4 *>(k + k_at[n]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int8_t *ve = v + (e / 4 * 8 + e % 4) * dim;
+#pragma unroll
+            for (int n = 0; n < kVItems; n++) x.v[n][e] = *reinterpret_cast<const unsigned *>(ve + v_at[n]);
         }
         // lanes 0 .. 15: key scales, 16 .. 31: value scales; zeros for tokens outside the range
         const int token = t + (lane & 15);
-        x.scale = 0.0f;
-        if (there && lane < 32 && token >= low && token < high) x.scale = (lane < 16 ? a.c.k_scale : a.c.v_scale)[row + (lane & 15)];
+        x.scale = ((lane & 16) == 0 ? a.c.k_scale : a.c.v_scale)[row + (lane & 15)];
+        if (!there(page) || token < low || token >= high) x.scale = 0.0f;
     };
-    // places of 16-byte pieces that put any 16 rows' pieces of one column on different banks
-    const auto k_place = [](int row, int piece) {
-        const int turn = DP == 64 ? row / 2 & 7 : DP == 96 ? row / 4 & 3 : row & 15;
-        return row * (DP * 2) + (piece ^ turn) * 16;
-    };
-    const auto v_place = [](int row, int piece) { return row * (kTile * 2) + (piece ^ ((row / 2 ^ row / 16) & 7)) * 16; };
+    // V's rows lie in the order d = 0, 4, 8 .., 1, 5, 9 ..: lanes next to each
+    // other write rows next to each other, and a lane's sums are runs of four d.
     const auto put = [&](const Stage &x, int buffer, int page) {
         int8_t *k = lds + buffer * (kK + kV), *v = k + kK;
 #pragma unroll
         for (int n = 0; n < kKItems; n++) {
             const int item = n * 64 + lane, at = item / (DP / 16), piece = item % (DP / 16) * 2;
-            if (DP % 64 && at >= 16) continue;
+            if (DP == 96 && at >= 16) continue;
 #pragma unroll
             for (int e = 0; e < 2; e++)
-                *reinterpret_cast<half8_t *>(k + k_place(16 * wave + at, piece + e)) = codes8(x.k[n][2 * e], x.k[n][2 * e + 1]);
+                *reinterpret_cast<half8_t *>(k + (16 * wave + at) * kKPitch + (piece + e) * 16) = codes8(x.k[n][2 * e], x.k[n][2 * e + 1]);
         }
 #pragma unroll
         for (int n = 0; n < kVItems; n++) {
-            const int item = n * 64 + lane, d = item % (DP / 4) * 4, half = item / (DP / 4);
-            if (DP % 128 && half >= 2) continue;
+            const int item = n * 64 + lane, dq = item % (DP / 4), half = item / (DP / 4);
+            if (DP < 128 && half >= 2) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const unsigned sel = 0x0c000c00u | ((4u + e) << 16) | e;
                 const half8_t y = join(codes_to_half(x.v[n][1], x.v[n][0], sel), codes_to_half(x.v[n][3], x.v[n][2], sel),
                                        codes_to_half(x.v[n][5], x.v[n][4], sel), codes_to_half(x.v[n][7], x.v[n][6], sel));
-                *reinterpret_cast<half8_t *>(v + v_place(d + e, 2 * wave + half)) = y;
+                *reinterpret_cast<half8_t *>(v + (e * (DP / 4) + dq) * kVPitch + (2 * wave + half) * 16) = y;
             }
         }
         if (lane < 32) scales[buffer][lane / 16][16 * wave + lane % 16] = x.scale;
-        if (lane == 0) whole[buffer][wave] = page >= 0;
+        if (lane == 0) whole[buffer][wave] = there(page);
     };
-    const auto use = [&](int buffer, int tile) {
-        const int8_t *k = lds + buffer * (kK + kV), *v = k + kK;
-        const int at = tile * kTile;
-        if (at >= any_to || at + kTile <= any_from) return;
-        floatx16 sc[2];
+    floatx16 sc[2];
+    const auto scores = [&](int buffer) {
+        const int8_t *k = lds + buffer * (kK + kV);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[t][e] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < DP / 16; x++) {
-                const half8_t kf = *reinterpret_cast<const half8_t *>(k + k_place(32 * t + col, 2 * x + h));
+        for (int x = 0; x < DP / 16; x++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const half8_t kf = *reinterpret_cast<const half8_t *>(k + (32 * t + col) * kKPitch + (2 * x + h) * 16);
 #pragma unroll
                 for (int w = 0; w < kParts; w++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][w], sc[t], 0, 0, 0);
             }
-        }
-        const intx4 ok = *reinterpret_cast<const intx4 *>(whole[buffer]);
-        const bool clear = at >= low && at + kTile <= high && at >= all_from && at + kTile <= all_to &&
-                           __builtin_amdgcn_readfirstlane(ok[0] & ok[1] & ok[2] & ok[3]);
+    };
+    // clear: every row of the wave reads every token of the tile
+    const auto use = [&](bool clear, int buffer, int tile, intx4 ok) {
+        const int8_t *v = lds + buffer * (kK + kV) + kK;
+        // this lane's first and last token of the tile, counted from its first one there
+        const int from_at = max(low, start) - tile * kTile - 4 * h, to_at = min(high - 1, last) - tile * kTile - 4 * h;
         float most = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -557,8 +572,8 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const int token = at + 32 * t + 8 * (e / 4) + 4 * h + e % 4;
-                    const bool keep = token >= low && token < high && token <= last && token >= start && ok[2 * t + e / 8];
+                    const int token = 32 * t + 8 * (e / 4) + e % 4;
+                    const bool keep = token >= from_at && token <= to_at && ok[2 * t + e / 8];
                     sc[t][e] = keep ? sc[t][e] : -__builtin_inff();
                 }
         }
@@ -597,18 +612,29 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
                 for (int u = 0; u < 4; u++) {
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][e + u], factor, from));
                     l += p;
-                    // 0 where the row masks the token, whose scale may be NaN
-                    const float w = !clear && sc[t][e + u] == -__builtin_inff() ? 0.0f : p * vs[u];
+                    float w = p * vs[u];
+                    if constexpr (kWide) once(w);
                     const _Float16 hi = static_cast<_Float16>(w);
                     pf[2 * t + e / 8][0][e % 8 + u] = hi;
                     if constexpr (kWide) pf[2 * t + e / 8][kParts - 1][e % 8 + u] = static_cast<_Float16>(w - static_cast<float>(hi));
                 }
             }
+        // a scale that is not finite reaches no row that masks its token
+        if (!clear && __any(!(fabsf(mine) < __builtin_inff()))) {
 #pragma unroll
-        for (int j = 0; j < DP / 32; j++)
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const half8_t vf = *reinterpret_cast<const half8_t *>(v + v_place(32 * j + col, 2 * g + h));
+                for (int e = 0; e < 16; e++)
+#pragma unroll
+                    for (int w = 0; w < kParts; w++)
+                        if (sc[t][e] == -__builtin_inff()) pf[2 * t + e / 8][w][e % 8] = static_cast<_Float16>(0.0f);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) {
+                const half8_t vf = *reinterpret_cast<const half8_t *>(v + (32 * j + col) * kVPitch + (2 * g + h) * 16);
 #pragma unroll
                 for (int w = 0; w < kParts; w++) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[g][w], acc[j], 0, 0, 0);
             }
@@ -617,23 +643,33 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     const int first = max(low, 0) / kTile, end = high > low ? (high + kTile - 1) / kTile : 0;
     if (first < end) {
         Stage x;
-        int page = page_of(first);
+        int page = page_of(first), then = page_of(first + 1), later = page_of(first + 2);
         fetch(x, first, page);
         put(x, first & 1, page);
-        page = first + 1 < end ? page_of(first + 1) : -1;
+        fetch(x, min(first + 1, end - 1), then);
         __syncthreads();
         for (int tile = first; tile < end; tile++) {
-            const int then = page;
-            if (tile + 1 < end) {
-                fetch(x, tile + 1, then);
-                if (tile + 2 < end) page = page_of(tile + 2);
+            const int buffer = tile & 1, at = tile * kTile;
+            // the next tile is turned while this one's scores are multiplied, the one after it is loaded meanwhile
+            scores(buffer);
+            put(x, buffer ^ 1, then);
+            __builtin_amdgcn_sched_barrier(0);
+            then = later;
+            fetch(x, min(tile + 2, end - 1), then);
+            later = page_of(tile + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            if (at < any_to && at + kTile > any_from) {
+                intx4 ok = *reinterpret_cast<const intx4 *>(whole[buffer]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) ok[e] = __builtin_amdgcn_readfirstlane(ok[e]);
+                use(at >= low && at + kTile <= high && at >= all_from && at + kTile <= all_to && (ok[0] & ok[1] & ok[2] & ok[3]), buffer, tile, ok);
             }
-            use(tile & 1, tile);
-            if (tile + 1 < end) put(x, ~tile & 1, then);
             __syncthreads();
         }
     }
 
+    // the sum of d = 32 q + 16 h + 4 u + e
+    const auto sum = [&](int q, int u, int e) { return acc[(e * (DP / 32) + q) / 4][(e * (DP / 32) + q) % 4 * 4 + u]; };
     l += __shfl_xor(l, 32);
     if (a.splits > 1) {
         if (!in) return;
@@ -641,12 +677,11 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         const float back = __builtin_amdgcn_exp2f(-base);
         const int64_t at_row = ((s.row0 + i) * a.heads + q_head) * a.splits + split;
 #pragma unroll
-        for (int j = 0; j < DP / 32; j++)
+        for (int q = 0; q < DP / 32; q++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 32 * j + 2 * e + 4 * h;
-                if (d < dim)
-                    *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d) = floatx4{acc[j][e], acc[j][e + 1], acc[j][e + 2], acc[j][e + 3]} * back;
+            for (int u = 0; u < 4; u++) {
+                const int d = 32 * q + 16 * h + 4 * u;
+                if (d < dim) *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d) = floatx4{sum(q, u, 0), sum(q, u, 1), sum(q, u, 2), sum(q, u, 3)} * back;
             }
         if (h == 0) {
             a.stats[2 * at_row] = m;
@@ -661,9 +696,9 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 #pragma unroll
     for (int j = 0; j < DP / 32; j++) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const float o[4] = {acc[j][e] * part, acc[j][e + 1] * part, acc[j][e + 2] * part, acc[j][e + 3] * part};
-            store_floats<4>(turn + col * kPitch + 2 * e + 4 * h, o);
+        for (int u = 0; u < 4; u++) {
+            const float o[4] = {sum(j, u, 0) * part, sum(j, u, 1) * part, sum(j, u, 2) * part, sum(j, u, 3) * part};
+            store_floats<4>(turn + col * kPitch + 16 * h + 4 * u, o);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         constexpr int kLanes = 32 / kPiece;
