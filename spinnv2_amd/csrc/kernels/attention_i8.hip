@@ -390,10 +390,12 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    // the heaviest rows of a causal mask first; a sequence's and head's blocks
-    // on one XCD where their number is a multiple of eight
-    const int pairs = a.sequences * a.c.kv_heads;
-    const int pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    // The heaviest rows of a causal mask first; a sequence's and head's blocks
+    // on one XCD where the pairs are a multiple of eight, in an order that turns,
+    // since an XCD's workgroups go to its four engines in turn too: without the
+    // turn two sequences of 4001 and 6007 tokens keep an engine each.
+    const unsigned pairs = a.sequences * a.c.kv_heads, rest = blockIdx.x / pairs;
+    const int pair = (blockIdx.x + rest / 2 % pairs * 8) % pairs;
     const int b = pair / a.c.kv_heads, head = pair - b * a.c.kv_heads;
     const int split = rest % a.splits, block = a.row_blocks - 1 - rest / a.splits;
     const int dim = a.c.head_dim;
