@@ -385,8 +385,9 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     constexpr int kK = kTile * kKPitch, kV = DP * kVPitch;  // bytes
     constexpr int kKItems = (DP + 63) / 64, kVItems = (DP / 2 + 63) / 64;
     __shared__ __align__(16) int8_t lds[2 * (kK + kV)];
-    __shared__ __align__(16) float scales[2][2][kTile];
-    __shared__ __align__(16) int whole[2][4];
+    __shared__ __align__(16) float scales[2][4][kTile];  // keys', values', and twice what no one reads
+    __shared__ __align__(16) unsigned held[2][4];  // kThere, and a bit for each of 16 tokens
+    constexpr unsigned kThere = 1u << 16;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
@@ -415,11 +416,9 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     const int last = a.causal ? s.position + i : s.length - 1;
     const int start = a.causal && a.window ? last + 1 - a.window : 0;
     const int wave_first = w0 / a.group, wave_last = (min(rows, w0 + 32) - 1) / a.group;  // queries
-    // tokens that all of the wave's rows read, and that any does
+    // tokens that all of the wave's rows read
     const int all_from = a.causal && a.window ? s.position + wave_last + 1 - a.window : 0;
     const int all_to = a.causal ? s.position + wave_first + 1 : s.length;
-    const int any_from = a.causal && a.window ? s.position + wave_first + 1 - a.window : 0;
-    const int any_to = w0 >= rows ? 0 : a.causal ? s.position + wave_last + 1 : s.length;
 
     half8_t qf[DP / 16][kParts];
     float factor;
@@ -474,7 +473,8 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         const unsigned t = min(tile * kTile + 16 * wave, high - 1);
         return table[(static_cast<uint64_t>(t) * a.page_mul) >> a.page_shift];
     };
-    const auto there = [&](int page) { return page >= 0 && page < a.c.pages; };
+    const unsigned pages = static_cast<unsigned>(a.c.pages);
+    const auto there = [&](int page) { return static_cast<unsigned>(page) < pages; };
     // This wave's 16 tokens of a tile.  Where a page is missing (its tokens are
     // masked) page 0 is read; codes past the head's, which meet zeros of q or
     // give columns that are not stored, are other codes of the token.
@@ -489,33 +489,43 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         const int item = n * 64 + lane;
         v_at[n] = min(item / (DP / 4), 1) * 4 * dim + min(item % (DP / 4) * 4, dim - 4);
     }
-    const auto fetch = [&](Stage &x, int tile, int page) {
+    // a token's row in the cache, in two parts: its page's first row (of this head), and the row in the page
+    const int64_t page_rows = static_cast<int64_t>(a.c.kv_heads) * a.c.page_size;
+    const int8_t *k_head = a.c.k + static_cast<int64_t>(head) * a.c.page_size * dim, *v_head = a.c.v + static_cast<int64_t>(head) * a.c.page_size * dim;
+    const float *k_scale = a.c.k_scale + static_cast<int64_t>(head) * a.c.page_size, *v_scale = a.c.v_scale + static_cast<int64_t>(head) * a.c.page_size;
+    const auto row_of = [&](int tile, int page) {
         const int t = tile * kTile + 16 * wave;
         const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
-        const int64_t row = (static_cast<int64_t>(there(page) ? page : 0) * a.c.kv_heads + head) * a.c.page_size + (t - page_at * a.c.page_size);
-        const int8_t *k = a.c.k + row * dim, *v = a.c.v + row * dim;
-        // the lanes' offsets are added by the loads: sums made ahead of the loop would take two registers each
+        page = __builtin_amdgcn_readfirstlane(page);
+        return (there(page) ? page : 0) * page_rows + (t - page_at * a.c.page_size);
+    };
+    // The lanes' offsets are added by the loads: sums made ahead of the loop would take two registers each.
+    const auto fetch = [&](Stage &x, int tile, int page) {
+        const int64_t row = row_of(tile, page);
+        const int8_t *k = k_head + row * dim;
 #pragma unroll
-        for (int n = 0; n < kKItems; n++) asm("" : "+v"(k_at[n]));
+        for (int n = 0; n < kKItems; n++) {
+            asm("" : "+v"(k_at[n]));
+            x.k[n] = *reinterpret_cast<const uintx4 *>(k + k_at[n]);
+        }
+        // lanes 0 .. 15: key scales, 16 .. 31: value scales; zeros for tokens outside the range
+        const int token = tile * kTile + 16 * wave + (lane & 15);
+        x.scale = ((lane & 16) == 0 ? k_scale : v_scale)[row + (lane & 15)];
+        if (!there(page) || token < low || token >= high) x.scale = 0.0f;
+        const int8_t *v = v_head + row * dim;
 #pragma unroll
         for (int n = 0; n < kVItems; n++) asm("" : "+v"(v_at[n]));
-#pragma unroll
-        for (int n = 0; n < kKItems; n++) x.k[n] = *reinterpret_cast<const uintx4 *>(k + k_at[n]);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int8_t *ve = v + (e / 4 * 8 + e % 4) * dim;
 #pragma unroll
             for (int n = 0; n < kVItems; n++) x.v[n][e] = *reinterpret_cast<const unsigned *>(ve + v_at[n]);
         }
-        // lanes 0 .. 15: key scales, 16 .. 31: value scales; zeros for tokens outside the range
-        const int token = t + (lane & 15);
-        x.scale = ((lane & 16) == 0 ? a.c.k_scale : a.c.v_scale)[row + (lane & 15)];
-        if (!there(page) || token < low || token >= high) x.scale = 0.0f;
     };
     // V's rows lie in the order d = 0, 4, 8 .., 1, 5, 9 ..: lanes next to each
     // other write rows next to each other, and a lane's sums are runs of four d.
     const auto put = [&](const Stage &x, int buffer, int page) {
-        int8_t *k = lds + buffer * (kK + kV), *v = k + kK;
+        int8_t *k = lds + buffer * kK, *v = lds + 2 * kK + buffer * kV;
 #pragma unroll
         for (int n = 0; n < kKItems; n++) {
             const int item = n * 64 + lane, at = item / (DP / 16), piece = item % (DP / 16) * 2;
@@ -524,6 +534,11 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
             for (int e = 0; e < 2; e++)
                 *reinterpret_cast<half8_t *>(k + (16 * wave + at) * kKPitch + (piece + e) * 16) = codes8(x.k[n][2 * e], x.k[n][2 * e + 1]);
         }
+        // a value's scale that is not finite is one of the bits of `held`, and 0 in the product
+        const bool odd = (lane & 16) && !(fabsf(x.scale) < __builtin_inff());
+        const unsigned odds = static_cast<unsigned>(__ballot(odd)) >> 16;
+        scales[buffer][lane / 16][16 * wave + lane % 16] = odd ? 0.0f : x.scale;
+        held[buffer][wave] = there(page) ? kThere | odds : 0;
 #pragma unroll
         for (int n = 0; n < kVItems; n++) {
             const int item = n * 64 + lane, dq = item % (DP / 4), half = item / (DP / 4);
@@ -536,12 +551,10 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
                 *reinterpret_cast<half8_t *>(v + (e * (DP / 4) + dq) * kVPitch + (2 * wave + half) * 16) = y;
             }
         }
-        if (lane < 32) scales[buffer][lane / 16][16 * wave + lane % 16] = x.scale;
-        if (lane == 0) whole[buffer][wave] = there(page);
     };
     floatx16 sc[2];
     const auto scores = [&](int buffer) {
-        const int8_t *k = lds + buffer * (kK + kV);
+        const int8_t *k = lds + buffer * kK;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -555,11 +568,26 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
                 for (int w = 0; w < kParts; w++) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][w], sc[t], 0, 0, 0);
             }
     };
-    // clear: every row of the wave reads every token of the tile
-    const auto use = [&](bool clear, int buffer, int tile, intx4 ok) {
-        const int8_t *v = lds + buffer * (kK + kV) + kK;
-        // this lane's first and last token of the tile, counted from its first one there
-        const int from_at = max(low, start) - tile * kTile - 4 * h, to_at = min(high - 1, last) - tile * kTile - 4 * h;
+    const auto add_values = [&](int buffer, const half8_t (&pf)[4][kParts]) {
+        const int8_t *v = lds + 2 * kK + buffer * kV;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) {
+                const half8_t vf = *reinterpret_cast<const half8_t *>(v + (32 * j + col) * kVPitch + (2 * g + h) * 16);
+#pragma unroll
+                for (int w = 0; w < kParts; w++) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[g][w], acc[j], 0, 0, 0);
+            }
+    };
+    const auto weights = [&](int buffer, int tile, half8_t (&pf)[4][kParts]) {
+        const uintx4 bits = *reinterpret_cast<const uintx4 *>(held[buffer]);
+        unsigned ok[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) ok[e] = __builtin_amdgcn_readfirstlane(bits[e]);
+        const bool plain = ok[0] == kThere && ok[1] == kThere && ok[2] == kThere && ok[3] == kThere;
+        const int at = tile * kTile;
+        // every row of the wave reads every token of the tile
+        const bool clear = at >= low && at + kTile <= high && at >= all_from && at + kTile <= all_to && plain;
         float most = -__builtin_inff();
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -570,21 +598,29 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
                 for (int u = 0; u < 4; u++) sc[t][e + u] *= ks[u];
             }
         if (!clear) {
+            // this lane's first and last token of the tile, counted from its first one there
+            const int from_at = max(low, start) - at - 4 * h, to_at = min(high - 1, last) - at - 4 * h;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int token = 32 * t + 8 * (e / 4) + e % 4;
-                    const bool keep = token >= from_at && token <= to_at && ok[2 * t + e / 8];
+                    const bool keep = token >= from_at && token <= to_at && (ok[2 * t + e / 8] & kThere);
                     sc[t][e] = keep ? sc[t][e] : -__builtin_inff();
                 }
+            if ((ok[0] | ok[1] | ok[2] | ok[3]) & (kThere - 1)) {  // NaN for the rows that read such a token, and only those
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if ((ok[2 * t + e / 8] >> (8 * (e / 4 % 2) + 4 * h + e % 4) & 1) && sc[t][e] != -__builtin_inff()) sc[t][e] = __builtin_nanf("");
+            }
         }
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) most = fmaxf(most, sc[t][e]);
-        const float mine = scales[buffer][1][lane];
-        const float value = mine < __builtin_inff() ? mine : 0.0f;
+        const float value = scales[buffer][1][lane];
         if (__any(most * factor > m + kSlack || value > unit)) {
             float up = value;
 #pragma unroll
@@ -604,7 +640,6 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
             for (int j = 0; j < DP / 32; j++) acc[j] *= ratio;
         }
         const float from = m > -__builtin_inff() ? base - m : 0.0f;
-        half8_t pf[4][kParts];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -621,25 +656,6 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
                     if constexpr (kWide) pf[2 * t + e / 8][kParts - 1][e % 8 + u] = static_cast<_Float16>(w - static_cast<float>(hi));
                 }
             }
-        // a scale that is not finite reaches no row that masks its token
-        if (!clear && __any(!(fabsf(mine) < __builtin_inff()))) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-#pragma unroll
-                    for (int w = 0; w < kParts; w++)
-                        if (sc[t][e] == -__builtin_inff()) pf[2 * t + e / 8][w][e % 8] = static_cast<_Float16>(0.0f);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-#pragma unroll
-            for (int j = 0; j < DP / 32; j++) {
-                const half8_t vf = *reinterpret_cast<const half8_t *>(v + (32 * j + col) * kVPitch + (2 * g + h) * 16);
-#pragma unroll
-                for (int w = 0; w < kParts; w++) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[g][w], acc[j], 0, 0, 0);
-            }
     };
 
     const int first = max(low, 0) / kTile, end = high > low ? (high + kTile - 1) / kTile : 0;
@@ -650,22 +666,16 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         put(x, first & 1, page);
         fetch(x, min(first + 1, end - 1), then);
         __syncthreads();
+        // the next tile is turned while this one's scores are multiplied, the one after it is loaded meanwhile
         for (int tile = first; tile < end; tile++) {
-            const int buffer = tile & 1, at = tile * kTile;
-            // the next tile is turned while this one's scores are multiplied, the one after it is loaded meanwhile
-            scores(buffer);
-            put(x, buffer ^ 1, then);
-            __builtin_amdgcn_sched_barrier(0);
+            scores(tile & 1);
+            put(x, ~tile & 1, then);
+            fetch(x, min(tile + 2, end - 1), later);
             then = later;
-            fetch(x, min(tile + 2, end - 1), then);
             later = page_of(tile + 3);
-            __builtin_amdgcn_sched_barrier(0);
-            if (at < any_to && at + kTile > any_from) {
-                intx4 ok = *reinterpret_cast<const intx4 *>(whole[buffer]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) ok[e] = __builtin_amdgcn_readfirstlane(ok[e]);
-                use(at >= low && at + kTile <= high && at >= all_from && at + kTile <= all_to && (ok[0] & ok[1] & ok[2] & ok[3]), buffer, tile, ok);
-            }
+            half8_t pf[4][kParts];
+            weights(tile & 1, tile, pf);
+            add_values(tile & 1, pf);
             __syncthreads();
         }
     }
@@ -691,9 +701,11 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         }
         return;
     }
-    // through this wave's part of LDS, 32 of d at a time, to 16-byte pieces (every wave is past its last tile)
+    // Through this wave's part of LDS, 32 of d at a time, to 16-byte pieces: the
+    // part of K, which every wave is past; V's last tile may still be read.
     constexpr int kPitch = 32 + 16 / static_cast<int>(sizeof(T)), kPiece = 16 / static_cast<int>(sizeof(T));
-    T *turn = reinterpret_cast<T *>(lds + wave * ((kK + kV) / 2));
+    T *turn = reinterpret_cast<T *>(lds + wave * (kK / 2));
+    static_assert(32 * kPitch * sizeof(T) <= kK / 2, "a wave's part of LDS holds 32 rows of 32");
     const float part = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int j = 0; j < DP / 32; j++) {
