@@ -85,6 +85,38 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
     return s;
 }
 
+// A split in which rows r0 .. r1 read no token: no sums, and a total of 0.
+__device__ __forceinline__ void nothing(const AttnArgs &a, const Sequence &s, int head, int split, int r0, int r1) {
+    for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += 256) {
+        const int i = r / a.group;
+        const int64_t at = ((s.row0 + i) * a.heads + head * a.group + (r - i * a.group)) * a.splits + split;
+        a.stats[2 * at] = -__builtin_inff();
+        a.stats[2 * at + 1] = 0.0f;
+    }
+}
+
+// Which rows and tokens are a workgroup's: the first split of every sequence and
+// head first, the heaviest rows of a causal mask ahead, so that what runs at the
+// end is short.  A sequence's and head's blocks are on one XCD where the pairs
+// are a multiple of eight, in an order that turns, since an XCD's workgroups go
+// to its four engines in turn too.  With the splits side by side each XCD had
+// its own, most of them empty on two of the eight (64 sequences of 3001 to 16384
+// tokens: 420 us, 305 in this order); without the turn two sequences of 4001 and
+// 6007 tokens kept two engines each (619 us, 530 with it).
+struct Place {
+    int b, head, split, block;
+};
+__device__ __forceinline__ Place place(const AttnArgs &a) {
+    const unsigned pairs = a.sequences * a.c.kv_heads, rest = blockIdx.x / pairs;
+    const int pair = (blockIdx.x + rest / 2 % pairs * 8) % pairs;
+    Place p;
+    p.b = pair / a.c.kv_heads;
+    p.head = pair - p.b * a.c.kv_heads;
+    p.split = rest / a.row_blocks;
+    p.block = a.row_blocks - 1 - rest % a.row_blocks;
+    return p;
+}
+
 // One workgroup: RT tiles of 16 rows (query, head of the group) of one
 // sequence and kv head, and one split of its tokens.  Scores are taken
 // transposed, S^T = K q^T on 16x16 tiles: a lane then holds four tokens'
@@ -99,7 +131,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
 //   V: those tokens' codes VPL (l % 16) .. + VPL (VPL = DP / 16); product j
 //      takes d = VPL r + j as its row r
 template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
+__global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) attend_rows(AttnArgs a) {
     constexpr bool kWide = sizeof(T) == 4;  // rows of 22 bits: two fp16 parts
     constexpr int kParts = kWide ? 2 : 1;
     constexpr int kPieces = DP / 64;  // 16-byte pieces of K a lane
@@ -110,9 +142,8 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int head = blockIdx.y;
-    const int at_x = blockIdx.x / a.splits, split = blockIdx.x - at_x * a.splits;
-    const int b = at_x / a.row_blocks, block = at_x - b * a.row_blocks;
+    const Place at_block = place(a);
+    const int b = at_block.b, head = at_block.head, split = at_block.split, block = at_block.block;
     const int dim = a.c.head_dim;
     const Sequence s = sequence(a, b);
     const int rows = s.count * a.group, r0 = block * 16 * RT;
@@ -122,6 +153,11 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
     if (a.causal) {
         high = min(high, s.position + last_q + 1);
         if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+    }
+
+    if (a.splits > 1 && low >= high) {
+        nothing(a, s, head, split, r0, min(rows, r0 + 16 * RT));
+        return;
     }
 
     // the rows' masks and queries, scaled by a power of two to 2^14 .. 2^15
@@ -170,14 +206,21 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
         floatx4 ks[2], vs[2];
         bool ok[2];
     };
-    auto fetch = [&](Chunk &x, int at) {
+    // Pages of the wave's next 32 chunks, two a chunk, one a lane: a chunk's
+    // loads wait for no load of its page.
+    const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
+    int ahead = 0;
+    auto look = [&](int at) {
+        const int t = at + lane / 2 * (kWaves * kChunk) + lane % 2 * 16;
+        ahead = -1;
+        if (t < high) ahead = table[(static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift];
+    };
+    auto fetch = [&](Chunk &x, int at, int n) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int t = at + 16 * h;
             const int page_at = static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift);
-            int page = -1;
-            if (t < high) page = a.table[static_cast<int64_t>(b) * a.table_width + page_at];
-            page = __builtin_amdgcn_readfirstlane(page);
+            const int page = __builtin_amdgcn_readlane(ahead, 2 * (n & 31) + h);
             x.ok[h] = page >= 0 && page < a.c.pages;
             x.ks[h] = x.vs[h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -289,15 +332,12 @@ __global__ void __launch_bounds__(256) attend_rows(AttnArgs a) {
     };
 
     const int first = low / kChunk * kChunk;
-    Chunk now, next;
-    int at = first + wave * kChunk;
-    if (at < high) fetch(now, at);
-    while (at < high) {
-        const int then = at + kWaves * kChunk;
-        if (then < high) fetch(next, then);
+    Chunk now;
+    int n = 0;
+    for (int at = first + wave * kChunk; at < high; at += kWaves * kChunk, n++) {
+        if ((n & 31) == 0) look(at);
+        fetch(now, at, n);
         use(now, at);
-        now = next;
-        at = then;
     }
 
     // the waves' sums, joined in wave order
@@ -391,14 +431,8 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    // The heaviest rows of a causal mask first; a sequence's and head's blocks
-    // on one XCD where the pairs are a multiple of eight, in an order that turns,
-    // since an XCD's workgroups go to its four engines in turn too: without the
-    // turn two sequences of 4001 and 6007 tokens keep an engine each.
-    const unsigned pairs = a.sequences * a.c.kv_heads, rest = blockIdx.x / pairs;
-    const int pair = (blockIdx.x + rest / 2 % pairs * 8) % pairs;
-    const int b = pair / a.c.kv_heads, head = pair - b * a.c.kv_heads;
-    const int split = rest % a.splits, block = a.row_blocks - 1 - rest / a.splits;
+    const Place at_block = place(a);
+    const int b = at_block.b, head = at_block.head, split = at_block.split, block = at_block.block;
     const int dim = a.c.head_dim;
     const Sequence s = sequence(a, b);
     const int rows = s.count * a.group, r0 = block * 128;
@@ -408,6 +442,11 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     if (a.causal) {
         high = min(high, s.position + last_q + 1);
         if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+    }
+
+    if (a.splits > 1 && low >= high) {
+        nothing(a, s, head, split, r0, min(rows, r0 + 128));
+        return;
     }
 
     // this wave's rows
@@ -730,7 +769,9 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     }
 }
 
-// A wave a row of q and head: its splits' sums, joined in their order.
+// A wave a row of q and head: its splits' sums, joined in their order.  A lane
+// takes one split's maximum and total, so that these come by one load, and four
+// splits' sums at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
     const int head = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -739,23 +780,46 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
     const Sequence s = sequence(a, b);
     if (i >= s.count) return;
     const int64_t at = ((s.row0 + i) * a.heads + head) * a.splits;
+    const int dim = a.c.head_dim;
     float most = -__builtin_inff();
-    for (int p = 0; p < a.splits; p++) most = fmaxf(most, a.stats[2 * (at + p)]);
+    for (int p = lane; p < a.splits; p += 64) most = fmaxf(most, a.stats[2 * (at + p)]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     const bool none = !(most > -__builtin_inff());
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
-    for (int p = 0; p < a.splits; p++) {
-        const float sum = a.stats[2 * (at + p) + 1];
-        if (sum == 0.0f) continue;  // no token of this split is the row's
-        const float r = none ? 1.0f : __builtin_amdgcn_exp2f(a.stats[2 * (at + p)] - most);
-        total += r * sum;
+    for (int p0 = 0; p0 < a.splits; p0 += 64) {
+        float share = 0.0f, sum = 0.0f;
+        if (p0 + lane < a.splits) {
+            sum = a.stats[2 * (at + p0 + lane) + 1];
+            share = none ? 1.0f : __builtin_amdgcn_exp2f(a.stats[2 * (at + p0 + lane)] - most);
+        }
+        const int end = min(64, a.splits - p0);
+        for (int p = 0; p < end; p += 4) {
+            float part[4][4], r[4], c[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (lane + 64 * e < a.c.head_dim) o[e] += r * a.part[(at + p) * a.c.head_dim + lane + 64 * e];
+            for (int u = 0; u < 4; u++) {
+                r[u] = __shfl(share, p + u);
+                c[u] = __shfl(sum, p + u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int d = lane + 64 * e;
+                    // no sums where a split holds no token of the row's
+                    part[u][e] = p + u < end && c[u] != 0.0f && d < dim ? a.part[(at + p0 + p + u) * dim + d] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (c[u] == 0.0f) continue;
+                total += r[u] * c[u];
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] += r[u] * part[u][e];
+            }
+        }
     }
-    T *y = static_cast<T *>(a.out) + (s.row0 + i) * a.out_stride + static_cast<int64_t>(head) * a.c.head_dim;
+    T *y = static_cast<T *>(a.out) + (s.row0 + i) * a.out_stride + static_cast<int64_t>(head) * dim;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < a.c.head_dim) y[lane + 64 * e] = static_cast<T>(total == 0.0f ? 0.0f : o[e] / total);
+        if (lane + 64 * e < dim) y[lane + 64 * e] = static_cast<T>(total == 0.0f ? 0.0f : o[e] / total);
 }
 
 struct Plan {
@@ -770,10 +834,12 @@ Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
     const int64_t rows = std::min(g.max_queries, g.queries) * (g.heads / c.kv_heads);
     p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
     p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
-    // enough workgroups for four on each CU, and no split shorter than a chunk for each wave
-    const int64_t base = static_cast<int64_t>(g.sequences) * c.kv_heads * p.row_blocks;
-    const int64_t step = kWaves * kChunk;
-    int64_t splits = std::min<int64_t>(p.tiles == 8 ? std::max<int64_t>(512 / base, 1) : (2048 + base - 1) / base, (g.max_length + step - 1) / step);
+    // Enough workgroups for eight on each CU (two where they take 128 rows), and
+    // no split shorter than four chunks for each wave (two tiles): a second
+    // kernel costs more than a few steps do.
+    const int64_t base = g.sequences * c.kv_heads * p.row_blocks;
+    const int64_t step = kWaves * kChunk, least = p.tiles == 8 ? 128 : 512;
+    int64_t splits = std::min<int64_t>(p.tiles == 8 ? 512 / base : (2048 + base - 1) / base, (g.max_length + least - 1) / least);
     splits = std::max<int64_t>(splits, 1);
     int64_t tokens = (g.max_length + splits - 1) / splits;
     tokens = std::max<int64_t>((tokens + step - 1) / step * step, step);
@@ -844,7 +910,7 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
             using T = decltype(t);
             const char *what = "attention_i8";
             auto go = [&](auto one, auto two) {
-                return launch(what, p.tiles == 1 ? one : two, dim3(blocks, c->kv_heads), dim3(256), stream, a);
+                return launch(what, p.tiles == 1 ? one : two, dim3(blocks * c->kv_heads), dim3(256), stream, a);
             };
             auto many = [&](auto kernel) { return launch(what, kernel, dim3(blocks * c->kv_heads), dim3(256), stream, a); };
             const int dim = c->head_dim;
