@@ -26,7 +26,6 @@ struct AttnArgs {
     int page_shift;
 };
 
-constexpr int kWaves = 4;    // of a workgroup: they deal a split's chunks out among them
 constexpr int kChunk = 32;   // tokens a wave takes at a time, as two tiles of 16
 // The running maximum of a row follows its scores only when one passes it by
 // more than 2^kSlack; weights are held as 2^kLift p in fp16, below 2^15.
@@ -53,6 +52,15 @@ __device__ __forceinline__ half8_t codes8(unsigned a, unsigned b) {
 // into the conversion to its high part, but not into the low part's, would give
 // parts of two values, a step of fp16 apart where one lies next to a tie.
 __device__ __forceinline__ void once(float &v) { asm("" : "+v"(v)); }
+
+// eight elements at p, of any alignment
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
+    Vec<T, 8> v;
+    __builtin_memcpy(v.v, p, sizeof(v.v));
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = static_cast<float>(v.v[e]);
+}
 
 __device__ __forceinline__ float over_groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -87,7 +95,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
 
 // A split in which rows r0 .. r1 read no token: no sums, and a total of 0.
 __device__ __forceinline__ void nothing(const AttnArgs &a, const Sequence &s, int head, int split, int r0, int r1) {
-    for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += 256) {
+    for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += blockDim.x) {
         const int i = r / a.group;
         const int64_t at = ((s.row0 + i) * a.heads + head * a.group + (r - i * a.group)) * a.splits + split;
         a.stats[2 * at] = -__builtin_inff();
@@ -130,15 +138,15 @@ __device__ __forceinline__ Place place(const AttnArgs &a) {
 //   scores, weights: tokens 4 g .. + 4 of each tile
 //   V: those tokens' codes VPL (l % 16) .. + VPL (VPL = DP / 16); product j
 //      takes d = VPL r + j as its row r
-template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) attend_rows(AttnArgs a) {
+template <typename T, int DP, int RT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / WAVES : 1) attend_rows(AttnArgs a) {
     constexpr bool kWide = sizeof(T) == 4;  // rows of 22 bits: two fp16 parts
     constexpr int kParts = kWide ? 2 : 1;
     constexpr int kPieces = DP / 64;  // 16-byte pieces of K a lane
     constexpr int kVpl = DP / 16;     // V codes a lane
     constexpr int kVw = kVpl / 4;
-    __shared__ __align__(16) float joined[kWaves * 64 * 4 * kVpl];
-    __shared__ float wave_max[kWaves][RT * 16], wave_sum[kWaves][RT * 16];
+    __shared__ __align__(16) float joined[WAVES * 64 * 4 * kVpl];
+    __shared__ float wave_max[WAVES][RT * 16], wave_sum[WAVES][RT * 16];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
@@ -160,46 +168,6 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
         return;
     }
 
-    // the rows' masks and queries, scaled by a power of two to 2^14 .. 2^15
-    half8_t qf[RT][DP / 32][kParts];
-    float factor[RT], m[RT], l[RT];
-    int last[RT], start[RT];
-    floatx4 acc[RT][kVpl];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int r = r0 + t * 16 + col, i = r / a.group;
-        const bool in = r < rows;
-        last[t] = a.causal ? s.position + i : s.length - 1;
-        start[t] = a.causal && a.window ? last[t] + 1 - a.window : 0;
-        const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_stride +
-                     static_cast<int64_t>(head * a.group + (r - i * a.group)) * dim;
-        float f[DP / 4];
-        float top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < DP / 4; e++) {
-            const int d = g * (DP / 4) + e;
-            f[e] = in && d < dim ? static_cast<float>(q[d]) : 0.0f;
-            top = fmaxf(top, fabsf(f[e]));
-        }
-        top = over_groups_max(top);
-        const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
-        factor[t] = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
-#pragma unroll
-        for (int x = 0; x < DP / 32; x++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = ldexpf(f[x * 8 + e], 14 - ex);
-                const _Float16 hi = static_cast<_Float16>(v);
-                qf[t][x][0][e] = hi;
-                if constexpr (kWide) qf[t][x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
-            }
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kVpl; j++) acc[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    float unit = 0.0f, per_unit = 0.0f;  // a power of two no value scale is above, and kLift / unit
-
     struct Chunk {
         uintx4 k[2][kPieces];
         unsigned v[8][kVw];
@@ -211,7 +179,7 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
     const int32_t *table = a.table + static_cast<int64_t>(b) * a.table_width;
     int ahead = 0;
     auto look = [&](int at) {
-        const int t = at + lane / 2 * (kWaves * kChunk) + lane % 2 * 16;
+        const int t = at + lane / 2 * (WAVES * kChunk) + lane % 2 * 16;
         ahead = -1;
         if (t < high) ahead = table[(static_cast<uint64_t>(static_cast<unsigned>(t)) * a.page_mul) >> a.page_shift];
     };
@@ -248,6 +216,60 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
             }
         }
     };
+    // the first chunk is on its way while the queries are split
+    Chunk now;
+    int at = low / kChunk * kChunk + wave * kChunk, n = 0;
+    if (at < high) {
+        look(at);
+        fetch(now, at, 0);
+    }
+
+    // the rows' masks and queries, scaled by a power of two to 2^14 .. 2^15
+    half8_t qf[RT][DP / 32][kParts];
+    float factor[RT], m[RT], l[RT];
+    int last[RT], start[RT];
+    floatx4 acc[RT][kVpl];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = r0 + t * 16 + col, i = r / a.group;
+        const bool in = r < rows;
+        last[t] = a.causal ? s.position + i : s.length - 1;
+        start[t] = a.causal && a.window ? last[t] + 1 - a.window : 0;
+        // without a branch, so that all loads are on their way at once: rows past the last are the last
+        const int rq = min(r, rows - 1), iq = rq / a.group;
+        const T *q = static_cast<const T *>(a.q) + (s.row0 + iq) * a.q_stride +
+                     static_cast<int64_t>(head * a.group + (rq - iq * a.group)) * dim;
+        float f[DP / 32][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int x = 0; x < DP / 32; x++) {
+            const int d = g * (DP / 4) + 8 * x;
+            load8(q + min(d, dim - 8), f[x]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f[x][e] = in && d < dim ? f[x][e] : 0.0f;
+                top = fmaxf(top, fabsf(f[x][e]));
+            }
+        }
+        top = over_groups_max(top);
+        const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
+        factor[t] = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
+#pragma unroll
+        for (int x = 0; x < DP / 32; x++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = ldexpf(f[x][e], 14 - ex);
+                const _Float16 hi = static_cast<_Float16>(v);
+                qf[t][x][0][e] = hi;
+                if constexpr (kWide) qf[t][x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+            }
+        m[t] = -__builtin_inff();
+        l[t] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kVpl; j++) acc[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float unit = 0.0f, per_unit = 0.0f;  // a power of two no value scale is above, and kLift / unit
+
     auto use = [&](const Chunk &x, int at) {
         floatx4 sc[RT][2];
 #pragma unroll
@@ -331,13 +353,13 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
         }
     };
 
-    const int first = low / kChunk * kChunk;
-    Chunk now;
-    int n = 0;
-    for (int at = first + wave * kChunk; at < high; at += kWaves * kChunk, n++) {
+    while (at < high) {
+        use(now, at);
+        at += WAVES * kChunk;
+        n++;
+        if (at >= high) break;
         if ((n & 31) == 0) look(at);
         fetch(now, at, n);
-        use(now, at);
     }
 
     // the waves' sums, joined in wave order
@@ -355,11 +377,11 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
     for (int t = 0; t < RT; t++) {
         float most = wave_max[0][t * 16 + col];
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) most = fmaxf(most, wave_max[w][t * 16 + col]);
+        for (int w = 1; w < WAVES; w++) most = fmaxf(most, wave_max[w][t * 16 + col]);
         const bool none = !(most > -__builtin_inff());
         float total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             const float r = none ? 1.0f : __builtin_amdgcn_exp2f(wave_max[w][t * 16 + col] - most);
             total += r * wave_sum[w][t * 16 + col];
         }
@@ -372,12 +394,13 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
                 *reinterpret_cast<floatx4 *>(joined + (((wave * 4 + i) * kVw + j / 4) * 64 + lane) * 4) =
                     floatx4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]} * mine;
         __syncthreads();
+        if (wave >= 4) continue;  // the columns are four waves' quarters
         float o[kVpl];
 #pragma unroll
         for (int j = 0; j < kVpl; j += 4) {
             floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < kWaves; w++)
+            for (int w = 0; w < WAVES; w++)
                 sum += *reinterpret_cast<const floatx4 *>(joined + (((w * 4 + wave) * kVw + j / 4) * 64 + lane) * 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) o[j + e] = sum[e];
@@ -397,9 +420,11 @@ __global__ void __launch_bounds__(256, DP * RT * sizeof(T) <= 256 ? 3 : 1) atten
             }
         } else {
             T *y = static_cast<T *>(a.out) + (s.row0 + i) * a.out_stride + static_cast<int64_t>(h) * dim + d;
-            const float r_total = 1.0f / total;
+            const float r_total = total == 0.0f ? 0.0f : 1.0f / total;
+            Vec<T, kVpl> v;
 #pragma unroll
-            for (int j = 0; j < kVpl; j++) y[j] = static_cast<T>(total == 0.0f ? 0.0f : o[j] * r_total);
+            for (int j = 0; j < kVpl; j++) v.v[j] = static_cast<T>(o[j] * r_total);
+            __builtin_memcpy(y, v.v, sizeof(v.v));
         }
     }
 }
@@ -462,18 +487,18 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     half8_t qf[DP / 16][kParts];
     float factor;
     {
-        const T *q = static_cast<const T *>(a.q) + (s.row0 + i) * a.q_stride + static_cast<int64_t>(q_head) * dim;
+        // without a branch, so that all loads are on their way at once: rows past the last are the last
+        const int rq = min(r, rows - 1), iq = rq / a.group;
+        const T *q = static_cast<const T *>(a.q) + (s.row0 + iq) * a.q_stride + static_cast<int64_t>(head * a.group + (rq - iq * a.group)) * dim;
         float f[DP / 16][8];
         float top = 0.0f;
 #pragma unroll
         for (int x = 0; x < DP / 16; x++) {
             const int d = 16 * x + 8 * h;
-            Vec<T, 8> v;
-            const bool there = in && d < dim;
-            if (there) __builtin_memcpy(v.v, q + d, sizeof(v.v));
+            load8(q + min(d, dim - 8), f[x]);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                f[x][e] = there ? static_cast<float>(v.v[e]) : 0.0f;
+                f[x][e] = in && d < dim ? f[x][e] : 0.0f;
                 top = fmaxf(top, fabsf(f[x][e]));
             }
         }
@@ -824,6 +849,7 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
 
 struct Plan {
     int tiles;  // of 16 rows a workgroup
+    int waves;  // that deal tokens out among them (few rows)
     int64_t row_blocks;  // up to 2^36: queries and heads are bounded
     int split_tokens, splits;
     size_t part, stats;  // bytes
@@ -835,16 +861,18 @@ Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
     p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
     p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
     // Enough workgroups for eight on each CU (two where they take 128 rows), and
-    // no split shorter than four chunks for each wave (two tiles): a second
-    // kernel costs more than a few steps do.
+    // no split shorter than four chunks for each of four waves (two tiles): a
+    // second kernel costs more than a few steps do.  Fewer workgroups than CUs
+    // are of eight waves: one sequence of 333 tokens ENC.
     const int64_t base = g.sequences * c.kv_heads * p.row_blocks;
-    const int64_t step = kWaves * kChunk, least = p.tiles == 8 ? 128 : 512;
+    const int64_t step = 128, least = p.tiles == 8 ? 128 : 512;
     int64_t splits = std::min<int64_t>(p.tiles == 8 ? 512 / base : (2048 + base - 1) / base, (g.max_length + least - 1) / least);
     splits = std::max<int64_t>(splits, 1);
     int64_t tokens = (g.max_length + splits - 1) / splits;
     tokens = std::max<int64_t>((tokens + step - 1) / step * step, step);
     p.split_tokens = static_cast<int>(tokens);
     p.splits = static_cast<int>(std::max<int64_t>((g.max_length + tokens - 1) / tokens, 1));
+    p.waves = p.tiles == 1 && base * p.splits <= 256 ? 8 : 4;
     const size_t parts = p.splits > 1 ? static_cast<size_t>(g.queries) * g.heads * p.splits : 0;
     p.part = parts * c.head_dim * sizeof(float);
     p.stats = parts * 2 * sizeof(float);
@@ -909,8 +937,8 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             const char *what = "attention_i8";
-            auto go = [&](auto one, auto two) {
-                return launch(what, p.tiles == 1 ? one : two, dim3(blocks * c->kv_heads), dim3(256), stream, a);
+            auto go = [&](auto one, auto eight, auto two) {
+                return launch(what, p.waves == 8 ? eight : p.tiles == 1 ? one : two, dim3(blocks * c->kv_heads), dim3(64 * p.waves), stream, a);
             };
             auto many = [&](auto kernel) { return launch(what, kernel, dim3(blocks * c->kv_heads), dim3(256), stream, a); };
             const int dim = c->head_dim;
@@ -918,9 +946,9 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
             if (p.tiles == 8) {
                 rc = dim <= 64 ? many(attend_tiles<T, 64>) : dim <= 96 ? many(attend_tiles<T, 96>) : dim <= 128 ? many(attend_tiles<T, 128>) : many(attend_tiles<T, 256>);
             } else {
-                rc = dim <= 64    ? go(attend_rows<T, 64, 1>, attend_rows<T, 64, 2>)
-                     : dim <= 128 ? go(attend_rows<T, 128, 1>, attend_rows<T, 128, 2>)
-                                  : go(attend_rows<T, 256, 1>, attend_rows<T, 256, 2>);
+                rc = dim <= 64 ? go(attend_rows<T, 64, 1, 4>, attend_rows<T, 64, 1, 8>, attend_rows<T, 64, 2, 4>)
+                     : dim <= 128 ? go(attend_rows<T, 128, 1, 4>, attend_rows<T, 128, 1, 8>, attend_rows<T, 128, 2, 4>)
+                                  : go(attend_rows<T, 256, 1, 4>, attend_rows<T, 256, 1, 8>, attend_rows<T, 256, 2, 4>);
             }
             if (rc || p.splits == 1) return rc;
             const dim3 rows(static_cast<unsigned>(g->sequences * a.max_queries), (g->heads + 3) / 4);
