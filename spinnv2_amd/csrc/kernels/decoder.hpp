@@ -71,20 +71,34 @@ template <int N, typename P>
 __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N]) {
     const float inv = 127.0f / static_cast<float>(top);
     float r[N];
-    bool near = false;
+    bool far[N], all = true;
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const float t = static_cast<float>(x[i]) * inv;
         r[i] = rintf(t);
-        near |= !(fabsf(t - r[i]) < 0.5f - 0x1p-14f);
+        far[i] = fabsf(t - r[i]) < 0.5f - 0x1p-14f;
+        all &= far[i];
     }
-    if (near) {
+    if (!all) {
 #pragma unroll
         for (int i = 0; i < N; i++)
-            r[i] = static_cast<float>(rint(static_cast<double>(x[i]) * 127.0 / static_cast<double>(top)));
+            if (!far[i]) r[i] = static_cast<float>(rint(static_cast<double>(x[i]) * 127.0 / static_cast<double>(top)));
     }
 #pragma unroll
     for (int i = 0; i < N; i++) q[i] = static_cast<int8_t>(static_cast<int>(r[i]));
+}
+
+// The largest of v over groups of LANES neighbouring lanes (8, 16 or 32), in
+// each of them: within 16 by lane moves of the adder's own, past that by LDS's
+// crossbar.
+template <int LANES>
+__device__ __forceinline__ unsigned max_over(unsigned v) {
+    v = max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));   // lanes 1 0 3 2
+    v = max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));   // lanes 2 3 0 1
+    v = max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 0xF, 0xF, true)));  // eight lanes mirrored
+    if constexpr (LANES >= 16) v = max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 0xF, 0xF, true)));  // 16 mirrored
+    if constexpr (LANES >= 32) v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 16)));
+    return v;
 }
 
 // ---- host ------------------------------------------------------------------

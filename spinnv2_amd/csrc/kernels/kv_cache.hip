@@ -1,10 +1,13 @@
 // A paged key/value cache in int8: tokens quantised as they are written, and
-// read back.
+// read back.  Both are bound by HBM, a call of a few tokens by its launch.
 //
 // Write: each head's vector of a token is quantised by its own largest
 // absolute value.  One pass, a group of lanes a vector, 8 elements a lane, the
-// maximum joined over the group's lanes.  Read: 16 codes a lane, scaled.  Both
-// bound by HBM; a call of a few tokens by its launch.
+// maximum joined over the group's lanes.  A workgroup takes one head of
+// neighbouring tokens, whose rows and scales lie next to each other in a page:
+// with the heads side by side instead, a page's line of scales was written a
+// few bytes at a time from several XCDs (3 x 8191 tokens of 8 heads of 128,
+// 152 MB: 45 us, WWW so).  Read: 16 codes a lane, scaled (30 us).
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -16,45 +19,50 @@ struct WriteArgs {
     const void *k, *v;
     const int64_t *slots;
     int64_t tokens, k_stride, v_stride;
+    unsigned page_mul;  // slot / page_size, by multiplication; 0: slots pass 2^31
+    int page_shift;
 };
 
-// LANES lanes (of which head_dim / 8 have elements) a vector; blockIdx.y: k, v
+// LANES lanes (of which head_dim / 8 have elements) a vector
 template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) kv_write(WriteArgs a) {
-    const int64_t vec = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int64_t token = vec / a.c.kv_heads;
-    const int head = static_cast<int>(vec - token * a.c.kv_heads);
+    const int head = blockIdx.x % a.c.kv_heads, lane = threadIdx.x % LANES;
+    const int64_t token = static_cast<int64_t>(blockIdx.x / a.c.kv_heads) * (256 / LANES) + threadIdx.x / LANES;
     if (token >= a.tokens) return;  // whole groups of lanes
-    const int64_t slot = a.slots[token];
-    const int64_t page = slot / a.c.page_size;
-    if (slot < 0 || page >= a.c.pages) return;
-    const int at = static_cast<int>(slot - page * a.c.page_size);
-    const bool is_v = blockIdx.y != 0;
-    const T *x = static_cast<const T *>(is_v ? a.v : a.k) + token * (is_v ? a.v_stride : a.k_stride) +
-                 static_cast<int64_t>(head) * a.c.head_dim + lane * 8;
-    const int64_t row = (page * a.c.kv_heads + head) * a.c.page_size + at;
     const bool in = lane * 8 < a.c.head_dim;
-    float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (in) {
-        if constexpr (VEC) load_floats<8>(x, f);
-        else {
+    const int64_t at_head = static_cast<int64_t>(head) * a.c.head_dim + lane * 8;
+    float f[2][8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = static_cast<float>(x[j]);
+    for (int n = 0; n < 2; n++) {
+        const T *x = static_cast<const T *>(n ? a.v : a.k) + token * (n ? a.v_stride : a.k_stride) + at_head;
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[n][j] = 0.0f;
+        if (in) {
+            if constexpr (VEC) load_floats<8>(x, f[n]);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[n][j] = static_cast<float>(x[j]);
+            }
         }
     }
-    unsigned top = 0;
+    const int64_t slot = a.slots[token];
+    if (slot < 0 || slot >= a.c.pages * a.c.page_size) return;  // below 2^51
+    const int64_t page = a.page_mul ? static_cast<int64_t>((static_cast<uint64_t>(slot) * a.page_mul) >> a.page_shift) : slot / a.c.page_size;
+    const int64_t row = (page * a.c.kv_heads + head) * a.c.page_size + (slot - page * a.c.page_size);
 #pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, abs_bits(f[j]));
+    for (int n = 0; n < 2; n++) {
+        unsigned top = 0;
 #pragma unroll
-    for (int d = LANES / 2; d; d >>= 1) top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), d, LANES)));
-    const bool finite = top < kInfBits;
-    Vec<int8_t, 8> q;
+        for (int j = 0; j < 8; j++) top = max(top, abs_bits(f[n][j]));
+        top = max_over<LANES>(top);
+        const bool finite = top < kInfBits;
+        Vec<int8_t, 8> q;
 #pragma unroll
-    for (int j = 0; j < 8; j++) q.v[j] = 0;
-    if (finite && top) quantise<8>(f, __uint_as_float(top), q.v);
-    if (in) *reinterpret_cast<Vec<int8_t, 8> *>((is_v ? a.c.v : a.c.k) + row * a.c.head_dim + lane * 8) = q;
-    if (lane == 0) (is_v ? a.c.v_scale : a.c.k_scale)[row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
+        for (int j = 0; j < 8; j++) q.v[j] = 0;
+        if (finite && top) quantise<8>(f[n], __uint_as_float(top), q.v);
+        if (in) *reinterpret_cast<Vec<int8_t, 8> *>((n ? a.c.v : a.c.k) + row * a.c.head_dim + lane * 8) = q;
+        if (lane == 0) (n ? a.c.v_scale : a.c.k_scale)[row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
+    }
 }
 
 struct ReadArgs {
@@ -141,13 +149,14 @@ extern "C" int spkv2_mi355x_kv_write_i8(const Spkv2KvCacheI8 *c, const Spkv2KvWr
         if (g->tokens > INT32_MAX) return unsupported("kv_write_i8: more than 2^31 tokens");
         const size_t size = dtype_size(g->dtype);
         const bool vec = aligned(g->k, 16) && aligned(g->v, 16) && (g->k_stride * size) % 16 == 0 && (g->v_stride * size) % 16 == 0;
-        const WriteArgs a{*c, g->k, g->v, g->slots, g->tokens, g->k_stride, g->v_stride};
+        WriteArgs a{*c, g->k, g->v, g->slots, g->tokens, g->k_stride, g->v_stride, 0, 0};
+        if (c->pages * c->page_size <= INT32_MAX) div_magic(static_cast<unsigned>(c->page_size), &a.page_mul, &a.page_shift);
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             auto go = [&](auto kernel, int lanes) {
-                const int64_t vecs = g->tokens * c->kv_heads, blocks = (vecs + 256 / lanes - 1) / (256 / lanes);
-                if (blocks > INT32_MAX) return unsupported("kv_write_i8: too many tokens for one launch");
-                return launch("kv_write_i8", kernel, dim3(static_cast<unsigned>(blocks), 2), dim3(256), stream, a);
+                const int64_t blocks = (g->tokens + 256 / lanes - 1) / (256 / lanes) * c->kv_heads;
+                if (blocks >= 1 << 24) return unsupported("kv_write_i8: too many tokens for one launch");
+                return launch("kv_write_i8", kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), stream, a);
             };
             if (c->head_dim <= 64) return vec ? go(kv_write<T, 8, true>, 8) : go(kv_write<T, 8, false>, 8);
             if (c->head_dim <= 128) return vec ? go(kv_write<T, 16, true>, 16) : go(kv_write<T, 16, false>, 16);
