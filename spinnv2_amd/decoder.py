@@ -31,6 +31,7 @@ _FP32, _INT8, _FP16, _BF16, _INT32, _INT64 = 1, 2, 3, 4, 101, 102
 #: dtype -> the library's code; torch's own dtype objects join at first sight
 _CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64}
 _FLOATS = (_FP32, _FP16, _BF16)
+_FP32S, _INT8S, _INT32S, _INT64S = (_FP32,), (_INT8,), (_INT32,), (_INT64,)
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -160,6 +161,7 @@ def to_bfloat16(values) -> np.ndarray:
 
 
 def _code(t) -> int:
+    """The library's code of a tensor's dtype; torch's dtype objects join _CODES here."""
     code = _CODES.get(t.dtype)
     if code is None:
         code = _CODES.get(str(t.dtype).replace("torch.", ""))
@@ -173,18 +175,20 @@ def _fail(name: str, why: str):
     raise ValueError(f"{name}: {why}")
 
 
-def _refuse(name: str, t, codes, shape):
-    """Says which of a tensor's type, shape and place does not fit."""
+def _refuse(name: str, t, codes, shape) -> None:
+    """Says which of a tensor's type, shape and place does not fit; nothing
+    where its dtype object was only met for the first time."""
     if _code(t) not in codes:
         _fail(name, f"unexpected dtype {t.dtype}")
-    if tuple(t.shape) != shape:
-        _fail(name, f"shape {tuple(t.shape)}, expected {shape}")
-    _fail(name, "not on the GPU")
+    if t.shape != shape:
+        _fail(name, f"shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_cuda:
+        _fail(name, "not on the GPU")
 
 
 def _rows(name: str, t, codes, shape) -> int:
     """A 2-d tensor's row stride, its type and shape checked."""
-    if _code(t) not in codes or t.shape != shape or not t.is_cuda:
+    if t.shape != shape or _CODES.get(t.dtype) not in codes or not t.is_cuda:
         _refuse(name, t, codes, shape)
     row, step = t.stride()
     if step != 1 and shape[1] > 1:
@@ -194,16 +198,16 @@ def _rows(name: str, t, codes, shape) -> int:
 
 def _vector(name: str, t, codes, n: int) -> int:
     """A contiguous vector's address, its type and length checked."""
-    if _code(t) not in codes or t.shape != (n,) or not t.is_cuda:
+    if t.shape != (n,) or _CODES.get(t.dtype) not in codes or not t.is_cuda:
         _refuse(name, t, codes, (n,))
-    if n > 1 and t.stride()[0] != 1:
+    if t.stride() != (1,) and n > 1:
         _fail(name, "not contiguous")
     return t.data_ptr()
 
 
 def _heads(name: str, t, codes, shape) -> int:
     """A [tokens, heads, dim] tensor's token stride: the heads have to lie one after the other."""
-    if _code(t) not in codes or t.shape != shape or not t.is_cuda:
+    if t.shape != shape or _CODES.get(t.dtype) not in codes or not t.is_cuda:
         _refuse(name, t, codes, shape)
     row, head, step = t.stride()
     if step != 1 or (head != shape[2] and shape[1] > 1):
@@ -213,10 +217,10 @@ def _heads(name: str, t, codes, shape) -> int:
 
 def _table(t) -> tuple:
     """(sequences, width) of a page table."""
-    if len(t.shape) != 2:
+    shape = t.shape
+    if len(shape) != 2:
         _fail("table", "not two-dimensional")
-    shape = tuple(t.shape)
-    if _rows("table", t, (_INT32,), shape) != shape[1] and shape[0] > 1:
+    if _rows("table", t, _INT32S, shape) != shape[1] and shape[0] > 1:
         _fail("table", "not contiguous")
     return shape
 
@@ -237,19 +241,19 @@ def quantize_i8(x, q, scale, *, stream: int = 0) -> None:
 
 
 def _norm_rows(x, weight, q, scale, residual, residual_out, norm, eps, stream) -> None:
-    shape, code = tuple(x.shape), _code(x)
+    shape, code = x.shape, _code(x)
     if len(shape) != 2:
         _fail("x", "not two-dimensional")
     rows, cols = shape
     w = w_code = r = r_stride = h = h_stride = 0
     if weight is not None:
-        w, w_code = _vector("weight", weight, (code, _FP32), cols), _code(weight)
+        w, w_code = _vector("weight", weight, (code, _FP32), cols), _CODES[weight.dtype]
     if residual is not None:
         r_stride, r = _rows("residual", residual, (code,), shape), residual.data_ptr()
     if residual_out is not None:
         h_stride, h = _rows("residual_out", residual_out, (code,), shape), residual_out.data_ptr()
-    a = _pack_norm(x.data_ptr(), r, w, h, q.data_ptr(), _vector("scale", scale, (_FP32,), rows), rows, cols,
-                   _rows("x", x, _FLOATS, shape), r_stride, h_stride, _rows("q", q, (_INT8,), shape), code, w_code, norm, eps)
+    a = _pack_norm(x.data_ptr(), r, w, h, q.data_ptr(), _vector("scale", scale, _FP32S, rows), rows, cols,
+                   _rows("x", x, _FLOATS, shape), r_stride, h_stride, _rows("q", q, _INT8S, shape), code, w_code, norm, eps)
     lib = load_library()
     if code := lib.spkv2_mi355x_rmsnorm_i8(a, stream):
         _check(lib, code, "rmsnorm_i8")
@@ -257,12 +261,12 @@ def _norm_rows(x, weight, q, scale, residual, residual_out, norm, eps, stream) -
 
 def dequantize_i8(q, scale, out, *, stream: int = 0) -> None:
     """out = q * scale, row by row; out float32, float16 or bfloat16."""
-    shape = tuple(q.shape)
+    shape = q.shape
     if len(shape) != 2:
         _fail("q", "not two-dimensional")
     rows, cols = shape
-    a = _pack_dequantize(q.data_ptr(), _vector("scale", scale, (_FP32,), rows), out.data_ptr(), rows, cols,
-                         _rows("q", q, (_INT8,), shape), _rows("out", out, _FLOATS, shape), _code(out), 0)
+    a = _pack_dequantize(q.data_ptr(), _vector("scale", scale, _FP32S, rows), out.data_ptr(), rows, cols,
+                         _rows("q", q, _INT8S, shape), _rows("out", out, _FLOATS, shape), _code(out), 0)
     lib = load_library()
     if code := lib.spkv2_mi355x_dequantize_i8(a, stream):
         _check(lib, code, "dequantize_i8")
@@ -277,9 +281,9 @@ def matmul_i8(a, a_scale, b, b_scale, out, *, bias=None, stream: int = 0) -> Non
     if len(a.shape) != 2 or len(b.shape) != 2:
         _fail("a, b", "not two-dimensional")
     (m, k), n = a.shape, b.shape[0]
-    g = _pack_matmul(a.data_ptr(), b.data_ptr(), _vector("a_scale", a_scale, (_FP32,), m), _vector("b_scale", b_scale, (_FP32,), n),
-                     0 if bias is None else _vector("bias", bias, (_FP32,), n), out.data_ptr(), m, n, k,
-                     _rows("a", a, (_INT8,), (m, k)), _rows("b", b, (_INT8,), (n, k)), _rows("out", out, _FLOATS, (m, n)),
+    g = _pack_matmul(a.data_ptr(), b.data_ptr(), _vector("a_scale", a_scale, _FP32S, m), _vector("b_scale", b_scale, _FP32S, n),
+                     0 if bias is None else _vector("bias", bias, _FP32S, n), out.data_ptr(), m, n, k,
+                     _rows("a", a, _INT8S, (m, k)), _rows("b", b, _INT8S, (n, k)), _rows("out", out, _FLOATS, (m, n)),
                      _code(out), 0)
     lib = load_library()
     if code := lib.spkv2_mi355x_matmul_i8(g, stream):
@@ -322,7 +326,7 @@ class KvCache:
         [tokens]; negative ones, and those past the cache, are not written)."""
         shape = (k.shape[0], self.kv_heads, self.head_dim)
         code = _code(k)
-        a = _pack_write(k.data_ptr(), v.data_ptr(), _vector("slots", slots, (_INT64,), shape[0]), shape[0],
+        a = _pack_write(k.data_ptr(), v.data_ptr(), _vector("slots", slots, _INT64S, shape[0]), shape[0],
                         _heads("k", k, _FLOATS, shape), _heads("v", v, (code,), shape), code, 0)
         lib = load_library()
         if code := lib.spkv2_mi355x_kv_write_i8(self._ref, a, stream):
@@ -335,8 +339,8 @@ class KvCache:
         shape = (k.shape[0], self.kv_heads, self.head_dim)
         seqs, width = _table(table)
         code = _code(k)
-        a = _pack_read(table.data_ptr(), 0 if first is None else _vector("first", first, (_INT32,), seqs),
-                       _vector("offsets", offsets, (_INT32,), seqs + 1), k.data_ptr(), v.data_ptr(), shape[0],
+        a = _pack_read(table.data_ptr(), 0 if first is None else _vector("first", first, _INT32S, seqs),
+                       _vector("offsets", offsets, _INT32S, seqs + 1), k.data_ptr(), v.data_ptr(), shape[0],
                        _heads("k", k, _FLOATS, shape), _heads("v", v, (code,), shape), seqs, width, code, 0)
         lib = load_library()
         if code := lib.spkv2_mi355x_kv_read_i8(self._ref, a, stream):
@@ -366,9 +370,9 @@ def attention(q, cache: KvCache, table, lengths, offsets, out, *, max_queries: i
     lengths; workspace: a buffer of attention_workspace() bytes; scale: 1 /
     sqrt(head_dim) by default.
     """
-    shape = tuple(q.shape)
+    shape = q.shape
     if len(shape) != 3 or shape[2] != cache.head_dim:
-        _fail("q", f"shape {shape}, expected [queries, heads, {cache.head_dim}]")
+        _fail("q", f"shape {tuple(shape)}, expected [queries, heads, {cache.head_dim}]")
     seqs, width = _table(table)
     code = _code(q)
     size = at = 0
@@ -377,8 +381,8 @@ def attention(q, cache: KvCache, table, lengths, offsets, out, *, max_queries: i
         if _code_size(workspace) != 1 or not workspace.is_cuda:
             _fail("workspace", "not bytes on the GPU")
         at = workspace.data_ptr() if size else 0
-    a = _pack_attention(q.data_ptr(), out.data_ptr(), table.data_ptr(), _vector("lengths", lengths, (_INT32,), seqs),
-                        _vector("offsets", offsets, (_INT32,), seqs + 1), at, size, shape[0], _heads("q", q, _FLOATS, shape),
+    a = _pack_attention(q.data_ptr(), out.data_ptr(), table.data_ptr(), _vector("lengths", lengths, _INT32S, seqs),
+                        _vector("offsets", offsets, _INT32S, seqs + 1), at, size, shape[0], _heads("q", q, _FLOATS, shape),
                         _heads("out", out, (code,), shape), max_queries, max_length, seqs, width, shape[1], code, 1 if causal else 0,
                         window, cache.head_dim ** -0.5 if scale is None else scale, 0)
     lib = load_library()
