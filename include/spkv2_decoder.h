@@ -79,8 +79,9 @@ int spkv2_mi355x_dequantize_i8(const Spkv2DequantizeI8 *args, void *stream);
 /* ---- product ------------------------------------------------------------- */
 
 /* out[m, n] = a_scale[m] b_scale[n] sum_k a[m, k] b[n, k] + bias[n]: int32
- * sums, which are exact up to k = 2^17 (larger k is refused), scaled in fp32
- * and rounded once to out's type. */
+ * sums, which are exact up to k = 2^17 (larger k is refused, and m above 2^21
+ * or n above 2^26), scaled in fp32 and rounded once to out's type: the same
+ * bits whatever the strides and the sizes beside a row and a channel. */
 typedef struct {
     const int8_t *a;      /* [m, k]: one row for each token */
     const int8_t *b;      /* [n, k]: one row for each output channel */
@@ -150,9 +151,12 @@ int spkv2_mi355x_kv_read_i8(const Spkv2KvCacheI8 *cache, const Spkv2KvRead *args
  * whose mask leaves nothing (no tokens yet; a position before the first) gets
  * zeros.  Tokens past a table's end, or on a page that the cache does not
  * have, are as masked.
- * The cached codes are read as 16-bit floats, exactly; queries and softmax
- * weights are rounded to 11 bits (22 for fp32 rows) relative to their row's
- * largest, sums and softmax statistics are fp32.
+ * The cached codes are read as 16-bit floats, exactly; queries are held with
+ * 11 bits relative to themselves (22 for fp32 rows), softmax weights times
+ * their tokens' value scales too, sums and softmax statistics are fp32.  Value
+ * scales are meant to lie between 2^-96 and 2^96; smaller ones lose bits.  A
+ * token whose key or value scale is not finite makes the rows that read it
+ * NaN, and no other.
  *
  * max_queries and max_length bound the sequences' counts of queries and
  * lengths; what a sequence has beyond them is not computed (queries) or not

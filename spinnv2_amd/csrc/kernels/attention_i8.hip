@@ -71,6 +71,12 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// The exponent of a power of two above a value scale.  Scales below 2^-96 share
+// one, under which their weights lose low bits: 2^7 / unit has to stay a float.
+__device__ __forceinline__ int unit_exponent(float scale) {
+    return min(max(static_cast<int>(__float_as_uint(scale) >> 23) - 126, -96), 127);
+}
+
 struct Sequence {
     int64_t row0;   // its first row of q
     int count;      // queries computed
@@ -295,10 +301,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
         for (int e = 0; e < 8; e++) {
             const int token = at + 16 * (e / 4) + 4 * g + e % 4;
             vs[e] = whole || (token >= low && token < high && x.ok[e / 4]) ? x.vs[e / 4][e % 4] : 0.0f;
-            top = fmaxf(top, vs[e]);
+            if (vs[e] < __builtin_inff()) top = fmaxf(top, vs[e]);
         }
         if (__any(top > unit)) {
-            const float now = __uint_as_float((__float_as_uint(fmaxf(over_groups_max(top), unit)) & kInfBits) + 0x00800000u);
+            const float now = ldexpf(1.0f, unit_exponent(fmaxf(over_groups_max(top), unit)));
             const float ratio = unit / now;
             unit = now;
             per_unit = kLift / now;
@@ -693,8 +699,7 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
             float ratio = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - now) : 0.0f;
             m = now;
             if (up > unit) {
-                const unsigned bits = (__float_as_uint(up) & kInfBits) + 0x00800000u;
-                const int ex = min(max(static_cast<int>(bits >> 23) - 127, -96), 127);
+                const int ex = unit_exponent(up);
                 ratio *= __builtin_amdgcn_exp2f(7.0f - static_cast<float>(ex) - base);
                 unit = ldexpf(1.0f, ex);
                 base = 7.0f - static_cast<float>(ex);
@@ -887,6 +892,8 @@ int check(const Spkv2KvCacheI8 *c, const Spkv2AttentionI8 *g) {
         return bad("attention_i8: negative size");
     if (g->heads < 1 || g->heads % c->kv_heads) return bad("attention_i8: heads is not a multiple of kv_heads");
     if (g->window < 0 || (g->window && !g->causal)) return bad("attention_i8: window is negative, or not causal");
+    if (std::min(g->max_queries, g->queries) * (g->heads / c->kv_heads) > (1 << 30))
+        return unsupported("attention_i8: more than 2^30 rows of one sequence and kv head");
     if (g->queries > (1 << 24) || g->heads > 65535 || g->sequences > 65535 || g->max_length > (1 << 30))
         return unsupported("attention_i8: more than 2^24 queries, 65535 heads or sequences, or 2^30 tokens");
     return 0;
@@ -922,8 +929,9 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         const Plan p = plan(*c, *g);
         if (p.splits > 1 && (!g->workspace || g->workspace_size < p.part + p.stats || !aligned(g->workspace, 16)))
             return bad("attention_i8: the workspace is missing, too small or not 16-byte aligned");
-        if (g->sequences * p.row_blocks > INT32_MAX / p.splits / c->kv_heads ||
-            g->sequences * std::min(g->max_queries, g->queries) > INT32_MAX)
+        // a launch has fewer than 2^32 threads
+        if (g->sequences * p.row_blocks >= (1 << 23) / c->kv_heads / p.splits ||
+            (p.splits > 1 && g->sequences * std::min(g->max_queries, g->queries) >= (1 << 24)))
             return unsupported("attention_i8: too many queries and sequences for one launch");
         unsigned mul;
         int shift;

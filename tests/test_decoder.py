@@ -195,7 +195,8 @@ def test_cache_is_refused_by_every_entry(cache, code):
     (dict(max_length=4096, workspace=PTR, workspace_size=64), -1), (dict(max_length=4096, workspace=PTR + 8, workspace_size=1 << 30), -1),
     (dict(heads=65538), UNSUPPORTED), (dict(sequences=65536), UNSUPPORTED), (dict(max_length=(1 << 30) + 1), UNSUPPORTED),
     (dict(queries=(1 << 24) + 1), UNSUPPORTED),
-    (dict(queries=1 << 24, max_queries=1 << 40, sequences=65535), UNSUPPORTED)])
+    (dict(queries=1 << 24, max_queries=1 << 40, sequences=65535), UNSUPPORTED),
+    (dict(queries=1 << 24, max_queries=1 << 24, heads=256, q_stride=1 << 20, out_stride=1 << 20), UNSUPPORTED)])
 def test_attention_entry_refuses(kw, code):
     _refused("attention", _attention(**kw), code)
 

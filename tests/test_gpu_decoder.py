@@ -489,6 +489,25 @@ def test_attention_with_wide_values(gpu, dtype):
     _attend_case([256, 100], [200, 60], 4, 2, 64, 64, dtype, edit=grow, causal=False, scale=0.5)
 
 
+@pytest.mark.parametrize("size", [1e-25, 1e-12, 1e20])
+def test_attention_with_value_scales_of_any_size(gpu, size):
+    def edit(q, codes, scales, table):
+        scales[1][:] = scales[1] * np.float32(size)
+
+    _attend_case([100, 300], [1, 1], 4, 2, 64, 16, "float32", edit=edit)
+    _attend_case([100, 300], [1, 1], 4, 2, 128, 16, "bfloat16", edit=edit)
+    _attend_case([100, 300], [80, 50], 4, 2, 64, 16, "float32", edit=edit)
+    _attend_case([100, 300], [80, 50], 4, 2, 128, 16, "bfloat16", edit=edit)
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [90, 60]])
+def test_attention_with_other_scales_of_scores(gpu, counts):
+    """Negative, zero, and large enough that one token takes almost all."""
+    for scale in (-0.2, 0.0, 2.0):
+        _attend_case([100, 300], counts, 4, 2, 64, 16, "float32", scale=scale)
+        _attend_case([100, 300], counts, 4, 2, 80, 16, "float16", scale=scale)
+
+
 def test_attention_in_far_slots(gpu):
     """Pages whose bytes lie past 2^32: a cache of 4.5 GiB of keys."""
     heads, page, dim = 1, 256, 256
