@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const float o[4] = {sum(j, u, 0) * part, sum(j, u, 1) * part, sum(j, u, 2) * part, sum(j, u, 3) * part};
-            store_floats<4>(turn + col * kPitch + 16 * h + 4 * u, o);
+            put_floats<4>(turn + col * kPitch + 16 * h + 4 * u, o);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         constexpr int kLanes = 32 / kPiece;

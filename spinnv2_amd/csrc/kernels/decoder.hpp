@@ -31,14 +31,16 @@ struct alignas(sizeof(T) * N) Vec {
     T v[N];
 };
 
-// N elements at p as floats: N > 1 takes a pointer aligned to the smaller of
-// 16 bytes and all N elements.
+// N elements at p as floats, 16 bytes an instruction.  Any alignment will do:
+// the memory units take wide accesses at every address, and one that crosses
+// a line costs a second request, not a byte's each.
 template <int N, typename T>
 __device__ __forceinline__ void load_floats(const T *p, float (&f)[N]) {
     constexpr int kPer = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
 #pragma unroll
     for (int i = 0; i < N; i += kPer) {
-        const Vec<T, kPer> x = *reinterpret_cast<const Vec<T, kPer> *>(p + i);
+        Vec<T, kPer> x;
+        __builtin_memcpy(x.v, p + i, sizeof(x.v));
 #pragma unroll
         for (int j = 0; j < kPer; j++) f[i + j] = static_cast<float>(x.v[j]);
     }
@@ -51,8 +53,60 @@ __device__ __forceinline__ void store_floats(T *p, const float (&f)[N]) {
         Vec<T, kPer> x;
 #pragma unroll
         for (int j = 0; j < kPer; j++) x.v[j] = static_cast<T>(f[i + j]);
-        *reinterpret_cast<Vec<T, kPer> *>(p + i) = x;
+        __builtin_memcpy(p + i, x.v, sizeof(x.v));
     }
+}
+// To LDS, aligned to all N elements.
+template <int N, typename T>
+__device__ __forceinline__ void put_floats(T *p, const float (&f)[N]) {
+    Vec<T, N> x;
+#pragma unroll
+    for (int j = 0; j < N; j++) x.v[j] = static_cast<T>(f[j]);
+    *reinterpret_cast<Vec<T, N> *>(p) = x;
+}
+// N elements that were loaded from min(i, cols - N) of a row of `cols`, as those
+// from i on, zeros past the row's end.  All lanes load so, without a branch:
+// under one each of a row's loads is waited for by itself.  TAIL: cols is no
+// multiple of N.
+template <int N, bool TAIL>
+__device__ __forceinline__ void settle(int i, int cols, float (&f)[N]) {
+    const int past = i + N - cols;
+    if constexpr (TAIL) {
+        if (past > 0) {
+#pragma unroll
+            for (int step = 1; step < N; step *= 2)
+#pragma unroll
+                for (int j = 0; j < N; j++) f[j] = past & step ? (j + step < N ? f[(j + step) % N] : 0.0f) : f[j];
+#pragma unroll
+            for (int j = 0; j < N; j++) f[j] = past >= N ? 0.0f : f[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) f[j] = past > 0 ? 0.0f : f[j];
+    }
+}
+// The first `left` of N elements.
+template <int N, typename T>
+__device__ __forceinline__ void store_some(T *p, int left, const float (&f)[N]) {
+    if (left >= N) {
+        store_floats<N>(p, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < left) p[i] = static_cast<T>(f[i]);
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec(const T *p) {
+    Vec<T, N> x;
+    __builtin_memcpy(x.v, p, sizeof(x.v));
+    return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Vec<T, N> &x, float (&f)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) f[j] = static_cast<float>(x.v[j]);
 }
 
 constexpr unsigned kInfBits = 0x7f800000u;

@@ -12,6 +12,8 @@
 // One pass: a thread keeps its part of the row in registers between the
 // statistics and the codes, so each input is read once and each output
 // written once.  Bound by HBM.
+#include <type_traits>
+
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -63,8 +65,8 @@ __device__ __forceinline__ U wave_max(U v) {
 
 // THREADS threads a row (a wave: several rows a workgroup), each with CHUNKS
 // runs of VEC neighbouring elements in registers; CHUNKS = 0: rows of any
-// length, read again for the codes.
-template <typename T, typename W, int THREADS, int VEC, int CHUNKS>
+// length, read again for the codes.  TAIL: cols is no multiple of VEC.
+template <typename T, typename W, int THREADS, int VEC, int CHUNKS, bool TAIL>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(RowArgs a) {
     using P = typename Product<T, W>::type;
     using U = decltype(abs_bits(P{}));
@@ -82,28 +84,37 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
     float hv[CHUNKS ? CHUNKS : 1][VEC];
     double sum = 0.0;
     U top = 0;
-    auto load = [&](int c, float(&f)[VEC], bool store) {
+    auto from = [&](int c) { return min((c * THREADS + tid) * VEC, a.cols - VEC); };
+    struct Raw {
+        Vec<T, VEC> x, r;
+    };
+    auto fetch = [&](int c, Raw &v) {
+        v.x = load_vec<T, VEC>(x + from(c));
+        if (r) v.r = load_vec<T, VEC>(r + from(c));
+    };
+    auto sum_up = [&](int c, const Raw &v, float(&f)[VEC]) {
         const int i = (c * THREADS + tid) * VEC;
-        if (i >= a.cols) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) f[j] = 0.0f;
-            return;
-        }
-        load_floats<VEC>(x + i, f);
+        widen(v.x, f);
         if (r) {
             float g[VEC];
-            load_floats<VEC>(r + i, g);
+            widen(v.r, g);
 #pragma unroll
             for (int j = 0; j < VEC; j++) f[j] = static_cast<float>(static_cast<T>(f[j] + g[j]));
         }
-        if (h && store) store_floats<VEC>(h + i, f);
+        settle<VEC, TAIL>(i, a.cols, f);
+    };
+    auto keep = [&](int c, const float(&f)[VEC]) {
+        const int i = (c * THREADS + tid) * VEC;
+        if (h && i < a.cols) store_some<VEC>(h + i, TAIL ? a.cols - i : VEC, f);
     };
     auto products = [&](int c, const float(&f)[VEC], P(&p)[VEC]) {
-        const int i = (c * THREADS + tid) * VEC;
         float g[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; j++) g[j] = 1.0f;
-        if (w && i < a.cols) load_floats<VEC>(w + i, g);
+        if (w) {
+            widen(load_vec<W, VEC>(w + from(c)), g);
+            settle<VEC, TAIL>((c * THREADS + tid) * VEC, a.cols, g);
+        }
 #pragma unroll
         for (int j = 0; j < VEC; j++) p[j] = static_cast<P>(f[j]) * static_cast<P>(g[j]);
     };
@@ -119,13 +130,21 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
         }
     };
     if constexpr (CHUNKS > 0) {
+        Raw raw[CHUNKS];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c++) load(c, hv[c], true);
+        for (int c = 0; c < CHUNKS; c++) fetch(c, raw[c]);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) sum_up(c, raw[c], hv[c]);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) keep(c, hv[c]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) statistics(c, hv[c]);
     } else {
         for (int c = 0; c < chunks; c++) {
-            load(c, hv[0], true);
+            Raw raw;
+            fetch(c, raw);
+            sum_up(c, raw, hv[0]);
+            keep(c, hv[0]);
             statistics(c, hv[0]);
         }
     }
@@ -164,7 +183,13 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
 #pragma unroll
         for (int j = 0; j < VEC; j++) out.v[j] = 0;
         if (finite && top != 0) quantise<VEC>(p, amax, out.v);
-        if (i < a.cols) *reinterpret_cast<Vec<int8_t, VEC> *>(q + i) = out;
+        if (i + VEC <= a.cols) {
+            __builtin_memcpy(q + i, out.v, VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (i + j < a.cols) q[i + j] = out.v[j];
+        }
     };
     if constexpr (CHUNKS > 0) {
 #pragma unroll
@@ -172,15 +197,22 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
     } else {
         for (int c = 0; c < chunks; c++) {
             // h is read back where it was stored: x may have been overwritten by it
-            const int i = (c * THREADS + tid) * VEC;
-            if (!h) load(c, hv[0], false);
-            else if (i < a.cols) load_floats<VEC>(h + i, hv[0]);
+            Raw raw;
+            if (h) {
+                const int i = (c * THREADS + tid) * VEC;
+                // this thread's own elements: past them others may not have stored yet
+#pragma unroll
+                for (int j = 0; j < VEC; j++) hv[0][j] = i + j < a.cols ? static_cast<float>(h[i + j]) : 0.0f;
+            } else {
+                fetch(c, raw);
+                sum_up(c, raw, hv[0]);
+            }
             codes(c, hv[0]);
         }
     }
 }
 
-template <typename T, typename W, int VEC>
+template <typename T, typename W>
 int launch_rows(const RowArgs &a, void *stream) {
     const char *what = "rmsnorm_i8";
     auto go = [&](auto kernel, int threads) {
@@ -188,16 +220,20 @@ int launch_rows(const RowArgs &a, void *stream) {
         return launch(what, kernel, dim3(static_cast<unsigned>((a.rows + rows - 1) / rows)), dim3(threads < 256 ? 256 : threads),
                       stream, a);
     };
-    constexpr int kOne = VEC == 1 ? 8 : 1;  // runs that hold as much as one of 8
     // a wave a row up to 1024 elements: no barrier; then as few threads as
-    // hold the row in 8 runs of 8, since the statistics' join grows with them
-    if (a.cols <= 64 * 8) return go(rmsnorm_rows<T, W, 64, VEC, kOne>, 64);
-    if (a.cols <= 64 * 16) return go(rmsnorm_rows<T, W, 64, VEC, 2 * kOne>, 64);
-    if (a.cols <= 256 * 8) return go(rmsnorm_rows<T, W, 256, VEC, kOne>, 256);
-    if (a.cols <= 256 * 16) return go(rmsnorm_rows<T, W, 256, VEC, 2 * kOne>, 256);
-    if (a.cols <= 512 * 16) return go(rmsnorm_rows<T, W, 512, VEC, 2 * kOne>, 512);
-    if (a.cols <= 1024 * 16) return go(rmsnorm_rows<T, W, 1024, VEC, 2 * kOne>, 1024);
-    return go(rmsnorm_rows<T, W, 1024, VEC, 0>, 1024);
+    // hold the row in two runs of 8, since the statistics' join grows with them
+    if (a.cols < 8) return go(rmsnorm_rows<T, W, 64, 1, 1, false>, 64);
+    auto by_length = [&](auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        if (a.cols <= 64 * 8) return go(rmsnorm_rows<T, W, 64, 8, 1, TAIL>, 64);
+        if (a.cols <= 64 * 16) return go(rmsnorm_rows<T, W, 64, 8, 2, TAIL>, 64);
+        if (a.cols <= 256 * 8) return go(rmsnorm_rows<T, W, 256, 8, 1, TAIL>, 256);
+        if (a.cols <= 256 * 16) return go(rmsnorm_rows<T, W, 256, 8, 2, TAIL>, 256);
+        if (a.cols <= 512 * 16) return go(rmsnorm_rows<T, W, 512, 8, 2, TAIL>, 512);
+        if (a.cols <= 1024 * 16) return go(rmsnorm_rows<T, W, 1024, 8, 2, TAIL>, 1024);
+        return go(rmsnorm_rows<T, W, 1024, 8, 0, TAIL>, 1024);
+    };
+    return a.cols % 8 ? by_length(std::true_type{}) : by_length(std::false_type{});
 }
 
 struct DequantArgs {
@@ -208,8 +244,9 @@ struct DequantArgs {
     int cols, runs;  // runs of VEC elements a row
 };
 
-// A workgroup takes 256 runs of VEC elements of one row after the other's.
-template <typename T, int VEC>
+// A workgroup takes 256 runs of VEC elements, one row's after the other's.
+// TAIL: cols is no multiple of VEC; it is VEC at least.
+template <typename T, int VEC, bool TAIL>
 __global__ void __launch_bounds__(256) dequantize_rows(DequantArgs a) {
     const int64_t total = a.rows * a.runs;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < total;
@@ -217,17 +254,13 @@ __global__ void __launch_bounds__(256) dequantize_rows(DequantArgs a) {
         const int64_t row = t / a.runs;
         const int i = static_cast<int>(t - row * a.runs) * VEC;
         const float s = a.scale[row];
-        const Vec<int8_t, VEC> c = *reinterpret_cast<const Vec<int8_t, VEC> *>(a.q + row * a.q_stride + i);
         float f[VEC];
+        widen(load_vec<int8_t, VEC>(a.q + row * a.q_stride + min(i, a.cols - VEC)), f);
+        if constexpr (TAIL) settle<VEC, true>(i, a.cols, f);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) f[j] = s * static_cast<float>(c.v[j]);
-        store_floats<VEC>(static_cast<T *>(a.out) + row * a.out_stride + i, f);
+        for (int j = 0; j < VEC; j++) f[j] *= s;
+        store_some<VEC>(static_cast<T *>(a.out) + row * a.out_stride + i, TAIL ? a.cols - i : VEC, f);
     }
-}
-
-bool vec_rows(const void *p, int64_t stride, size_t size, int vec) {
-    const size_t to = size * vec < 16 ? size * vec : 16;
-    return aligned(p, to) && (stride * size) % to == 0;
 }
 
 }  // namespace
@@ -253,18 +286,12 @@ extern "C" int spkv2_mi355x_rmsnorm_i8(const Spkv2RmsNormI8 *g, void *stream) {
                 return bad("rmsnorm_i8: a stride is below cols");
         }
         if (g->cols > (1 << 24) || g->rows > INT32_MAX) return unsupported("rmsnorm_i8: more than 2^24 columns or 2^31 rows");
-        const size_t size = dtype_size(g->dtype);
         const RowArgs a{g->x, g->residual, g->weight, g->residual_out, g->q, g->scale, g->rows, g->x_stride,
                         g->residual_stride, g->residual_out_stride, g->q_stride, static_cast<int>(g->cols), g->norm, g->eps};
-        const bool vec = g->cols % 8 == 0 && vec_rows(g->x, g->x_stride, size, 8) &&
-                         (!g->residual || vec_rows(g->residual, g->residual_stride, size, 8)) &&
-                         (!g->residual_out || vec_rows(g->residual_out, g->residual_out_stride, size, 8)) &&
-                         (!g->weight || aligned(g->weight, 16)) && vec_rows(g->q, g->q_stride, 1, 8);
         const bool wide = g->weight && g->weight_dtype == SPKV2_DTYPE_FP32;
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
-            if (wide) return vec ? launch_rows<T, float, 8>(a, stream) : launch_rows<T, float, 1>(a, stream);
-            return vec ? launch_rows<T, T, 8>(a, stream) : launch_rows<T, T, 1>(a, stream);
+            return wide ? launch_rows<T, float>(a, stream) : launch_rows<T, T>(a, stream);
         });
     });
 }
@@ -278,22 +305,16 @@ extern "C" int spkv2_mi355x_dequantize_i8(const Spkv2DequantizeI8 *g, void *stre
         if (!g->q || !g->scale || !g->out) return bad("dequantize_i8: q, scale or out is NULL");
         if (g->rows > 1 && (g->q_stride < g->cols || g->out_stride < g->cols)) return bad("dequantize_i8: a stride is below cols");
         if (g->cols > INT32_MAX || g->rows > INT32_MAX) return unsupported("dequantize_i8: more than 2^31 rows or columns");
-        const size_t size = dtype_size(g->dtype);
-        auto vec = [&](int n) {
-            return g->cols % n == 0 && vec_rows(g->q, g->q_stride, 1, n) && vec_rows(g->out, g->out_stride, size, n);
-        };
-        DequantArgs a{g->q, g->scale, g->out, g->q_stride, g->out_stride, g->rows, static_cast<int>(g->cols), 0};
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
-            auto go = [&](auto kernel, int n) {
-                a.runs = a.cols / n;
+            auto go = [&](auto kernel, int run) {
+                const DequantArgs a{g->q, g->scale, g->out, g->q_stride, g->out_stride, g->rows, static_cast<int>(g->cols),
+                                    static_cast<int>((g->cols + run - 1) / run)};
                 const int64_t blocks = (a.rows * a.runs + 255) / 256;
-                return launch("dequantize_i8", kernel, dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536)), dim3(256),
-                              stream, a);
+                return launch("dequantize_i8", kernel, dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536)), dim3(256), stream, a);
             };
-            if (vec(16)) return go(dequantize_rows<T, 16>, 16);
-            if (vec(4)) return go(dequantize_rows<T, 4>, 4);
-            return go(dequantize_rows<T, 1>, 1);
+            if (g->cols < 16) return go(dequantize_rows<T, 1, false>, 1);
+            return g->cols % 16 ? go(dequantize_rows<T, 16, true>, 16) : go(dequantize_rows<T, 16, false>, 16);
         });
     });
 }

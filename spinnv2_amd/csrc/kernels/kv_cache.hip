@@ -24,7 +24,7 @@ struct WriteArgs {
 };
 
 // LANES lanes (of which head_dim / 8 have elements) a vector
-template <typename T, int LANES, bool VEC>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) kv_write(WriteArgs a) {
     const int head = blockIdx.x % a.c.kv_heads, lane = threadIdx.x % LANES;
     const int64_t token = static_cast<int64_t>(blockIdx.x / a.c.kv_heads) * (256 / LANES) + threadIdx.x / LANES;
@@ -37,13 +37,7 @@ __global__ void __launch_bounds__(256) kv_write(WriteArgs a) {
         const T *x = static_cast<const T *>(n ? a.v : a.k) + token * (n ? a.v_stride : a.k_stride) + at_head;
 #pragma unroll
         for (int j = 0; j < 8; j++) f[n][j] = 0.0f;
-        if (in) {
-            if constexpr (VEC) load_floats<8>(x, f[n]);
-            else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) f[n][j] = static_cast<float>(x[j]);
-            }
-        }
+        if (in) load_floats<8>(x, f[n]);
     }
     const int64_t slot = a.slots[token];
     if (slot < 0 || slot >= a.c.pages * a.c.page_size) return;  // below 2^51
@@ -82,7 +76,7 @@ __device__ __forceinline__ int sequence_of(const int32_t *offsets, int sequences
 }
 
 // 16 codes a lane, pieces of the token's heads one after the other
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(256) kv_read(ReadArgs a) {
     const int pieces = a.c.kv_heads * (a.c.head_dim / 16);
     const bool is_v = blockIdx.y != 0;
@@ -110,11 +104,7 @@ __global__ void __launch_bounds__(256) kv_read(ReadArgs a) {
             for (int j = 0; j < 16; j++) f[j] = scale * static_cast<float>(q.v[j]);
         }
         T *y = out + t * (is_v ? a.r.v_stride : a.r.k_stride) + static_cast<int64_t>(head) * a.c.head_dim + d;
-        if constexpr (VEC) store_floats<16>(y, f);
-        else {
-#pragma unroll
-            for (int j = 0; j < 16; j++) y[j] = static_cast<T>(f[j]);
-        }
+        store_floats<16>(y, f);
     }
 }
 
@@ -147,8 +137,6 @@ extern "C" int spkv2_mi355x_kv_write_i8(const Spkv2KvCacheI8 *c, const Spkv2KvWr
         const int64_t width = static_cast<int64_t>(c->kv_heads) * c->head_dim;
         if (g->tokens > 1 && (g->k_stride < width || g->v_stride < width)) return bad("kv_write_i8: a stride is below the heads' width");
         if (g->tokens > INT32_MAX) return unsupported("kv_write_i8: more than 2^31 tokens");
-        const size_t size = dtype_size(g->dtype);
-        const bool vec = aligned(g->k, 16) && aligned(g->v, 16) && (g->k_stride * size) % 16 == 0 && (g->v_stride * size) % 16 == 0;
         WriteArgs a{*c, g->k, g->v, g->slots, g->tokens, g->k_stride, g->v_stride, 0, 0};
         if (c->pages * c->page_size <= INT32_MAX) div_magic(static_cast<unsigned>(c->page_size), &a.page_mul, &a.page_shift);
         return with_type(g->dtype, [&](auto t) {
@@ -158,9 +146,9 @@ extern "C" int spkv2_mi355x_kv_write_i8(const Spkv2KvCacheI8 *c, const Spkv2KvWr
                 if (blocks >= 1 << 24) return unsupported("kv_write_i8: too many tokens for one launch");
                 return launch("kv_write_i8", kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), stream, a);
             };
-            if (c->head_dim <= 64) return vec ? go(kv_write<T, 8, true>, 8) : go(kv_write<T, 8, false>, 8);
-            if (c->head_dim <= 128) return vec ? go(kv_write<T, 16, true>, 16) : go(kv_write<T, 16, false>, 16);
-            return vec ? go(kv_write<T, 32, true>, 32) : go(kv_write<T, 32, false>, 32);
+            if (c->head_dim <= 64) return go(kv_write<T, 8>, 8);
+            if (c->head_dim <= 128) return go(kv_write<T, 16>, 16);
+            return go(kv_write<T, 32>, 32);
         });
     });
 }
@@ -177,15 +165,12 @@ extern "C" int spkv2_mi355x_kv_read_i8(const Spkv2KvCacheI8 *c, const Spkv2KvRea
         if (g->tokens > 1 && ((g->k && g->k_stride < width) || (g->v && g->v_stride < width)))
             return bad("kv_read_i8: a stride is below the heads' width");
         if (g->tokens > INT32_MAX) return unsupported("kv_read_i8: more than 2^31 tokens");
-        const size_t size = dtype_size(g->dtype);
-        const bool vec = aligned(g->k, 16) && aligned(g->v, 16) && (g->k_stride * size) % 16 == 0 && (g->v_stride * size) % 16 == 0;
         const ReadArgs a{*c, *g};
         const int64_t blocks = (g->tokens * c->kv_heads * (c->head_dim / 16) + 255) / 256;
         const dim3 grid(static_cast<unsigned>(blocks < 65536 ? blocks : 65536), 2);
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
-            return vec ? launch("kv_read_i8", kv_read<T, true>, grid, dim3(256), stream, a)
-                       : launch("kv_read_i8", kv_read<T, false>, grid, dim3(256), stream, a);
+            return launch("kv_read_i8", kv_read<T>, grid, dim3(256), stream, a);
         });
     });
 }

@@ -27,7 +27,6 @@ struct MatmulArgs {
     int64_t a_stride, b_stride, out_stride;
     int m, n, k;
     int m_tiles, n_tiles;
-    bool vec_out;  // rows of the output are 16-byte aligned
 };
 
 // 16 bytes at p, of which `left` are inside the row: zeros past them
@@ -287,33 +286,24 @@ __global__ void __launch_bounds__(256, B >= 4 ? 1 : 2) matmul_tiles(MatmulArgs a
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = scaled(acc[i][j][r + e], sa, sb[i][r + e], bias[i][r + e]);
-                store_floats<4>(row + i * 32 + 2 * r, v);
+                put_floats<4>(row + i * 32 + 2 * r, v);
             }
         wait_lds();
-        if (a.vec_out) {
-            constexpr int kLanes = kCols / kPiece, kRows = 64 / kLanes;
-            const int c = lane % kLanes * kPiece;
-            T *out = static_cast<T *>(a.out) + (m + lane / kLanes) * a.out_stride + n0 + wn + c;
+        constexpr int kLanes = kCols / kPiece, kRows = 64 / kLanes;
+        const int c = lane % kLanes * kPiece;
+        T *out = static_cast<T *>(a.out) + (m + lane / kLanes) * a.out_stride + n0 + wn + c;
 #pragma unroll
-            for (int r = 0; r < 32; r += kRows) {
-                const Vec<T, kPiece> v = *reinterpret_cast<const Vec<T, kPiece> *>(mine + (r + lane / kLanes) * (kOutPitch / static_cast<int>(sizeof(T))) + c);
-                if (m + r + lane / kLanes < a.m) {
-                    if (c + kPiece <= left) {
-                        *reinterpret_cast<Vec<T, kPiece> *>(out + r * a.out_stride) = v;
-                    } else {
+        for (int r = 0; r < 32; r += kRows) {
+            const Vec<T, kPiece> v = *reinterpret_cast<const Vec<T, kPiece> *>(mine + (r + lane / kLanes) * (kOutPitch / static_cast<int>(sizeof(T))) + c);
+            if (m + r + lane / kLanes < a.m) {
+                if (c + kPiece <= left) {
+                    __builtin_memcpy(out + r * a.out_stride, v.v, sizeof(v.v));
+                } else {
 #pragma unroll
-                        for (int e = 0; e < kPiece; e++)
-                            if (c + e < left) out[r * a.out_stride + e] = v.v[e];
-                    }
+                    for (int e = 0; e < kPiece; e++)
+                        if (c + e < left) out[r * a.out_stride + e] = v.v[e];
                 }
             }
-        } else {
-            T *out = static_cast<T *>(a.out) + m * a.out_stride + n0 + wn;
-            constexpr int kLanes = kCols < 64 ? kCols : 64;
-            for (int r = lane / kLanes; r < min(32, a.m - m); r += 64 / kLanes)
-#pragma unroll
-                for (int c = lane % kLanes; c < kCols; c += kLanes)
-                    if (c < left) out[r * a.out_stride + c] = mine[r * (kOutPitch / static_cast<int>(sizeof(T))) + c];
         }
         wait_lds();
     }
@@ -426,13 +416,7 @@ __global__ void __launch_bounds__(64 * WAVES) matmul_rows(MatmulArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = scaled(total[e], sa, sb[e], bias[e]);
         T *out = static_cast<T *>(a.out) + m * a.out_stride + n;
-        if (a.vec_out && left >= 4) {
-            store_floats<4>(out, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (e < left) out[e] = static_cast<T>(v[e]);
-        }
+        store_some<4>(out, left, v);
     }
 }
 
@@ -485,10 +469,9 @@ extern "C" int spkv2_mi355x_matmul_i8(const Spkv2MatmulI8 *g, void *stream) {
         if (g->k > (1 << 17)) return unsupported("matmul_i8: k above 2^17, whose sums may pass 32 bits");
         if (g->m > (1 << 21) || g->n > (1 << 26)) return unsupported("matmul_i8: m above 2^21 or n above 2^26");
         MatmulArgs a{g->a, g->b, g->a_scale, g->b_scale, g->bias, g->out, g->a_stride, g->b_stride, g->out_stride,
-                     static_cast<int>(g->m), static_cast<int>(g->n), static_cast<int>(g->k), 0, 0, false};
+                     static_cast<int>(g->m), static_cast<int>(g->n), static_cast<int>(g->k), 0, 0};
         if (g->m == 1) a.a_stride = 0, a.out_stride = 0;
         if (g->n == 1) a.b_stride = 0;
-        a.vec_out = aligned(g->out, 16) && (a.out_stride * dtype_size(g->dtype)) % 16 == 0;
         const bool far = a.a_stride >= (1 << 23) || a.b_stride >= (1 << 23);  // 256 rows pass 2^31 bytes
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
