@@ -6,8 +6,8 @@
 // fp16 matrix cores; a token's key scale multiplies its scores, its value
 // scale its weights.
 //
-// attend_rows takes up to 32 rows (query, head of the group) of a sequence and
-// kv head, single tokens above all: bound by the cache's bytes (64 sequences of
+// attend_rows takes 16 rows (query, head of the group) of a sequence and kv head
+// a workgroup, for single tokens above all: bound by the cache's bytes (64 sequences of
 // 3001 to 16384 tokens, 8 kv heads of 128, 1.31 GB: 271 us, 4.8 TB/s), one
 // short sequence by its loads' latency (333 tokens 9.7 us).  attend_tiles takes
 // 128 rows a workgroup: bound by two waves a SIMD whose arithmetic and matrix
@@ -139,8 +139,8 @@ __device__ __forceinline__ Place place(const AttnArgs &a) {
     return p;
 }
 
-// One workgroup: RT tiles of 16 rows (query, head of the group) of one
-// sequence and kv head, and one split of its tokens.  Scores are taken
+// One workgroup: 16 rows (query, head of the group) of one sequence and kv
+// head, and one split of its tokens.  Scores are taken
 // transposed, S^T = K q^T on 16x16 tiles: a lane then holds four tokens'
 // scores of one row, which are the weights' operand of O^T = V^T P^T as they
 // are, if V's rows are taken in the same order.  So nothing passes through LDS
@@ -152,15 +152,15 @@ __device__ __forceinline__ Place place(const AttnArgs &a) {
 //   scores, weights: tokens 4 g .. + 4 of each tile
 //   V: those tokens' codes VPL (l % 16) .. + VPL (VPL = DP / 16); product j
 //      takes d = VPL r + j as its row r
-template <typename T, int DP, int RT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / WAVES : 1) attend_rows(AttnArgs a) {
+template <typename T, int DP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES : 1) attend_rows(AttnArgs a) {
     constexpr bool kWide = sizeof(T) == 4;  // rows of 22 bits: two fp16 parts
     constexpr int kParts = kWide ? 2 : 1;
     constexpr int kPieces = DP / 64;  // 16-byte pieces of K a lane
     constexpr int kVpl = DP / 16;     // V codes a lane
     constexpr int kVw = kVpl / 4;
     __shared__ __align__(16) float joined[WAVES * 64 * 4 * kVpl];
-    __shared__ float wave_max[WAVES][RT * 16], wave_sum[WAVES][RT * 16];
+    __shared__ float wave_max[WAVES][16], wave_sum[WAVES][16];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
@@ -168,9 +168,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
     const int b = at_block.b, head = at_block.head, split = at_block.split, block = at_block.block;
     const int dim = a.c.head_dim;
     const Sequence s = sequence(a, b);
-    const int rows = s.count * a.group, r0 = block * 16 * RT;
+    const int rows = s.count * a.group, r0 = block * 16;
     if (r0 >= rows) return;
-    const int first_q = r0 / a.group, last_q = (min(rows, r0 + 16 * RT) - 1) / a.group;
+    const int first_q = r0 / a.group, last_q = (min(rows, r0 + 16) - 1) / a.group;
     int low = split * a.split_tokens, high = min(s.length, low + a.split_tokens);
     if (a.causal) {
         high = min(high, s.position + last_q + 1);
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
     }
 
     if (a.splits > 1 && low >= high) {
-        nothing(a, s, head, split, r0, min(rows, r0 + 16 * RT));
+        nothing(a, s, head, split, r0, min(rows, r0 + 16));
         return;
     }
 
@@ -239,16 +239,15 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
     }
 
     // the rows' masks and queries, scaled by a power of two to 2^14 .. 2^15
-    half8_t qf[RT][DP / 32][kParts];
-    float factor[RT], m[RT], l[RT];
-    int last[RT], start[RT];
-    floatx4 acc[RT][kVpl];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int r = r0 + t * 16 + col, i = r / a.group;
+    half8_t qf[DP / 32][kParts];
+    float factor, m, l;
+    int last, start;
+    floatx4 acc[kVpl];
+    {
+        const int r = r0 + col, i = r / a.group;
         const bool in = r < rows;
-        last[t] = a.causal ? s.position + i : s.length - 1;
-        start[t] = a.causal && a.window ? last[t] + 1 - a.window : 0;
+        last = a.causal ? s.position + i : s.length - 1;
+        start = a.causal && a.window ? last + 1 - a.window : 0;
         // without a branch, so that all loads are on their way at once: rows past the last are the last
         const int rq = min(r, rows - 1), iq = rq / a.group;
         const T *q = static_cast<const T *>(a.q) + (s.row0 + iq) * a.q_stride +
@@ -267,27 +266,26 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
         }
         top = over_groups_max(top);
         const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
-        factor[t] = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
+        factor = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
 #pragma unroll
         for (int x = 0; x < DP / 32; x++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = ldexpf(f[x][e], 14 - ex);
                 const _Float16 hi = static_cast<_Float16>(v);
-                qf[t][x][0][e] = hi;
-                if constexpr (kWide) qf[t][x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+                qf[x][0][e] = hi;
+                if constexpr (kWide) qf[x][kParts - 1][e] = static_cast<_Float16>(v - static_cast<float>(hi));
             }
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
+        m = -__builtin_inff();
+        l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kVpl; j++) acc[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < kVpl; j++) acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float unit = 0.0f, per_unit = 0.0f;  // a power of two no value scale is above, and kLift / unit
 
     auto use = [&](const Chunk &x, int at) {
-        floatx4 sc[RT][2];
-#pragma unroll
-        for (int t = 0; t < RT; t++) sc[t][0] = sc[t][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        floatx4 sc[2];
+        sc[0] = sc[1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -296,10 +294,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
                 for (int e = 0; e < 2; e++) {
                     const half8_t kf = codes8(x.k[h][p][2 * e], x.k[h][p][2 * e + 1]);
 #pragma unroll
-                    for (int t = 0; t < RT; t++)
-#pragma unroll
                         for (int w = 0; w < kParts; w++)
-                            sc[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][2 * p + e][w], sc[t][h], 0, 0, 0);
+                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[2 * p + e][w], sc[h], 0, 0, 0);
                 }
         // value scales: those of masked tokens may be anything in the cache
         float vs[8];
@@ -317,41 +313,38 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
             unit = now;
             per_unit = kLift / now;
 #pragma unroll
-            for (int t = 0; t < RT; t++)
-#pragma unroll
-                for (int j = 0; j < kVpl; j++) acc[t][j] *= ratio;
+                for (int j = 0; j < kVpl; j++) acc[j] *= ratio;
         }
-        half8_t pf[RT][kParts];
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
+        half8_t pf[kParts];
+        {
             float v[8], most = -__builtin_inff();
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int token = at + 16 * (e / 4) + 4 * g + e % 4;
-                v[e] = sc[t][e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor[t]);
-                const bool keep = token >= low && token < high && x.ok[e / 4] && token <= last[t] && token >= start[t];
+                v[e] = sc[e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor);
+                const bool keep = token >= low && token < high && x.ok[e / 4] && token <= last && token >= start;
                 v[e] = keep ? v[e] : -__builtin_inff();
                 most = fmaxf(most, v[e]);
             }
-            if (__any(most > m[t] + kSlack)) {
-                const float now = fmaxf(m[t], over_groups_max(most));
-                const float ratio = m[t] > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[t] - now) : 0.0f;
-                m[t] = now;
-                l[t] *= ratio;
+            if (__any(most > m + kSlack)) {
+                const float now = fmaxf(m, over_groups_max(most));
+                const float ratio = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - now) : 0.0f;
+                m = now;
+                l *= ratio;
 #pragma unroll
-                for (int j = 0; j < kVpl; j++) acc[t][j] *= ratio;
+                for (int j = 0; j < kVpl; j++) acc[j] *= ratio;
             }
-            const float from = m[t] > -__builtin_inff() ? m[t] : 0.0f;
+            const float from = m > -__builtin_inff() ? m : 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float p = __builtin_amdgcn_exp2f(v[e] - from);
-                l[t] += p;
+                l += p;
                 // 0 where the row masks the token, whose scale may be NaN
                 float w = v[e] == -__builtin_inff() ? 0.0f : p * (vs[e] * per_unit);
                 if constexpr (kWide) once(w);
                 const _Float16 hi = static_cast<_Float16>(w);
-                pf[t][0][e] = hi;
-                if constexpr (kWide) pf[t][kParts - 1][e] = static_cast<_Float16>(w - static_cast<float>(hi));
+                pf[0][e] = hi;
+                if constexpr (kWide) pf[kParts - 1][e] = static_cast<_Float16>(w - static_cast<float>(hi));
             }
         }
 #pragma unroll
@@ -360,10 +353,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
             const half8_t vf = join(codes_to_half(x.v[1][j / 4], x.v[0][j / 4], sel), codes_to_half(x.v[3][j / 4], x.v[2][j / 4], sel),
                                     codes_to_half(x.v[5][j / 4], x.v[4][j / 4], sel), codes_to_half(x.v[7][j / 4], x.v[6][j / 4], sel));
 #pragma unroll
-            for (int t = 0; t < RT; t++)
-#pragma unroll
                 for (int w = 0; w < kParts; w++)
-                    acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t][w], acc[t][j], 0, 0, 0);
+                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[w], acc[j], 0, 0, 0);
         }
     };
 
@@ -378,37 +369,34 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
 
     // the waves' sums, joined in wave order
     const float back = unit / kLift;
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        l[t] = over_groups_sum(l[t]);
+    {
+        l = over_groups_sum(l);
         if (g == 0) {
-            wave_max[wave][t * 16 + col] = m[t];
-            wave_sum[wave][t * 16 + col] = l[t];
+            wave_max[wave][col] = m;
+            wave_sum[wave][col] = l;
         }
     }
     __syncthreads();
+    {
+        float most = wave_max[0][col];
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        float most = wave_max[0][t * 16 + col];
-#pragma unroll
-        for (int w = 1; w < WAVES; w++) most = fmaxf(most, wave_max[w][t * 16 + col]);
+        for (int w = 1; w < WAVES; w++) most = fmaxf(most, wave_max[w][col]);
         const bool none = !(most > -__builtin_inff());
         float total = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
-            const float r = none ? 1.0f : __builtin_amdgcn_exp2f(wave_max[w][t * 16 + col] - most);
-            total += r * wave_sum[w][t * 16 + col];
+            const float r = none ? 1.0f : __builtin_amdgcn_exp2f(wave_max[w][col] - most);
+            total += r * wave_sum[w][col];
         }
-        const float mine = (none ? 1.0f : __builtin_amdgcn_exp2f(m[t] - most)) * back;
-        if (t) __syncthreads();
+        const float mine = (none ? 1.0f : __builtin_amdgcn_exp2f(m - most)) * back;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < kVpl; j += 4)
                 *reinterpret_cast<floatx4 *>(joined + (((wave * 4 + i) * kVw + j / 4) * 64 + lane) * 4) =
-                    floatx4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]} * mine;
+                    floatx4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]} * mine;
         __syncthreads();
-        if (wave >= 4) continue;  // the columns are four waves' quarters
+        if (wave >= 4) return;  // the columns are four waves' quarters
         float o[kVpl];
 #pragma unroll
         for (int j = 0; j < kVpl; j += 4) {
@@ -420,8 +408,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP * RT * sizeof(T) <= 256 ? 12 / 
             for (int e = 0; e < 4; e++) o[j + e] = sum[e];
         }
         // this wave's quarter of the columns: d = VPL (4 g + wave) + j
-        const int r = r0 + t * 16 + col, i = r / a.group, d = kVpl * (4 * g + wave);
-        if (r >= rows || d >= dim) continue;
+        const int r = r0 + col, i = r / a.group, d = kVpl * (4 * g + wave);
+        if (r >= rows || d >= dim) return;
         const int h = head * a.group + (r - i * a.group);
         if (a.splits > 1) {
             const int64_t at_row = ((s.row0 + i) * a.heads + h) * a.splits + split;
@@ -861,8 +849,8 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
 }
 
 struct Plan {
-    int tiles;  // of 16 rows a workgroup
-    int waves;  // that deal tokens out among them (few rows)
+    bool wide;  // 128 rows a workgroup (attend_tiles), otherwise 16 (attend_rows)
+    int waves;  // of attend_rows
     int64_t row_blocks;  // up to 2^36: queries and heads are bounded
     int split_tokens, splits;
     size_t part, stats;  // bytes
@@ -871,22 +859,27 @@ struct Plan {
 Plan plan(const Spkv2KvCacheI8 &c, const Spkv2AttentionI8 &g) {
     Plan p;
     const int64_t rows = std::min(g.max_queries, g.queries) * (g.heads / c.kv_heads);
-    p.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
-    p.row_blocks = (rows + 16 * p.tiles - 1) / (16 * p.tiles);
+    // attend_tiles reads a tile of tokens once for 128 rows, attend_rows for 16,
+    // but spreads few tokens over more waves.  Where 16 rows do not hold them
+    // all, rows times tokens of all sequences and kv heads decide (us, rows'
+    // kernel against tiles'): 192 x 32 K 30 and 35, 120 x 64 K 28 and 33, 32 x
+    // 256 K 36 and 34, 192 x 48 K 38 and 34, 40 x 1 M 125 and 85.
+    p.wide = rows > 16 && static_cast<double>(rows) * g.sequences * c.kv_heads * g.max_length > 8e6;
+    p.row_blocks = p.wide ? (rows + 127) / 128 : (rows + 15) / 16;
     // Enough workgroups for eight on each CU (two where they take 128 rows), and
     // no split shorter than four chunks for each of four waves (two tiles): a
     // second kernel costs more than a few steps do.  Fewer workgroups than CUs
     // are of eight waves: one sequence of 333
     // tokens 13.1 us with four, 12.2 with eight.
     const int64_t base = g.sequences * c.kv_heads * p.row_blocks;
-    const int64_t step = 128, least = p.tiles == 8 ? 128 : 512;
-    int64_t splits = std::min<int64_t>(p.tiles == 8 ? 512 / base : (2048 + base - 1) / base, (g.max_length + least - 1) / least);
+    const int64_t step = 128, least = p.wide ? 128 : 512;
+    int64_t splits = std::min<int64_t>(p.wide ? 512 / base : (2048 + base - 1) / base, (g.max_length + least - 1) / least);
     splits = std::max<int64_t>(splits, 1);
     int64_t tokens = (g.max_length + splits - 1) / splits;
     tokens = std::max<int64_t>((tokens + step - 1) / step * step, step);
     p.split_tokens = static_cast<int>(tokens);
     p.splits = static_cast<int>(std::max<int64_t>((g.max_length + tokens - 1) / tokens, 1));
-    p.waves = p.tiles == 1 && base * p.splits <= 256 ? 8 : 4;
+    p.waves = base * p.splits <= 256 ? 8 : 4;
     const size_t parts = p.splits > 1 ? static_cast<size_t>(g.queries) * g.heads * p.splits : 0;
     p.part = parts * c.head_dim * sizeof(float);
     p.stats = parts * 2 * sizeof(float);
@@ -954,18 +947,21 @@ extern "C" int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *c, const Spkv2Att
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             const char *what = "attention_i8";
-            auto go = [&](auto one, auto eight, auto two) {
-                return launch(what, p.waves == 8 ? eight : p.tiles == 1 ? one : two, dim3(blocks * c->kv_heads), dim3(64 * p.waves), stream, a);
-            };
             auto many = [&](auto kernel) { return launch(what, kernel, dim3(blocks * c->kv_heads), dim3(256), stream, a); };
+            auto few = [&](auto four, auto eight) {
+                return launch(what, p.waves == 8 ? eight : four, dim3(blocks * c->kv_heads), dim3(64 * p.waves), stream, a);
+            };
             const int dim = c->head_dim;
             int rc;
-            if (p.tiles == 8) {
-                rc = dim <= 64 ? many(attend_tiles<T, 64>) : dim <= 96 ? many(attend_tiles<T, 96>) : dim <= 128 ? many(attend_tiles<T, 128>) : many(attend_tiles<T, 256>);
+            if (p.wide) {
+                rc = dim <= 64    ? many(attend_tiles<T, 64>)
+                     : dim <= 96  ? many(attend_tiles<T, 96>)
+                     : dim <= 128 ? many(attend_tiles<T, 128>)
+                                  : many(attend_tiles<T, 256>);
             } else {
-                rc = dim <= 64 ? go(attend_rows<T, 64, 1, 4>, attend_rows<T, 64, 1, 8>, attend_rows<T, 64, 2, 4>)
-                     : dim <= 128 ? go(attend_rows<T, 128, 1, 4>, attend_rows<T, 128, 1, 8>, attend_rows<T, 128, 2, 4>)
-                                  : go(attend_rows<T, 256, 1, 4>, attend_rows<T, 256, 1, 8>, attend_rows<T, 256, 2, 4>);
+                rc = dim <= 64    ? few(attend_rows<T, 64, 4>, attend_rows<T, 64, 8>)
+                     : dim <= 128 ? few(attend_rows<T, 128, 4>, attend_rows<T, 128, 8>)
+                                  : few(attend_rows<T, 256, 4>, attend_rows<T, 256, 8>);
             }
             if (rc || p.splits == 1) return rc;
             const dim3 rows(static_cast<unsigned>(g->sequences * a.max_queries), (g->heads + 3) / 4);

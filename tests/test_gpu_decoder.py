@@ -509,6 +509,68 @@ def test_attention_with_other_scales_of_scores(gpu, counts):
         _attend_case([100, 300], counts, 4, 2, 80, 16, "float16", scale=scale)
 
 
+# A bound far above the lengths makes calls of many rows take the kernel for
+# long ones, 128 rows a workgroup, at sizes that a plain implementation holds.
+FAR = 1 << 20
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 64), (12, 12, 64, 32), (8, 1, 80, 16), (2, 1, 256, 16), (10, 2, 48, 16), (4, 2, 96, 48), (3, 3, 192, 16)])
+def test_attention_of_many_rows(gpu, heads, kv, dim, page, dtype):
+    _attend_case([70, 200, 1, 33, 9], [70, 37, 1, 0, 12], heads, kv, dim, page, dtype, max_length=FAR)
+    _attend_case([150, 64, 0], [77, 5, 1], heads, kv, dim, page, dtype, max_length=FAR, causal=False)
+
+
+@pytest.mark.parametrize("window", [1, 16, 100, 1000])
+def test_attention_of_many_rows_in_a_window(gpu, window):
+    for dtype, dim in (("bfloat16", 128), ("float16", 64), ("float32", 80)):
+        _attend_case([300, 40, 7], [150, 40, 3], 4, 2, dim, 16, dtype, window=window, max_length=FAR)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_attention_of_many_rows_past_what_is_not_finite(gpu, dtype):
+    def bad(q, codes, scales, table):
+        table[0, 1], table[0, 3], table[1, 0], table[2, :] = -1, 2 ** 31 - 1, 10 ** 6, -7
+
+    def nan(q, codes, scales, table):
+        scales[0][table[0, 45 // 16], :, 45 % 16] = np.nan
+        scales[1][table[1, 30 // 16], 0, 30 % 16] = np.nan
+
+    def grow(q, codes, scales, table):
+        scales[0][:] = scales[0] * (1 + np.arange(scales[0].shape[2]) / 8).astype(np.float32)
+        scales[1][:, 0] *= np.float32(1e-6)
+        scales[1][:, 1] *= np.float32(3e4)
+        q[1] *= 0.0
+        q[2] *= 2.0 ** -12
+        q[3, 1] = rounded(q[3, 1] * 100, dtype)
+
+    for causal in (True, False):
+        _attend_case([120, 90, 20], [30, 70, 2], 4, 2, 64, 16, dtype, edit=bad, causal=causal, max_length=FAR)
+    got, want = _attend_case([70, 60], [70, 60], 4, 2, 64, 16, dtype, edit=nan, max_length=FAR)
+    assert np.isnan(want[45:70]).all() and np.isfinite(want[:45]).all() and np.isnan(want[100:130, :2]).all()
+    _attend_case([256, 100], [200, 60], 4, 2, 128, 64, dtype, edit=grow, max_length=FAR)
+    _attend_case([256, 100], [200, 60], 4, 2, 64, 64, dtype, edit=grow, causal=False, scale=0.5, max_length=FAR)
+    for scale in (-0.2, 0.0, 2.0):
+        _attend_case([100, 300], [90, 60], 4, 2, 80, 16, dtype, scale=scale, max_length=FAR)
+    for size in (1e-25, 1e-12, 1e20):
+        _attend_case([100, 300], [80, 50], 4, 2, 64, 16, "float32", max_length=FAR,
+                     edit=lambda q, c, s, t: s[1].__imul__(np.float32(size)))
+
+
+def test_attention_of_many_rows_strided_and_bounded(gpu):
+    for dtype, pad in (("bfloat16", 8), ("float16", 3), ("float32", 1)):
+        _attend_case([100, 90, 80], [40, 17, 80], 4, 2, 64, 16, dtype, pad=pad, extra_rows=3, max_length=FAR)
+    _attend_case([200, 90], [50, 90], 4, 2, 128, 16, "float16", max_queries=49, max_length=FAR)
+    # long enough by themselves, and cut by the bound
+    _attend_case([2600, 2100], [300, 290], 8, 2, 64, 64, "float16", max_length=2000)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_attention_of_many_rows_without_a_join(gpu, dtype):
+    """Enough sequences and heads that no split is made: rows leave through LDS."""
+    _attend_case([20 + 31 * i for i in range(8)], [20 + 25 * i for i in range(8)], 32, 32, 64, 16, dtype, max_length=FAR)
+
+
 def test_attention_in_far_slots(gpu):
     """Pages whose bytes lie past 2^32: a cache of 4.5 GiB of keys."""
     heads, page, dim = 1, 256, 256
