@@ -12,10 +12,10 @@
 // One pass: a thread keeps its part of the row in registers between the
 // statistics and the codes, so each input is read once and each output
 // written once.  Bound by HBM: 8190 x 4096 of bf16 with a residual, 235 MB, in
-// 45 us (5.2 TB/s), its codes back to values, 101 MB, in 18 (5.5 TB/s); a few
-// rows by the launch (4 x 2048: 3.3 us and 2.0).  Rows of odd lengths lie at
-// any alignment and are read 16 bytes a lane all the same, the row's end moved
-// into place: 1596 x 9233 51 us, 100 an element at a time.
+// 44 us (5.3 TB/s), its codes back to values, 101 MB, in 16.5 (6.1 TB/s); a
+// few rows by the launch (4 x 2048: 3.3 us and 2.0).  Rows of odd lengths lie
+// at any alignment and are read 16 bytes a lane all the same, the row's end
+// moved into place: 1596 x 9233 and back 35 us, 100 an element at a time.
 #include <type_traits>
 
 #include "decoder.hpp"
