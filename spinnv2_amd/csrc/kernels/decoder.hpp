@@ -19,7 +19,6 @@ typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef int intx4 __attribute__((ext_vector_type(4)));
-typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWave = 64;
@@ -166,7 +165,6 @@ inline int unsupported(const char *text) {
     return SPKV2_E_UNSUPPORTED;
 }
 inline bool is_dtype(int d) { return d == SPKV2_DTYPE_FP32 || d == SPKV2_DTYPE_FP16 || d == SPKV2_DTYPE_BF16; }
-inline size_t dtype_size(int d) { return d == SPKV2_DTYPE_FP32 ? 4 : 2; }
 inline bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 // (mul, shift) with n / d = n mul >> shift for 0 <= n < 2^31, d >= 1: mul =
