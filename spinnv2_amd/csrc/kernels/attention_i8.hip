@@ -95,7 +95,7 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
     Sequence s;
     const int o0 = a.offsets[b], o1 = a.offsets[b + 1];
-    s.true_length = a.lengths[b];
+    s.true_length = max(a.lengths[b], 0);
     s.row0 = o0;
     s.count = min(o1 - o0, a.max_queries);
     if (o0 < 0) s.count = 0;
@@ -105,6 +105,14 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
     s.length = max(0, min(s.true_length, a.max_length));
     if (s.length > held) s.length = static_cast<int>(held);
     return s;
+}
+
+// The first token that the window leaves to the query at `position`; 0 where
+// there is none.  No difference is formed that could pass 32 bits: with a window
+// of 2^31 - 1 and a query ahead of the first token it would turn into a token far
+// past the table.
+__device__ __forceinline__ int window_from(const AttnArgs &a, int position) {
+    return a.causal && a.window && position >= a.window ? position + 1 - a.window : 0;
 }
 
 // A split in which rows r0 .. r1 read no token: no sums, and a total of 0.
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
     int low = split * a.split_tokens, high = min(s.length, low + a.split_tokens);
     if (a.causal) {
         high = min(high, s.position + last_q + 1);
-        if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+        low = max(low, window_from(a, s.position + first_q));
     }
 
     if (a.splits > 1 && low >= high) {
@@ -247,7 +255,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
         const int r = r0 + col, i = r / a.group;
         const bool in = r < rows;
         last = a.causal ? s.position + i : s.length - 1;
-        start = a.causal && a.window ? last + 1 - a.window : 0;
+        start = window_from(a, last);
         // without a branch, so that all loads are on their way at once: rows past the last are the last
         const int rq = min(r, rows - 1), iq = rq / a.group;
         const T *q = static_cast<const T *>(a.q) + (s.row0 + iq) * a.q_stride +
@@ -468,7 +476,7 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     int low = split * a.split_tokens, high = min(s.length, low + a.split_tokens);
     if (a.causal) {
         high = min(high, s.position + last_q + 1);
-        if (a.window) low = max(low, s.position + first_q + 1 - a.window);
+        low = max(low, window_from(a, s.position + first_q));
     }
 
     if (a.splits > 1 && low >= high) {
@@ -480,10 +488,10 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     const int w0 = r0 + 32 * wave, r = w0 + col, i = r / a.group, q_head = head * a.group + (r - i * a.group);
     const bool in = r < rows;
     const int last = a.causal ? s.position + i : s.length - 1;
-    const int start = a.causal && a.window ? last + 1 - a.window : 0;
+    const int start = window_from(a, last);
     const int wave_first = w0 / a.group, wave_last = (min(rows, w0 + 32) - 1) / a.group;  // queries
     // tokens that all of the wave's rows read
-    const int all_from = a.causal && a.window ? s.position + wave_last + 1 - a.window : 0;
+    const int all_from = window_from(a, s.position + wave_last);
     const int all_to = a.causal ? s.position + wave_first + 1 : s.length;
 
     half8_t qf[DP / 16][kParts];
