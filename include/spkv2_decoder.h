@@ -152,11 +152,13 @@ int spkv2_mi355x_kv_read_i8(const Spkv2KvCacheI8 *cache, const Spkv2KvRead *args
  * zeros.  Tokens past a table's end, or on a page that the cache does not
  * have, are as masked.
  * The cached codes are read as 16-bit floats, exactly; queries are held with
- * 11 bits relative to themselves (22 for fp32 rows), softmax weights times
- * their tokens' value scales too, sums and softmax statistics are fp32.  Value
- * scales are meant to lie between 2^-96 and 2^96; smaller ones lose bits.  A
- * token whose key or value scale is not finite makes the rows that read it
- * NaN, and no other.
+ * 11 bits (22 for fp32 rows), and to within 2^-39 of their row's largest
+ * element; softmax weights times their tokens' value scales with as many, and
+ * to within 2^-28 of the largest of those that the row reads; sums and softmax
+ * statistics are fp32.  Value scales are meant to lie between 2^-96 and 2^96;
+ * smaller ones lose bits.  A token whose key or value scale is not finite makes
+ * the rows that read it NaN, and no other; what a row does not read changes no
+ * bit of it.
  *
  * max_queries and max_length bound the sequences' counts of queries and
  * lengths; what a sequence has beyond them is not computed (queries) or not

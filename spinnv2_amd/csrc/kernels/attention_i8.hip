@@ -24,7 +24,7 @@ struct AttnArgs {
     const void *q;
     void *out;
     const int32_t *table, *lengths, *offsets;
-    float *part, *stats;  // [row][split][head_dim] sums, [row][split][2] maximum and total; row = row of q * heads + head
+    float *part, *stats;  // [row][split][head_dim] sums, [row][split][2] base and total; row = row of q * heads + head
     int64_t queries, q_stride, out_stride;
     int max_queries, max_length, table_width, heads, group, sequences;
     int causal, window;
@@ -35,10 +35,16 @@ struct AttnArgs {
 };
 
 constexpr int kChunk = 32;   // tokens a wave takes at a time, as two tiles of 16
-// The running maximum of a row follows its scores only when one passes it by
-// more than 2^kSlack; weights are held as kLift p in fp16, below 2^15.
-constexpr float kSlack = 8.0f;
-constexpr float kLift = 128.0f;
+// A row's weights are 2^(score - base), and times their tokens' value scales
+// (their size) they are fp16.  The base is kLift below the largest size so far,
+// and follows it only when one passes it by kSlack more: sizes stay below 2^15,
+// and the largest at 2^7 or more (2^3 where it is bounded by a tile's largest
+// value scale).  So the base goes by what the row itself reads: neither a token
+// that its mask leaves out, nor one of large values and next to no weight, costs
+// it bits.
+constexpr float kSlack = 8.0f, kLift = 7.0f;
+// the least logarithm of a value scale: 2^(score - base) stays a float
+constexpr float kLeastLog = -96.0f;
 
 // Two codes of a dword, picked by `sel` into the low bytes of two halves, as
 // fp16: 0x6400 + (code + 128) is 1024 + 128 + code.
@@ -79,10 +85,15 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// The exponent of a power of two above a value scale.  Scales below 2^-96 share
-// one, under which their weights lose low bits: 2^7 / unit has to stay a float.
-__device__ __forceinline__ int unit_exponent(float scale) {
-    return min(max(static_cast<int>(__float_as_uint(scale) >> 23) - 126, -96), 127);
+// log2 of a value scale, kLeastLog at least.  Infinity or NaN gives what fmaxf
+// passes over beside a masked token's score of -infinity.
+__device__ __forceinline__ float log_scale(float scale) { return fmaxf(__builtin_amdgcn_logf(fabsf(scale)), kLeastLog); }
+
+// Sums relative to `from`, now relative to `to`: a factor that is applied twice,
+// since 2^(from - to) may be 0 where the totals of tokens with tiny values still
+// count.
+__device__ __forceinline__ float half_ratio(float from, float to) {
+    return from > -__builtin_inff() ? __builtin_amdgcn_exp2f((from - to) * 0.5f) : 0.0f;
 }
 
 struct Sequence {
@@ -107,12 +118,12 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs &a, int b) {
     return s;
 }
 
-// The first token that the window leaves to the query at `position`; 0 where
-// there is none.  No difference is formed that could pass 32 bits: with a window
+// The first token that the window (causal calls only have one) leaves to the
+// query at `position`; 0 without one.  No difference is formed that could pass 32 bits: with a window
 // of 2^31 - 1 and a query ahead of the first token it would turn into a token far
 // past the table.
 __device__ __forceinline__ int window_from(const AttnArgs &a, int position) {
-    return a.causal && a.window && position >= a.window ? position + 1 - a.window : 0;
+    return a.window && position >= a.window ? position + 1 - a.window : 0;
 }
 
 // A split in which rows r0 .. r1 read no token: no sums, and a total of 0.
@@ -289,8 +300,6 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
 #pragma unroll
         for (int j = 0; j < kVpl; j++) acc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float unit = 0.0f, per_unit = 0.0f;  // a power of two no value scale is above, and kLift / unit
-
     auto use = [&](const Chunk &x, int at) {
         floatx4 sc[2];
         sc[0] = sc[1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -305,42 +314,26 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
                         for (int w = 0; w < kParts; w++)
                             sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[2 * p + e][w], sc[h], 0, 0, 0);
                 }
-        // value scales: those of masked tokens may be anything in the cache
-        float vs[8];
-        float top = 0.0f;
-        const bool whole = at >= low && at + kChunk <= high && x.ok[0] && x.ok[1];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int token = at + 16 * (e / 4) + 4 * g + e % 4;
-            vs[e] = whole || (token >= low && token < high && x.ok[e / 4]) ? x.vs[e / 4][e % 4] : 0.0f;
-            if (vs[e] < __builtin_inff()) top = fmaxf(top, vs[e]);
-        }
-        if (__any(top > unit)) {
-            const float now = ldexpf(1.0f, unit_exponent(fmaxf(over_groups_max(top), unit)));
-            const float ratio = unit / now;
-            unit = now;
-            per_unit = kLift / now;
-#pragma unroll
-                for (int j = 0; j < kVpl; j++) acc[j] *= ratio;
-        }
         half8_t pf[kParts];
         {
-            float v[8], most = -__builtin_inff();
+            float v[8], most = -__builtin_inff();  // the largest size, as a logarithm
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int token = at + 16 * (e / 4) + 4 * g + e % 4;
                 v[e] = sc[e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor);
                 const bool keep = token >= low && token < high && x.ok[e / 4] && token <= last && token >= start;
                 v[e] = keep ? v[e] : -__builtin_inff();
-                most = fmaxf(most, v[e]);
+                most = fmaxf(most, v[e] + log_scale(x.vs[e / 4][e % 4]));
             }
-            if (__any(most > m + kSlack)) {
-                const float now = fmaxf(m, over_groups_max(most));
-                const float ratio = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - now) : 0.0f;
+            if (__any(most > m + (kLift + kSlack))) {
+                // a row whose own sizes have not passed keeps its base
+                most = over_groups_max(most);
+                const float now = most > m + (kLift + kSlack) ? most - kLift : m;
+                const float half = half_ratio(m, now);
                 m = now;
-                l *= ratio;
+                l = l * half * half;
 #pragma unroll
-                for (int j = 0; j < kVpl; j++) acc[j] *= ratio;
+                for (int j = 0; j < kVpl; j++) acc[j] *= half * half;
             }
             const float from = m > -__builtin_inff() ? m : 0.0f;
 #pragma unroll
@@ -348,7 +341,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
                 const float p = __builtin_amdgcn_exp2f(v[e] - from);
                 l += p;
                 // 0 where the row masks the token, whose scale may be NaN
-                float w = v[e] == -__builtin_inff() ? 0.0f : p * (vs[e] * per_unit);
+                float w = v[e] == -__builtin_inff() ? 0.0f : p * x.vs[e / 4][e % 4];
                 if constexpr (kWide) once(w);
                 const _Float16 hi = static_cast<_Float16>(w);
                 pf[0][e] = hi;
@@ -376,7 +369,6 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
     }
 
     // the waves' sums, joined in wave order
-    const float back = unit / kLift;
     {
         l = over_groups_sum(l);
         if (g == 0) {
@@ -393,10 +385,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
         float total = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
-            const float r = none ? 1.0f : __builtin_amdgcn_exp2f(wave_max[w][col] - most);
-            total += r * wave_sum[w][col];
+            const float half = none ? 1.0f : half_ratio(wave_max[w][col], most);
+            total += wave_sum[w][col] * half * half;
         }
-        const float mine = (none ? 1.0f : __builtin_amdgcn_exp2f(m - most)) * back;
+        const float mine = none ? 1.0f : __builtin_amdgcn_exp2f(m - most);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -452,7 +444,7 @@ constexpr int kTile = 64;  // tokens
 // the same order: the 16 tokens of a product as 0-3, 8-11 (lanes 0 .. 31), 4-7,
 // 12-15 (lanes 32 .. 63).
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) attend_tiles(AttnArgs a) {
+__global__ void __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) attend_tiles(AttnArgs a) {
     constexpr bool kWide = sizeof(T) == 4;
     constexpr int kParts = kWide ? 2 : 1;
     // 16 bytes past each row: any 16 rows' pieces of one column lie on different banks
@@ -460,7 +452,7 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     constexpr int kK = kTile * kKPitch, kV = DP * kVPitch;  // bytes
     constexpr int kKItems = (DP + 63) / 64, kVItems = (DP / 2 + 63) / 64;
     __shared__ __align__(16) int8_t lds[2 * (kK + kV)];
-    __shared__ __align__(16) float scales[2][4][kTile];  // keys', values', and twice what no one reads
+    __shared__ __align__(16) float scales[2][4][kTile];  // keys', values', what no one reads, log_scale() of the values'
     __shared__ __align__(16) unsigned held[2][4];  // kThere, and a bit for each of 16 tokens
     constexpr unsigned kThere = 1u << 16;
 
@@ -532,10 +524,10 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     for (int j = 0; j < DP / 32; j++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[j][e] = 0.0f;
-    // Weights are held as 2^base p in fp16, base = 7 - log2(unit) with `unit` a
-    // power of two that no value scale reaches, so that a weight times its
-    // token's scale stays below 2^15; sums and totals carry the same factor.
-    float m = -__builtin_inff(), l = 0.0f, unit = 0.0f, base = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+    // A power of two above the value scales of a tile that every row of the wave reads, and its logarithm: what bounds
+    // the sizes of every such tile whose scales lie between a sixteenth of it and itself, without a sum for each score.
+    float top_scale = 0.0f, top_log = kLeastLog;
 
     struct Stage {
         uintx4 k[kKItems];
@@ -611,7 +603,8 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
         // a value's scale that is not finite is one of the bits of `held`, and 0 in the product
         const bool odd = (lane & 16) && !(fabsf(x.scale) < __builtin_inff());
         const unsigned odds = static_cast<unsigned>(__ballot(odd)) >> 16;
-        scales[buffer][lane / 16][16 * wave + lane % 16] = odd ? 0.0f : x.scale;
+        const float scale = odd ? 0.0f : x.scale;
+        scales[buffer][lane / 16][16 * wave + lane % 16] = lane < 48 ? scale : log_scale(scale);
         held[buffer][wave] = there(page) ? kThere | odds : 0;
 #pragma unroll
         for (int n = 0; n < kVItems; n++) {
@@ -695,24 +688,39 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 #pragma unroll
             for (int e = 0; e < 16; e++) most = fmaxf(most, sc[t][e]);
         const float value = scales[buffer][1][lane];
-        if (__any(most * factor > m + kSlack || value > unit)) {
-            float up = value;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) up = fmaxf(up, __shfl_xor(up, d));
-            const float now = fmaxf(m, fmaxf(most, __shfl_xor(most, 32)) * factor);
-            float ratio = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - now) : 0.0f;
-            m = now;
-            if (up > unit) {
-                const int ex = unit_exponent(up);
-                ratio *= __builtin_amdgcn_exp2f(7.0f - static_cast<float>(ex) - base);
-                unit = ldexpf(1.0f, ex);
-                base = 7.0f - static_cast<float>(ex);
+        const auto fits = [&]() { return value <= top_scale && value * 16.0f >= top_scale; };
+        float size = __builtin_fmaf(most, factor, top_log);
+        if (!clear || __any(!fits() || size > m + (kLift + kSlack))) {
+            bool even = clear && __all(fits());
+            if (clear && !even) {
+                const unsigned half = max_over<32>(abs_bits(value));
+                const unsigned up = max(__builtin_amdgcn_readlane(half, 0), __builtin_amdgcn_readlane(half, 32));
+                top_log = ceilf(log_scale(__uint_as_float(up)));
+                top_scale = ldexpf(1.0f, static_cast<int>(top_log));
+                size = __builtin_fmaf(most, factor, top_log);
+                even = __all(fits());
             }
-            l *= ratio;
+            if (!even) {
+                size = -__builtin_inff();
 #pragma unroll
-            for (int j = 0; j < DP / 32; j++) acc[j] *= ratio;
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const floatx4 logs = *reinterpret_cast<const floatx4 *>(&scales[buffer][3][32 * t + 2 * e + 4 * h]);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) size = fmaxf(size, __builtin_fmaf(sc[t][e + u], factor, logs[u]));
+                    }
+            }
+            // a row whose own sizes have not passed keeps its base
+            size = fmaxf(size, __shfl_xor(size, 32));
+            const float now = size > m + (kLift + kSlack) ? size - kLift : m;
+            const float half = half_ratio(m, now);
+            m = now;
+            l = l * half * half;
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) acc[j] *= half * half;
         }
-        const float from = m > -__builtin_inff() ? base - m : 0.0f;
+        const float from = m > -__builtin_inff() ? -m : 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -758,19 +766,17 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
     l += __shfl_xor(l, 32);
     if (a.splits > 1) {
         if (!in) return;
-        // totals and sums without 2^base, which is this split's own
-        const float back = __builtin_amdgcn_exp2f(-base);
         const int64_t at_row = ((s.row0 + i) * a.heads + q_head) * a.splits + split;
 #pragma unroll
         for (int q = 0; q < DP / 32; q++)
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const int d = 32 * q + 16 * h + 4 * u;
-                if (d < dim) *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d) = floatx4{sum(q, u, 0), sum(q, u, 1), sum(q, u, 2), sum(q, u, 3)} * back;
+                if (d < dim) *reinterpret_cast<floatx4 *>(a.part + at_row * dim + d) = floatx4{sum(q, u, 0), sum(q, u, 1), sum(q, u, 2), sum(q, u, 3)};
             }
         if (h == 0) {
             a.stats[2 * at_row] = m;
-            a.stats[2 * at_row + 1] = l * back;
+            a.stats[2 * at_row + 1] = l;
         }
         return;
     }
@@ -804,7 +810,7 @@ __global__ void __launch_bounds__(256, DP > 128 || sizeof(T) == 4 ? 1 : 2) atten
 }
 
 // A wave a row of q and head: its splits' sums, joined in their order.  A lane
-// takes one split's maximum and total, so that these come by one load, and four
+// takes one split's base and total, so that these come by one load, and four
 // splits' sums at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
@@ -822,17 +828,17 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
     const bool none = !(most > -__builtin_inff());
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
     for (int p0 = 0; p0 < a.splits; p0 += 64) {
-        float share = 0.0f, sum = 0.0f;
+        float half = 0.0f, sum = 0.0f;
         if (p0 + lane < a.splits) {
             sum = a.stats[2 * (at + p0 + lane) + 1];
-            share = none ? 1.0f : __builtin_amdgcn_exp2f(a.stats[2 * (at + p0 + lane)] - most);
+            half = none ? 1.0f : half_ratio(a.stats[2 * (at + p0 + lane)], most);
         }
         const int end = min(64, a.splits - p0);
         for (int p = 0; p < end; p += 4) {
             float part[4][4], r[4], c[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                r[u] = __shfl(share, p + u);
+                r[u] = __shfl(half, p + u);
                 c[u] = __shfl(sum, p + u);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -844,7 +850,8 @@ __global__ void __launch_bounds__(256) join_splits(AttnArgs a) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 if (c[u] == 0.0f) continue;
-                total += r[u] * c[u];
+                total += c[u] * r[u] * r[u];
+                r[u] *= r[u];
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[e] += r[u] * part[u][e];
             }

@@ -4,9 +4,13 @@ kernels.  References in 64 bits or in whole numbers, as in test_gpu_decoder."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
-from .test_gpu_decoder import FAR, _attend_case
+from spinnv2_amd import decoder
+from spinnv2_amd.decoder import DeviceArray as Array, KvCache
+
+from .test_gpu_decoder import FAR, HALF, _attend_case, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +24,91 @@ def test_attention_in_a_window_past_every_token(gpu, window, dtype):
     for bound in ({}, {"max_length": FAR}):
         _attend_case([1, 40, 9, 70], [5, 12, 41, 70], 4, 2, 64, 16, dtype, window=window, **bound)
     _attend_case([1, 700], [1, 1], 4, 2, 64, 16, dtype, window=window)
+
+
+def _cached(lengths, kv, dim, page, seed=3):
+    rng = np.random.default_rng(seed)
+    need = [max(1, -(-n // page)) for n in lengths]
+    pages = sum(need) + 1
+    codes = [np.clip(np.rint(rng.standard_normal((pages, kv, page, dim)) * 45), -127, 127).astype(np.int8) for _ in range(2)]
+    scales = [(0.01 + 0.01 * rng.random((pages, kv, page))).astype(np.float32) for _ in range(2)]
+    order = rng.permutation(pages - 1).astype(np.int32) + 1
+    table, at = np.zeros((len(lengths), max(need)), np.int32), 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+    return codes, scales, table
+
+
+def _attend(codes, scales, table, lengths, counts, q, dtype, bound, **kw):
+    """out [queries, heads, dim] of one call"""
+    cache = KvCache(*(Array.of(v) for v in codes + scales))
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    kw |= dict(max_queries=max(counts), max_length=bound or max(lengths))
+    size = decoder.attention_workspace(len(lengths), len(q), q.shape[1], cache, max_queries=kw["max_queries"], max_length=kw["max_length"])
+    out = Array(q.shape, dtype)
+    decoder.attention(Array.of(q, dtype), cache, Array.of(table), Array.of(np.array(lengths, np.int32)), Array.of(offsets), out,
+                      workspace=Array((size,), "int8") if size else None, **kw)
+    return out.download()
+
+
+# counts, lengths and max_length (0: the longest): single tokens without and with splits, few and many rows, many rows with splits
+FORMS = [([1, 1], [200, 90], 0), ([1, 1], [2000, 1500], 0), ([40, 90], [100, 90], 0), ([40, 90], [100, 90], FAR),
+         ([300, 150], [700, 400], 1 << 15)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("window", [0, 30])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_does_not_depend_on_what_is_not_read(gpu, counts, lengths, bound, window, dtype):
+    """The same bits whatever the value scales of tokens behind a row's own, or ahead of its window."""
+    heads, kv, dim, page = 4, 2, 64, 16
+    codes, scales, table = _cached(lengths, kv, dim, page)
+    q = rounded(np.random.default_rng(1).standard_normal((sum(counts), heads, dim)), dtype)
+    plain = _attend(codes, scales, table, lengths, counts, q, dtype, bound, window=window)
+    for size in (2.0 ** 30, 2.0 ** 60):
+        changed = [scales[0], scales[1].copy()]
+        at = [n - 1 if c > 1 else n // 2 for n, c in zip(lengths, counts)]
+        for i, t in enumerate(at):
+            changed[1][table[i, t // page], :, t % page] *= np.float32(size)
+        got = _attend(codes, changed, table, lengths, counts, q, dtype, bound, window=window)
+        row = 0
+        for n, c, t in zip(lengths, counts, at):
+            place = np.arange(n - c, n)
+            reads = (place >= t) & ((place < t + window) if window else True)
+            np.testing.assert_array_equal(got[row:row + c][~reads], plain[row:row + c][~reads])
+            row += c
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_with_values_of_very_different_sizes(gpu, counts, lengths, bound, dtype):
+    """One token's values are far larger than the others', its weight next to nothing."""
+    for size in (2.0 ** 20, 2.0 ** 32):
+        def edit(q, codes, scales, table):
+            np.abs(q, out=q)
+            for i, n in enumerate(lengths):
+                p, r = table[i, (n // 3) // 16], (n // 3) % 16
+                codes[0][p, :, r] = -127
+                scales[0][p, :, r] = 0.25  # scores below -100
+                scales[1][p, :, r] *= np.float32(size)
+
+        got, want = _attend_case(lengths, counts, 4, 2, 64, 16, dtype, edit=edit, **({"max_length": bound} if bound else {}))
+        # values of the others: 127 times 0.02 at most; weights of 11 or 22 bits (2^-11, 2^-23), their scores (2^-14.4), sums of up to 2000 tokens (2^-12)
+        off = 127 * 0.02 * (2.0 ** -11 if dtype == "float32" else 2.0 ** -10) + HALF[dtype] * np.abs(want) + 2.0 ** -24
+        assert (np.abs(got - want) <= off).all(), float((np.abs(got - want) / off).max())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_with_small_values_first(gpu, counts, lengths, bound, dtype):
+    """The first tokens' values are tiny, or zero, and count among the weights all the same."""
+    for small, large in ((2.0 ** -80, 2.0 ** 8 if dtype == "float16" else 2.0 ** 55), (0.0, 2.0 ** 8 if dtype == "float16" else 2.0 ** 55), (2.0 ** -80, 1.0)):
+        def edit(q, codes, scales, table):
+            first = np.zeros(scales[1].shape, bool)
+            for i, n in enumerate(lengths):
+                for t in range(n // 2):
+                    first[table[i, t // 16], :, t % 16] = True
+            scales[1][:] = np.where(first, scales[1] * np.float32(small), scales[1] * np.float32(large))
+
+        _attend_case(lengths, counts, 4, 2, 64, 16, dtype, edit=edit, **({"max_length": bound} if bound else {}))
