@@ -317,10 +317,20 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
         half8_t pf[kParts];
         {
             float v[8], most = -__builtin_inff();  // the largest size, as a logarithm
+            unsigned widest = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] = sc[e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor);
+                widest = max(widest, max(abs_bits(x.ks[e / 4][e % 4]), abs_bits(x.vs[e / 4][e % 4])));
+            }
+            if (__any(widest >= kInfBits)) {  // an infinite key scale may have given -infinity, which stands for masked
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (max(abs_bits(x.ks[e / 4][e % 4]), abs_bits(x.vs[e / 4][e % 4])) >= kInfBits) v[e] = __builtin_nanf("");
+            }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int token = at + 16 * (e / 4) + 4 * g + e % 4;
-                v[e] = sc[e / 4][e % 4] * (x.ks[e / 4][e % 4] * factor);
                 const bool keep = token >= low && token < high && x.ok[e / 4] && token <= last && token >= start;
                 v[e] = keep ? v[e] : -__builtin_inff();
                 most = fmaxf(most, v[e] + log_scale(x.vs[e / 4][e % 4]));
@@ -600,9 +610,9 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) attend_tile
             for (int e = 0; e < 2; e++)
                 *reinterpret_cast<half8_t *>(k + (16 * wave + at) * kKPitch + (piece + e) * 16) = codes8(x.k[n][2 * e], x.k[n][2 * e + 1]);
         }
-        // a value's scale that is not finite is one of the bits of `held`, and 0 in the product
-        const bool odd = (lane & 16) && !(fabsf(x.scale) < __builtin_inff());
-        const unsigned odds = static_cast<unsigned>(__ballot(odd)) >> 16;
+        // a token with a scale that is not finite is one of the bits of `held`, and the scale 0 in the product
+        const bool odd = !(fabsf(x.scale) < __builtin_inff());
+        const unsigned both = static_cast<unsigned>(__ballot(odd)), odds = (both | both >> 16) & (kThere - 1);
         const float scale = odd ? 0.0f : x.scale;
         scales[buffer][lane / 16][16 * wave + lane % 16] = lane < 48 ? scale : log_scale(scale);
         held[buffer][wave] = there(page) ? kThere | odds : 0;

@@ -112,3 +112,32 @@ def test_attention_with_small_values_first(gpu, counts, lengths, bound, dtype):
             scales[1][:] = np.where(first, scales[1] * np.float32(small), scales[1] * np.float32(large))
 
         _attend_case(lengths, counts, 4, 2, 64, 16, dtype, edit=edit, **({"max_length": bound} if bound else {}))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_with_infinite_scales(gpu, counts, lengths, bound, value, which, dtype):
+    """As NaN: the rows that read the token are NaN, also where its score would be -inf, and the others have the bits that they have without it."""
+    heads, kv, dim, page = 4, 2, 64, 16
+    codes, scales, table = _cached(lengths, kv, dim, page)
+    rng = np.random.default_rng(1)
+    q = np.abs(rounded(rng.standard_normal((sum(counts), heads, dim)), dtype))
+    at = [n // 2 for n in lengths]
+    for i, t in enumerate(at):
+        codes[0][table[i, t // page], :, t % page] = np.where(np.arange(kv) % 2, 100, -100)[:, None]  # scores of both signs
+    plain = _attend(codes, scales, table, lengths, counts, q, dtype, bound)
+    got = []
+    for v in (np.nan, value):
+        changed = [s.copy() for s in scales]
+        for i, t in enumerate(at):
+            changed[which][table[i, t // page], :, t % page] = v
+        got.append(_attend(codes, changed, table, lengths, counts, q, dtype, bound))
+    np.testing.assert_array_equal(got[1], got[0])
+    row = 0
+    for n, c, t in zip(lengths, counts, at):
+        reads = np.arange(n - c, n) >= t
+        assert np.isnan(got[0][row:row + c][reads]).all()
+        np.testing.assert_array_equal(got[0][row:row + c][~reads], plain[row:row + c][~reads])
+        row += c
