@@ -284,6 +284,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP * sizeof(T) <= 256 ? 12 / WAVES
             }
         }
         top = over_groups_max(top);
+        // an infinite query's scores are not finite whatever the codes, and all of -infinity would read as masked
+        if (top == __builtin_inff()) f[0][0] = __builtin_nanf("");
         const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
         factor = ldexpf(a.scale * 1.44269504088896340736f, ex - 14);
 #pragma unroll
@@ -515,6 +517,8 @@ __global__ void __launch_bounds__(256, DP * sizeof(T) > 256 ? 1 : 2) attend_tile
             }
         }
         top = fmaxf(top, __shfl_xor(top, 32));
+        // an infinite query's scores are not finite whatever the codes, and all of -infinity would read as masked
+        if (top == __builtin_inff()) f[0][0] = __builtin_nanf("");
         const int ex = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
         const bool negative = a.scale < 0.0f;  // q takes the sign, so that the largest score has the largest product
         // above zero, since masked scores are -inf times it

@@ -141,3 +141,20 @@ def test_attention_with_infinite_scales(gpu, counts, lengths, bound, value, whic
         assert np.isnan(got[0][row:row + c][reads]).all()
         np.testing.assert_array_equal(got[0][row:row + c][~reads], plain[row:row + c][~reads])
         row += c
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_of_infinite_queries(gpu, counts, lengths, bound, dtype):
+    """A query with an infinity gives NaN, also where all of its scores are -infinity, and zeros where it reads nothing."""
+    heads, kv, dim, page = 4, 2, 64, 16
+    codes, scales, table = _cached(lengths, kv, dim, page)
+    codes[0][..., 7] = -np.abs(codes[0][..., 7]) - 1
+    q = rounded(np.random.default_rng(1).standard_normal((sum(counts), heads, dim)), dtype)
+    plain = _attend(codes, scales, table, lengths, counts, q, dtype, bound)
+    q[::2, 1, 7] = np.inf
+    got = _attend(codes, scales, table, lengths, counts, q, dtype, bound)
+    assert np.isnan(got[::2, 1]).all()
+    got[::2, 1] = plain[::2, 1]
+    np.testing.assert_array_equal(got, plain)
+    assert (_attend(codes, scales, table, [0 for n in lengths], counts, q, dtype, bound or max(lengths)) == 0).all()
