@@ -118,8 +118,9 @@ __device__ __forceinline__ uint64_t abs_bits(double x) {
 // x, 127 / top and their product each rounded to fp32, t is within 127 * 4 *
 // 2^-24 < 2^-15 of the quotient, so it has the quotient's nearest integer
 // unless it lies within 2^-14 of the border of two.  One value in eight
-// thousand does, and where 127 / top or a wide x leaves fp32's range all do
-// (t is then infinite or NaN): those are divided in 64 bits.
+// thousand does, and where 127 / top or a wide x leaves fp32's range all do (t
+// is then infinite or NaN): those are divided in 64 bits, and so is every value
+// where a wide top passes fp32's range, 127 / top is 0 and t says nothing.
 template <int N, typename P>
 __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N]) {
     const float inv = 127.0f / static_cast<float>(top);
@@ -129,7 +130,7 @@ __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N])
     for (int i = 0; i < N; i++) {
         const float t = static_cast<float>(x[i]) * inv;
         r[i] = rintf(t);
-        far[i] = fabsf(t - r[i]) < 0.5f - 0x1p-14f;
+        far[i] = inv > 0.0f && fabsf(t - r[i]) < 0.5f - 0x1p-14f;
         all &= far[i];
     }
     if (!all) {

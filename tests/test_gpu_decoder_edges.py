@@ -4,6 +4,8 @@ kernels.  References in 64 bits or in whole numbers, as in test_gpu_decoder."""
 
 from __future__ import annotations
 
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -13,6 +15,40 @@ from spinnv2_amd.decoder import DeviceArray as Array, KvCache
 from .test_gpu_decoder import FAR, HALF, _attend_case, rounded
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------- norm
+
+def _exact_codes(p, top):
+    """rint(127 p / top) in rationals: round() of a Fraction takes ties to the even one."""
+    return 0 if top == 0 else round(127 * Fraction(float(p)) / Fraction(float(top)))
+
+
+def _norm_exactly(h, w, dtype, weight_dtype, eps=0.0):
+    """h [rows, cols] and w [cols] hold values of their types; products of two of them are exact in float64."""
+    rows, cols = h.shape
+    q, s = Array((rows, cols), "int8"), Array((rows,), "float32")
+    decoder.rmsnorm_i8(Array.of(h, dtype), Array.of(w, weight_dtype), q, s, eps=eps)
+    p = h * w
+    top = np.abs(p).max(1)
+    codes = np.array([[_exact_codes(v, t) for v in row] for row, t in zip(p, top)])
+    np.testing.assert_array_equal(q.download(), codes)
+    want = top / 127 / np.sqrt((h * h).sum(1) / cols + eps)
+    np.testing.assert_allclose(s.download().astype(np.float64), want, rtol=2.0 ** -24 * 1.001 + cols * 2.0 ** -52, atol=2.0 ** -150)
+
+
+@pytest.mark.parametrize("dtype,weight_dtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float32")])
+@pytest.mark.parametrize("cols", [3, 40, 1003, 2056])
+def test_norm_of_products_past_float32(gpu, cols, dtype, weight_dtype):
+    """Rows whose largest product with the weights passes fp32's largest value, or is far below its smallest."""
+    rng = np.random.default_rng(cols)
+    sizes = np.array([2.0 ** 124, 2.0 ** 120, 2.0 ** -100, 1.0, 2.0 ** 60])[:, None] if dtype != "float16" else np.array([2.0 ** 13, 1.0, 2.0 ** -8])[:, None]
+    h = rounded(np.clip(rng.standard_normal((len(sizes), cols)), -7, 7) * sizes, dtype)
+    for w_size in (4.0, 2.0 ** -60) if dtype != "float16" else (2.0 ** 120, 2.0 ** -140):
+        w = rounded((1 + rng.random(cols)) * w_size, weight_dtype)
+        _norm_exactly(h, w, dtype, weight_dtype)
+    w = rounded(2.0 ** rng.uniform(-100, 20, cols), weight_dtype)
+    _norm_exactly(h, w, dtype, weight_dtype)
 
 
 # -------------------------------------------------------------- attention
