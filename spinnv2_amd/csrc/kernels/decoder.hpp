@@ -114,6 +114,17 @@ __device__ __forceinline__ uint64_t abs_bits(double x) {
     return static_cast<uint64_t>(__double_as_longlong(x)) & 0x7fffffffffffffffull;
 }
 
+// rint(127 x / top) in exact arithmetic, 0 <= x <= top, both of at most 48 bits
+// (products of two fp32 values).  127 x has up to 55 bits and a quotient may lie
+// closer to a border of two codes than a double tells, so only its integer part
+// n is taken from one; whether the border n + 1/2 is passed, (2 n + 1) top <
+// 254 x, is one fused product: 256 x - (2 n + 1) top is a multiple of 2^-47 of
+// x's power of two, so where it is near 2 x it has at most 50 bits and no rounding.
+__device__ __forceinline__ double exact_code(double x, double top) {
+    const double n = floor(x * 127.0 / top), rest = __builtin_fma(-(2.0 * n + 1.0), top, 256.0 * x);
+    return rest > 2.0 * x || (rest == 2.0 * x && (static_cast<int>(n) & 1)) ? n + 1.0 : n;
+}
+
 // Codes rint(127 x / top) of N values with |x| <= top, top > 0 finite.  With
 // x, 127 / top and their product each rounded to fp32, t is within 127 * 4 *
 // 2^-24 < 2^-15 of the quotient, so it has the quotient's nearest integer
@@ -136,7 +147,7 @@ __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N])
     if (!all) {
 #pragma unroll
         for (int i = 0; i < N; i++)
-            if (!far[i]) r[i] = static_cast<float>(rint(static_cast<double>(x[i]) * 127.0 / static_cast<double>(top)));
+            if (!far[i]) r[i] = static_cast<float>(copysign(exact_code(fabs(static_cast<double>(x[i])), static_cast<double>(top)), static_cast<double>(x[i])));
     }
 #pragma unroll
     for (int i = 0; i < N; i++) q[i] = static_cast<int8_t>(static_cast<int>(r[i]));

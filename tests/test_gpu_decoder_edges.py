@@ -51,6 +51,21 @@ def test_norm_of_products_past_float32(gpu, cols, dtype, weight_dtype):
     _norm_exactly(h, w, dtype, weight_dtype)
 
 
+# Whole numbers a b and c d whose quotient 127 a b / (c d) is a border of two codes, or less than 2^-52 of itself beside one.
+BORDERS = [(8940899, 9729239, 10614406, 10566517), (11295405, 9747045, 9645777, 13871550), (9160570, 12577316, 12957651, 10603233),
+           (14745699, 11389702, 14989556, 14745699), (14594146, 7324835, 12089229, 9639527), (12585681, 8392783, 12248134, 10790721)]
+
+
+@pytest.mark.parametrize("border", BORDERS)
+def test_norm_codes_next_to_a_border(gpu, border):
+    """127 a b has 55 bits: in float64 it is rounded past the border, or off it."""
+    a, b, c, d = border
+    h = np.array([[c, a, -a, 0, a, c, 1, 2, 3, 4], [-c, a, -a, 0, a, 0, 1, 2, 3, 4]], np.float64)
+    w = np.array([d, b, b, 1, -b, 1, 1, 1, 1, 1], np.float64)
+    _norm_exactly(h, w, "float32", "float32")
+    _norm_exactly(h * 2.0 ** -60, w * 2.0 ** -40, "float32", "float32")
+
+
 # -------------------------------------------------------------- attention
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
