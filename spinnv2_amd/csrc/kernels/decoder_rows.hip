@@ -7,7 +7,10 @@
 // The norm is one factor of the whole row, so it cancels out of q: the codes
 // are those of p = h w, and only the scale needs the sum of squares.  Codes
 // are therefore exact: of 16-bit rows p has at most 22 bits and is held in
-// fp32, with an fp32 factor in it at most 48, held in fp64.
+// fp32, with an fp32 factor in it at most 48, held in fp64.  A product of two
+// bf16 may leave fp32's range: a row whose largest does, or is so small that
+// others would lose bits that their codes need, is multiplied again in fp64
+// (8190 x 4096 and back takes 66.9 us so, 68.8 with fp64 for every row).
 //
 // One pass: a thread keeps its part of the row in registers between the
 // statistics and the codes, so each input is read once and each output
@@ -111,7 +114,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
         const int i = (c * THREADS + tid) * VEC;
         if (h && i < a.cols) store_some<VEC>(h + i, TAIL ? a.cols - i : VEC, f);
     };
-    auto products = [&](int c, const float(&f)[VEC], P(&p)[VEC]) {
+    auto products = [&](int c, const float(&f)[VEC], auto &p) {
+        using Q = std::decay_t<decltype(p[0])>;
         float g[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; j++) g[j] = 1.0f;
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
             settle<VEC, TAIL>((c * THREADS + tid) * VEC, a.cols, g);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; j++) p[j] = static_cast<P>(f[j]) * static_cast<P>(g[j]);
+        for (int j = 0; j < VEC; j++) p[j] = static_cast<Q>(f[j]) * static_cast<Q>(g[j]);
     };
     auto statistics = [&](int c, const float(&f)[VEC]) {
         P p[VEC];
@@ -170,50 +174,88 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
             top = tops[i] > top ? tops[i] : top;
         }
     }
-    constexpr U kInf = sizeof(U) == 8 ? static_cast<U>(0x7ff0000000000000ull) : static_cast<U>(kInfBits);
-    const bool finite = top < kInf;
-    const P amax = __builtin_bit_cast(P, top);
-    if (tid == 0) {
-        double s = static_cast<double>(amax) / 127.0;
-        if (a.norm) s /= sqrt(sum / a.cols + static_cast<double>(a.eps));
-        // 0 of a row of zeros, whose norm may be 0 / 0
-        a.scale[row] = !finite ? __builtin_nanf("") : top == 0 ? 0.0f : static_cast<float>(s);
-    }
-    auto codes = [&](int c, const float(&f)[VEC]) {
-        const int i = (c * THREADS + tid) * VEC;
-        P p[VEC];
-        products(c, f, p);
-        Vec<int8_t, VEC> out;
+    // chunk c of h once more
+    auto again = [&](int c, float(&f)[VEC]) {
+        if constexpr (CHUNKS > 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) out.v[j] = 0;
-        if (finite && top != 0) quantise<VEC>(p, amax, out.v);
-        if (i + VEC <= a.cols) {
-            __builtin_memcpy(q + i, out.v, VEC);
+            for (int j = 0; j < VEC; j++) f[j] = hv[c][j];
+        } else if (h) {
+            // read back where it was stored: x may have been overwritten by it
+            const int i = (c * THREADS + tid) * VEC;
+            // this thread's own elements: past them others may not have stored yet
+#pragma unroll
+            for (int j = 0; j < VEC; j++) f[j] = i + j < a.cols ? static_cast<float>(h[i + j]) : 0.0f;
         } else {
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (i + j < a.cols) q[i + j] = out.v[j];
+            Raw raw;
+            fetch(c, raw);
+            sum_up(c, raw, f);
         }
     };
-    if constexpr (CHUNKS > 0) {
+    auto over_row = [&](auto &&work) {
+        if constexpr (CHUNKS > 0) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c++) codes(c, hv[c]);
-    } else {
-        for (int c = 0; c < chunks; c++) {
-            // h is read back where it was stored: x may have been overwritten by it
-            Raw raw;
-            if (h) {
-                const int i = (c * THREADS + tid) * VEC;
-                // this thread's own elements: past them others may not have stored yet
+            for (int c = 0; c < CHUNKS; c++) work(c);
+        } else {
+            for (int c = 0; c < chunks; c++) work(c);
+        }
+    };
+    // the scale, and the codes of the products as Q
+    auto finish = [&](auto top) {
+        using Q = std::conditional_t<sizeof(top) == 8, double, float>;
+        constexpr auto kInf = sizeof(top) == 8 ? static_cast<decltype(top)>(0x7ff0000000000000ull) : static_cast<decltype(top)>(kInfBits);
+        const bool finite = top < kInf;
+        const Q amax = __builtin_bit_cast(Q, top);
+        if (tid == 0) {
+            double s = static_cast<double>(amax) / 127.0;
+            if (a.norm) s /= sqrt(sum / a.cols + static_cast<double>(a.eps));
+            // 0 of a row of zeros, whose norm may be 0 / 0
+            a.scale[row] = !finite ? __builtin_nanf("") : top == 0 ? 0.0f : static_cast<float>(s);
+        }
+        over_row([&](int c) {
+            const int i = (c * THREADS + tid) * VEC;
+            float f[VEC];
+            again(c, f);
+            Q p[VEC];
+            products(c, f, p);
+            Vec<int8_t, VEC> out;
 #pragma unroll
-                for (int j = 0; j < VEC; j++) hv[0][j] = i + j < a.cols ? static_cast<float>(h[i + j]) : 0.0f;
+            for (int j = 0; j < VEC; j++) out.v[j] = 0;
+            if (finite && top != 0) quantise<VEC>(p, amax, out.v);
+            if (i + VEC <= a.cols) {
+                __builtin_memcpy(q + i, out.v, VEC);
             } else {
-                fetch(c, raw);
-                sum_up(c, raw, hv[0]);
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if (i + j < a.cols) q[i + j] = out.v[j];
             }
-            codes(c, hv[0]);
+        });
+    };
+    if constexpr (std::is_same_v<P, float> && std::is_same_v<T, __bf16>) {
+        // Products below 2^-126 lose bits: next to a top of 2^-90 their codes are 0 all the same.  The row's
+        // threads have one top, and turn here together.
+        if (w && (top < __builtin_bit_cast(unsigned, 0x1p-90f) || top >= kInfBits)) {
+            uint64_t wide = 0;
+            over_row([&](int c) {
+                float f[VEC];
+                again(c, f);
+                double p[VEC];
+                products(c, f, p);
+#pragma unroll
+                for (int j = 0; j < VEC; j++) wide = max(wide, abs_bits(p[j]));
+            });
+            wide = wave_max(wide);
+            if constexpr (THREADS > kWave) {
+                __shared__ uint64_t wides[THREADS / kWave];
+                if ((tid & (kWave - 1)) == 0) wides[tid / kWave] = wide;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < THREADS / kWave; i++) wide = max(wide, wides[i]);
+            }
+            finish(wide);
+            return;
         }
     }
+    finish(top);
 }
 
 template <typename T, typename W>

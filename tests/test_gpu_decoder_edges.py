@@ -24,11 +24,14 @@ def _exact_codes(p, top):
     return 0 if top == 0 else round(127 * Fraction(float(p)) / Fraction(float(top)))
 
 
-def _norm_exactly(h, w, dtype, weight_dtype, eps=0.0):
+def _norm_exactly(h, w, dtype, weight_dtype, eps=0.0, in_place=False):
     """h [rows, cols] and w [cols] hold values of their types; products of two of them are exact in float64."""
     rows, cols = h.shape
     q, s = Array((rows, cols), "int8"), Array((rows,), "float32")
-    decoder.rmsnorm_i8(Array.of(h, dtype), Array.of(w, weight_dtype), q, s, eps=eps)
+    x, more = Array.of(h, dtype), {}
+    if in_place:
+        more = dict(residual=Array.of(np.zeros_like(h), dtype), residual_out=x)
+    decoder.rmsnorm_i8(x, Array.of(w, weight_dtype), q, s, eps=eps, **more)
     p = h * w
     top = np.abs(p).max(1)
     codes = np.array([[_exact_codes(v, t) for v in row] for row, t in zip(p, top)])
@@ -37,8 +40,8 @@ def _norm_exactly(h, w, dtype, weight_dtype, eps=0.0):
     np.testing.assert_allclose(s.download().astype(np.float64), want, rtol=2.0 ** -24 * 1.001 + cols * 2.0 ** -52, atol=2.0 ** -150)
 
 
-@pytest.mark.parametrize("dtype,weight_dtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float32")])
-@pytest.mark.parametrize("cols", [3, 40, 1003, 2056])
+@pytest.mark.parametrize("dtype,weight_dtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float32"), ("bfloat16", "bfloat16")])
+@pytest.mark.parametrize("cols", [3, 40, 1003, 2056, 17000])
 def test_norm_of_products_past_float32(gpu, cols, dtype, weight_dtype):
     """Rows whose largest product with the weights passes fp32's largest value, or is far below its smallest."""
     rng = np.random.default_rng(cols)
@@ -48,7 +51,7 @@ def test_norm_of_products_past_float32(gpu, cols, dtype, weight_dtype):
         w = rounded((1 + rng.random(cols)) * w_size, weight_dtype)
         _norm_exactly(h, w, dtype, weight_dtype)
     w = rounded(2.0 ** rng.uniform(-100, 20, cols), weight_dtype)
-    _norm_exactly(h, w, dtype, weight_dtype)
+    _norm_exactly(h, w, dtype, weight_dtype, in_place=True)
 
 
 # Whole numbers a b and c d whose quotient 127 a b / (c d) is a border of two codes, or less than 2^-52 of itself beside one.
