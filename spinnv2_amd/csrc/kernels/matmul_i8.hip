@@ -3,9 +3,11 @@
 //
 //   out[m, n] = sa[m] sb[n] sum_k a[m, k] b[n, k] + bias[n]
 //
-// int32 sums on the int8 matrix cores, exact whatever their order (127 128 2^17
-// < 2^31), scaled in fp32 and rounded once.  So every kernel here gives the
-// same bits, and which one runs is a question of time alone.
+// int32 sums on the int8 matrix cores, exact whatever their order, scaled in
+// fp32 and rounded once.  So every kernel here gives the same bits, and which
+// one runs is a question of time alone.  Up to k = 2^17 the sums lie between
+// -127 128 2^17 > -2^31 and 128 128 2^17 = 2^31: that one, of 2^17 products of
+// -128, is held as -2^31, which no other sum is.
 //
 // matmul_tiles serves many tokens: bound by the matrix cores (8192^3 in 470 us,
 // 2.3 POP/s, 66 us more than the time that its products take at the clock that
@@ -61,7 +63,8 @@ __device__ __forceinline__ intx4 behind(int cut) {
 }
 
 __device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
-    return __builtin_fmaf(static_cast<float>(sum) * sa, sb, bias);
+    const float x = sum == INT32_MIN ? 0x1p31f : static_cast<float>(sum);
+    return __builtin_fmaf(x * sa, sb, bias);
 }
 
 // LDS of one wave alone: its writes are done before its reads, and the other way round

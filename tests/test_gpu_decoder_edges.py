@@ -69,6 +69,20 @@ def test_norm_codes_next_to_a_border(gpu, border):
     _norm_exactly(h * 2.0 ** -60, w * 2.0 ** -40, "float32", "float32")
 
 
+# ---------------------------------------------------------------- product
+
+@pytest.mark.parametrize("m,n", [(2, 16), (70, 130), (300, 520), (1500, 1300)])
+def test_matmul_of_sums_of_2_to_the_31(gpu, m, n):
+    """2^17 products of -128 and -128: one more than int32 holds."""
+    k = 1 << 17
+    u, v = np.full(m, -128.0), np.full(n, -128.0)
+    u[0], v[n // 2] = 127, 127
+    a, b = (np.repeat(x.astype(np.int8)[:, None], k, 1) for x in (u, v))
+    out = Array((m, n), "float32")
+    decoder.matmul_i8(Array.of(a), Array.of(np.ones(m, np.float32)), Array.of(b), Array.of(np.ones(n, np.float32)), out)
+    np.testing.assert_array_equal(out.download(), np.outer(u, v) * k)
+
+
 # -------------------------------------------------------------- attention
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
