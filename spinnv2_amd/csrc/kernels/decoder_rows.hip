@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
     using P = typename Product<T, W>::type;
     using U = decltype(abs_bits(P{}));
     constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (kRows > 1 ? threadIdx.x / THREADS : 0);
-    if (kRows > 1 && row >= a.rows) return;
+    const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kRows + (kRows > 1 ? threadIdx.x / THREADS : 0);
+    if (row >= a.rows) return;  // whole waves, or workgroups
     const int tid = kRows > 1 ? threadIdx.x % THREADS : threadIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.r_stride : nullptr;
@@ -263,8 +263,10 @@ int launch_rows(const RowArgs &a, void *stream) {
     const char *what = "rmsnorm_i8";
     auto go = [&](auto kernel, int threads) {
         const int rows = threads < 256 ? 256 / threads : 1;
-        return launch(what, kernel, dim3(static_cast<unsigned>((a.rows + rows - 1) / rows)), dim3(threads < 256 ? 256 : threads),
-                      stream, a);
+        // a launch has fewer than 2^32 threads along an axis: up to 2^21 workgroups, then as many again
+        const int64_t blocks = (a.rows + rows - 1) / rows, x = std::min<int64_t>(blocks, 1 << 21);
+        return launch(what, kernel, dim3(static_cast<unsigned>(x), static_cast<unsigned>((blocks + x - 1) / x)),
+                      dim3(threads < 256 ? 256 : threads), stream, a);
     };
     // a wave a row up to 1024 elements: no barrier; then as few threads as hold
     // the row in three runs of 8, since the statistics' join grows with them and

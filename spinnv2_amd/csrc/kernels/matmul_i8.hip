@@ -446,7 +446,7 @@ int fastest(int64_t m, int64_t n, int64_t k, bool tiles) {
     for (int i = 0; i < 8; i++) {
         const Form &f = kForms[i];
         const int64_t down = (m + f.tokens - 1) / f.tokens, across = (n + f.channels - 1) / f.channels;
-        if (f.waves == 1 ? !tiles || down * across > 1 << 24 : down > 65535) continue;
+        if (f.waves == 1 ? !tiles || down * across >= 1 << 24 : down > 65535) continue;  // fewer than 2^32 threads along an axis
         const int64_t steps = ((k + 127) / 128 + f.waves - 1) / f.waves, each = (down * across + 255) / 256;
         const float time = f.launch + steps * std::max(f.step, each * f.work) + each * f.sums;
         if (least == 0.0f || time < least) least = time, best = i;

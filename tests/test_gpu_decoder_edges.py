@@ -69,6 +69,16 @@ def test_norm_codes_next_to_a_border(gpu, border):
     _norm_exactly(h * 2.0 ** -60, w * 2.0 ** -40, "float32", "float32")
 
 
+def test_norm_of_more_rows_than_a_launch_has_waves(gpu):
+    """A wave takes a row up to 1024 columns: 2^26 rows are 2^32 threads."""
+    rows = (1 << 26) + 5
+    x = np.arange(rows, dtype=np.int64) % 7 - 3
+    dx, q, s = Array.of(x.astype(np.float16)[:, None]), Array((rows, 1), "int8"), Array((rows,), "float32")
+    decoder.quantize_i8(dx, q, s)
+    np.testing.assert_array_equal(q.download()[:, 0], np.sign(x) * 127)
+    np.testing.assert_array_equal(s.download(), (np.abs(x) / 127).astype(np.float32))
+
+
 # ---------------------------------------------------------------- product
 
 @pytest.mark.parametrize("m,n", [(2, 16), (70, 130), (300, 520), (1500, 1300)])
