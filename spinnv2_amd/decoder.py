@@ -380,6 +380,8 @@ def attention(q, cache: KvCache, table, lengths, offsets, out, *, max_queries: i
         size = math.prod(workspace.shape)
         if _code_size(workspace) != 1 or not workspace.is_cuda:
             _fail("workspace", "not bytes on the GPU")
+        if workspace.stride() != (1,) and not _contiguous(workspace):
+            _fail("workspace", "not contiguous")
         at = workspace.data_ptr() if size else 0
     a = _pack_attention(q.data_ptr(), out.data_ptr(), table.data_ptr(), _vector("lengths", lengths, _INT32S, seqs),
                         _vector("offsets", offsets, _INT32S, seqs + 1), at, size, shape[0], _heads("q", q, _FLOATS, shape),
@@ -388,6 +390,16 @@ def attention(q, cache: KvCache, table, lengths, offsets, out, *, max_queries: i
     lib = load_library()
     if code := lib.spkv2_mi355x_attention_i8(cache._ref, a, stream):
         _check(lib, code, "attention_i8")
+
+
+def _contiguous(t) -> bool:
+    """Whether a tensor's elements lie one after the other; an axis of one element may have any stride."""
+    step = 1
+    for n, stride in zip(reversed(t.shape), reversed(t.stride())):
+        if n != 1 and stride != step:
+            return False
+        step *= n
+    return True
 
 
 def _code_size(t) -> int:
