@@ -308,7 +308,7 @@ class KvCache:
                                      ("v_scale", v_scale, _FP32, tuple(k.shape)[:3])):
             if _code(t) != code or tuple(t.shape) != shape or not t.is_cuda:
                 _fail(name, f"expected {shape} of another type or place")
-            if tuple(t.stride()) != tuple(math.prod(shape[i + 1:]) for i in range(len(shape))):
+            if not _contiguous(t):
                 _fail(name, "not contiguous")
         self.buffers = (k, v, k_scale, v_scale)  # held as long as the cache is
         self._c = _Cache(*(t.data_ptr() for t in self.buffers), self.pages, self.kv_heads, self.page_size, self.head_dim, 0)

@@ -17,3 +17,16 @@ def test_attention_refuses_a_workspace_that_is_not_contiguous():
                  Fake((1 << 15, 1 << 15), "int8", strides=(1, 1 << 15))):
         with pytest.raises(ValueError):
             decoder.attention(q, c, table, lengths, offsets, q, max_queries=2, max_length=4096, workspace=work)
+
+
+def test_cache_takes_any_stride_of_an_axis_of_one():
+    """One head, or one page, made by moving axes: contiguous, whatever the stride that the axis carries."""
+    pages, page, dim = 4, 16, 64
+    codes, scales = Fake((pages, 1, page, dim), "int8", strides=(page * dim, dim, dim, 1)), Fake((pages, 1, page), "float32", strides=(page, 1, 1))
+    decoder.KvCache(codes, codes, scales, scales)
+    codes, scales = Fake((1, 2, page, dim), "int8", strides=(7, page * dim, dim, 1)), Fake((1, 2, page), "float32", strides=(0, page, 1))
+    decoder.KvCache(codes, codes, scales, scales)
+    for strides in ((2 * page * dim, page * dim, dim, 1), (page * dim, page * dim, dim, 2), (0, page * dim, dim, 1)):
+        bad = Fake((pages, 1, page, dim), "int8", strides=strides)
+        with pytest.raises(ValueError):
+            decoder.KvCache(bad, bad, Fake((pages, 1, page), "float32"), Fake((pages, 1, page), "float32"))
