@@ -98,7 +98,8 @@ class DeviceArray:
 
     ``dtype`` is one of float32, float16, bfloat16, int8, int32, int64;
     bfloat16 values come and go as float32 arrays.  ``at`` elements from the
-    buffer's start; ``strides`` in elements (default: contiguous).
+    buffer's start; ``strides`` in elements, none below zero (default:
+    contiguous).
     """
 
     is_cuda = True
@@ -113,7 +114,7 @@ class DeviceArray:
         extent = 1 + sum((d - 1) * s for d, s in zip(self.shape, self.strides)) if math.prod(self.shape) else 0
         if buffer is None:
             buffer = DeviceBuffer(max(16, (at + extent) * self.itemsize))
-        if (at + extent) * self.itemsize > buffer.nbytes:
+        if at < 0 or min(self.strides, default=0) < 0 or (at + extent) * self.itemsize > buffer.nbytes:
             raise ValueError("the array does not fit its buffer")
         self.buffer = buffer
 

@@ -30,3 +30,14 @@ def test_cache_takes_any_stride_of_an_axis_of_one():
         bad = Fake((pages, 1, page, dim), "int8", strides=strides)
         with pytest.raises(ValueError):
             decoder.KvCache(bad, bad, Fake((pages, 1, page), "float32"), Fake((pages, 1, page), "float32"))
+
+
+def test_arrays_outside_their_buffer_are_refused():
+    class Buffer:
+        nbytes = 1024
+
+    for kw in (dict(at=-1), dict(at=250), dict(strides=(-8, 1)), dict(strides=(8, -1)), dict(at=64, strides=(-8, 1)), dict(strides=(300, 1))):
+        with pytest.raises(ValueError):
+            decoder.DeviceArray((4, 8), "float32", buffer=Buffer(), **kw)
+    decoder.DeviceArray((4, 8), "float32", buffer=Buffer(), at=224)
+    decoder.DeviceArray((4, 8), "float32", buffer=Buffer(), strides=(0, 1))
