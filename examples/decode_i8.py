@@ -73,10 +73,10 @@ class Decoder:
         """Logits after the last of each sequence's new tokens (one array of ids for each sequence, none of them empty)."""
         s = self.sizes
         counts = np.array([len(t) for t in tokens], np.int32)
+        if (self.lengths + counts).max() > self.longest:
+            raise ValueError("a sequence is longer than its pages")
         place = [np.arange(n, n + c) for n, c in zip(self.lengths, counts)]
         self.lengths = self.lengths + counts
-        if self.lengths.max() > self.longest:
-            raise ValueError("a sequence is longer than its pages")
         slots = np.concatenate([self.table[i, p // s.page].astype(np.int64) * s.page + p % s.page for i, p in enumerate(place)])
         offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         total, widest, bound = int(offsets[-1]), int(counts.max()), int(self.lengths.max())

@@ -5,6 +5,7 @@ kernels.  References in 64 bits or in whole numbers, as in test_gpu_decoder."""
 from __future__ import annotations
 
 from fractions import Fraction
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -236,3 +237,19 @@ def test_attention_of_infinite_queries(gpu, counts, lengths, bound, dtype):
     got[::2, 1] = plain[::2, 1]
     np.testing.assert_array_equal(got, plain)
     assert (_attend(codes, scales, table, [0 for n in lengths], counts, q, dtype, bound or max(lengths)) == 0).all()
+
+
+# ---------------------------------------------------------------- example
+
+def test_example_goes_on_after_a_refusal(gpu, monkeypatch):
+    """Tokens that do not fit are refused and leave the sequences as they were."""
+    monkeypatch.syspath_prepend(str(Path(__file__).resolve().parent.parent / "examples"))
+    from decode_i8 import Decoder, Sizes
+
+    prompt = np.arange(9)
+    plain, refused = Decoder(Sizes(layers=1), 1, 16), Decoder(Sizes(layers=1), 1, 16)
+    plain.forward([prompt])
+    refused.forward([prompt])
+    with pytest.raises(ValueError):
+        refused.forward([np.zeros(8, np.int64)])
+    np.testing.assert_array_equal(refused.forward([prompt[:2]]), plain.forward([prompt[:2]]))
