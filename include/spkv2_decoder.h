@@ -95,6 +95,10 @@ typedef struct {
     int32_t reserved;
 } Spkv2MatmulI8;
 int spkv2_mi355x_matmul_i8(const Spkv2MatmulI8 *args, void *stream);
+/* name of the kernel that the call takes at these sizes, strides and type
+ * ("matmul_tiles<128x128>", ...; its pointers are not looked at; empty: none),
+ * for reports and tests */
+int spkv2_mi355x_matmul_i8_kernel_name(const Spkv2MatmulI8 *args, char *buf, size_t buf_size);
 
 /* ---- key/value cache ----------------------------------------------------- */
 
@@ -190,6 +194,8 @@ typedef struct {
 int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI8 *args, void *stream);
 /* bytes of workspace that the call needs (its pointers and workspace are not looked at); -1 codes as above */
 int spkv2_mi355x_attention_i8_workspace(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI8 *args, size_t *size);
+/* name of the kernel that the call takes ("attend_rows<waves=4,splits=3>", ...), likewise, for reports and tests */
+int spkv2_mi355x_attention_i8_kernel_name(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI8 *args, char *buf, size_t buf_size);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,8 @@
 // 128 rows a workgroup: bound by two waves a SIMD whose arithmetic and matrix
 // products hide little of each other (4001 queries of 32 heads on 4001 and 6007
 // tokens, 394 GFLOP: 505 us, 780 TFLOP/s, half of what a large product reaches).
+#include <cstdio>
+
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -944,6 +946,19 @@ extern "C" int spkv2_mi355x_attention_i8_workspace(const Spkv2KvCacheI8 *c, cons
         if (g->queries == 0 || g->sequences == 0 || g->max_queries == 0) return 0;
         const Plan p = plan(*c, *g);
         *size = p.part + p.stats;
+        return 0;
+    });
+}
+
+extern "C" int spkv2_mi355x_attention_i8_kernel_name(const Spkv2KvCacheI8 *c, const Spkv2AttentionI8 *g, char *buf, size_t buf_size) {
+    return entry([&]() -> int {
+        if (!buf || !buf_size) return bad("attention_i8: nowhere to put the name");
+        if (int rc = check(c, g)) return rc;
+        buf[0] = 0;
+        if (g->queries == 0 || g->sequences == 0 || g->max_queries == 0) return 0;
+        const Plan p = plan(*c, *g);
+        if (p.wide) snprintf(buf, buf_size, "attend_tiles<splits=%d>", p.splits);
+        else snprintf(buf, buf_size, "attend_rows<waves=%d,splits=%d>", p.waves, p.splits);
         return 0;
     });
 }

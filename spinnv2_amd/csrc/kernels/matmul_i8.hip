@@ -14,6 +14,8 @@
 // the chip keeps under them).  matmul_rows serves few: bound by the weights'
 // bytes (1 x 16384 x 4096 in 15 us, 4.5 TB/s) or, where they are few, by its
 // launch (64 x 1000 x 2048 in 5 us).
+#include <cstdio>
+
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -454,28 +456,52 @@ int fastest(int64_t m, int64_t n, int64_t k, bool tiles) {
     return best;
 }
 
+// the kernel of a call that check() took, as an index of kForms
+int form(const Spkv2MatmulI8 &g) {
+    const bool far = (g.m > 1 && g.a_stride >= (1 << 23)) || (g.n > 1 && g.b_stride >= (1 << 23));  // 256 rows pass 2^31 bytes
+    return fastest(g.m, g.n, g.k, !far && g.k >= 16);
+}
+
+int check(const Spkv2MatmulI8 *g, bool pointers) {
+    if (!g) return bad("matmul_i8: no arguments");
+    if (!is_dtype(g->dtype)) return bad("matmul_i8: unknown dtype");
+    if (g->m < 0 || g->n < 0 || g->k < 0) return bad("matmul_i8: negative size");
+    if (g->m == 0 || g->n == 0) return 0;
+    if (pointers && (!g->out || !g->a_scale || !g->b_scale || (g->k && (!g->a || !g->b)))) return bad("matmul_i8: a NULL pointer");
+    if ((g->m > 1 && (g->a_stride < g->k || g->out_stride < g->n)) || (g->n > 1 && g->b_stride < g->k))
+        return bad("matmul_i8: a stride is below its row's length");
+    if (g->k > (1 << 17)) return unsupported("matmul_i8: k above 2^17, whose sums may pass 32 bits");
+    if (g->m > (1 << 21) || g->n > (1 << 26)) return unsupported("matmul_i8: m above 2^21 or n above 2^26");
+    return 0;
+}
+
 }  // namespace
 
 }  // namespace spk::dec
 
 using namespace spk::dec;
 
+extern "C" int spkv2_mi355x_matmul_i8_kernel_name(const Spkv2MatmulI8 *g, char *buf, size_t buf_size) {
+    return entry([&]() -> int {
+        if (!buf || !buf_size) return bad("matmul_i8: nowhere to put the name");
+        if (int rc = check(g, false)) return rc;
+        buf[0] = 0;
+        if (g->m == 0 || g->n == 0) return 0;
+        const Form &f = kForms[form(*g)];
+        if (f.waves == 1) snprintf(buf, buf_size, "matmul_tiles<%dx%d>", f.tokens, f.channels);
+        else snprintf(buf, buf_size, "matmul_rows<%dx%d,waves=%d>", f.tokens, f.channels, f.waves);
+        return 0;
+    });
+}
+
 extern "C" int spkv2_mi355x_matmul_i8(const Spkv2MatmulI8 *g, void *stream) {
     return entry([&]() -> int {
-        if (!g) return bad("matmul_i8: no arguments");
-        if (!is_dtype(g->dtype)) return bad("matmul_i8: unknown dtype");
-        if (g->m < 0 || g->n < 0 || g->k < 0) return bad("matmul_i8: negative size");
+        if (int rc = check(g, true)) return rc;
         if (g->m == 0 || g->n == 0) return 0;
-        if (!g->out || !g->a_scale || !g->b_scale || (g->k && (!g->a || !g->b))) return bad("matmul_i8: a NULL pointer");
-        if ((g->m > 1 && (g->a_stride < g->k || g->out_stride < g->n)) || (g->n > 1 && g->b_stride < g->k))
-            return bad("matmul_i8: a stride is below its row's length");
-        if (g->k > (1 << 17)) return unsupported("matmul_i8: k above 2^17, whose sums may pass 32 bits");
-        if (g->m > (1 << 21) || g->n > (1 << 26)) return unsupported("matmul_i8: m above 2^21 or n above 2^26");
         MatmulArgs a{g->a, g->b, g->a_scale, g->b_scale, g->bias, g->out, g->a_stride, g->b_stride, g->out_stride,
                      static_cast<int>(g->m), static_cast<int>(g->n), static_cast<int>(g->k), 0, 0};
         if (g->m == 1) a.a_stride = 0, a.out_stride = 0;
         if (g->n == 1) a.b_stride = 0;
-        const bool far = a.a_stride >= (1 << 23) || a.b_stride >= (1 << 23);  // 256 rows pass 2^31 bytes
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             const char *what = "matmul_i8";
@@ -488,7 +514,7 @@ extern "C" int spkv2_mi355x_matmul_i8(const Spkv2MatmulI8 *g, void *stream) {
                 a.n_tiles = (a.n + 64 * blocks - 1) / (64 * blocks);
                 return launch(what, kernel, dim3(static_cast<unsigned>(a.m_tiles * a.n_tiles)), dim3(256), stream, a);
             };
-            switch (fastest(g->m, g->n, g->k, !far && g->k >= 16)) {
+            switch (form(*g)) {
                 case 0: return rows(matmul_rows<T, 1, 1, 8>, 1, 1, 8);
                 case 1: return rows(matmul_rows<T, 1, 2, 8>, 1, 2, 8);
                 case 2: return rows(matmul_rows<T, 2, 2, 8>, 2, 2, 8);

@@ -106,10 +106,12 @@ SIGNATURES = {
     "spkv2_mi355x_rmsnorm_i8": (I, [VP, VP]),
     "spkv2_mi355x_dequantize_i8": (I, [VP, VP]),
     "spkv2_mi355x_matmul_i8": (I, [VP, VP]),
+    "spkv2_mi355x_matmul_i8_kernel_name": (I, [VP, ctypes.c_char_p, SZ]),
     "spkv2_mi355x_kv_write_i8": (I, [VP, VP, VP]),
     "spkv2_mi355x_kv_read_i8": (I, [VP, VP, VP]),
     "spkv2_mi355x_attention_i8": (I, [VP, VP, VP]),
     "spkv2_mi355x_attention_i8_workspace": (I, [VP, VP, ctypes.POINTER(SZ)]),
+    "spkv2_mi355x_attention_i8_kernel_name": (I, [VP, VP, ctypes.c_char_p, SZ]),
 }
 
 _LIB = None

@@ -13,7 +13,8 @@ import pytest
 from spinnv2_amd import decoder
 from spinnv2_amd.decoder import DeviceArray as Array, KvCache
 
-from .test_gpu_decoder import FAR, HALF, _attend_case, rounded
+from .test_decoder_edges import PRODUCTS, SPLIT, matmul_kernel
+from .test_gpu_decoder import FAR, HALF, _attend_case, _matmul_case, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -92,6 +93,67 @@ def test_matmul_of_sums_of_2_to_the_31(gpu, m, n):
     out = Array((m, n), "float32")
     decoder.matmul_i8(Array.of(a), Array.of(np.ones(m, np.float32)), Array.of(b), Array.of(np.ones(n, np.float32)), out)
     np.testing.assert_array_equal(out.download(), np.outer(u, v) * k)
+
+
+@pytest.mark.parametrize("kernel,m,n,k,dtype,bias,pads,at", PRODUCTS)
+def test_matmul_of_every_kernel(gpu, kernel, m, n, k, dtype, bias, pads, at):
+    _matmul_case(m, n, k, dtype, bias, pads, at)
+
+
+@pytest.mark.parametrize("kernel,m,n,k", [p[:4] for p in PRODUCTS if p[3] in (15, 333, 2111)])
+def test_matmul_of_every_kernel_with_extreme_codes(gpu, kernel, m, n, k):
+    _matmul_case(m, n, k, "float32", extreme=True)
+
+
+@pytest.mark.parametrize("kernel,m,n,k", [p[:4] for p in PRODUCTS if p[3] in (15, 200, 2048)])
+def test_matmul_of_every_kernel_with_scales_that_are_not_finite(gpu, kernel, m, n, k):
+    """A token's NaN is its row's, a channel's infinity its column's, and no other's."""
+    a, b = np.ones((m, k), np.int8), np.ones((n, k), np.int8)
+    sa, sb = np.ones(m, np.float32), np.ones(n, np.float32)
+    sa[m // 2], sb[n - 2] = np.nan, np.inf
+    out = Array((m, n), "float32")
+    decoder.matmul_i8(Array.of(a), Array.of(sa), Array.of(b), Array.of(sb), out)
+    want = np.full((m, n), np.float32(k))
+    want[:, n - 2], want[m // 2] = np.inf, np.nan
+    np.testing.assert_array_equal(out.download(), want)
+
+
+def test_matmul_gives_the_same_bits_in_every_kernel(gpu):
+    """One row and channel among fewer or more others, 333 and 2111 codes each."""
+    rng = np.random.default_rng(6)
+    for k, m, n, parts in ((333, 3001, 4100, [(9, 333), (3, 4100), (17, 4100), (65, 3001), (3001, 130), (700, 3001)]), (2111, 700, 4100, [(129, 4100), (9, 333)])):
+        a, b = rng.integers(-127, 128, (m, k), dtype=np.int8), rng.integers(-127, 128, (n, k), dtype=np.int8)
+        sa, sb, c = rng.random(m).astype(np.float32), rng.random(n).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+
+        def product(m, n):
+            out = Array((m, n), "float32")
+            decoder.matmul_i8(Array.of(a[:m]), Array.of(sa[:m]), Array.of(b[:n]), Array.of(sb[:n]), out, bias=Array.of(c[:n]))
+            return out.download()
+
+        whole = product(m, n)
+        kernels = {matmul_kernel(m, n, k, "float32")}
+        for rows, cols in parts:
+            np.testing.assert_array_equal(product(rows, cols), whole[:rows, :cols])
+            kernels.add(matmul_kernel(rows, cols, k, "float32"))
+        assert len(kernels) == len(parts) + 1
+
+
+def test_matmul_of_rows_far_apart(gpu):
+    """260 rows of more than 2^23 bytes: the last ones lie past 2^31."""
+    rng = np.random.default_rng(8)
+    m, n, k, stride = 260, 70, 200, (1 << 23) + 16
+    a, b = rng.integers(-127, 128, (m, k), dtype=np.int8), rng.integers(-127, 128, (n, k), dtype=np.int8)
+    far = Array((m, k), "int8", strides=(stride, 1))
+    for i, row in enumerate(a):
+        assert gpu.spkv2_device_memcpy_h2d(far.data_ptr() + i * stride, row.ctypes.data, k) == 0
+    sums = a.astype(np.float64) @ b.astype(np.float64).T
+    ones = [Array.of(np.ones(x, np.float32)) for x in (m, n)]
+    out = Array((m, n), "float32")
+    decoder.matmul_i8(far, ones[0], Array.of(b), ones[1], out)
+    np.testing.assert_array_equal(out.download(), sums)
+    out = Array((n, m), "float32")
+    decoder.matmul_i8(Array.of(b), ones[1], far, ones[0], out)
+    np.testing.assert_array_equal(out.download(), sums.T)
 
 
 # -------------------------------------------------------------- attention
@@ -237,6 +299,27 @@ def test_attention_of_infinite_queries(gpu, counts, lengths, bound, dtype):
     got[::2, 1] = plain[::2, 1]
     np.testing.assert_array_equal(got, plain)
     assert (_attend(codes, scales, table, [0 for n in lengths], counts, q, dtype, bound or max(lengths)) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("window", [20, 100, 700])
+def test_attention_in_a_window_over_splits(gpu, window, dtype):
+    """Splits ahead of the window hold nothing for a row."""
+    _attend_case([1500, 2600, 90], [1, 1, 1], 4, 1, 128, 64, dtype, window=window)
+    _attend_case([1500, 2600], [3, 5], 4, 2, 64, 16, dtype, window=window)
+    _attend_case([700, 530], [80, 60], 4, 2, 64, 16, dtype, window=window, max_length=1 << 15)
+
+
+@pytest.mark.parametrize("counts,lengths,bound,heads,kv,dim,dtype,causal", SPLIT)
+def test_attention_of_many_rows_over_splits(gpu, counts, lengths, bound, heads, kv, dim, dtype, causal):
+    _attend_case(lengths, counts, heads, kv, dim, 16, dtype, causal=causal, max_length=bound)
+
+
+def test_attention_of_lengths_below_zero(gpu):
+    """As of no tokens."""
+    for counts in ([1, 1, 1], [40, 30, 2]):
+        for causal in (True, False):
+            _attend_case([-3, 40, -2 ** 31], counts, 4, 2, 64, 16, "bfloat16", causal=causal)
 
 
 # ---------------------------------------------------------------- example
