@@ -9,16 +9,20 @@
 // are therefore exact: of 16-bit rows p has at most 22 bits and is held in
 // fp32, with an fp32 factor in it at most 48, held in fp64.  A product of two
 // bf16 may leave fp32's range: a row whose largest does, or is so small that
-// others would lose bits that their codes need, is multiplied again in fp64
-// (8190 x 4096 and back takes 66.9 us so, 68.8 with fp64 for every row).
+// others would lose bits that their codes need, is multiplied again in fp64, an
+// element at a time, so that the other rows pay no registers for it (1596 x 9233
+// and back 44.5 us, 48.4 with runs of 8 in registers there too; 8190 x 4096
+// 66.6, 68.8 with fp64 for every row).
 //
 // One pass: a thread keeps its part of the row in registers between the
 // statistics and the codes, so each input is read once and each output
 // written once.  Bound by HBM: 8190 x 4096 of bf16 with a residual, 235 MB, in
-// 44 us (5.3 TB/s), its codes back to values, 101 MB, in 16.5 (6.1 TB/s); a
-// few rows by the launch (4 x 2048: 3.3 us and 2.0).  Rows of odd lengths lie
-// at any alignment and are read 16 bytes a lane all the same, the row's end
-// moved into place: 1596 x 9233 and back 35 us, 100 an element at a time.
+// 47 us (5.0 TB/s), its codes back to values, 101 MB, in 20 (5.1 TB/s; 16.8
+// right behind the norm, whose codes the cache still holds); a few rows by the
+// launch (4 x 2048: 3.3 us and 1.8).  Rows of odd lengths lie at any alignment
+// and are read 16 bytes a lane all the same, the row's end moved into place:
+// 1596 x 9233 without a residual 19 us, and back 9.  Rows of more than 16384
+// elements are read twice (1000 x 17000 with a residual 44.5 us, 28 of 16384).
 #include <type_traits>
 
 #include "decoder.hpp"
@@ -114,8 +118,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
         const int i = (c * THREADS + tid) * VEC;
         if (h && i < a.cols) store_some<VEC>(h + i, TAIL ? a.cols - i : VEC, f);
     };
-    auto products = [&](int c, const float(&f)[VEC], auto &p) {
-        using Q = std::decay_t<decltype(p[0])>;
+    auto products = [&](int c, const float(&f)[VEC], P(&p)[VEC]) {
         float g[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; j++) g[j] = 1.0f;
@@ -124,7 +127,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
             settle<VEC, TAIL>((c * THREADS + tid) * VEC, a.cols, g);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; j++) p[j] = static_cast<Q>(f[j]) * static_cast<Q>(g[j]);
+        for (int j = 0; j < VEC; j++) p[j] = static_cast<P>(f[j]) * static_cast<P>(g[j]);
     };
     auto statistics = [&](int c, const float(&f)[VEC]) {
         P p[VEC];
@@ -174,88 +177,89 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) rmsnorm_rows(Ro
             top = tops[i] > top ? tops[i] : top;
         }
     }
-    // chunk c of h once more
-    auto again = [&](int c, float(&f)[VEC]) {
-        if constexpr (CHUNKS > 0) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) f[j] = hv[c][j];
-        } else if (h) {
-            // read back where it was stored: x may have been overwritten by it
-            const int i = (c * THREADS + tid) * VEC;
-            // this thread's own elements: past them others may not have stored yet
-#pragma unroll
-            for (int j = 0; j < VEC; j++) f[j] = i + j < a.cols ? static_cast<float>(h[i + j]) : 0.0f;
-        } else {
-            Raw raw;
-            fetch(c, raw);
-            sum_up(c, raw, f);
-        }
-    };
-    auto over_row = [&](auto &&work) {
-        if constexpr (CHUNKS > 0) {
-#pragma unroll
-            for (int c = 0; c < CHUNKS; c++) work(c);
-        } else {
-            for (int c = 0; c < chunks; c++) work(c);
-        }
-    };
-    // the scale, and the codes of the products as Q
-    auto finish = [&](auto top) {
-        using Q = std::conditional_t<sizeof(top) == 8, double, float>;
-        constexpr auto kInf = sizeof(top) == 8 ? static_cast<decltype(top)>(0x7ff0000000000000ull) : static_cast<decltype(top)>(kInfBits);
-        const bool finite = top < kInf;
-        const Q amax = __builtin_bit_cast(Q, top);
-        if (tid == 0) {
-            double s = static_cast<double>(amax) / 127.0;
-            if (a.norm) s /= sqrt(sum / a.cols + static_cast<double>(a.eps));
-            // 0 of a row of zeros, whose norm may be 0 / 0
-            a.scale[row] = !finite ? __builtin_nanf("") : top == 0 ? 0.0f : static_cast<float>(s);
-        }
-        over_row([&](int c) {
-            const int i = (c * THREADS + tid) * VEC;
-            float f[VEC];
-            again(c, f);
-            Q p[VEC];
-            products(c, f, p);
-            Vec<int8_t, VEC> out;
-#pragma unroll
-            for (int j = 0; j < VEC; j++) out.v[j] = 0;
-            if (finite && top != 0) quantise<VEC>(p, amax, out.v);
-            if (i + VEC <= a.cols) {
-                __builtin_memcpy(q + i, out.v, VEC);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if (i + j < a.cols) q[i + j] = out.v[j];
-            }
-        });
+    auto put_scale = [&](double amax) {  // infinite or NaN: the row is
+        double s = amax / 127.0;
+        if (a.norm) s /= sqrt(sum / a.cols + static_cast<double>(a.eps));
+        // 0 of a row of zeros, whose norm may be 0 / 0
+        a.scale[row] = !(amax < __builtin_inf()) ? __builtin_nanf("") : amax == 0.0 ? 0.0f : static_cast<float>(s);
     };
     if constexpr (std::is_same_v<P, float> && std::is_same_v<T, __bf16>) {
         // Products below 2^-126 lose bits: next to a top of 2^-90 their codes are 0 all the same.  The row's
         // threads have one top, and turn here together.
         if (w && (top < __builtin_bit_cast(unsigned, 0x1p-90f) || top >= kInfBits)) {
-            uint64_t wide = 0;
-            over_row([&](int c) {
-                float f[VEC];
-                again(c, f);
-                double p[VEC];
-                products(c, f, p);
-#pragma unroll
-                for (int j = 0; j < VEC; j++) wide = max(wide, abs_bits(p[j]));
-            });
-            wide = wave_max(wide);
+            // h as it was stored, if it was: x may have been overwritten by it
+            auto product = [&](int i) {
+                const float f = h ? static_cast<float>(h[i]) : r ? static_cast<float>(static_cast<T>(static_cast<float>(x[i]) + static_cast<float>(r[i]))) : static_cast<float>(x[i]);
+                return static_cast<double>(f) * static_cast<double>(static_cast<float>(w[i]));
+            };
+            // this thread's own elements: others may not have stored theirs yet
+            auto over_own = [&](auto &&work) {
+#pragma unroll 1
+                for (int e = 0; e < chunks * VEC; e++) {
+                    const int i = (e / VEC * THREADS + tid) * VEC + e % VEC;
+                    if (i < a.cols) work(i);
+                }
+            };
+            uint64_t bits = 0;
+            over_own([&](int i) { bits = max(bits, abs_bits(product(i))); });
+            bits = wave_max(bits);
             if constexpr (THREADS > kWave) {
                 __shared__ uint64_t wides[THREADS / kWave];
-                if ((tid & (kWave - 1)) == 0) wides[tid / kWave] = wide;
+                if ((tid & (kWave - 1)) == 0) wides[tid / kWave] = bits;
                 __syncthreads();
-#pragma unroll
-                for (int i = 0; i < THREADS / kWave; i++) wide = max(wide, wides[i]);
+#pragma unroll 1
+                for (int i = 0; i < THREADS / kWave; i++) bits = max(bits, wides[i]);
             }
-            finish(wide);
+            const double wide = __builtin_bit_cast(double, bits);
+            if (tid == 0) put_scale(wide);
+            over_own([&](int i) {
+                const double p[1] = {product(i)};
+                int8_t code[1] = {0};
+                if (wide < __builtin_inf() && wide != 0.0) quantise<1>(p, wide, code);
+                q[i] = code[0];
+            });
             return;
         }
     }
-    finish(top);
+    constexpr U kInf = sizeof(U) == 8 ? static_cast<U>(0x7ff0000000000000ull) : static_cast<U>(kInfBits);
+    const bool finite = top < kInf;
+    const P amax = __builtin_bit_cast(P, top);
+    if (tid == 0) put_scale(static_cast<double>(amax));
+    auto codes = [&](int c, const float(&f)[VEC]) {
+        const int i = (c * THREADS + tid) * VEC;
+        P p[VEC];
+        products(c, f, p);
+        Vec<int8_t, VEC> out;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) out.v[j] = 0;
+        if (finite && top != 0) quantise<VEC>(p, amax, out.v);
+        if (i + VEC <= a.cols) {
+            __builtin_memcpy(q + i, out.v, VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (i + j < a.cols) q[i + j] = out.v[j];
+        }
+    };
+    if constexpr (CHUNKS > 0) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) codes(c, hv[c]);
+    } else {
+        for (int c = 0; c < chunks; c++) {
+            // h is read back where it was stored: x may have been overwritten by it
+            Raw raw;
+            if (h) {
+                const int i = (c * THREADS + tid) * VEC;
+                // this thread's own elements: past them others may not have stored yet
+#pragma unroll
+                for (int j = 0; j < VEC; j++) hv[0][j] = i + j < a.cols ? static_cast<float>(h[i + j]) : 0.0f;
+            } else {
+                fetch(c, raw);
+                sum_up(c, raw, hv[0]);
+            }
+            codes(c, hv[0]);
+        }
+    }
 }
 
 template <typename T, typename W>
