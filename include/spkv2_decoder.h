@@ -78,9 +78,9 @@ int spkv2_mi355x_dequantize_i8(const Spkv2DequantizeI8 *args, void *stream);
 
 /* ---- product ------------------------------------------------------------- */
 
-/* out[m, n] = a_scale[m] b_scale[n] sum_k a[m, k] b[n, k] + bias[n]: int32
- * sums, which are exact up to k = 2^17 (larger k is refused, and m above 2^21
- * or n above 2^26), scaled in fp32 and rounded once to out's type: the same
+/* out[m, n] = a_scale[m] b_scale[n] sum_k a[m, k] b[n, k] + bias[n]: sums
+ * that are exact up to k = 2^17, of -128 too (larger k is refused, and m above
+ * 2^21 or n above 2^26), scaled in fp32 and rounded once to out's type: the same
  * bits whatever the strides and the sizes beside a row and a channel. */
 typedef struct {
     const int8_t *a;      /* [m, k]: one row for each token */
@@ -159,10 +159,10 @@ int spkv2_mi355x_kv_read_i8(const Spkv2KvCacheI8 *cache, const Spkv2KvRead *args
  * 11 bits (22 for fp32 rows), and to within 2^-39 of their row's largest
  * element; softmax weights times their tokens' value scales with as many, and
  * to within 2^-28 of the largest of those that the row reads; sums and softmax
- * statistics are fp32.  Value scales are meant to lie between 2^-96 and 2^96;
- * smaller ones lose bits.  A token whose key or value scale is not finite makes
- * the rows that read it NaN, and no other; what a row does not read changes no
- * bit of it.
+ * statistics are fp32.  Value scales are meant to lie between 2^-96 and 2^96,
+ * where smaller ones lose bits, key scales below 2^64.  A token whose key or
+ * value scale is not finite makes the rows that read it NaN, and no other; what
+ * a row does not read changes no bit of it.
  *
  * max_queries and max_length bound the sequences' counts of queries and
  * lengths; what a sequence has beyond them is not computed (queries) or not

@@ -8,11 +8,17 @@
 //
 // attend_rows takes 16 rows (query, head of the group) of a sequence and kv head
 // a workgroup, for single tokens above all: bound by the cache's bytes (64 sequences of
-// 3001 to 16384 tokens, 8 kv heads of 128, 1.31 GB: 271 us, 4.8 TB/s), one
+// 3001 to 16384 tokens, 8 kv heads of 128, 1.31 GB: 270 us, 4.9 TB/s), one
 // short sequence by its loads' latency (333 tokens 9.7 us).  attend_tiles takes
 // 128 rows a workgroup: bound by two waves a SIMD whose arithmetic and matrix
 // products hide little of each other (4001 queries of 32 heads on 4001 and 6007
-// tokens, 394 GFLOP: 505 us, 780 TFLOP/s, half of what a large product reaches).
+// tokens, 394 GFLOP: 507 to 523 us on three chips, 770 TFLOP/s, half of what a
+// large product reaches).
+//
+// Weights are rounded to fp16's 11 bits for the second product, except of fp32
+// rows, where they are two parts: bf16 results do not show it (relative error
+// 1.7e-3 with either), of fp16 rows 2.1e-4 becomes 2.9e-4, and a second part
+// would double the products that the kernel for many rows is bound by.
 #include <cstdio>
 
 #include "decoder.hpp"

@@ -7,7 +7,7 @@
 // neighbouring tokens, whose rows and scales lie next to each other in a page:
 // with the heads side by side instead, a page's line of scales was written a
 // few bytes at a time from several XCDs (3 x 8191 tokens of 8 heads of 128,
-// 152 MB: 45 us, 37 so, 4.1 TB/s).  Read: 16 codes a lane, scaled (31 us, 5.0
+// 152 MB: 45 us, 38 so, 4.0 TB/s).  Read: 16 codes a lane, scaled (31 us, 4.9
 // TB/s).
 #include "decoder.hpp"
 

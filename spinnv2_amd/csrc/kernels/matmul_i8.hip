@@ -9,11 +9,10 @@
 // -127 128 2^17 > -2^31 and 128 128 2^17 = 2^31: that one, of 2^17 products of
 // -128, is held as -2^31, which no other sum is.
 //
-// matmul_tiles serves many tokens: bound by the matrix cores (8192^3 in 470 us,
-// 2.3 POP/s, 66 us more than the time that its products take at the clock that
-// the chip keeps under them).  matmul_rows serves few: bound by the weights'
-// bytes (1 x 16384 x 4096 in 15 us, 4.5 TB/s) or, where they are few, by its
-// launch (64 x 1000 x 2048 in 5 us).
+// matmul_tiles serves many tokens: bound by the matrix cores, which work in 64%
+// of the busy cycles (8192^3 in 474 to 487 us on three chips, 2.3 POP/s).  matmul_rows serves few:
+// bound by the weights' bytes (1 x 16384 x 4096 in 13.4 us, 5.0 TB/s) or, where
+// they are few, by its launch (64 x 1000 x 2048 in 3.8 us).
 #include <cstdio>
 
 #include "decoder.hpp"
@@ -110,14 +109,14 @@ __device__ __forceinline__ void interleave() {
 // 64 B tokens x 64 B channels a workgroup of four waves (2 x 2), each B x B
 // tiles of 32 x 32; 128 bytes of k a step, in two buffers of LDS.
 //
-// The widest tile takes a CU: its sums are 256 registers of each lane, and it
-// reads 64 bytes of LDS a product of 32 cycles, half of what LDS gives (128 x
-// 64 a wave would need all of it).  A step's pieces wait in registers from one
-// step to the next, so that memory has a step's time to answer, and each piece
-// is written to LDS and loaded anew among the products, a few at a time: all at
-// once, the four waves' loads stand in line while no product runs (8192^3 495
-// against 465 us).  The next phase's operands are read a phase ahead, across
-// the step's one barrier too.
+// The widest tile takes a CU: its sums are 256 registers of each lane, and each
+// of its four waves reads 512 bytes of LDS a product of 32 cycles, together 64
+// bytes a cycle, half of what LDS gives (96 with 128 x 64 a wave).  A step's
+// pieces wait in registers from one step to the next, so that memory has a
+// step's time to answer, and each piece is written to LDS and loaded anew among
+// the products, a few at a time: all at once, the four waves' loads stand in
+// line while no product runs (8192^3 495 against 465 us).  The next phase's
+// operands are read a phase ahead, across the step's one barrier too.
 template <typename T, int B>
 __global__ void __launch_bounds__(256, B >= 4 ? 1 : 2) matmul_tiles(MatmulArgs a) {
     constexpr int TM = B, TN = B;

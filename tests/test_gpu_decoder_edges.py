@@ -301,6 +301,18 @@ def test_attention_of_infinite_queries(gpu, counts, lengths, bound, dtype):
     assert (_attend(codes, scales, table, [0 for n in lengths], counts, q, dtype, bound or max(lengths)) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -40, 2.0 ** 40, 2.0 ** 64])
+@pytest.mark.parametrize("counts,lengths,bound", FORMS)
+def test_attention_with_key_scales_of_any_size(gpu, counts, lengths, bound, size, dtype):
+    """Large keys and small queries, and the other way round: the same scores."""
+    def edit(q, codes, scales, table):
+        scales[0][:] = scales[0] * np.float32(size)
+        q /= size
+
+    _attend_case(lengths, counts, 4, 2, 64, 16, dtype, edit=edit, **({"max_length": bound} if bound else {}))
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("window", [20, 100, 700])
 def test_attention_in_a_window_over_splits(gpu, window, dtype):
