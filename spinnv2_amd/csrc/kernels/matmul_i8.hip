@@ -7,7 +7,7 @@
 // fp32 and rounded once.  So every kernel here gives the same bits, and which
 // one runs is a question of time alone.  Up to k = 2^17 the sums lie between
 // -127 128 2^17 > -2^31 and 128 128 2^17 = 2^31: that one, of 2^17 products of
-// -128, is held as -2^31, which no other sum is.
+// -128, comes out as -2^31, which no other sum does.
 //
 // matmul_tiles serves many tokens: bound by the matrix cores, which work in 64%
 // of the busy cycles (8192^3 in 474 to 487 us on three chips, 2.3 POP/s).  matmul_rows serves few:
@@ -64,9 +64,13 @@ __device__ __forceinline__ intx4 behind(int cut) {
 }
 
 __device__ __forceinline__ float scaled(int sum, float sa, float sb, float bias) {
-    const float x = sum == INT32_MIN ? 0x1p31f : static_cast<float>(sum);
-    return __builtin_fmaf(x * sa, sb, bias);
+    return __builtin_fmaf(static_cast<float>(sum) * sa, sb, bias);
 }
+
+// A sum of 2^31 that came out as -2^31, as the int32 that fp32 rounds to it.
+// Only k = 2^17 has one: asked of every sum it costs 4 us of 8192 x 8192 x 2048.
+__device__ __forceinline__ int unwrapped(int sum) { return sum == INT32_MIN ? INT32_MAX : sum; }
+constexpr int kMostTerms = 1 << 17;
 
 // LDS of one wave alone: its writes are done before its reads, and the other way round
 __device__ __forceinline__ void wait_lds() {
@@ -258,6 +262,15 @@ __global__ void __launch_bounds__(256, B >= 4 ? 1 : 2) matmul_tiles(MatmulArgs a
         multiply(1);
     }
 
+    if (a.k == kMostTerms) {
+#pragma unroll
+        for (int i = 0; i < TN; i++)
+#pragma unroll
+            for (int j = 0; j < TM; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[i][j][r] = unwrapped(acc[i][j][r]);
+    }
+
     // Scaled and rounded, each 32 tokens go through this wave's own part of LDS
     // (every wave is past its last read of the buffers), so that a row's
     // channels leave as 16-byte pieces one after the other.
@@ -410,6 +423,10 @@ __global__ void __launch_bounds__(64 * WAVES) matmul_rows(MatmulArgs a) {
         intx4 total = sums(0, i, j);
 #pragma unroll
         for (int w = 1; w < WAVES; w++) total += sums(w, i, j);
+        if (a.k == kMostTerms) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) total[e] = unwrapped(total[e]);
+        }
         const int m = m0 + 16 * j + col, n = n0 + 16 * i + 4 * g, left = a.n - n;
         if (m >= a.m || left <= 0) continue;
         float sb[4], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -469,7 +486,7 @@ int check(const Spkv2MatmulI8 *g, bool pointers) {
     if (pointers && (!g->out || !g->a_scale || !g->b_scale || (g->k && (!g->a || !g->b)))) return bad("matmul_i8: a NULL pointer");
     if ((g->m > 1 && (g->a_stride < g->k || g->out_stride < g->n)) || (g->n > 1 && g->b_stride < g->k))
         return bad("matmul_i8: a stride is below its row's length");
-    if (g->k > (1 << 17)) return unsupported("matmul_i8: k above 2^17, whose sums may pass 32 bits");
+    if (g->k > kMostTerms) return unsupported("matmul_i8: k above 2^17, whose sums may pass 32 bits");
     if (g->m > (1 << 21) || g->n > (1 << 26)) return unsupported("matmul_i8: m above 2^21 or n above 2^26");
     return 0;
 }

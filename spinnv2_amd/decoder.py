@@ -14,7 +14,8 @@ before this library is loaded, so that both use one HIP runtime) or a
 hipStream_t as a number, torch's ``Stream.cuda_stream``; 0 is the default
 stream), return without waiting, and write into tensors of the caller's: keep
 every tensor of a call until its work is done.  Shapes and types that do not
-fit raise ValueError, what the library refuses raises RuntimeError_.
+fit raise ValueError, numbers past the C types' ranges struct.error, what the
+library refuses raises RuntimeError_.
 """
 
 from __future__ import annotations

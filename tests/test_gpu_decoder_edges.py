@@ -83,7 +83,8 @@ def test_norm_of_more_rows_than_a_launch_has_waves(gpu):
 
 # ---------------------------------------------------------------- product
 
-@pytest.mark.parametrize("m,n", [(2, 16), (70, 130), (300, 520), (1500, 1300)])
+# each kernel of the product by one of these
+@pytest.mark.parametrize("m,n", [(2, 16), (70, 130), (3, 4100), (300, 520), (65, 3001), (129, 4100), (1500, 1300), (2050, 2050), (2050, 4100)])
 def test_matmul_of_sums_of_2_to_the_31(gpu, m, n):
     """2^17 products of -128 and -128: one more than int32 holds."""
     k = 1 << 17
