@@ -1,6 +1,7 @@
 /*
  * Operators of a decoder layer that holds activations, weights and the
- * key/value cache as int8 with scales, for programs that decode token by
+ * key/value cache as int8 with scales, or activations and weights as 8-bit
+ * floats with scales for blocks of 128, for programs that decode token by
  * token on one MI355X.
  *
  * None of these has a counterpart in the reference runtime, whose packages
@@ -196,6 +197,164 @@ int spkv2_mi355x_attention_i8(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI
 int spkv2_mi355x_attention_i8_workspace(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI8 *args, size_t *size);
 /* name of the kernel that the call takes ("attend_rows<waves=4,splits=3>", ...), likewise, for reports and tests */
 int spkv2_mi355x_attention_i8_kernel_name(const Spkv2KvCacheI8 *cache, const Spkv2AttentionI8 *args, char *buf, size_t buf_size);
+
+/* ---- positions ------------------------------------------------------------ */
+
+/* Norms of queries and keys head by head, and the rotation of their positions:
+ *
+ *   y = x weight / sqrt(mean(x^2) + eps)   over a head's head_dim (norm = 0: y = x)
+ *   angle = position[axis[i]] frequencies[i]
+ *   (y[i], y[j]) -> (y[i] cos - y[j] sin, y[j] cos + y[i] sin)   for each pair i
+ *
+ * with j = i + pairs, or 2 i and 2 i + 1 for i and j where interleaved.  What
+ * lies past 2 pairs is not turned.  All of it is held in 64 bits and rounded
+ * once; angles are meant below 2^40.
+ * With a cache the keys, as rounded, and the values go into their slots as
+ * spkv2_mi355x_kv_write_i8 writes them, with the same bits; k_out may be NULL
+ * then, and a token without a slot is not written to the cache.  Without one,
+ * v and slots are not looked at. */
+typedef struct {
+    const void *q;  /* [tokens, heads, head_dim], heads contiguous; heads = 0: no queries */
+    void *q_out;    /* likewise; may be q's own memory (with its stride) */
+    const void *k;  /* [tokens, kv_heads, head_dim], heads contiguous; kv_heads = 0: no keys */
+    void *k_out;    /* likewise; may be k's own memory (with its stride) */
+    const void *v;  /* [tokens, kv_heads, head_dim], heads contiguous */
+    const void *q_weight, *k_weight; /* [head_dim], or NULL: ones; with the norm only */
+    const int32_t *positions;        /* [tokens, axes] */
+    const float *frequencies;        /* [pairs]: radians a position */
+    const int32_t *axis;             /* [pairs]: each pair's axis, or NULL: 0; a pair of no axis is not turned */
+    const int64_t *slots;            /* [tokens] */
+    int64_t tokens;
+    int64_t q_stride, q_out_stride, k_stride, k_out_stride, v_stride, position_stride; /* elements between tokens */
+    int32_t heads, kv_heads;
+    int32_t head_dim; /* a multiple of 16, at most 256 */
+    int32_t pairs;    /* at most head_dim / 2 */
+    int32_t axes;     /* at least 1 */
+    int32_t interleaved, norm;
+    int32_t dtype;        /* of q, k, v and the outputs */
+    int32_t weight_dtype; /* dtype, or SPKV2_DTYPE_FP32 */
+    float eps;            /* at least 0 */
+} Spkv2Rotate;
+int spkv2_mi355x_rotate(const Spkv2KvCacheI8 *cache, const Spkv2Rotate *args, void *stream);
+
+/* ---- rows in 8-bit floats -------------------------------------------------- */
+
+/* 8-bit floats are e4m3 with 0x7f and 0xff for NaN and no infinity (the OCP
+ * format): eight values to a power of two from 2^-6 to 448, multiples of 2^-9
+ * below.  Each 128 columns of a row (the last block may be shorter) become
+ * codes 448 v / max|v|, rounded to the nearest, ties to even, and one float
+ * scale max|v| / 448.  The codes are those of exact arithmetic (of the gate:
+ * of 64-bit).  A block of zeros has scale 0; one that holds a NaN or an
+ * infinity has scale NaN and codes 0.  A scale below 2^-126 loses bits. */
+#define SPKV2_F8_BLOCK 128
+
+enum {
+    SPKV2_F8_VALUES = 0, /* v = x */
+    SPKV2_F8_NORM = 1,   /* h = x + residual (rounded to the rows' type, as it is stored), v = h weight / sqrt(mean(h^2) + eps) */
+    SPKV2_F8_GATE = 2    /* x [rows, 2 cols]: v = silu(x[:, :cols]) x[:, cols:], silu(t) = t / (1 + exp(-t)) */
+};
+typedef struct {
+    const void *x;        /* [rows, cols], or [rows, 2 cols] */
+    const void *residual; /* [rows, cols], or NULL: h = x; this and the next two with the norm only */
+    const void *weight;   /* [cols], or NULL: ones */
+    void *residual_out;   /* [rows, cols]: h; may be x's or residual's own memory (with its stride); NULL: not stored */
+    uint8_t *q;           /* [rows, cols] */
+    float *scale;         /* [rows, blocks], blocks = ceil(cols / 128) */
+    int64_t rows, cols;
+    int64_t x_stride, residual_stride, residual_out_stride, q_stride, scale_stride; /* elements between rows */
+    int32_t kind;
+    int32_t dtype;        /* of x, residual and residual_out */
+    int32_t weight_dtype; /* dtype, or SPKV2_DTYPE_FP32 */
+    float eps;            /* at least 0; with the norm only */
+} Spkv2RowsF8;
+int spkv2_mi355x_rows_f8(const Spkv2RowsF8 *args, void *stream);
+
+/* out = scale q, block by block */
+typedef struct {
+    const uint8_t *q;   /* [rows, cols] */
+    const float *scale; /* [rows, blocks] */
+    void *out;          /* [rows, cols] */
+    int64_t rows, cols;
+    int64_t q_stride, scale_stride, out_stride;
+    int32_t dtype; /* of out */
+    int32_t reserved;
+} Spkv2DequantizeF8;
+int spkv2_mi355x_dequantize_f8(const Spkv2DequantizeF8 *args, void *stream);
+
+/* ---- products in 8-bit floats ---------------------------------------------- */
+
+/* out[m, n] = sum over blocks t of 128 of k: a_scale[m, t] b_scale[n / 128, t]
+ * sum_{k in t} a[m, k] b[n, k], + bias[n].  A block's products are summed by
+ * the matrix cores, scaled and added in fp32, and rounded once to out's type.
+ * The order of the blocks' sums depends on the sizes.  Products of two scales
+ * are meant to lie between 2^-126 and 2^100. */
+typedef struct {
+    const uint8_t *a;     /* [m, k]: one row for each token */
+    const uint8_t *b;     /* [n, k]: one row for each output channel */
+    const float *a_scale; /* [m, blocks of k] */
+    const float *b_scale; /* [blocks of n, blocks of k] */
+    const float *bias;    /* [n], or NULL */
+    void *out;            /* [m, n] */
+    int64_t m, n, k;
+    int64_t a_stride, b_stride, out_stride, a_scale_stride, b_scale_stride;
+    int32_t dtype; /* of out */
+    int32_t reserved;
+} Spkv2MatmulF8;
+int spkv2_mi355x_matmul_f8(const Spkv2MatmulF8 *args, void *stream);
+/* name of the kernel that the call takes, for reports and tests (see spkv2_mi355x_matmul_i8_kernel_name) */
+int spkv2_mi355x_matmul_f8_kernel_name(const Spkv2MatmulF8 *args, char *buf, size_t buf_size);
+
+/* The same for rows sorted by expert: rows offsets[e] .. offsets[e + 1] of out
+ * are products with expert e's weights.  Row r's input is row r of a, or with
+ * an order row order[r] / per_token of a (spkv2_mi355x_sort_tokens gives it).
+ * Rows of out behind offsets[experts] are left as they were; an input row that
+ * a does not have counts as zeros. */
+typedef struct {
+    Spkv2MatmulF8 product;  /* m: rows of out; b [experts, n, k], b_scale [experts, blocks of n, blocks of k], bias [experts, n] */
+    const int32_t *offsets; /* [experts + 1], from 0, not decreasing; what passes m is not computed */
+    const int32_t *order;   /* [m], or NULL */
+    int64_t a_rows;         /* rows of a and a_scale */
+    int64_t b_expert_stride, b_scale_expert_stride; /* elements between experts */
+    int32_t experts;        /* at most 4096 */
+    int32_t per_token;      /* at least 1 */
+} Spkv2MatmulF8Experts;
+int spkv2_mi355x_matmul_f8_experts(const Spkv2MatmulF8Experts *args, void *stream);
+int spkv2_mi355x_matmul_f8_experts_kernel_name(const Spkv2MatmulF8Experts *args, char *buf, size_t buf_size);
+
+/* ---- tokens sorted by expert, and back -------------------------------------- */
+
+/* Sorts the choices c = token per_token + j by their expert, those of one
+ * expert by c: order[r] is the choice that is row r of the sorted rows, place
+ * its inverse, offsets[e] expert e's first row.  A choice of no expert (below
+ * zero, or experts and above) has no row: its place is -1, and order is left
+ * as it was from offsets[experts] on. */
+typedef struct {
+    const void *ids;  /* [tokens, per_token] */
+    int32_t *offsets; /* [experts + 1] */
+    int32_t *order;   /* [tokens per_token] */
+    int32_t *place;   /* [tokens, per_token] */
+    int64_t tokens;
+    int32_t per_token;
+    int32_t experts;  /* at most 4096 */
+    int32_t wide_ids; /* 0: ids are int32, 1: int64 */
+    int32_t reserved;
+} Spkv2SortTokens;
+int spkv2_mi355x_sort_tokens(const Spkv2SortTokens *args, void *stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] y[place[t, j]]: fp32 sums in the
+ * order of j, rounded once.  A place that y does not have adds nothing. */
+typedef struct {
+    const void *y;          /* [rows, cols] */
+    const int32_t *place;   /* [tokens, per_token] */
+    const float *weights;   /* [tokens, per_token] */
+    const void *residual;   /* [tokens, cols], or NULL */
+    void *out;              /* [tokens, cols]; may be residual's own memory (with its stride) */
+    int64_t rows, tokens, cols;
+    int64_t y_stride, residual_stride, out_stride;
+    int32_t per_token; /* at least 1 */
+    int32_t dtype;     /* of y, residual and out */
+} Spkv2Combine;
+int spkv2_mi355x_combine(const Spkv2Combine *args, void *stream);
 
 #ifdef __cplusplus
 }

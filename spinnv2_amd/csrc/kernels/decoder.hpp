@@ -153,6 +153,46 @@ __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N])
     for (int i = 0; i < N; i++) q[i] = static_cast<int8_t>(static_cast<int>(r[i]));
 }
 
+// A code of 448 x / top rounded to four bits (ties to even) in exact arithmetic,
+// without its sign: 0 <= x <= top, both of at most 48 bits.  The quotient is a
+// number of steps, 2^-9 or its power of two's eighth, of which a double gives the
+// integer part n (or, where it rounds up to it, n of the border below); whether
+// the border n + 1/2 is passed is one fused product, whose sign is exact.
+__device__ __forceinline__ unsigned exact_code_f8(double x, double top) {
+    const double y = x * 448.0 / top;
+    const int e = y < 0x1p-6 ? -6 : min(ilogb(y), 8);
+    const double step = ldexp(1.0, e - 3), n = floor(ldexp(y, 3 - e));
+    const double rest = __builtin_fma(-(n + 0.5) * step, top, 448.0 * x);
+    const unsigned whole = static_cast<unsigned>(n);
+    return static_cast<unsigned>((e + 6) * 8) + whole + (rest > 0.0 || (rest == 0.0 && (whole & 1)) ? 1u : 0u);
+}
+
+// Two floats as 8-bit floats, in bytes 0 and 1, rounded to the nearest, ties to even
+__device__ __forceinline__ unsigned two_f8(float a, float b) {
+    return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false)) & 0xffffu;
+}
+
+// Codes of 448 v / top of N values, |v| <= top, both within 2^-(SLACK + 2) of
+// their values in 64 bits.  The quotient in fp32, of four roundings more, is then
+// within 2^-SLACK: where it and what lies that far on both sides have one code,
+// that is it.  Returns a bit for each of the others, which have to be divided in
+// 64 bits; so have all where top is so small or large that quotients lose bits.
+template <int N, int SLACK>
+__device__ __forceinline__ unsigned quantise_f8(const float (&v)[N], float top, uint8_t (&q)[N]) {
+    constexpr float kLess = 1.0f - 1.0f / (1 << SLACK), kMore = 1.0f + 1.0f / (1 << SLACK);
+    const float inv = 448.0f / top;
+    unsigned near = 0;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const float a = v[j] * inv, b = v[j + 1] * inv;
+        const unsigned code = two_f8(a * kLess, b * kLess), differ = code ^ two_f8(a * kMore, b * kMore);
+        q[j] = static_cast<uint8_t>(code);
+        q[j + 1] = static_cast<uint8_t>(code >> 8);
+        near |= (differ & 0xffu ? 1u << j : 0u) | (differ >> 8 ? 2u << j : 0u);
+    }
+    return top > 0x1p-90f && top < 0x1p120f ? near : (1u << N) - 1u;
+}
+
 // The largest of v over groups of LANES neighbouring lanes (8, 16 or 32), in
 // each of them: within 16 by lane moves of the adder's own, past that by LDS's
 // crossbar.

@@ -1,0 +1,177 @@
+// Tokens sorted by expert, and their experts' rows weighted and added back.
+//
+// sort_tokens: the choices of one expert keep their order, so a choice's row is
+// the count of choices of lower experts and of earlier ones of its own.  A
+// workgroup an expert counts and places its own: every id is read once for each
+// expert, from L2, but there is one launch, no atomics and no order that changes
+// from run to run.
+//
+// combine: bound by the bytes of the rows picked.
+#include "decoder.hpp"
+
+namespace spk::dec {
+
+namespace {
+
+struct SortArgs {
+    const void *ids;
+    int32_t *offsets, *order, *place;
+    int count, experts;
+};
+
+// WAVES waves, each with a run of the choices, 64 at a time
+template <typename I, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) sort_choices(SortArgs a) {
+    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const I *ids = static_cast<const I *>(a.ids);
+    const int per = (a.count + 64 * WAVES - 1) / (64 * WAVES) * 64;  // counts up to 2^30
+    const int first = min(wave * per, a.count), end = min(first + per, a.count);
+    constexpr int kAhead = 8;
+    int lower = 0, own = 0;
+    for (int c0 = first; c0 < end; c0 += 64 * kAhead) {
+        I id[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int c = c0 + 64 * u + lane;
+            id[u] = c < end ? ids[c] : static_cast<I>(-1);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            lower += __popcll(__ballot(id[u] >= 0 && id[u] < e));
+            own += __popcll(__ballot(id[u] == e));
+        }
+    }
+    __shared__ int lowers[WAVES], owns[WAVES];
+    if (lane == 0) {
+        lowers[wave] = lower;
+        owns[wave] = own;
+    }
+    __syncthreads();
+    int row = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        row += lowers[w] + (w < wave ? owns[w] : 0);
+        all += lowers[w] + owns[w];
+    }
+    if (threadIdx.x == 0) {
+        a.offsets[e] = row;
+        if (e == a.experts - 1) a.offsets[a.experts] = all;
+    }
+    const uint64_t before = (uint64_t(1) << lane) - 1;
+    for (int c0 = first; c0 < end; c0 += 64 * kAhead) {
+        I id[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int c = c0 + 64 * u + lane;
+            id[u] = c < end ? ids[c] : static_cast<I>(0);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int c = c0 + 64 * u + lane;
+            const uint64_t mine = __ballot(c < end && id[u] == e);
+            if (c < end && id[u] == e) {
+                const int r = row + __popcll(mine & before);
+                a.order[r] = c;
+                a.place[c] = r;
+            }
+            row += __popcll(mine);
+            // the first expert's workgroup also marks the choices of none
+            if (e == 0 && c < end && (id[u] < 0 || id[u] >= a.experts)) a.place[c] = -1;
+        }
+    }
+}
+
+struct CombineArgs {
+    const void *y, *residual;
+    const int32_t *place;
+    const float *weights;
+    void *out;
+    int64_t rows, tokens, y_stride, residual_stride, out_stride;
+    int cols, per_token, runs;  // runs of VEC elements a row
+};
+
+// A run of VEC elements of a token a thread.  TAIL: cols is no multiple of VEC; it is VEC at least.
+template <typename T, int VEC, bool TAIL>
+__global__ void __launch_bounds__(256) combine_rows(CombineArgs a) {
+    const int64_t total = a.tokens * a.runs;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < total; t += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t token = t / a.runs;
+        const int i = static_cast<int>(t - token * a.runs) * VEC, from = min(i, a.cols - VEC);
+        float sum[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) sum[e] = 0.0f;
+        if (a.residual) load_floats<VEC>(static_cast<const T *>(a.residual) + token * a.residual_stride + from, sum);
+        const int32_t *place = a.place + token * a.per_token;
+        const float *weights = a.weights + token * a.per_token;
+        for (int j = 0; j < a.per_token; j += 4) {
+            Vec<T, VEC> v[4];
+            float w[4];
+            bool there[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int at = min(j + u, a.per_token - 1);
+                const int64_t row = place[at];
+                w[u] = weights[at];
+                there[u] = j + u < a.per_token && row >= 0 && row < a.rows;
+                if (there[u]) v[u] = load_vec<T, VEC>(static_cast<const T *>(a.y) + row * a.y_stride + from);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (there[u]) {
+                    float f[VEC];
+                    widen(v[u], f);
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) sum[e] = __builtin_fmaf(w[u], f[e], sum[e]);
+                }
+        }
+        if constexpr (TAIL) settle<VEC, true>(i, a.cols, sum);
+        store_some<VEC>(static_cast<T *>(a.out) + token * a.out_stride + i, TAIL ? a.cols - i : VEC, sum);
+    }
+}
+
+}  // namespace
+
+}  // namespace spk::dec
+
+using namespace spk::dec;
+
+extern "C" int spkv2_mi355x_sort_tokens(const Spkv2SortTokens *g, void *stream) {
+    return entry([&]() -> int {
+        if (!g) return bad("sort_tokens: no arguments");
+        if (g->tokens < 0 || g->per_token < 0 || g->experts < 1) return bad("sort_tokens: a negative size, or no expert");
+        if (g->experts > 4096) return unsupported("sort_tokens: more than 4096 experts");
+        if (g->per_token && g->tokens > (1 << 30) / g->per_token) return unsupported("sort_tokens: more than 2^30 choices");
+        const int64_t count = g->tokens * g->per_token;
+        if (!g->offsets || (count && (!g->ids || !g->order || !g->place))) return bad("sort_tokens: a NULL pointer");
+        const SortArgs a{g->ids, g->offsets, g->order, g->place, static_cast<int>(count), g->experts};
+        auto go = [&](auto kernel, int waves) { return launch("sort_tokens", kernel, dim3(g->experts), dim3(64 * waves), stream, a); };
+        if (g->wide_ids) return count <= 4096 ? go(sort_choices<int64_t, 4>, 4) : go(sort_choices<int64_t, 16>, 16);
+        return count <= 4096 ? go(sort_choices<int32_t, 4>, 4) : go(sort_choices<int32_t, 16>, 16);
+    });
+}
+
+extern "C" int spkv2_mi355x_combine(const Spkv2Combine *g, void *stream) {
+    return entry([&]() -> int {
+        if (!g) return bad("combine: no arguments");
+        if (!is_dtype(g->dtype)) return bad("combine: unknown dtype");
+        if (g->rows < 0 || g->tokens < 0 || g->cols < 0) return bad("combine: negative size");
+        if (g->per_token < 1) return bad("combine: per_token is below 1");
+        if (g->tokens == 0 || g->cols == 0) return 0;
+        if (!g->place || !g->weights || !g->out || (g->rows && !g->y)) return bad("combine: a NULL pointer");
+        if ((g->rows > 1 && g->y_stride < g->cols) || (g->tokens > 1 && (g->out_stride < g->cols || (g->residual && g->residual_stride < g->cols))))
+            return bad("combine: a stride is below cols");
+        if (g->tokens > INT32_MAX || g->cols > INT32_MAX) return unsupported("combine: more than 2^31 tokens or columns");
+        return with_type(g->dtype, [&](auto t) {
+            using T = decltype(t);
+            auto go = [&](auto kernel, int run) {
+                const CombineArgs a{g->y, g->residual, g->place, g->weights, g->out, g->rows, g->tokens, g->y_stride, g->residual_stride,
+                                    g->out_stride, static_cast<int>(g->cols), g->per_token, static_cast<int>((g->cols + run - 1) / run)};
+                const int64_t blocks = (a.tokens * a.runs + 255) / 256;
+                return launch("combine", kernel, dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536)), dim3(256), stream, a);
+            };
+            constexpr int kRun = 16 / static_cast<int>(sizeof(T));
+            if (g->cols < kRun) return go(combine_rows<T, 1, false>, 1);
+            return g->cols % kRun ? go(combine_rows<T, kRun, true>, kRun) : go(combine_rows<T, kRun, false>, kRun);
+        });
+    });
+}

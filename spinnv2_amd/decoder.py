@@ -1,11 +1,20 @@
 """Operators of a decoder layer in 8 bits (include/spkv2_decoder.h) from Python.
 
-    rmsnorm_i8      residual + root-mean-square norm -> int8 rows with scales
-    quantize_i8     rows -> int8 rows with scales
-    dequantize_i8   int8 rows -> values
-    matmul_i8       int8 rows x int8 weights, a scale for each row and channel
-    KvCache         a paged int8 key/value cache: write, read
-    attention       attention of new tokens to a KvCache
+    rmsnorm_i8          residual + root-mean-square norm -> int8 rows with scales
+    quantize_i8         rows -> int8 rows with scales
+    dequantize_i8       int8 rows -> values
+    matmul_i8           int8 rows x int8 weights, a scale for each row and channel
+    KvCache             a paged int8 key/value cache: write, read
+    attention           attention of new tokens to a KvCache
+    rotate              norms of queries and keys, their positions, and the way into a KvCache
+    rmsnorm_f8          residual + root-mean-square norm -> 8-bit float rows, a scale for each 128 columns
+    quantize_f8         rows -> 8-bit float rows
+    gate_f8             silu(gate) * up -> 8-bit float rows
+    dequantize_f8       8-bit float rows -> values
+    matmul_f8           8-bit float rows x weights, a scale for each 128 columns and 128 x 128 weights
+    matmul_f8_experts   the same for rows sorted by expert, each with its expert's weights
+    sort_tokens         the order of tokens sorted by expert
+    combine             experts' rows, weighted and added back to their tokens
 
 No counterpart in the reference.  A tensor is anything with ``data_ptr()``,
 ``shape``, ``stride()`` and ``dtype`` on the GPU: a torch tensor (import torch
@@ -28,11 +37,14 @@ import numpy as np
 
 from .runtime import DeviceBuffer, _check, load_library
 
-_FP32, _INT8, _FP16, _BF16, _INT32, _INT64 = 1, 2, 3, 4, 101, 102
+_FP32, _INT8, _FP16, _BF16, _INT32, _INT64, _F8 = 1, 2, 3, 4, 101, 102, 103
 #: dtype -> the library's code; torch's own dtype objects join at first sight
-_CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64}
+_CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64,
+          "float8_e4m3fn": _F8}
 _FLOATS = (_FP32, _FP16, _BF16)
-_FP32S, _INT8S, _INT32S, _INT64S = (_FP32,), (_INT8,), (_INT32,), (_INT64,)
+_FP32S, _INT8S, _INT32S, _INT64S, _F8S = (_FP32,), (_INT8,), (_INT32,), (_INT64,), (_F8,)
+#: columns of a row of 8-bit floats, and rows and columns of weights, that share a scale
+F8_BLOCK = 128
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -78,6 +90,51 @@ class _Attention(ctypes.Structure):
                 ("dtype", _I32), ("causal", _I32), ("window", _I32), ("scale", _F), ("reserved", _I32)]
 
 
+class _Rotate(ctypes.Structure):
+    _fields_ = [("q", _P), ("q_out", _P), ("k", _P), ("k_out", _P), ("v", _P), ("q_weight", _P), ("k_weight", _P),
+                ("positions", _P), ("frequencies", _P), ("axis", _P), ("slots", _P), ("tokens", _I64), ("q_stride", _I64),
+                ("q_out_stride", _I64), ("k_stride", _I64), ("k_out_stride", _I64), ("v_stride", _I64), ("position_stride", _I64),
+                ("heads", _I32), ("kv_heads", _I32), ("head_dim", _I32), ("pairs", _I32), ("axes", _I32), ("interleaved", _I32),
+                ("norm", _I32), ("dtype", _I32), ("weight_dtype", _I32), ("eps", _F)]
+
+
+class _RowsF8(ctypes.Structure):
+    _fields_ = [("x", _P), ("residual", _P), ("weight", _P), ("residual_out", _P), ("q", _P), ("scale", _P),
+                ("rows", _I64), ("cols", _I64), ("x_stride", _I64), ("residual_stride", _I64),
+                ("residual_out_stride", _I64), ("q_stride", _I64), ("scale_stride", _I64), ("kind", _I32), ("dtype", _I32),
+                ("weight_dtype", _I32), ("eps", _F)]
+
+
+class _DequantizeF8(ctypes.Structure):
+    _fields_ = [("q", _P), ("scale", _P), ("out", _P), ("rows", _I64), ("cols", _I64), ("q_stride", _I64),
+                ("scale_stride", _I64), ("out_stride", _I64), ("dtype", _I32), ("reserved", _I32)]
+
+
+_PRODUCT = [("a", _P), ("b", _P), ("a_scale", _P), ("b_scale", _P), ("bias", _P), ("out", _P), ("m", _I64), ("n", _I64),
+            ("k", _I64), ("a_stride", _I64), ("b_stride", _I64), ("out_stride", _I64), ("a_scale_stride", _I64),
+            ("b_scale_stride", _I64), ("dtype", _I32), ("reserved", _I32)]
+
+
+class _MatmulF8(ctypes.Structure):
+    _fields_ = _PRODUCT
+
+
+class _MatmulF8Experts(ctypes.Structure):
+    _fields_ = _PRODUCT + [("offsets", _P), ("order", _P), ("a_rows", _I64), ("b_expert_stride", _I64),
+                           ("b_scale_expert_stride", _I64), ("experts", _I32), ("per_token", _I32)]
+
+
+class _SortTokens(ctypes.Structure):
+    _fields_ = [("ids", _P), ("offsets", _P), ("order", _P), ("place", _P), ("tokens", _I64), ("per_token", _I32),
+                ("experts", _I32), ("wide_ids", _I32), ("reserved", _I32)]
+
+
+class _Combine(ctypes.Structure):
+    _fields_ = [("y", _P), ("place", _P), ("weights", _P), ("residual", _P), ("out", _P), ("rows", _I64), ("tokens", _I64),
+                ("cols", _I64), ("y_stride", _I64), ("residual_stride", _I64), ("out_stride", _I64), ("per_token", _I32),
+                ("dtype", _I32)]
+
+
 _LETTERS = {_P: "P", _I32: "i", _I64: "q", _F: "f", ctypes.c_size_t: "N"}
 
 
@@ -92,13 +149,15 @@ def _packer(cls):
 
 _pack_norm, _pack_dequantize, _pack_matmul = _packer(_RmsNorm), _packer(_Dequantize), _packer(_Matmul)
 _pack_write, _pack_read, _pack_attention = _packer(_Write), _packer(_Read), _packer(_Attention)
+_pack_rotate, _pack_rows_f8, _pack_dequantize_f8 = _packer(_Rotate), _packer(_RowsF8), _packer(_DequantizeF8)
+_pack_matmul_f8, _pack_experts, _pack_sort, _pack_combine = _packer(_MatmulF8), _packer(_MatmulF8Experts), _packer(_SortTokens), _packer(_Combine)
 
 
 class DeviceArray:
     """A tensor in a `DeviceBuffer`, for callers without torch.
 
-    ``dtype`` is one of float32, float16, bfloat16, int8, int32, int64;
-    bfloat16 values come and go as float32 arrays.  ``at`` elements from the
+    ``dtype`` is one of float32, float16, bfloat16, float8_e4m3fn, int8, int32,
+    int64; bfloat16 and float8_e4m3fn values come and go as float32 arrays.  ``at`` elements from the
     buffer's start; ``strides`` in elements, none below zero (default:
     contiguous).
     """
@@ -110,7 +169,7 @@ class DeviceArray:
             raise ValueError(f"unknown dtype {dtype!r}")
         self.shape, self.dtype = tuple(int(d) for d in shape), dtype
         self.strides = tuple(strides) if strides else tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
-        self.itemsize = 2 if dtype == "bfloat16" else np.dtype(dtype).itemsize
+        self.itemsize = self._kind().itemsize
         self.at = at
         extent = 1 + sum((d - 1) * s for d, s in zip(self.shape, self.strides)) if math.prod(self.shape) else 0
         if buffer is None:
@@ -137,8 +196,11 @@ class DeviceArray:
         _check(self.buffer.lib, self.buffer.lib.spkv2_device_memcpy_d2h(raw.ctypes.data, self.buffer.ptr, raw.nbytes), "d2h")
         return raw
 
+    def _kind(self) -> np.dtype:
+        return np.dtype({"bfloat16": np.uint16, "float8_e4m3fn": np.uint8}.get(self.dtype, self.dtype))
+
     def _view(self, raw: np.ndarray) -> np.ndarray:
-        kind = np.dtype(np.uint16 if self.dtype == "bfloat16" else self.dtype)
+        kind = self._kind()
         flat = raw[: raw.nbytes // kind.itemsize * kind.itemsize].view(kind)[self.at:]
         return np.lib.stride_tricks.as_strided(flat, self.shape, [s * kind.itemsize for s in self.strides])
 
@@ -146,11 +208,14 @@ class DeviceArray:
         """Writes the values, rounded to the array's type; what lies between strided rows stays."""
         values = np.broadcast_to(np.asarray(values), self.shape)
         raw = self._whole()
-        self._view(raw)[...] = to_bfloat16(values) if self.dtype == "bfloat16" else values.astype(self.dtype)
+        to = {"bfloat16": to_bfloat16, "float8_e4m3fn": to_float8}.get(self.dtype)
+        self._view(raw)[...] = to(values) if to else values.astype(self.dtype)
         self.buffer.upload(raw)
 
     def download(self) -> np.ndarray:
         a = self._view(self._whole()).copy()
+        if self.dtype == "float8_e4m3fn":
+            return _FLOAT8[a]
         return (a.astype(np.uint32) << 16).view(np.float32) if self.dtype == "bfloat16" else a
 
 
@@ -160,6 +225,29 @@ def to_bfloat16(values) -> np.ndarray:
     u = f.view(np.uint32)
     r = ((u.astype(np.uint64) + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
     return np.where(np.isnan(f), np.uint16(0x7FC0), r)
+
+
+def _float8() -> np.ndarray:
+    """The values of the 256 codes of 8-bit floats (e4m3, 0x7f and 0xff for NaN)."""
+    u = np.arange(128)
+    e, m = u >> 3, u & 7
+    v = np.where(e > 0, (8 + m) * 2.0 ** (e - 10.0), m * 2.0 ** -9).astype(np.float32)
+    v[127] = np.nan
+    return np.concatenate([v, -v])
+
+
+_FLOAT8 = _float8()
+
+
+def to_float8(values) -> np.ndarray:
+    """Values rounded to the nearest 8-bit float, ties to even, as its 8 bits; NaN for what is not finite or rounds past 448."""
+    v = np.asarray(values, np.float64)
+    border = (_FLOAT8[1:127].astype(np.float64) + _FLOAT8[:126]) / 2
+    size = np.abs(v)
+    # at a border itself the even one of both codes
+    low, high = np.searchsorted(border, size, side="left"), np.searchsorted(border, size, side="right")
+    code = np.where((low != high) & (low % 2 == 1), high, low)
+    return np.where(size <= 464, code | np.where(np.signbit(v), 0x80, 0), 0x7F).astype(np.uint8)
 
 
 def _code(t) -> int:
@@ -392,6 +480,236 @@ def attention(q, cache: KvCache, table, lengths, offsets, out, *, max_queries: i
     lib = load_library()
     if code := lib.spkv2_mi355x_attention_i8(cache._ref, a, stream):
         _check(lib, code, "attention_i8")
+
+
+def rotate(q, k, positions, frequencies, q_out, k_out, *, axes=None, norm: bool = False, q_weight=None, k_weight=None,
+           eps: float = 1e-6, interleaved: bool = False, cache: KvCache | None = None, v=None, slots=None, stream: int = 0) -> None:
+    """Norms of queries and keys head by head, and the rotation of their positions.
+
+    q, q_out [tokens, heads, head_dim], k, k_out [tokens, kv_heads, head_dim],
+    of one type; q and q_out, or k and k_out, may be None, and q_out may be q,
+    k_out k.  frequencies float32 [pairs], radians a position; positions int32
+    [tokens] or [tokens, axes]; axes int32 [pairs]: each pair's axis (default:
+    0).  Pair i are elements i and i + pairs of a head, or 2 i and 2 i + 1 where
+    interleaved.  norm: each head is divided by its root mean square first and
+    multiplied by q_weight, k_weight [head_dim] (of the heads' type or float32,
+    or None).  With a cache, the rotated keys and v [tokens, kv_heads,
+    head_dim] are written into its slots (as KvCache.write takes them), and
+    k_out may be None.
+    """
+    x = k if q is None else q
+    if x is None:
+        _fail("q, k", "neither is there")
+    if len(x.shape) != 3:
+        _fail("q, k", "not [tokens, heads, head_dim]")
+    code, (tokens, _, dim) = _code(x), x.shape
+    if len(frequencies.shape) != 1:
+        _fail("frequencies", "not one-dimensional")
+    pairs = frequencies.shape[0]
+    heads = kv_heads = qp = qs = qo = qos = kp = ks = ko = kos = vp = vs = sp = qw = kw = w_code = 0
+    if q is not None:
+        shape = (tokens, q.shape[1], dim)
+        heads, qp, qs = shape[1], q.data_ptr(), _heads("q", q, _FLOATS, shape)
+        if q_out is None:
+            _fail("q_out", "queries without an output")
+        qo, qos = q_out.data_ptr(), _heads("q_out", q_out, (code,), shape)
+    if k is not None:
+        if len(k.shape) != 3:
+            _fail("k", "not [tokens, kv_heads, head_dim]")
+        shape = (tokens, k.shape[1], dim)
+        kv_heads, kp, ks = shape[1], k.data_ptr(), _heads("k", k, (code,) if q is not None else _FLOATS, shape)
+        if k_out is not None:
+            ko, kos = k_out.data_ptr(), _heads("k_out", k_out, (code,), shape)
+        elif cache is None:
+            _fail("k_out", "keys without an output or a cache")
+    if cache is not None:
+        if k is None or v is None or slots is None:
+            _fail("cache", "keys, values or slots are missing")
+        if (kv_heads, dim) != (cache.kv_heads, cache.head_dim):
+            _fail("k", f"{kv_heads} heads of {dim}, the cache has {cache.kv_heads} of {cache.head_dim}")
+        vp, vs, sp = v.data_ptr(), _heads("v", v, (code,), shape), _vector("slots", slots, _INT64S, tokens)
+    if norm:
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None:
+                at = _vector(name, w, (code, _FP32), dim)
+                if w_code and w_code != _CODES[w.dtype]:
+                    _fail(name, "the weights are of different types")
+                w_code = _CODES[w.dtype]
+                if name == "q_weight":
+                    qw = at
+                else:
+                    kw = at
+    if len(positions.shape) == 1:
+        count, stride, at = 1, 1, _vector("positions", positions, _INT32S, tokens)
+    else:
+        if len(positions.shape) != 2:
+            _fail("positions", "not [tokens] or [tokens, axes]")
+        count, at = positions.shape[1], positions.data_ptr()
+        stride = _rows("positions", positions, _INT32S, (tokens, count))
+    a = _pack_rotate(qp, qo, kp, ko, vp, qw, kw, at, _vector("frequencies", frequencies, _FP32S, pairs),
+                     0 if axes is None else _vector("axes", axes, _INT32S, pairs), sp, tokens, qs, qos, ks, kos, vs, stride, heads, kv_heads,
+                     dim, pairs, count, 1 if interleaved else 0, 1 if norm else 0, code, w_code, eps)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_rotate(None if cache is None else cache._ref, a, stream):
+        _check(lib, code, "rotate")
+
+
+def _blocks(n: int) -> int:
+    return -(-n // F8_BLOCK)
+
+
+def rmsnorm_f8(x, weight, q, scale, *, residual=None, residual_out=None, eps: float = 1e-6, stream: int = 0) -> None:
+    """h = x + residual; q, scale = 8-bit float rows of h * weight / sqrt(mean(h^2) + eps).
+
+    As rmsnorm_i8, but q [rows, cols] is float8_e4m3fn and scale [rows,
+    blocks] float32 holds one scale for each 128 columns.
+    """
+    _rows_f8(1, x, weight, q, scale, residual, residual_out, eps, stream)
+
+
+def quantize_f8(x, q, scale, *, stream: int = 0) -> None:
+    """q, scale = 8-bit float rows of x, a scale for each 128 columns."""
+    _rows_f8(0, x, None, q, scale, None, None, 0.0, stream)
+
+
+def gate_f8(x, q, scale, *, stream: int = 0) -> None:
+    """q, scale = 8-bit float rows of silu(x[:, :cols]) * x[:, cols:]; x [rows, 2 cols]."""
+    _rows_f8(2, x, None, q, scale, None, None, 0.0, stream)
+
+
+def _rows_f8(kind, x, weight, q, scale, residual, residual_out, eps, stream) -> None:
+    shape, code = q.shape, _code(x)
+    if len(shape) != 2:
+        _fail("q", "not two-dimensional")
+    rows, cols = shape
+    w = w_code = r = r_stride = h = h_stride = 0
+    if weight is not None:
+        w, w_code = _vector("weight", weight, (code, _FP32), cols), _CODES[weight.dtype]
+    if residual is not None:
+        r_stride, r = _rows("residual", residual, (code,), shape), residual.data_ptr()
+    if residual_out is not None:
+        h_stride, h = _rows("residual_out", residual_out, (code,), shape), residual_out.data_ptr()
+    a = _pack_rows_f8(x.data_ptr(), r, w, h, q.data_ptr(), scale.data_ptr(), rows, cols, _rows("x", x, _FLOATS, (rows, 2 * cols) if kind == 2 else shape),
+                      r_stride, h_stride, _rows("q", q, _F8S, shape), _rows("scale", scale, _FP32S, (rows, _blocks(cols))), kind, code, w_code, eps)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_rows_f8(a, stream):
+        _check(lib, code, "rows_f8")
+
+
+def dequantize_f8(q, scale, out, *, stream: int = 0) -> None:
+    """out = q * scale, each 128 columns by their scale; out float32, float16 or bfloat16."""
+    shape = q.shape
+    if len(shape) != 2:
+        _fail("q", "not two-dimensional")
+    rows, cols = shape
+    a = _pack_dequantize_f8(q.data_ptr(), scale.data_ptr(), out.data_ptr(), rows, cols, _rows("q", q, _F8S, shape),
+                            _rows("scale", scale, _FP32S, (rows, _blocks(cols))), _rows("out", out, _FLOATS, shape), _code(out), 0)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_dequantize_f8(a, stream):
+        _check(lib, code, "dequantize_f8")
+
+
+def matmul_f8(a, a_scale, b, b_scale, out, *, bias=None, stream: int = 0) -> None:
+    """out[m, n] = sum over blocks t of 128 of k: a_scale[m, t] b_scale[n // 128, t] sum_{k in t} a[m, k] b[n, k], + bias[n].
+
+    a [m, k] and b [n, k] float8_e4m3fn, a_scale [m, blocks of k], b_scale
+    [blocks of n, blocks of k] and bias [n] float32, out [m, n] float32,
+    float16 or bfloat16.
+    """
+    if len(a.shape) != 2 or len(b.shape) != 2:
+        _fail("a, b", "not two-dimensional")
+    (m, k), n = a.shape, b.shape[0]
+    g = _pack_matmul_f8(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), 0 if bias is None else _vector("bias", bias, _FP32S, n),
+                        out.data_ptr(), m, n, k, _rows("a", a, _F8S, (m, k)), _rows("b", b, _F8S, (n, k)), _rows("out", out, _FLOATS, (m, n)),
+                        _rows("a_scale", a_scale, _FP32S, (m, _blocks(k))), _rows("b_scale", b_scale, _FP32S, (_blocks(n), _blocks(k))), _code(out), 0)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_matmul_f8(g, stream):
+        _check(lib, code, "matmul_f8")
+
+
+def matmul_f8_experts(a, a_scale, b, b_scale, offsets, out, *, order=None, per_token: int = 1, bias=None, stream: int = 0) -> None:
+    """matmul_f8 for rows sorted by expert: rows offsets[e] .. offsets[e + 1] of out with expert e's weights.
+
+    b [experts, n, k], b_scale [experts, blocks of n, blocks of k], bias
+    [experts, n]; offsets int32 [experts + 1].  Row r's input is row r of a, or
+    with an order (int32 [rows of out], sort_tokens' own) row order[r] //
+    per_token.  Rows behind offsets[experts] are left as they were.
+    """
+    if len(a.shape) != 2 or len(b.shape) != 3 or len(out.shape) != 2:
+        _fail("a, b, out", "not of two, three and two axes")
+    (rows, k), (experts, n, _), m = a.shape, b.shape, out.shape[0]
+    shapes = []
+    for name, t, codes, shape in (("b", b, _F8S, (experts, n, k)), ("b_scale", b_scale, _FP32S, (experts, _blocks(n), _blocks(k)))):
+        if t.shape != shape or _CODES.get(t.dtype) not in codes or not t.is_cuda:
+            _refuse(name, t, codes, shape)
+        expert, row, step = t.stride()
+        if step != 1 and shape[2] > 1:
+            _fail(name, "its last axis is not contiguous")
+        shapes.append((expert, row))
+    if bias is not None:
+        stride = _rows("bias", bias, _FP32S, (experts, n))
+        if stride != n and experts > 1:
+            _fail("bias", "not contiguous")
+    g = _pack_experts(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
+                      m, n, k, _rows("a", a, _F8S, (rows, k)), shapes[0][1], _rows("out", out, _FLOATS, (m, n)),
+                      _rows("a_scale", a_scale, _FP32S, (rows, _blocks(k))), shapes[1][1], _code(out), 0,
+                      _vector("offsets", offsets, _INT32S, experts + 1), 0 if order is None else _vector("order", order, _INT32S, m), rows,
+                      shapes[0][0], shapes[1][0], experts, per_token)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_matmul_f8_experts(g, stream):
+        _check(lib, code, "matmul_f8_experts")
+
+
+def _matrix(name: str, t, codes, shape) -> int:
+    """A contiguous matrix's address, its type and shape checked."""
+    if _rows(name, t, codes, shape) != shape[1] and shape[0] > 1:
+        _fail(name, "not contiguous")
+    return t.data_ptr()
+
+
+def sort_tokens(experts, offsets, order, place, *, stream: int = 0) -> None:
+    """Sorts the tokens' choices of experts: experts int32 or int64 [tokens, per_token].
+
+    order int32 [tokens * per_token]: the choice (token * per_token + j) that
+    is each sorted row; place int32 [tokens, per_token]: each choice's row;
+    offsets int32 [count of experts + 1]: each expert's first row.  Choices of
+    one expert keep their order.  A choice below zero, or of an expert that is
+    not there, has no row and the place -1.
+    """
+    shape = experts.shape
+    if len(shape) != 2:
+        _fail("experts", "not two-dimensional")
+    if len(offsets.shape) != 1:
+        _fail("offsets", "not one-dimensional")
+    tokens, per_token = shape
+    count = offsets.shape[0] - 1
+    a = _pack_sort(_matrix("experts", experts, (_INT32, _INT64), shape), _vector("offsets", offsets, _INT32S, count + 1),
+                   _vector("order", order, _INT32S, tokens * per_token), _matrix("place", place, _INT32S, shape), tokens, per_token, count,
+                   1 if _CODES[experts.dtype] == _INT64 else 0, 0)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_sort_tokens(a, stream):
+        _check(lib, code, "sort_tokens")
+
+
+def combine(y, place, weights, out, *, residual=None, stream: int = 0) -> None:
+    """out[t] = residual[t] + sum over j of weights[t, j] * y[place[t, j]].
+
+    y [rows, cols], out and residual [tokens, cols] (out may be residual) of
+    one type; place int32 and weights float32 [tokens, per_token].  A place
+    that y does not have adds nothing.
+    """
+    if len(y.shape) != 2 or len(place.shape) != 2:
+        _fail("y, place", "not two-dimensional")
+    (rows, cols), shape, code = y.shape, place.shape, _code(y)
+    tokens, per_token = shape
+    r = r_stride = 0
+    if residual is not None:
+        r, r_stride = residual.data_ptr(), _rows("residual", residual, (code,), (tokens, cols))
+    a = _pack_combine(y.data_ptr(), _matrix("place", place, _INT32S, shape), _matrix("weights", weights, _FP32S, shape), r, out.data_ptr(), rows,
+                      tokens, cols, _rows("y", y, _FLOATS, (rows, cols)), r_stride, _rows("out", out, (code,), (tokens, cols)), per_token, code)
+    lib = load_library()
+    if code := lib.spkv2_mi355x_combine(a, stream):
+        _check(lib, code, "combine")
 
 
 def _contiguous(t) -> bool:

@@ -112,6 +112,15 @@ SIGNATURES = {
     "spkv2_mi355x_attention_i8": (I, [VP, VP, VP]),
     "spkv2_mi355x_attention_i8_workspace": (I, [VP, VP, ctypes.POINTER(SZ)]),
     "spkv2_mi355x_attention_i8_kernel_name": (I, [VP, VP, ctypes.c_char_p, SZ]),
+    "spkv2_mi355x_rotate": (I, [VP, VP, VP]),
+    "spkv2_mi355x_rows_f8": (I, [VP, VP]),
+    "spkv2_mi355x_dequantize_f8": (I, [VP, VP]),
+    "spkv2_mi355x_matmul_f8": (I, [VP, VP]),
+    "spkv2_mi355x_matmul_f8_kernel_name": (I, [VP, ctypes.c_char_p, SZ]),
+    "spkv2_mi355x_matmul_f8_experts": (I, [VP, VP]),
+    "spkv2_mi355x_matmul_f8_experts_kernel_name": (I, [VP, ctypes.c_char_p, SZ]),
+    "spkv2_mi355x_sort_tokens": (I, [VP, VP]),
+    "spkv2_mi355x_combine": (I, [VP, VP]),
 }
 
 _LIB = None
