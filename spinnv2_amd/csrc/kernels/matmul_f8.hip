@@ -11,6 +11,7 @@
 // outputs, with 2^-9 and 2^-12 of their own, do not show.  fp32 outputs would
 // (1.1e-5 relative where fp32 sums leave 3e-7), so theirs are computed on the fp16
 // cores, whose operands hold 8-bit floats exactly, at half the rate.
+#include <cmath>
 #include <cstdio>
 
 #include "decoder.hpp"
@@ -26,7 +27,7 @@ struct MatmulArgs {
     const float *a_scale, *b_scale, *bias;
     void *out;
     int64_t a_stride, b_stride, out_stride, sa_stride, sb_stride;
-    int m, n, k;
+    int m, n, k, n_tiles;
     // by expert
     const int32_t *offsets, *order;
     int64_t a_rows, b_expert, sb_expert;
@@ -136,13 +137,27 @@ __device__ __forceinline__ Rows rows_of(const MatmulArgs &a, int at, int height)
     return Rows{-1, 0, 0};
 }
 
+// How many there are
+__device__ __forceinline__ int tiles_of(const MatmulArgs &a, int height) {
+    const int lane = threadIdx.x & 63;
+    int tiles = 0;
+    for (int e = lane; e < a.experts; e += 64) {
+        const int low = min(max(a.offsets[e], 0), a.m);
+        tiles += (min(max(a.offsets[e + 1], low), a.m) - low + height - 1) / height;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) tiles += __shfl_xor(tiles, d);
+    return __builtin_amdgcn_readfirstlane(tiles);
+}
+
 // 16 TM tokens x 16 TN channels a workgroup, whose waves deal k out among them,
 // a block at a time, and join their sums in LDS.  A wave loads eight rows' 128
 // bytes an instruction and turns them in LDS of its own into the matrix cores'
 // order (16 rows' 16 bytes): loaded in that order, neighbouring lanes are
 // different rows and each is a request of its own.
-template <typename T, bool EXPERTS, int TM, int TN, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) matmul_rows(MatmulArgs a) {
+template <typename T, bool EXPERTS, int TM, int TN>
+__global__ void __launch_bounds__(512) matmul_rows(MatmulArgs a) {
+    constexpr int WAVES = 8;
     constexpr int kPieces = 2 * (TM + TN);  // loads of eight rows a block: 2 TM of a, then 2 TN of b
     constexpr int kAhead = kPieces <= 4 ? 4 : kPieces <= 8 ? 2 : 1;  // blocks loaded together
     constexpr int kTurn = (kPieces > TM * TN ? kPieces : TM * TN) * 1024;
@@ -268,6 +283,304 @@ __global__ void __launch_bounds__(64 * WAVES) matmul_rows(MatmulArgs a) {
     }
 }
 
+// 16 bytes a lane from base + offset into LDS, lane after lane from `to` on,
+// which is one for the wave.  The builtin for it makes the next read of any LDS
+// wait for the load; here wait_all() does, ahead of the reads of what was loaded.
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+    return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
+}
+__device__ __forceinline__ void load_lds16(const void *base, unsigned offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+// A barrier ahead of which every wave's loads into LDS have arrived.
+__device__ __forceinline__ void wait_all() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// WAVES_M x WAVES_N waves, each TJ x TI tiles of 16 x 16 (rows by channels), take
+// a block of k a step; where such tiles are few, WAVES_K groups of them take a
+// block each and join their sums in the end.
+//
+// DIRECT: rows are whole runs of 16 bytes, which are loaded into one of two
+// buffers of LDS while the other is multiplied.  Otherwise they wait in registers
+// for a step between memory and LDS.
+template <typename T, bool EXPERTS, bool DIRECT, int WAVES_M, int WAVES_N, int WAVES_K, int TJ, int TI>
+__global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ? 2 : sizeof(T) == 4 || WAVES_N == 4 ? 3 : 4)
+    matmul_tiles(MatmulArgs a) {
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int kWaves = WAVES_M * WAVES_N, kThreads = 64 * kWaves;  // of a group
+    constexpr int BM = 16 * TJ * WAVES_M, BN = 16 * TI * WAVES_N, BK = 128;
+    constexpr int kA = BM * 8 / kThreads, kB = BN * 8 / kThreads, kPieces = kA + kB;  // 16-byte pieces a thread
+    constexpr int kPart = (BM + BN) * BK, kBuffer = kPart * WAVES_K;
+    constexpr int kScales = BM < 64 ? 64 : BM;
+    __shared__ __align__(16) uint8_t lds[2 * kBuffer];
+    __shared__ __align__(16) float row_scales[2][kScales][4];  // of four blocks of k
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), tid = wave * 64 + lane;
+    const int col = lane & 15, g = lane >> 4;
+    // Workgroups go to the eight XCDs in turn; each XCD takes a run of tiles,
+    // four tiles of rows by the channels one after the other, whose operands
+    // its L2 then holds for several of them.
+    int m0, end_m = a.m, expert = 0, nt;
+    {
+        int m_tiles = (a.m + BM - 1) / BM;
+        if constexpr (EXPERTS) m_tiles = tiles_of(a, BM);
+        const int tiles = m_tiles * a.n_tiles, per = tiles / 8, rest = tiles % 8;
+        const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
+        if (local >= per + (xcd < rest ? 1 : 0)) return;
+        const int at = xcd * per + min(xcd, rest) + local;
+        constexpr int kGroup = 4;
+        const int grp = at / (kGroup * a.n_tiles), in = at - grp * kGroup * a.n_tiles, height = min(kGroup, m_tiles - grp * kGroup);
+        const int mt = grp * kGroup + in % height;
+        nt = in / height;
+        m0 = mt * BM;
+        if constexpr (EXPERTS) {
+            const Rows r = rows_of(a, mt, BM);
+            if (r.expert < 0) return;
+            expert = r.expert;
+            m0 = r.first;
+            end_m = r.end;
+        }
+    }
+    const int n0 = nt * BN;
+    const int wm = wave / WAVES_N * (16 * TJ), wn = wave % WAVES_N * (16 * TI);
+    const int blocks = (a.k + BK - 1) / BK, steps = (blocks + WAVES_K - 1) / WAVES_K;
+    const auto input = [&](int r) -> unsigned {  // ~0: a row that is not there, for which the first is read
+        r = min(r, end_m - 1);
+        if constexpr (!EXPERTS) return r;
+        const unsigned at = a.order ? static_cast<unsigned>(a.order[r]) / static_cast<unsigned>(a.per_token) : r;
+        return at < a.a_rows ? at : 0xffffffffu;
+    };
+
+    // A thread's pieces of a step: kA of a, then kB of b, kThreads / 8 rows apart.
+    // Row r's piece p lies at place p ^ (r / 2 % 8): any 16 rows' pieces of one
+    // column are then on different banks.
+    const int place = tid & 7, piece = place ^ (tid / 16 & 7);
+    const uint8_t *pa = a.a, *pb = a.b + expert * a.b_expert + n0 * a.b_stride;
+    if constexpr (!EXPERTS) pa += m0 * a.a_stride;
+    unsigned offset[kPieces];
+#pragma unroll
+    for (int c = 0; c < kPieces; c++) {
+        const int r = tid / 8 + (c < kA ? c : c - kA) * (kThreads / 8);
+        if (c >= kA) offset[c] = static_cast<unsigned>(min(r, a.n - 1 - n0)) * static_cast<unsigned>(a.b_stride) + piece * 16;
+        else if (EXPERTS) offset[c] = (input(m0 + r) == 0xffffffffu ? 0 : input(m0 + r)) * static_cast<unsigned>(a.a_stride) + piece * 16;
+        else offset[c] = static_cast<unsigned>(min(r, a.m - 1 - m0)) * static_cast<unsigned>(a.a_stride) + piece * 16;
+    }
+    // Rows' scales, four blocks of a row a lane: a row at a time they are a request
+    // each, of 4 bytes as of 16.  The last four of a row may be some of those before.
+    constexpr int kRuns = kScales / 64;  // waves that load them
+    const int scale_row = wave % kRuns * 64 + lane;
+    const float *sa = a.a_scale;
+    unsigned scale_at = 0;
+    if constexpr (EXPERTS) {
+        const unsigned row = input(m0 + scale_row % BM);
+        scale_at = (row == 0xffffffffu ? 0 : row) * static_cast<unsigned>(a.sa_stride) * 4;
+    } else {
+        sa += m0 * a.sa_stride;
+        scale_at = static_cast<unsigned>(min(scale_row % BM, a.m - 1 - m0)) * static_cast<unsigned>(a.sa_stride) * 4;
+    }
+    const bool scaler = part == 0 && wave < kRuns;
+    const auto quad_from = [&](int q) { return max(min(4 * q, blocks - 4), 0); };
+    if (blocks < 4 && scaler) {
+        for (int t = 0; t < blocks; t++)
+            row_scales[0][scale_row][t] = *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(sa + t) + scale_at);
+    }
+    // DIRECT: a step's loads into its buffer
+    const auto load = [&](int s) {
+        const int t = s * WAVES_K + part;
+        // the lanes' offsets are added by the loads: sums made ahead of the loop would take two registers each
+        asm("" : "+v"(scale_at));
+#pragma unroll
+        for (int c = 0; c < kPieces; c++) asm("" : "+v"(offset[c]));
+        if (t % 4 == 0 && blocks >= 4 && scaler) load_lds16(sa + quad_from(t / 4), scale_at, lds_address(&row_scales[t / 4 & 1][wave * 64]));
+        const uint8_t *fa = pa + t * BK, *fb = pb + t * BK;
+        uint8_t *to = lds + (s & 1) * kBuffer + part * kPart + wave * 1024;
+        if (t * BK + BK <= a.k) {
+#pragma unroll
+            for (int c = 0; c < kPieces; c++) load_lds16(c < kA ? fa : fb, offset[c], lds_address(to) + c * (kThreads * 16));
+        } else if (t < blocks) {
+            // the last block of a row, not whole: zeros past its end (the row's first bytes are loaded there)
+            const int past = t * BK + piece * 16 >= a.k ? t * BK + piece * 16 : 0;
+            intx4 last[kPieces];
+#pragma unroll
+            for (int c = 0; c < kPieces; c++) last[c] = load16((c < kA ? fa : fb) + offset[c], -past);
+#pragma unroll
+            for (int c = 0; c < kPieces; c++) *reinterpret_cast<intx4 *>(to + lane * 16 + c * (kThreads * 16)) = past ? intx4{0, 0, 0, 0} : last[c];
+        }
+    };
+    // otherwise: into registers, and from there into LDS
+    intx4 staged[kPieces];
+    floatx4 quad;
+    const auto fetch = [&](int s) {
+        const int t = s * WAVES_K + part;
+#pragma unroll
+        for (int c = 0; c < kPieces; c++) asm("" : "+v"(offset[c]));
+        if (t % 4 == 0 && t < blocks && blocks >= 4 && scaler)
+            __builtin_memcpy(&quad, reinterpret_cast<const uint8_t *>(sa + quad_from(t / 4)) + scale_at, 16);
+        const uint8_t *fa = pa + t * BK, *fb = pb + t * BK;
+        if (t * BK + BK <= a.k) {
+#pragma unroll
+            for (int c = 0; c < kPieces; c++) __builtin_memcpy(&staged[c], (c < kA ? fa : fb) + offset[c], 16);
+        } else if (t < blocks) {
+            // what passes the row's end is its last 16 bytes, cleared where another piece has them
+            const int back = max(t * BK + piece * 16 + 16 - a.k, 0);
+            const intx4 keep = behind(back);
+#pragma unroll
+            for (int c = 0; c < kPieces; c++) staged[c] = load16((c < kA ? fa : fb) + offset[c], -static_cast<int64_t>(back)) & keep;
+        }
+    };
+    const auto store = [&](int s) {
+        const int t = s * WAVES_K + part;
+        uint8_t *to = lds + (s & 1) * kBuffer + part * kPart + tid * 16;
+#pragma unroll
+        for (int c = 0; c < kPieces; c++) *reinterpret_cast<intx4 *>(to + c * (kThreads * 16)) = staged[c];
+        // over those that were last read four blocks ago
+        if (t % 4 == 0 && t < blocks && blocks >= 4 && scaler) *reinterpret_cast<floatx4 *>(row_scales[t / 4 & 1][scale_row]) = quad;
+    };
+    // The weights' scales of 64 blocks, one a lane: a scalar load in every step would have each of its reads of LDS
+    // wait for it, too.
+    const float *sb = a.b_scale + expert * a.sb_expert + min(n0 + wn, a.n - 1) / 128 * a.sb_stride;
+    float sb_ahead = 0.0f;
+
+    floatx4 acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; i++)
+#pragma unroll
+        for (int j = 0; j < TJ; j++) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int at0 = col * BK + (g ^ (col / 2)) * 16, at1 = col * BK + ((4 + g) ^ (col / 2)) * 16;
+    const auto read = [&](const uint8_t *rows, Operand<kWide> &x) {
+        x.set(*reinterpret_cast<const intx4 *>(rows + at0), *reinterpret_cast<const intx4 *>(rows + at1));
+    };
+    // a wave whose rows or channels are all past the end leaves the matrix cores to the others
+    const bool active = m0 + wm < end_m && n0 + wn < a.n;
+    const auto step = [&](int s) {
+        const int t = s * WAVES_K + part;
+        const uint8_t *now = lds + (s & 1) * kBuffer + part * kPart;
+        if (t % 64 < WAVES_K) {
+            sb_ahead = sb[min(t / 64 * 64 + lane, blocks - 1)];
+            asm volatile("" : "+v"(sb_ahead));  // waited for here, not in every step
+        }
+        const float sb_now = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sb_ahead), t % 64));
+        if (active && (WAVES_K == 1 || t < blocks)) {
+            Operand<kWide> fa[TJ], fb[2];
+            float scale[TJ];
+            read(now + (BM + wn) * BK, fb[0]);
+#pragma unroll
+            for (int j = 0; j < TJ; j++) read(now + (wm + 16 * j) * BK, fa[j]);
+#pragma unroll
+            for (int j = 0; j < TJ; j++) scale[j] = row_scales[t / 4 & 1][wm + 16 * j + col][t - quad_from(t / 4)];
+            if constexpr (!kWide) __builtin_amdgcn_sched_barrier(0);
+            // a product, and the sums of the one two before it, which has ended
+            floatx4 sum[3];
+            const auto add = [&](int p) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[p / TJ][p % TJ][e] = __builtin_fmaf(scale[p % TJ], sum[p % 3][e], acc[p / TJ][p % TJ][e]);
+            };
+#pragma unroll
+            for (int i = 0; i < TI; i++) {
+#pragma unroll
+                for (int j = 0; j < TJ; j++) {
+                    const int p = i * TJ + j;
+                    sum[p % 3] = product(fb[i & 1], fa[j]);
+                    if constexpr (!kWide) __builtin_amdgcn_sched_barrier(0);
+                    if (j == 0 && i + 1 < TI) read(now + (BM + wn + 16 * (i + 1)) * BK, fb[(i + 1) & 1]);
+                    if (p < TJ) scale[j] *= sb_now;
+                    if (p > 1) add(p - 2);
+                    if constexpr (!kWide) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            add(TI * TJ - 2);
+            add(TI * TJ - 1);
+        }
+    };
+    if constexpr (DIRECT) {
+        if (steps > 0) load(0);
+        for (int s = 0; s < steps; s++) {
+            // the barrier also ends the reads of the step before, whose buffer is loaded next
+            wait_all();
+            if (s + 1 < steps) load(s + 1);
+            step(s);
+        }
+    } else if (steps > 0) {
+        fetch(0);
+        store(0);
+        if (steps > 1) fetch(1);
+        for (int s = 0; s < steps; s++) {
+            __syncthreads();
+            if (s + 1 < steps) store(s + 1);
+            if (s + 2 < steps) fetch(s + 2);
+            step(s);
+        }
+    }
+    __syncthreads();
+    if constexpr (WAVES_K > 1) {
+        // the groups' sums, joined in their order
+        floatx4 *sums = reinterpret_cast<floatx4 *>(lds);
+        static_assert((WAVES_K - 1) * BM * BN * 4 <= 2 * kBuffer, "LDS holds the groups' sums");
+        if (part > 0) {
+#pragma unroll
+            for (int i = 0; i < TI; i++)
+#pragma unroll
+                for (int j = 0; j < TJ; j++) sums[((part - 1) * TI * TJ + i * TJ + j) * kThreads + tid] = acc[i][j];
+        }
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int j = 0; j < TJ; j++)
+#pragma unroll
+                for (int w = 1; w < WAVES_K; w++) acc[i][j] += sums[((w - 1) * TI * TJ + i * TJ + j) * kThreads + tid];
+        // this group's waves write over others' sums
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    // 16 rows at a time through this wave's own part of LDS (every wave is past
+    // its last read of the buffers), so that a row's channels leave as 16-byte
+    // pieces one after the other
+    constexpr int kCols = 16 * TI, kPiece = 16 / static_cast<int>(sizeof(T)), kPitch = kCols + kPiece;
+    static_assert(16 * kPitch * sizeof(T) <= 2 * kBuffer / kWaves, "a wave's part of LDS holds 16 rows");
+    T *mine = reinterpret_cast<T *>(lds + wave * (2 * kBuffer / kWaves));
+    const int left = a.n - n0 - wn;
+#pragma unroll
+    for (int j = 0; j < TJ; j++) {
+        const int m = m0 + wm + 16 * j;
+        if (m >= end_m) break;
+        const bool there = !EXPERTS || input(m + col) != 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < TI; i++) {
+            float v[4];
+            const int n = 16 * i + 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (there ? acc[i][j][e] : 0.0f) + (a.bias && n + e < left ? a.bias[static_cast<int64_t>(expert) * a.n + n0 + wn + n + e] : 0.0f);
+            put_floats<4>(mine + col * kPitch + n, v);
+        }
+        wait_lds();
+        constexpr int kLanes = kCols / kPiece, kRows = 64 / kLanes;
+        const int c = lane % kLanes * kPiece;
+#pragma unroll
+        for (int r = 0; r < 16; r += kRows) {
+            const int row = r + lane / kLanes;
+            if (row < 16 && m + row < end_m) {
+                const Vec<T, kPiece> v = *reinterpret_cast<const Vec<T, kPiece> *>(mine + row * kPitch + c);
+                T *out = static_cast<T *>(a.out) + (m + row) * a.out_stride + n0 + wn + c;
+                if (c + kPiece <= left) {
+                    __builtin_memcpy(out, v.v, sizeof(v.v));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPiece; e++)
+                        if (c + e < left) out[e] = v.v[e];
+                }
+            }
+        }
+        wait_lds();
+    }
+}
+
 int check(const Spkv2MatmulF8 *g, bool experts, bool pointers) {
     if (!g) return bad("matmul_f8: no arguments");
     if (!is_dtype(g->dtype)) return bad("matmul_f8: unknown dtype");
@@ -300,43 +613,135 @@ int check(const Spkv2MatmulF8Experts *g, bool pointers) {
 
 MatmulArgs arguments(const Spkv2MatmulF8 &g) {
     MatmulArgs a{g.a, g.b, g.a_scale, g.b_scale, g.bias, g.out, g.a_stride, g.b_stride, g.out_stride, g.a_scale_stride, g.b_scale_stride,
-                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), nullptr, nullptr, g.m, 0, 0, 1, 1};
-    if (g.m == 1) a.out_stride = 0;
+                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), 0, nullptr, nullptr, g.m, 0, 0, 1, 1};
+    if (g.m == 1) a.a_stride = 0, a.sa_stride = 0, a.out_stride = 0;
     if (g.n == 1) a.b_stride = 0;
     if (g.n <= 128) a.sb_stride = 0;
     return a;
 }
 
-struct Form {
-    int tokens, channels, waves;  // of a workgroup; waves that deal k out
+// A kernel's time: a launch's, then steps by every workgroup, of a block of k for
+// each of its groups of waves, which take `step` each where a CU's workgroups do
+// not fill it, or `work` for each of the CU's workgroups where they do, and the
+// workgroup's sums.  Fitted, in us, to 1100 products of log-uniform sizes (m 1 ..
+// 8192, n and k 64 .. 16384, up to 2^37 multiplications; half of them by expert):
+// the kernel of the least time by these is 2.4% slower than the fastest of
+// fourteen in the mean, 30% in one of a hundred.
+struct Cost {
+    float launch, step, work, sums;
 };
-constexpr Form kForms[] = {{16, 16, 8}, {64, 64, 4}};
+struct Form {
+    int tokens, channels, groups;  // of a workgroup; groups of waves that deal k out
+    bool tiles;
+    Cost cost[4];  // 16-bit outputs with rows of whole runs of 16 bytes, and others; fp32 outputs likewise
+};
+constexpr Form kForms[] = {
+    {16, 16, 8, false, {{1.23f, 0.550f, 0.630f, 1.655f}, {1.30f, 0.956f, 0.905f, 1.321f}, {1.16f, 0.666f, 0.701f, 1.710f}, {1.22f, 0.987f, 0.915f, 1.581f}}},
+    {16, 32, 8, false, {{1.67f, 0.818f, 1.007f, 1.048f}, {1.82f, 0.818f, 1.332f, 0.758f}, {1.56f, 0.484f, 1.071f, 1.164f}, {1.80f, 0.313f, 1.378f, 0.946f}}},
+    {16, 64, 8, false, {{1.55f, 0.180f, 1.584f, 0.975f}, {2.00f, 2.140f, 2.154f, 0.378f}, {1.60f, 1.575f, 1.622f, 1.063f}, {1.79f, 0.005f, 2.254f, 0.669f}}},
+    {32, 64, 8, false, {{0.37f, 1.013f, 1.866f, 2.328f}, {0.81f, 1.143f, 2.548f, 1.718f}, {0.53f, 1.752f, 2.063f, 2.287f}, {0.73f, 1.028f, 2.698f, 1.963f}}},
+    {64, 64, 1, true, {{3.10f, 0.382f, 0.277f, 1.069f}, {2.76f, 0.788f, 0.435f, 1.129f}, {3.21f, 0.496f, 0.325f, 1.247f}, {2.85f, 0.920f, 0.472f, 1.406f}}},
+    {64, 64, 2, true, {{2.18f, 0.542f, 0.514f, 2.152f}, {2.05f, 1.152f, 0.896f, 1.863f}, {2.18f, 0.741f, 0.627f, 2.309f}, {2.02f, 1.323f, 0.998f, 2.152f}}},
+    {64, 64, 4, true, {{0.00f, 0.621f, 0.965f, 4.945f}, {0.00f, 1.107f, 1.950f, 4.079f}, {0.00f, 1.018f, 1.272f, 5.070f}, {0.00f, 1.532f, 2.107f, 4.626f}}},
+    {32, 128, 1, true, {{3.05f, 0.428f, 0.344f, 1.235f}, {2.68f, 0.930f, 0.587f, 1.236f}, {2.92f, 0.530f, 0.374f, 1.561f}, {2.43f, 1.057f, 0.589f, 1.668f}}},
+    {128, 128, 1, true, {{3.42f, 0.418f, 0.652f, 3.066f}, {1.57f, 1.382f, 0.944f, 4.299f}, {2.25f, 1.076f, 0.893f, 4.346f}, {1.95f, 2.031f, 1.358f, 4.122f}}},
+    {256, 256, 1, true, {{0.00f, 0.100f, 1.110f, 10.122f}, {0.00f, 0.100f, 2.104f, 9.616f}, {}, {}}},
+};
+constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
 
-int form(int64_t m) { return m <= 16 ? 0 : 1; }
+// Workgroups along the rows.  By expert: at most, for the launch; about, for the time.
+int64_t most_down(const MatmulArgs &a, bool experts, int height) {
+    return experts ? a.m / height + std::min(a.experts, a.m) : (static_cast<int64_t>(a.m) + height - 1) / height;
+}
+double about_down(const MatmulArgs &a, bool experts, int height) {
+    if (!experts) return static_cast<double>(most_down(a, false, height));
+    // experts that rows chosen at random leave without one, and half a workgroup's rows missing of each other's last
+    const double used = a.experts * (1.0 - pow(1.0 - 1.0 / a.experts, a.m)), each = a.m / used;
+    return ceil(each < 0.5 * height ? used : used * (each / height + 0.5));
+}
+
+// whether rows are whole runs of 16 bytes at such addresses, as loads into LDS take them
+bool whole(const MatmulArgs &a) {
+    return a.k % 16 == 0 && aligned(a.a, 16) && aligned(a.b, 16) && a.a_stride % 16 == 0 && a.b_stride % 16 == 0 && a.b_expert % 16 == 0;
+}
+
+// the kernel of a call that check() took, as an index of kForms; -1: none
+int form(const MatmulArgs &a, bool experts, int dtype) {
+    const int kind = (dtype == SPKV2_DTYPE_FP32 ? 2 : 0) + (whole(a) ? 0 : 1);
+    // tiles hold offsets of a workgroup's rows (by expert, of all rows of a) in 32 bits
+    const int64_t held = experts ? a.a_rows : std::min(a.m, 256);
+    const bool near = held * a.a_stride < (int64_t(1) << 31) && held * a.sa_stride < (int64_t(1) << 29) && 256 * a.b_stride < (int64_t(1) << 31);
+    const int blocks = (a.k + 127) / 128;
+    int best = -1;
+    double least = 0.0;
+    for (int i = 0; i < kFormCount; i++) {
+        const Form &f = kForms[i];
+        const int64_t across = (static_cast<int64_t>(a.n) + f.channels - 1) / f.channels, down = most_down(a, experts, f.tokens);
+        // a launch has fewer than 2^32 threads along an axis, and as many workgroups along the second as 16 bits hold
+        if (f.tiles ? !near || a.k < 16 || down * across >= 1 << 22 : down > 65535) continue;
+        if (f.tokens == 256 && dtype == SPKV2_DTYPE_FP32) continue;  // two registers' operands do not fit beside its sums
+        const Cost &c = f.cost[kind];
+        const double steps = (blocks + f.groups - 1) / f.groups, each = ceil(about_down(a, experts, f.tokens) * across / 256.0);
+        const double time = c.launch + steps * std::max(static_cast<double>(c.step), each * c.work) + each * c.sums;
+        if (best < 0 || time < least) least = time, best = i;
+    }
+    return best;
+}
 
 template <bool EXPERTS>
-int run(const char *what, int dtype, const MatmulArgs &a, void *stream) {
+int run(const char *what, int dtype, MatmulArgs a, void *stream) {
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        auto rows = [&](auto kernel, int tm, int tn, int waves) {
-            int64_t down = (static_cast<int64_t>(a.m) + 16 * tm - 1) / (16 * tm);
-            // an expert's last workgroup may be partly empty
-            if (EXPERTS) down = a.m / (16 * tm) + std::min(a.experts, a.m);
-            if (down > 65535) return unsupported("matmul_f8: too many rows for one launch");
-            const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.n) + 16 * tn - 1) / (16 * tn)), static_cast<unsigned>(down));
-            return launch(what, kernel, grid, dim3(64 * waves), stream, a);
+        const int i = form(a, EXPERTS, dtype);
+        if (i < 0) return unsupported("matmul_f8: too many rows or channels for one launch");
+        const Form &f = kForms[i];
+        const unsigned across = static_cast<unsigned>((static_cast<int64_t>(a.n) + f.channels - 1) / f.channels);
+        const unsigned down = static_cast<unsigned>(most_down(a, EXPERTS, f.tokens));
+        a.n_tiles = static_cast<int>(across);
+        auto rows = [&](auto kernel) { return launch(what, kernel, dim3(across, down), dim3(64 * 8), stream, a); };
+        auto tiles = [&](auto direct, auto staged, int waves) {
+            return launch(what, whole(a) ? direct : staged, dim3(across * down), dim3(64 * waves), stream, a);
         };
-        if (form(a.m) == 0) return rows(matmul_rows<T, EXPERTS, 1, 1, 8>, 1, 1, 8);
-        return rows(matmul_rows<T, EXPERTS, 4, 4, 4>, 4, 4, 4);
+        switch (i) {
+            case 0: return rows(matmul_rows<T, EXPERTS, 1, 1>);
+            case 1: return rows(matmul_rows<T, EXPERTS, 1, 2>);
+            case 2: return rows(matmul_rows<T, EXPERTS, 1, 4>);
+            case 3: return rows(matmul_rows<T, EXPERTS, 2, 4>);
+            case 4: return tiles(matmul_tiles<T, EXPERTS, true, 2, 2, 1, 2, 2>, matmul_tiles<T, EXPERTS, false, 2, 2, 1, 2, 2>, 4);
+            case 5: return tiles(matmul_tiles<T, EXPERTS, true, 2, 2, 2, 2, 2>, matmul_tiles<T, EXPERTS, false, 2, 2, 2, 2, 2>, 8);
+            case 6: return tiles(matmul_tiles<T, EXPERTS, true, 2, 2, 4, 2, 2>, matmul_tiles<T, EXPERTS, false, 2, 2, 4, 2, 2>, 16);
+            case 7: return tiles(matmul_tiles<T, EXPERTS, true, 1, 4, 1, 2, 2>, matmul_tiles<T, EXPERTS, false, 1, 4, 1, 2, 2>, 4);
+            case 8: return tiles(matmul_tiles<T, EXPERTS, true, 2, 2, 1, 4, 4>, matmul_tiles<T, EXPERTS, false, 2, 2, 1, 4, 4>, 4);
+            default:
+                if constexpr (sizeof(T) == 4) return -1;
+                else return tiles(matmul_tiles<T, EXPERTS, true, 4, 2, 1, 4, 8>, matmul_tiles<T, EXPERTS, false, 4, 2, 1, 4, 8>, 8);
+        }
     });
 }
 
-int name(const Spkv2MatmulF8 &g, char *buf, size_t size) {
+int name(const MatmulArgs &a, bool experts, int dtype, char *buf, size_t size) {
     buf[0] = 0;
-    if (g.m == 0 || g.n == 0) return 0;
-    const Form &f = kForms[form(g.m)];
-    snprintf(buf, size, "matmul_rows<%dx%d,waves=%d>", f.tokens, f.channels, f.waves);
+    if (a.m == 0 || a.n == 0) return 0;
+    const int i = form(a, experts, dtype);
+    if (i < 0) return unsupported("matmul_f8: too many rows or channels for one launch");
+    const Form &f = kForms[i];
+    if (f.tiles) snprintf(buf, size, "matmul_tiles<%dx%d,groups=%d,%s>", f.tokens, f.channels, f.groups, whole(a) ? "direct" : "staged");
+    else snprintf(buf, size, "matmul_rows<%dx%d>", f.tokens, f.channels);
     return 0;
+}
+
+MatmulArgs arguments(const Spkv2MatmulF8Experts &g) {
+    MatmulArgs a = arguments(g.product);
+    a.offsets = g.offsets;
+    a.order = g.order;
+    a.a_rows = g.a_rows;
+    a.b_expert = g.experts > 1 ? g.b_expert_stride : 0;
+    a.sb_expert = g.experts > 1 ? g.b_scale_expert_stride : 0;
+    a.experts = g.experts;
+    a.per_token = g.per_token;
+    a.a_stride = g.product.a_stride, a.sa_stride = g.product.a_scale_stride;
+    if (g.a_rows == 1) a.a_stride = 0, a.sa_stride = 0;
+    return a;
 }
 
 }  // namespace
@@ -349,9 +754,7 @@ extern "C" int spkv2_mi355x_matmul_f8(const Spkv2MatmulF8 *g, void *stream) {
     return entry([&]() -> int {
         if (int rc = check(g, false, true)) return rc;
         if (g->m == 0 || g->n == 0) return 0;
-        MatmulArgs a = arguments(*g);
-        if (g->m == 1) a.a_stride = 0, a.sa_stride = 0;
-        return run<false>("matmul_f8", g->dtype, a, stream);
+        return run<false>("matmul_f8", g->dtype, arguments(*g), stream);
     });
 }
 
@@ -359,16 +762,7 @@ extern "C" int spkv2_mi355x_matmul_f8_experts(const Spkv2MatmulF8Experts *g, voi
     return entry([&]() -> int {
         if (int rc = check(g, true)) return rc;
         if (g->product.m == 0 || g->product.n == 0) return 0;
-        MatmulArgs a = arguments(g->product);
-        a.offsets = g->offsets;
-        a.order = g->order;
-        a.a_rows = g->a_rows;
-        a.b_expert = g->experts > 1 ? g->b_expert_stride : 0;
-        a.sb_expert = g->experts > 1 ? g->b_scale_expert_stride : 0;
-        a.experts = g->experts;
-        a.per_token = g->per_token;
-        if (g->a_rows == 1) a.a_stride = 0, a.sa_stride = 0;
-        return run<true>("matmul_f8_experts", g->product.dtype, a, stream);
+        return run<true>("matmul_f8_experts", g->product.dtype, arguments(*g), stream);
     });
 }
 
@@ -376,7 +770,7 @@ extern "C" int spkv2_mi355x_matmul_f8_kernel_name(const Spkv2MatmulF8 *g, char *
     return entry([&]() -> int {
         if (!buf || !buf_size) return bad("matmul_f8: nowhere to put the name");
         if (int rc = check(g, false, false)) return rc;
-        return name(*g, buf, buf_size);
+        return name(arguments(*g), false, g->dtype, buf, buf_size);
     });
 }
 
@@ -384,6 +778,6 @@ extern "C" int spkv2_mi355x_matmul_f8_experts_kernel_name(const Spkv2MatmulF8Exp
     return entry([&]() -> int {
         if (!buf || !buf_size) return bad("matmul_f8_experts: nowhere to put the name");
         if (int rc = check(g, false)) return rc;
-        return name(g->product, buf, buf_size);
+        return name(arguments(*g), true, g->product.dtype, buf, buf_size);
     });
 }

@@ -250,3 +250,50 @@ def test_float8_rounding():
     np.testing.assert_array_equal(decoder.to_float8(half * (1 - 1e-9)), np.arange(126))
     np.testing.assert_array_equal(decoder.to_float8(-half * (1 + 1e-9)), np.arange(1, 127) | 128)
     assert decoder.to_float8([np.inf, np.nan, 500, 464, -0.0]).tolist() == [127, 127, 127, 126, 128]
+
+
+# ------------------------------------------------------- which kernel a call takes
+
+FORMS = ["rows<16x16>", "rows<16x32>", "rows<16x64>", "rows<32x64>"] + [
+    f"tiles<{tile},{how}>" for tile in ("64x64,groups=1", "64x64,groups=2", "64x64,groups=4", "32x128,groups=1", "128x128,groups=1", "256x256,groups=1")
+    for how in ("direct", "staged")]
+TYPES = {"float32": FP32, "float16": FP16, "bfloat16": BF16}
+
+
+def kernel_of(dtype, m, n, k, experts=0, a_rows=0, pad=0):
+    """The kernel that a product of contiguous rows (rows `pad` elements apart) takes."""
+    name = ctypes.create_string_buffer(64)
+    blocks = -(-k // 128)
+    a = dict(m=m, n=n, k=k, a_stride=k + pad, b_stride=k + pad, out_stride=n, a_scale_stride=blocks, b_scale_stride=blocks, dtype=TYPES[dtype])
+    lib = load_library()
+    if experts:
+        a.update(a_rows=a_rows, b_expert_stride=n * (k + pad), b_scale_expert_stride=-(-n // 128) * blocks, experts=experts, per_token=1)
+        rc = lib.spkv2_mi355x_matmul_f8_experts_kernel_name(ctypes.byref(decoder._MatmulF8Experts(**a)), name, 64)
+    else:
+        rc = lib.spkv2_mi355x_matmul_f8_kernel_name(ctypes.byref(decoder._MatmulF8(**a)), name, 64)
+    assert rc == 0
+    return name.value.decode()
+
+
+def sizes_of_kernels(dtype, by_expert):
+    """For each kernel that some call takes, the smallest sizes found that take it, none of them a multiple of a tile."""
+    found = {}
+    for rows in (1, 3, 9, 18, 33, 50, 70, 100, 130, 200, 300, 520, 700, 1030, 1500, 2100, 3000, 4100):
+        for n in (17, 33, 65, 100, 130, 190, 260, 390, 515, 770, 1029, 2050, 4100):
+            for k in (47, 48, 129, 144, 300, 304, 513, 528, 1030, 1040, 2050, 2064, 4100, 4112, 8200, 8208):
+                for experts in ((1, 3, 7, 40) if by_expert else (0,)):
+                    if rows * n * k * max(experts, 1) > 4e9 or rows * n > 1.7e7:
+                        continue
+                    kernel = kernel_of(dtype, rows, n, k, experts, rows)
+                    size = rows * n * k + experts * n * k * 20
+                    if kernel not in found or size < found[kernel][0]:
+                        found[kernel] = (size, rows, n, k, experts)
+    return {kernel: v[1:] for kernel, v in found.items()}
+
+
+@pytest.mark.parametrize("by_expert", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_every_kernel_is_some_calls(dtype, by_expert):
+    wanted = {"matmul_" + f for f in FORMS if not (dtype == "float32" and "256x256" in f)}
+    missing = wanted - set(sizes_of_kernels(dtype, by_expert))
+    assert not missing, missing

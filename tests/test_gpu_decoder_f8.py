@@ -15,6 +15,7 @@ import pytest
 from spinnv2_amd import decoder
 from spinnv2_amd.decoder import DeviceArray as Array, KvCache, _FLOAT8, to_float8
 
+from .test_decoder_f8 import FORMS, kernel_of, sizes_of_kernels
 from .test_gpu_decoder import HALF, SMALLEST, Hip, gaps, rounded, strided
 
 pytestmark = pytest.mark.gpu
@@ -348,6 +349,21 @@ def test_matmul_variants(gpu, m, n, k, kw, dtype):
     _matmul_case(m, n, k, dtype, **kw)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_every_kernel_of_the_product(gpu, form, dtype):
+    """Each kernel at the smallest sizes that take it, with rows apart, a bias, a row of NaN and codes behind the rows' ends."""
+    sizes = sizes_of_kernels(dtype, False)
+    if "matmul_" + form not in sizes:
+        assert dtype == "float32" and "256x256" in form
+        return
+    m, n, k, _ = sizes["matmul_" + form]
+    _matmul_case(m, n, k, dtype)
+    pad = 0 if k % 16 else 16
+    if kernel_of(dtype, m, n, k, pad=pad) == "matmul_" + form:
+        _matmul_case(m, n, k, dtype, pad=pad, at=pad, bias=True, seed=2)
+
+
 def test_matmul_of_nothing(gpu):
     """k = 0: the bias alone, or zeros."""
     out = Array.of(np.full((3, 5), 9.0), "float32")
@@ -513,6 +529,32 @@ def _ids(rng, tokens, per_token, experts, kind):
 def test_experts(gpu, tokens, per_token, experts, n, k, kind, dtype):
     ids = _ids(np.random.default_rng(tokens), tokens, per_token, experts, kind)
     _experts_case(ids, experts, n, k, dtype, spare=5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_every_kernel_of_the_experts_product(gpu, form, dtype):
+    """Each kernel at the smallest sizes that take it, the experts of ragged counts of rows."""
+    sizes = sizes_of_kernels(dtype, True)
+    if "matmul_" + form not in sizes:
+        assert dtype == "float32" and "256x256" in form
+        return
+    m, n, k, experts = sizes["matmul_" + form]
+    rng = np.random.default_rng(m)
+    ids = np.minimum(rng.integers(0, experts, (m, 1)), rng.integers(0, experts, (m, 1))).astype(np.int32)
+    assert kernel_of(dtype, m, n, k, experts, m) == "matmul_" + form
+    _experts_case(ids, experts, n, k, dtype)
+
+
+def test_experts_rows_of_one_token(gpu):
+    """One output row, whose input is not the first of several."""
+    rng = np.random.default_rng(4)
+    a, b = _whole(rng, (4, 144)), _whole(rng, (2, 20, 144))
+    sa, sb = _twos(rng, (4, 2)), _twos(rng, (2, 1, 2))
+    out = Array((1, 20), "float32")
+    decoder.matmul_f8_experts(Array.of(a, F8), Array.of(sa, "float32"), Array.of(b, F8), Array.of(sb, "float32"),
+                              Array.of(np.array([0, 0, 1], np.int32)), out, order=Array.of(np.array([3], np.int32)))
+    np.testing.assert_array_equal(out.download(), _product(a[3:], sa[3:], b[1], sb[1]))
 
 
 @pytest.mark.parametrize("kw", [dict(by_order=False), dict(bias=True), dict(pad=3), dict(pad=16, bias=True, by_order=False)])
