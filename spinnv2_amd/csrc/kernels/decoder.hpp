@@ -157,41 +157,54 @@ __device__ __forceinline__ void quantise(const P (&x)[N], P top, int8_t (&q)[N])
 // without its sign: 0 <= x <= top, both of at most 48 bits.  The quotient is a
 // number of steps, 2^-9 or its power of two's eighth, of which a double gives the
 // integer part n (or, where it rounds up to it, n of the border below); whether
-// the border n + 1/2 is passed is one fused product, whose sign is exact.
+// the border n + 1/2 is passed is one fused product, whose sign is exact.  Where x
+// and top are themselves rounded to 64 bits (EXACT = false), a quotient within 2^-49
+// of a border is taken for a tie, which it then nearly always is in truth.
+template <bool EXACT>
 __device__ __forceinline__ unsigned exact_code_f8(double x, double top) {
     const double y = x * 448.0 / top;
     const int e = y < 0x1p-6 ? -6 : min(ilogb(y), 8);
     const double step = ldexp(1.0, e - 3), n = floor(ldexp(y, 3 - e));
-    const double rest = __builtin_fma(-(n + 0.5) * step, top, 448.0 * x);
+    double rest = EXACT ? __builtin_fma(-(n + 0.5) * step, top, 448.0 * x) : y - (n + 0.5) * step;
+    if (!EXACT && fabs(rest) <= y * 0x1p-49) rest = 0.0;
     const unsigned whole = static_cast<unsigned>(n);
     return static_cast<unsigned>((e + 6) * 8) + whole + (rest > 0.0 || (rest == 0.0 && (whole & 1)) ? 1u : 0u);
 }
 
-// Two floats as 8-bit floats, in bytes 0 and 1, rounded to the nearest, ties to even
-__device__ __forceinline__ unsigned two_f8(float a, float b) {
-    return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false)) & 0xffffu;
+// Four floats as 8-bit floats, rounded to the nearest, ties to even
+__device__ __forceinline__ unsigned four_f8(float a, float b, float c, float d) {
+    return static_cast<unsigned>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true));
 }
 
-// Codes of 448 v / top of N values, |v| <= top, both within 2^-(SLACK + 2) of
+// Codes of 448 v / top of eight values, |v| <= top, both within 2^-(SLACK + 2) of
 // their values in 64 bits.  The quotient in fp32, of four roundings more, is then
 // within 2^-SLACK: where it and what lies that far on both sides have one code,
-// that is it.  Returns a bit for each of the others, which have to be divided in
-// 64 bits; so have all where top is so small or large that quotients lose bits.
-template <int N, int SLACK>
-__device__ __forceinline__ unsigned quantise_f8(const float (&v)[N], float top, uint8_t (&q)[N]) {
-    constexpr float kLess = 1.0f - 1.0f / (1 << SLACK), kMore = 1.0f + 1.0f / (1 << SLACK);
-    const float inv = 448.0f / top;
-    unsigned near = 0;
+// that is it.  Returns whether some have not, or all may not since top is so small
+// or large that quotients lose bits; beside_f8() says which.
+template <int SLACK>
+struct F8 {
+    static constexpr float kLess = 1.0f - 1.0f / (1 << SLACK), kMore = 1.0f + 1.0f / (1 << SLACK);
+    static __device__ __forceinline__ bool plain(float top) { return top > 0x1p-90f && top < 0x1p120f; }
+    static __device__ __forceinline__ bool quantise(const float (&v)[8], float top, unsigned (&q)[2]) {
+        const float inv = 448.0f / top;
+        unsigned differ = 0;
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-        const float a = v[j] * inv, b = v[j + 1] * inv;
-        const unsigned code = two_f8(a * kLess, b * kLess), differ = code ^ two_f8(a * kMore, b * kMore);
-        q[j] = static_cast<uint8_t>(code);
-        q[j + 1] = static_cast<uint8_t>(code >> 8);
-        near |= (differ & 0xffu ? 1u << j : 0u) | (differ >> 8 ? 2u << j : 0u);
+        for (int h = 0; h < 2; h++) {
+            float t[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] = v[4 * h + j] * inv;
+            q[h] = four_f8(t[0] * kLess, t[1] * kLess, t[2] * kLess, t[3] * kLess);
+            differ |= q[h] ^ four_f8(t[0] * kMore, t[1] * kMore, t[2] * kMore, t[3] * kMore);
+        }
+        return differ || !plain(top);
     }
-    return top > 0x1p-90f && top < 0x1p120f ? near : (1u << N) - 1u;
-}
+    // whether a value's quotient lies beside the border of two codes
+    static __device__ __forceinline__ bool beside(float v, float top) {
+        const float t = v * (448.0f / top);
+        const unsigned codes = four_f8(t * kLess, t * kMore, 0.0f, 0.0f);
+        return !plain(top) || (codes & 0xffu) != (codes >> 8 & 0xffu);
+    }
+};
 
 // The largest of v over groups of LANES neighbouring lanes (8, 16 or 32), in
 // each of them: within 16 by lane moves of the adder's own, past that by LDS's

@@ -7,10 +7,17 @@
 // lanes take the sines and cosines of the pairs, which every head of the token
 // turns by, and groups of 8, 16 or 32 lanes a head each, 8 elements a lane.
 //
+// Bound by HBM and by its arithmetic, each two thirds of the time: 8190 tokens of
+// 32 + 8 heads of 128 in bf16, values too, into the cache in 48 us (185 MB, 3.9
+// TB/s), without a cache in 38 (168 MB, 4.4 TB/s); fp32 without a cache at 5.2
+// TB/s.
+//
 // In 64 bits: angles of far positions need it (position 70001 times a frequency
 // near 1 keeps 7 bits behind the point in fp32), and a key beside the border of
 // two bf16 values or two codes falls on its own side.  The vector units take
 // 64-bit products at the rate of 32-bit ones.
+#include <type_traits>
+
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -77,17 +84,57 @@ __device__ __forceinline__ double sum_over(double v) {
     return v;
 }
 
+// 1 / sqrt(v): the hardware's estimate of 2^-26 and a step of Newton's method, within 2^-51; infinite for 0
+__device__ __forceinline__ double inverse_root(double v) {
+    const double r = __builtin_amdgcn_rsq(v);
+    const double better = __builtin_fma(r * 0.5, __builtin_fma(-v * r, r, 1.0), r);
+    return v > 0.0 && v < __builtin_inf() ? better : r;
+}
+
+// Eight values rounded to T, as floats.  By way of fp32, rounded twice, unless one
+// of them may lie on a tie there, which is then taken straight from 64 bits: one
+// in thirty thousand of bf16, one in four thousand of fp16.
+template <typename T>
+__device__ __forceinline__ void rounded(const double (&v)[8], float (&y)[8]) {
+    // bits that are all 0 where a value may lie on a tie
+    constexpr unsigned kBelow = __is_same(T, __bf16) ? 0x7fffu : 0xfffu;
+    unsigned least = ~0u;
+    float smallest = 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        y[j] = static_cast<float>(v[j]);
+        least = min(least, __float_as_uint(y[j]) & kBelow);
+        smallest = fminf(smallest, fabsf(y[j]));
+    }
+    // fp16 values below 2^-14 have their ties elsewhere
+    const bool tie = least == 0 || (__is_same(T, _Float16) && smallest < 0x1p-14f);
+    if constexpr (sizeof(T) == 2) {
+        if (__any(tie)) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = static_cast<float>(static_cast<T>(v[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = static_cast<float>(static_cast<T>(y[j]));
+        }
+    }
+}
+
 // What a lane's 8 elements are multiplied by, and their partners: y = norm (x own + partner other)
 struct Turn {
     double own[8], other[8];
 };
 
-// PAIRED: a lane's elements have their partners in one lane: pairs side by side, or a multiple of 8 apart
-template <typename T, typename W, int LANES, bool PAIRED>
+// A lane's 8 elements of a head: four pairs, side by side (kBeside) or four of each
+// half (kApart: a multiple of 4 apart), or eight in a row whose partners other lanes
+// have (kAny), which LDS passes on.  Through LDS as well, pairs a multiple of 8 apart
+// took 8190 tokens of 32 + 8 heads of 128 to 56 us.
+enum Pairing { kBeside, kApart, kAny };
+
+template <typename T, typename W, int LANES, Pairing PAIRING>
 __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
     constexpr int kGroups = 64 / LANES, kDim = LANES * 8;
     __shared__ __align__(16) double table[4][2][128];
-    __shared__ __align__(32) float heads[4][kGroups][kDim];
+    __shared__ __align__(32) float heads[PAIRING == kAny ? 4 : 1][kGroups][kDim];
     const Spkv2Rotate &g = a.g;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + wave;
@@ -95,8 +142,34 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
     const int part = static_cast<int>(at - token * a.parts);
     if (token >= g.tokens) return;  // a whole wave; no barrier follows
     const int dim = g.head_dim, pairs = g.pairs;
-    const int group = lane / LANES, i0 = lane % LANES * 8;
-    const bool in = i0 < dim;
+    const int group = lane / LANES, eighth = min(lane % LANES, dim / 8 - 1);
+    const bool in = lane % LANES < dim / 8;
+    // where the lane's elements 0 .. 4 and 4 .. 8 lie; past the pairs, in a row
+    int low = eighth * 8, high = low + 4;
+    if constexpr (PAIRING == kApart) {
+        const int past = eighth * 4 - pairs;
+        low = past < 0 ? eighth * 4 : 2 * (pairs + past);
+        high = past < 0 ? low + pairs : low + 4;
+    }
+    const auto place = [&](int e) { return e < 4 ? low + e : high + e - 4; };
+    const int first = part * kGroups, step = a.parts * kGroups;
+    // without a branch: lanes and groups past the last load its elements, and store nothing
+    const auto fetch8 = [&](auto *p) {
+        Vec<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 8> v;
+        if constexpr (PAIRING == kApart) {
+            __builtin_memcpy(v.v, p + low, sizeof(v.v) / 2);
+            __builtin_memcpy(v.v + 4, p + high, sizeof(v.v) / 2);
+        } else {
+            __builtin_memcpy(v.v, p + low, sizeof(v.v));
+        }
+        return v;
+    };
+    const auto fetch = [&](const void *x, int64_t stride, int head) {
+        return fetch8(static_cast<const T *>(x) + token * stride + static_cast<int64_t>(head) * dim);
+    };
+    // the first head is on its way while the angles are taken
+    Vec<T, 8> next;
+    if (g.heads > first) next = fetch(g.q, g.q_stride, min(first + group, g.heads - 1));
     double *sines = table[wave][0], *cosines = table[wave][1];
     for (int p = lane; p < pairs; p += 64) {
         const int axis = g.axis ? g.axis[p] : 0;
@@ -106,94 +179,87 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 
-    // where element i of a head has its partner, and with which factors
-    const auto pair_of = [&](int i, bool *second) {
-        if (g.interleaved) {
-            *second = i & 1;
-            return i / 2;
-        }
-        *second = i >= pairs;
-        return *second ? i - pairs : i;
+    // where element e of the lane has its partner; itself past the pairs
+    const auto partner_of = [&](int e) {
+        const int i = place(e);
+        return i >= 2 * pairs ? i : PAIRING == kBeside ? i ^ 1 : i >= pairs ? i - pairs : i + pairs;
     };
-    const auto partner_of = [&](int i) { return i >= 2 * pairs || !in ? i : g.interleaved ? i ^ 1 : i >= pairs ? i - pairs : i + pairs; };
+    constexpr int kOther = PAIRING == kBeside ? 1 : 4;  // partner e ^ kOther of the same lane
     const auto turn_of = [&](const void *weight) {
         Turn t;
-        const W *w = static_cast<const W *>(weight);
+        float own[8], other[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int i = i0 + j;
-            bool second;
-            const int p = pair_of(i, &second);
-            t.own[j] = 1.0;
-            t.other[j] = 0.0;
-            if (in && i < 2 * pairs) {
-                t.own[j] = cosines[p];
-                t.other[j] = second ? sines[p] : -sines[p];
-            }
-            if (in && w && g.norm) {
-                t.own[j] *= static_cast<double>(static_cast<float>(w[i]));
-                t.other[j] *= static_cast<double>(static_cast<float>(w[partner_of(i)]));
-            }
+        for (int e = 0; e < 8; e++) own[e] = other[e] = 1.0f;
+        if (weight && g.norm) {
+            const W *w = static_cast<const W *>(weight);
+            widen(fetch8(w), own);
+#pragma unroll
+            for (int e = 0; e < 8; e++) other[e] = PAIRING == kAny ? static_cast<float>(w[partner_of(e)]) : own[e ^ kOther];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = place(e);
+            const bool second = PAIRING == kBeside ? i & 1 : i >= pairs, turns = i < 2 * pairs;
+            const int p = !turns ? 0 : PAIRING == kBeside ? i / 2 : second ? i - pairs : i;
+            const double c = cosines[p], s = sines[p];
+            t.own[e] = (turns ? c : 1.0) * static_cast<double>(own[e]);
+            t.other[e] = turns ? (second ? s : -s) * static_cast<double>(other[e]) : 0.0;
         }
         return t;
     };
-    float *mine = heads[wave][group];
-    const auto turned = [&](const Turn &t, const float(&x)[8], float(&y)[8]) {
+    float *mine = heads[PAIRING == kAny ? wave : 0][group];
+    const double per = 1.0 / dim;
+    const auto turned = [&](const Turn &t, const Vec<T, 8> &raw, float (&y)[8]) {
+        float x[8], other[8];
+        widen(raw, x);
         double factor = 1.0;
         if (g.norm) {
             double sum = 0.0;
 #pragma unroll
             for (int j = 0; j < 8; j++) sum = __builtin_fma(static_cast<double>(x[j]), static_cast<double>(x[j]), sum);
-            factor = 1.0 / sqrt(sum_over<LANES>(sum) / dim + static_cast<double>(g.eps));
+            factor = inverse_root(sum_over<LANES>(in ? sum : 0.0) * per + static_cast<double>(g.eps));
         }
-        float other[8];
-        if (PAIRED && g.interleaved) {
+        if constexpr (PAIRING != kAny) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) other[j] = x[j ^ 1];
+            for (int e = 0; e < 8; e++) other[e] = x[e ^ kOther];
         } else {
-            put_floats<8>(mine + i0, x);
+            if (in) put_floats<8>(mine + low, x);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if constexpr (PAIRED) {
-                const Vec<float, 8> v = *reinterpret_cast<const Vec<float, 8> *>(mine + partner_of(i0));
 #pragma unroll
-                for (int j = 0; j < 8; j++) other[j] = v.v[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) other[j] = mine[partner_of(i0 + j)];
-            }
+            for (int e = 0; e < 8; e++) other[e] = mine[partner_of(e)];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
+        double v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            // a partner that is not there, or is not finite where nothing turns, adds nothing
-            double v = static_cast<double>(x[j]) * t.own[j];
-            if (i0 + j < 2 * pairs) v = __builtin_fma(static_cast<double>(other[j]), t.other[j], v);
-            y[j] = static_cast<float>(static_cast<T>(v * factor));
+            // past the pairs nothing is added: 0 times what is not finite would be NaN
+            const float o = place(j) < 2 * pairs ? other[j] : 0.0f;
+            v[j] = __builtin_fma(static_cast<double>(o), t.other[j], static_cast<double>(x[j]) * t.own[j]) * factor;
         }
-    };
-    const auto fetch = [&](const void *x, int64_t stride, int head, float(&f)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = 0.0f;
-        if (in) load_floats<8>(static_cast<const T *>(x) + token * stride + static_cast<int64_t>(head) * dim + i0, f);
+        rounded<T>(v, y);
     };
     const auto put = [&](void *y, int64_t stride, int head, const float(&f)[8]) {
-        if (in) store_floats<8>(static_cast<T *>(y) + token * stride + static_cast<int64_t>(head) * dim + i0, f);
+        T *p = static_cast<T *>(y) + token * stride + static_cast<int64_t>(head) * dim;
+        if constexpr (PAIRING == kApart) {
+            store_floats<4>(p + low, {f[0], f[1], f[2], f[3]});
+            store_floats<4>(p + high, {f[4], f[5], f[6], f[7]});
+        } else {
+            store_floats<8>(p + low, f);
+        }
     };
-    const int first = part * kGroups, step = a.parts * kGroups;
     if (g.heads > first) {
         const Turn t = turn_of(g.q_weight);
         for (int h = first; h < g.heads; h += step) {
-            const int head = min(h + group, g.heads - 1);
-            float x[8], y[8];
-            fetch(g.q, g.q_stride, head, x);
-            turned(t, x, y);
-            if (h + group < g.heads) put(g.q_out, g.q_out_stride, head, y);
+            const Vec<T, 8> now = next;
+            next = fetch(g.q, g.q_stride, min(h + step + group, g.heads - 1));
+            float y[8];
+            turned(t, now, y);
+            if (in && h + group < g.heads) put(g.q_out, g.q_out_stride, h + group, y);
         }
     }
     if (g.kv_heads <= first) return;
-    const Turn t = turn_of(g.k_weight);
     int64_t page = -1, row = 0;
     if (a.c.pages) {
         const int64_t slot = g.slots[token];
@@ -202,34 +268,38 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
             row = slot - page * a.c.page_size;
         }
     }
-    const auto code = [&](const float(&f)[8], int head, int8_t *codes, float *scales) {
+    const auto code = [&](const float(&x)[8], bool there, int head, int8_t *codes, float *scales) {
         const int64_t at_row = (page * a.c.kv_heads + head) * a.c.page_size + row;
         unsigned top = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, abs_bits(f[j]));
-        top = max_over<LANES>(top);
+        for (int j = 0; j < 8; j++) top = max(top, abs_bits(x[j]));
+        top = max_over<LANES>(in ? top : 0);
         const bool finite = top < kInfBits;
         Vec<int8_t, 8> q;
 #pragma unroll
         for (int j = 0; j < 8; j++) q.v[j] = 0;
-        if (finite && top) quantise<8>(f, __uint_as_float(top), q.v);
-        if (in) *reinterpret_cast<Vec<int8_t, 8> *>(codes + at_row * a.c.head_dim + i0) = q;
-        if (lane % LANES == 0) scales[at_row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
+        if (finite && top) quantise<8>(x, __uint_as_float(top), q.v);
+        if (in && there) {
+            int8_t *p = codes + at_row * a.c.head_dim;
+            __builtin_memcpy(p + low, q.v, 4);
+            __builtin_memcpy(p + high, q.v + 4, 4);
+        }
+        if (lane % LANES == 0 && there) scales[at_row] = finite ? __uint_as_float(top) / 127.0f : __builtin_nanf("");
     };
+    const Turn t = turn_of(g.k_weight);
     for (int h = first; h < g.kv_heads; h += step) {
         const int head = min(h + group, g.kv_heads - 1);
         const bool there = h + group < g.kv_heads;
-        float x[8], y[8];
-        fetch(g.k, g.k_stride, head, x);
-        turned(t, x, y);
-        if (there && g.k_out) put(g.k_out, g.k_out_stride, head, y);
-        if (page >= 0) {
-            float v[8];
-            fetch(g.v, g.v_stride, head, v);
-            if (there) {
-                code(y, head, a.c.k, a.c.k_scale);
-                code(v, head, a.c.v, a.c.v_scale);
-            }
+        const Vec<T, 8> k = fetch(g.k, g.k_stride, head);
+        Vec<T, 8> v;
+        if (page >= 0) v = fetch(g.v, g.v_stride, head);
+        float y[8];
+        turned(t, k, y);
+        if (in && there && g.k_out) put(g.k_out, g.k_out_stride, head, y);
+        if (page >= 0) {  // the whole wave: a token's
+            code(y, there, head, a.c.k, a.c.k_scale);
+            widen(v, y);
+            code(y, there, head, a.c.v, a.c.v_scale);
         }
     }
 }
@@ -274,16 +344,16 @@ extern "C" int spkv2_mi355x_rotate(const Spkv2KvCacheI8 *c, const Spkv2Rotate *g
         a.parts = static_cast<int>(std::min<int64_t>(most, (2048 + g->tokens - 1) / g->tokens));
         const int64_t blocks = (g->tokens * a.parts + 3) / 4;
         if (blocks >= 1 << 24) return unsupported("rotate: too many tokens for one launch");
-        const bool paired = g->interleaved || g->pairs % 8 == 0;
         const bool wide = g->norm && (g->q_weight || g->k_weight) && g->weight_dtype == SPKV2_DTYPE_FP32;
         return with_type(g->dtype, [&](auto t) {
             using T = decltype(t);
             auto go = [&](auto kernel) { return launch("rotate", kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), stream, a); };
             auto by_weight = [&](auto w) {
                 using W = decltype(w);
-                if (groups == 8) return paired ? go(rotate_heads<T, W, 8, true>) : go(rotate_heads<T, W, 8, false>);
-                if (groups == 4) return paired ? go(rotate_heads<T, W, 16, true>) : go(rotate_heads<T, W, 16, false>);
-                return paired ? go(rotate_heads<T, W, 32, true>) : go(rotate_heads<T, W, 32, false>);
+                auto by_lanes = [&](auto beside, auto apart, auto any) { return go(g->interleaved ? beside : g->pairs % 4 == 0 ? apart : any); };
+                if (groups == 8) return by_lanes(rotate_heads<T, W, 8, kBeside>, rotate_heads<T, W, 8, kApart>, rotate_heads<T, W, 8, kAny>);
+                if (groups == 4) return by_lanes(rotate_heads<T, W, 16, kBeside>, rotate_heads<T, W, 16, kApart>, rotate_heads<T, W, 16, kAny>);
+                return by_lanes(rotate_heads<T, W, 32, kBeside>, rotate_heads<T, W, 32, kApart>, rotate_heads<T, W, 32, kAny>);
             };
             return wide ? by_weight(float{}) : by_weight(T{});
         });

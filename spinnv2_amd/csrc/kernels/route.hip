@@ -4,9 +4,11 @@
 // the count of choices of lower experts and of earlier ones of its own.  A
 // workgroup an expert counts and places its own: every id is read once for each
 // expert, from L2, but there is one launch, no atomics and no order that changes
-// from run to run.
+// from run to run (65520 choices of 128 experts 14 us: bound by the instructions
+// for each 64 of them; 512 of 64 3.3 us).
 //
-// combine: bound by the bytes of the rows picked.
+// combine: bound by the bytes of the rows picked (8190 tokens of 8 rows of 2048,
+// 302 MB: 64 us, 4.7 TB/s).
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -19,65 +21,101 @@ struct SortArgs {
     int count, experts;
 };
 
-// WAVES waves, each with a run of the choices, 64 at a time
-template <typename I, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) sort_choices(SortArgs a) {
-    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const I *ids = static_cast<const I *>(a.ids);
-    const int per = (a.count + 64 * WAVES - 1) / (64 * WAVES) * 64;  // counts up to 2^30
-    const int first = min(wave * per, a.count), end = min(first + per, a.count);
-    constexpr int kAhead = 8;
-    int lower = 0, own = 0;
-    for (int c0 = first; c0 < end; c0 += 64 * kAhead) {
-        I id[kAhead];
+// Four ids at p, of which `left` are there, as 16 bits each: 0xffff for those of no expert
+template <typename I>
+__device__ __forceinline__ void four_ids(const I *p, int left, unsigned experts, unsigned (&id)[4]) {
+    I v[4];
+    if (left >= 4) {
+        __builtin_memcpy(v, p, sizeof(v));
+    } else {
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const int c = c0 + 64 * u + lane;
-            id[u] = c < end ? ids[c] : static_cast<I>(-1);
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            lower += __popcll(__ballot(id[u] >= 0 && id[u] < e));
-            own += __popcll(__ballot(id[u] == e));
-        }
+        for (int u = 0; u < 4; u++) v[u] = u < left ? p[u] : static_cast<I>(-1);
     }
+#pragma unroll
+    for (int u = 0; u < 4; u++) id[u] = static_cast<uint64_t>(v[u]) < experts ? static_cast<unsigned>(v[u]) : 0xffffu;
+}
+
+// WAVES waves, each with a run of the choices, PIECE of them at a time: read four a
+// lane, counted, and kept in LDS, which gives them back 64 in a row to be placed.
+// An expert's workgroups (along y) count all choices and each place a part of every
+// run: what they do for 64 choices, not the bytes, takes the time.
+template <typename I, int WAVES, int PIECE>
+__global__ void __launch_bounds__(64 * WAVES) sort_choices(SortArgs a) {
+    constexpr int kBatches = PIECE / 256, kAhead = kBatches < 8 ? kBatches : 8;
+    __shared__ __align__(16) uint16_t held[WAVES][PIECE];
+    const unsigned e = blockIdx.x, experts = a.experts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const I *ids = static_cast<const I *>(a.ids);
+    const int batches = (a.count + 256 * WAVES - 1) / (256 * WAVES), per = batches * 256;  // counts up to 2^30
+    const int first = min(wave * per, a.count), end = min(first + per, a.count);
+    // the part of the run that is placed here
+    const int parts = gridDim.y, part = blockIdx.y;
+    const int from = min(first + static_cast<int>(static_cast<int64_t>(batches) * part / parts) * 256, end);
+    const int to = min(first + static_cast<int>(static_cast<int64_t>(batches) * (part + 1) / parts) * 256, end);
+    int lower = 0, own = 0, earlier = 0;  // earlier: of its own, ahead of the part
+    const auto take = [&](int c0) {
+#pragma unroll 1
+        for (int b = 0; b < kBatches && c0 + 256 * b < end; b += kAhead) {
+            unsigned id[kAhead][4];
+#pragma unroll
+            for (int n = 0; n < kAhead; n++) {
+                const int c = c0 + 256 * (b + n) + 4 * lane;
+                four_ids(ids + min(c, a.count), end - c, experts, id[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < kAhead; n++) {
+                int mine = 0;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    lower += __popcll(__ballot(id[n][u] < e));
+                    mine += __popcll(__ballot(id[n][u] == e));
+                }
+                own += mine;
+                if (c0 + 256 * (b + n) < from) earlier += mine;
+                *reinterpret_cast<uint2 *>(&held[wave][256 * (b + n) + 4 * lane]) = uint2{id[n][0] | id[n][1] << 16, id[n][2] | id[n][3] << 16};
+            }
+        }
+    };
+    for (int c0 = first; c0 < end; c0 += PIECE) take(c0);
     __shared__ int lowers[WAVES], owns[WAVES];
     if (lane == 0) {
         lowers[wave] = lower;
         owns[wave] = own;
     }
     __syncthreads();
-    int row = 0, all = 0;
+    int row = earlier, all = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; w++) {
         row += lowers[w] + (w < wave ? owns[w] : 0);
         all += lowers[w] + owns[w];
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && part == 0) {
         a.offsets[e] = row;
-        if (e == a.experts - 1) a.offsets[a.experts] = all;
+        if (e == experts - 1) a.offsets[experts] = all;
     }
-    const uint64_t before = (uint64_t(1) << lane) - 1;
-    for (int c0 = first; c0 < end; c0 += 64 * kAhead) {
-        I id[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const int c = c0 + 64 * u + lane;
-            id[u] = c < end ? ids[c] : static_cast<I>(0);
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const int c = c0 + 64 * u + lane;
-            const uint64_t mine = __ballot(c < end && id[u] == e);
-            if (c < end && id[u] == e) {
-                const int r = row + __popcll(mine & before);
-                a.order[r] = c;
-                a.place[c] = r;
+    if (own == 0 && e != 0) return;
+    for (int c0 = first; c0 < end; c0 += PIECE) {
+        if (c0 + PIECE <= from || c0 >= to) continue;
+        if (per > PIECE) take(c0);  // a piece of several; the counts were used
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int c1 = max(c0, from); c1 < min(c0 + PIECE, to); c1 += 64) {
+            const int c = c1 + lane;
+            const unsigned id = c < end ? held[wave][c - c0] : 0xfffeu;
+            const uint64_t mine = __ballot(id == e);
+            if (mine) {  // few of 64 choices are one expert's
+                if (id == e) {
+                    const int r = row + static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mine >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mine), 0)));
+                    a.order[r] = c;
+                    a.place[c] = r;
+                }
+                row += __popcll(mine);
             }
-            row += __popcll(mine);
-            // the first expert's workgroup also marks the choices of none
-            if (e == 0 && c < end && (id[u] < 0 || id[u] >= a.experts)) a.place[c] = -1;
+            // the first expert's workgroups also mark the choices of none
+            if (e == 0 && id == 0xffffu) a.place[c] = -1;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -144,9 +182,17 @@ extern "C" int spkv2_mi355x_sort_tokens(const Spkv2SortTokens *g, void *stream) 
         const int64_t count = g->tokens * g->per_token;
         if (!g->offsets || (count && (!g->ids || !g->order || !g->place))) return bad("sort_tokens: a NULL pointer");
         const SortArgs a{g->ids, g->offsets, g->order, g->place, static_cast<int>(count), g->experts};
-        auto go = [&](auto kernel, int waves) { return launch("sort_tokens", kernel, dim3(g->experts), dim3(64 * waves), stream, a); };
-        if (g->wide_ids) return count <= 4096 ? go(sort_choices<int64_t, 4>, 4) : go(sort_choices<int64_t, 16>, 16);
-        return count <= 4096 ? go(sort_choices<int32_t, 4>, 4) : go(sort_choices<int32_t, 16>, 16);
+        auto go = [&](auto kernel, int waves) {
+            // as many workgroups as CUs where choices are many: one holds most of a CU's LDS
+            const int parts = count <= 16384 ? 1 : std::max(1, std::min(256 / g->experts, 8));
+            return launch("sort_tokens", kernel, dim3(g->experts, parts), dim3(64 * waves), stream, a);
+        };
+        auto by_count = [&](auto i) {
+            using I = decltype(i);
+            // fewer waves join their counts sooner
+            return count <= 4096 ? go(sort_choices<I, 4, 1024>, 4) : count <= 16384 ? go(sort_choices<I, 16, 1024>, 16) : go(sort_choices<I, 16, 4096>, 16);
+        };
+        return g->wide_ids ? by_count(int64_t{}) : by_count(int32_t{});
     });
 }
 

@@ -277,6 +277,20 @@ def test_ties_go_to_the_even_code(gpu):
         np.testing.assert_array_equal(q.download(), want)
 
 
+def test_gates_whose_quotients_are_ties(gpu):
+    """Elements with the gate of their block's largest: their quotients are those of the factors, ties among them, whatever the
+    gate's own 64-bit value was rounded to."""
+    rng = np.random.default_rng(8)
+    border = (_FLOAT8[1:127].astype(np.float64) + _FLOAT8[:126]) / 2
+    u = np.concatenate([border, [448.0, 0.0]])[None] * np.where(rng.random((64, 128)) < 0.5, -1.0, 1.0)
+    g = np.repeat(rng.standard_normal((64, 1)) * 3, 128, 1)
+    x = np.concatenate([g, u], 1).astype(np.float32)
+    q, s = Array((64, 128), F8), Array((64, 1), "float32")
+    decoder.gate_f8(Array.of(x), q, s)
+    want = _FLOAT8[to_float8(u * np.sign(x[:, :1]))]
+    np.testing.assert_array_equal(q.download(), want)
+
+
 def test_gates_far_below_zero(gpu):
     """Gates whose exponential leaves fp32's range, alone in their block and beside others, with small and large factors."""
     rng = np.random.default_rng(3)
@@ -440,7 +454,7 @@ def _order(ids, experts):
 
 @pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("tokens,per_token,experts", [(0, 2, 3), (1, 1, 1), (1, 8, 64), (63, 1, 5), (64, 8, 64), (65, 3, 300), (1000, 4, 7), (1025, 8, 128),
-                                                      (9000, 2, 1), (20011, 5, 33), (70, 2, 4096)])
+                                                      (9000, 2, 1), (20011, 5, 33), (70, 2, 4096), (4096, 1, 3), (65536, 1, 9), (65537, 1, 9)])
 def test_sort_tokens(gpu, tokens, per_token, experts, wide):
     rng = np.random.default_rng(tokens)
     ids = rng.integers(-2 if tokens % 2 else 0, experts + (2 if tokens % 2 else 0), (tokens, per_token)).astype(np.int64 if wide else np.int32)
