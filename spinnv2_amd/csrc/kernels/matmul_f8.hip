@@ -276,9 +276,11 @@ __global__ void __launch_bounds__(512) matmul_rows(MatmulArgs a) {
         for (int w = 1; w < WAVES; w++) total += sums(w, i, j);
         const int m = m0 + 16 * j + col, n = n0 + 16 * i + 4 * g, left = a.n - n;
         if (m >= end_m || left <= 0) continue;
-        float v[4];
+        float v[4] = {total[0], total[1], total[2], total[3]};
+        if (a.bias) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = total[e] + (a.bias && e < left ? a.bias[static_cast<int64_t>(expert) * a.n + n + e] : 0.0f);
+            for (int e = 0; e < 4; e++) v[e] += a.bias[static_cast<int64_t>(expert) * a.n + min(n + e, a.n - 1)];
+        }
         store_some<4>(static_cast<T *>(a.out) + m * a.out_stride + n, left, v);
     }
 }
@@ -317,6 +319,7 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
     constexpr int kScales = BM < 64 ? 64 : BM;
     __shared__ __align__(16) uint8_t lds[2 * kBuffer];
     __shared__ __align__(16) float row_scales[2][kScales][4];  // of four blocks of k
+    __shared__ bool row_there[EXPERTS ? kScales : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), tid = wave * 64 + lane;
     const int col = lane & 15, g = lane >> 4;
@@ -382,6 +385,7 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         scale_at = static_cast<unsigned>(min(scale_row % BM, a.m - 1 - m0)) * static_cast<unsigned>(a.sa_stride) * 4;
     }
     const bool scaler = part == 0 && wave < kRuns;
+    if (EXPERTS && scaler) row_there[EXPERTS ? scale_row : 0] = input(m0 + scale_row % BM) != 0xffffffffu;
     const auto quad_from = [&](int q) { return max(min(4 * q, blocks - 4), 0); };
     if (blocks < 4 && scaler) {
         for (int t = 0; t < blocks; t++)
@@ -539,45 +543,67 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         asm volatile("" ::: "memory");
     }
 
-    // 16 rows at a time through this wave's own part of LDS (every wave is past
-    // its last read of the buffers), so that a row's channels leave as 16-byte
-    // pieces one after the other
-    constexpr int kCols = 16 * TI, kPiece = 16 / static_cast<int>(sizeof(T)), kPitch = kCols + kPiece;
-    static_assert(16 * kPitch * sizeof(T) <= 2 * kBuffer / kWaves, "a wave's part of LDS holds 16 rows");
-    T *mine = reinterpret_cast<T *>(lds + wave * (2 * kBuffer / kWaves));
-    const int left = a.n - n0 - wn;
+    // Through this wave's own part of LDS (every wave is past its last read of the
+    // buffers), so that a row's channels leave as 16-byte pieces one after the other.
+    // A row's piece p lies at place p ^ (row / rows of 256 bytes): the accumulators'
+    // 8-byte writes and the rows' reads are then on different banks.  Sixteen rows at
+    // a time, each asked whether it is inside, this took a tile of 256 x 256 8 us.
+    constexpr int kPiece = 16 / static_cast<int>(sizeof(T)), kLanes = 16 * TI / kPiece;  // elements of a piece, pieces of a row
+    constexpr int kRows = 64 / kLanes, kReads = 16 * TJ / kRows, kPitch = kLanes * 16;
+    static_assert(16 * TJ * kPitch <= 2 * kBuffer / kWaves, "a wave's part of LDS holds its tile");
+    uint8_t *mine = lds + wave * (2 * kBuffer / kWaves);
+    const auto spot = [&](int row, int p) { return mine + row * kPitch + ((p ^ (row / (16 / kLanes > 0 ? 16 / kLanes : 1))) & (kLanes - 1)) * 16; };
+    const int left = a.n - n0 - wn, rows = end_m - m0 - wm;
+    floatx4 bias[TI];
+#pragma unroll
+    for (int i = 0; i < TI; i++) bias[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (a.bias) {
+        const float *from = a.bias + static_cast<int64_t>(expert) * a.n;
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) bias[i][e] = from[min(n0 + wn + 16 * i + 4 * g + e, a.n - 1)];
+    }
 #pragma unroll
     for (int j = 0; j < TJ; j++) {
-        const int m = m0 + wm + 16 * j;
-        if (m >= end_m) break;
-        const bool there = !EXPERTS || input(m + col) != 0xffffffffu;
+        const bool there = !EXPERTS || row_there[EXPERTS ? wm + 16 * j + col : 0];
 #pragma unroll
         for (int i = 0; i < TI; i++) {
             float v[4];
-            const int n = 16 * i + 4 * g;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (there ? acc[i][j][e] : 0.0f) + (a.bias && n + e < left ? a.bias[static_cast<int64_t>(expert) * a.n + n0 + wn + n + e] : 0.0f);
-            put_floats<4>(mine + col * kPitch + n, v);
+            for (int e = 0; e < 4; e++) v[e] = (there ? acc[i][j][e] : 0.0f) + bias[i][e];
+            const int at = 16 * i + 4 * g;
+            put_floats<4>(reinterpret_cast<T *>(spot(16 * j + col, at / kPiece)) + at % kPiece, v);
         }
-        wait_lds();
-        constexpr int kLanes = kCols / kPiece, kRows = 64 / kLanes;
-        const int c = lane % kLanes * kPiece;
+    }
+    wait_lds();
+    const int c = lane % kLanes * kPiece, r0 = lane / kLanes;
+    T *out = static_cast<T *>(a.out) + (m0 + wm + r0) * a.out_stride + n0 + wn + c;
+    const auto piece_of = [&](int r) { return *reinterpret_cast<const Vec<T, kPiece> *>(spot(r + r0, lane % kLanes)); };
+    if (rows >= 16 * TJ && left >= 16 * TI) {
+        constexpr int kAhead = kReads < 8 ? kReads : 8;
 #pragma unroll
-        for (int r = 0; r < 16; r += kRows) {
-            const int row = r + lane / kLanes;
-            if (row < 16 && m + row < end_m) {
-                const Vec<T, kPiece> v = *reinterpret_cast<const Vec<T, kPiece> *>(mine + row * kPitch + c);
-                T *out = static_cast<T *>(a.out) + (m + row) * a.out_stride + n0 + wn + c;
-                if (c + kPiece <= left) {
-                    __builtin_memcpy(out, v.v, sizeof(v.v));
-                } else {
+        for (int q = 0; q < kReads; q += kAhead) {
+            Vec<T, kPiece> v[kAhead];
 #pragma unroll
-                    for (int e = 0; e < kPiece; e++)
-                        if (c + e < left) out[e] = v.v[e];
-                }
+            for (int u = 0; u < kAhead; u++) v[u] = piece_of((q + u) * kRows);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) __builtin_memcpy(out + static_cast<int64_t>((q + u) * kRows) * a.out_stride, v[u].v, 16);
+        }
+    } else {
+#pragma unroll 1
+        for (int r = 0; r < min(rows, 16 * TJ); r += kRows) {
+            const Vec<T, kPiece> v = piece_of(r);
+            if (r + r0 >= rows) continue;
+            T *y = out + static_cast<int64_t>(r) * a.out_stride;
+            if (c + kPiece <= left) {
+                __builtin_memcpy(y, v.v, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPiece; e++)
+                    if (c + e < left) y[e] = v.v[e];
             }
         }
-        wait_lds();
     }
 }
 
@@ -623,10 +649,10 @@ MatmulArgs arguments(const Spkv2MatmulF8 &g) {
 // A kernel's time: a launch's, then steps by every workgroup, of a block of k for
 // each of its groups of waves, which take `step` each where a CU's workgroups do
 // not fill it, or `work` for each of the CU's workgroups where they do, and the
-// workgroup's sums.  Fitted, in us, to 1100 products of log-uniform sizes (m 1 ..
+// workgroup's sums.  Fitted, in us, to 1300 products of log-uniform sizes (m 1 ..
 // 8192, n and k 64 .. 16384, up to 2^37 multiplications; half of them by expert):
-// the kernel of the least time by these is 2.4% slower than the fastest of
-// fourteen in the mean, 30% in one of a hundred.
+// the kernel of the least time by these is 2.0% slower than the fastest of them in
+// the mean, 28% in one of a hundred.
 struct Cost {
     float launch, step, work, sums;
 };
@@ -636,16 +662,16 @@ struct Form {
     Cost cost[4];  // 16-bit outputs with rows of whole runs of 16 bytes, and others; fp32 outputs likewise
 };
 constexpr Form kForms[] = {
-    {16, 16, 8, false, {{1.23f, 0.550f, 0.630f, 1.655f}, {1.30f, 0.956f, 0.905f, 1.321f}, {1.16f, 0.666f, 0.701f, 1.710f}, {1.22f, 0.987f, 0.915f, 1.581f}}},
-    {16, 32, 8, false, {{1.67f, 0.818f, 1.007f, 1.048f}, {1.82f, 0.818f, 1.332f, 0.758f}, {1.56f, 0.484f, 1.071f, 1.164f}, {1.80f, 0.313f, 1.378f, 0.946f}}},
-    {16, 64, 8, false, {{1.55f, 0.180f, 1.584f, 0.975f}, {2.00f, 2.140f, 2.154f, 0.378f}, {1.60f, 1.575f, 1.622f, 1.063f}, {1.79f, 0.005f, 2.254f, 0.669f}}},
-    {32, 64, 8, false, {{0.37f, 1.013f, 1.866f, 2.328f}, {0.81f, 1.143f, 2.548f, 1.718f}, {0.53f, 1.752f, 2.063f, 2.287f}, {0.73f, 1.028f, 2.698f, 1.963f}}},
-    {64, 64, 1, true, {{3.10f, 0.382f, 0.277f, 1.069f}, {2.76f, 0.788f, 0.435f, 1.129f}, {3.21f, 0.496f, 0.325f, 1.247f}, {2.85f, 0.920f, 0.472f, 1.406f}}},
-    {64, 64, 2, true, {{2.18f, 0.542f, 0.514f, 2.152f}, {2.05f, 1.152f, 0.896f, 1.863f}, {2.18f, 0.741f, 0.627f, 2.309f}, {2.02f, 1.323f, 0.998f, 2.152f}}},
-    {64, 64, 4, true, {{0.00f, 0.621f, 0.965f, 4.945f}, {0.00f, 1.107f, 1.950f, 4.079f}, {0.00f, 1.018f, 1.272f, 5.070f}, {0.00f, 1.532f, 2.107f, 4.626f}}},
-    {32, 128, 1, true, {{3.05f, 0.428f, 0.344f, 1.235f}, {2.68f, 0.930f, 0.587f, 1.236f}, {2.92f, 0.530f, 0.374f, 1.561f}, {2.43f, 1.057f, 0.589f, 1.668f}}},
-    {128, 128, 1, true, {{3.42f, 0.418f, 0.652f, 3.066f}, {1.57f, 1.382f, 0.944f, 4.299f}, {2.25f, 1.076f, 0.893f, 4.346f}, {1.95f, 2.031f, 1.358f, 4.122f}}},
-    {256, 256, 1, true, {{0.00f, 0.100f, 1.110f, 10.122f}, {0.00f, 0.100f, 2.104f, 9.616f}, {}, {}}},
+    {16, 16, 8, false, {{1.25f, 0.155f, 0.670f, 1.527f}, {1.62f, 0.194f, 0.868f, 1.268f}, {1.34f, 0.094f, 0.762f, 1.463f}, {1.38f, 1.038f, 0.948f, 1.380f}}},
+    {16, 32, 8, false, {{1.62f, 0.059f, 1.017f, 1.013f}, {1.97f, 1.164f, 1.304f, 0.741f}, {1.75f, 0.846f, 1.134f, 0.951f}, {1.88f, 0.818f, 1.449f, 0.760f}}},
+    {16, 64, 8, false, {{1.54f, 1.358f, 1.477f, 1.053f}, {1.93f, 1.262f, 2.150f, 0.464f}, {1.71f, 1.319f, 1.656f, 0.920f}, {1.76f, 2.152f, 2.447f, 0.357f}}},
+    {32, 64, 8, false, {{0.45f, 1.215f, 1.773f, 2.389f}, {1.02f, 2.192f, 2.541f, 1.621f}, {0.83f, 1.795f, 2.092f, 2.002f}, {0.88f, 2.868f, 2.883f, 1.528f}}},
+    {64, 64, 1, true, {{2.98f, 0.374f, 0.275f, 0.887f}, {2.96f, 0.792f, 0.433f, 0.838f}, {3.04f, 0.510f, 0.318f, 1.113f}, {2.78f, 0.980f, 0.507f, 1.003f}}},
+    {64, 64, 2, true, {{2.26f, 0.353f, 0.533f, 1.758f}, {2.25f, 1.141f, 0.854f, 1.516f}, {2.22f, 0.739f, 0.630f, 2.041f}, {2.08f, 1.403f, 1.029f, 1.644f}}},
+    {64, 64, 4, true, {{0.00f, 0.204f, 0.951f, 4.516f}, {0.39f, 0.832f, 1.875f, 3.531f}, {0.44f, 1.245f, 1.285f, 4.474f}, {0.39f, 2.212f, 2.228f, 3.669f}}},
+    {32, 128, 1, true, {{2.98f, 0.417f, 0.350f, 0.949f}, {2.99f, 0.907f, 0.568f, 0.789f}, {2.82f, 0.559f, 0.374f, 1.276f}, {2.54f, 1.102f, 0.636f, 1.094f}}},
+    {128, 128, 1, true, {{2.78f, 0.381f, 0.655f, 2.523f}, {2.57f, 1.406f, 0.998f, 2.355f}, {2.88f, 1.081f, 0.861f, 3.255f}, {2.36f, 2.117f, 1.439f, 2.945f}}},
+    {256, 256, 1, true, {{0.00f, 0.100f, 1.047f, 7.766f}, {0.00f, 2.080f, 2.113f, 7.675f}, {}, {}}},
 };
 constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
 
