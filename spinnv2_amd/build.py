@@ -5,7 +5,9 @@
 
 Every source under spinnv2_amd/csrc is compiled by hipcc for gfx950 only and
 linked into spinnv2_amd/lib/libspkv2_mi355x.so.  Packed-FP32 instruction
-selection is disabled (-packed-fp32-ops) for all device code.
+selection is disabled (-packed-fp32-ops) for all device code.  The host
+compiler builds spinnv2_amd/bindings, the decoder layer's calls for Python, into
+a module beside it.
 """
 
 from __future__ import annotations
@@ -16,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -25,6 +28,9 @@ BUILD = PKG / "_build"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libspkv2_mi355x.so"
 INCLUDE = ROOT / "include"
+BINDINGS = PKG / "bindings" / "decoder_calls.cpp"
+#: the module of the decoder layer's calls, for the interpreter that builds it
+CALLS = LIB_DIR / f"_decoder_calls{sysconfig.get_config_var('EXT_SUFFIX')}"
 ARCH = "gfx950"
 
 
@@ -78,6 +84,24 @@ def _compile(src: Path, force: bool, newest_header: float) -> tuple[Path, str]:
     return obj, warnings
 
 
+def build_calls(force: bool = False) -> Path:
+    """The module of the decoder layer's calls; host code only."""
+    newest = max(BINDINGS.stat().st_mtime, max(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if not force and CALLS.exists() and CALLS.stat().st_mtime >= newest:
+        return CALLS
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("no C++ compiler found (g++ or c++) for the decoder layer's calls")
+    tmp = CALLS.with_suffix(".so.tmp")
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-I{INCLUDE}",
+           f"-I{sysconfig.get_paths()['include']}", str(BINDINGS), "-o", str(tmp)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"compile failed: {BINDINGS}\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, CALLS)
+    return CALLS
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
     BUILD.mkdir(parents=True, exist_ok=True)
     LIB_DIR.mkdir(parents=True, exist_ok=True)
@@ -97,6 +121,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
     if proc.returncode != 0:
         raise RuntimeError(f"link failed\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, LIB)
+    build_calls(force)
     return LIB
 
 

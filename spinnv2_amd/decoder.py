@@ -30,6 +30,7 @@ library refuses raises RuntimeError_.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import math
 import struct
 
@@ -42,7 +43,7 @@ _FP32, _INT8, _FP16, _BF16, _INT32, _INT64, _F8 = 1, 2, 3, 4, 101, 102, 103
 _CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64,
           "float8_e4m3fn": _F8}
 _FLOATS = (_FP32, _FP16, _BF16)
-_FP32S, _INT8S, _INT32S, _INT64S, _F8S = (_FP32,), (_INT8,), (_INT32,), (_INT64,), (_F8,)
+_FP32S, _INT8S, _INT32S, _INT64S = (_FP32,), (_INT8,), (_INT32,), (_INT64,)
 #: columns of a row of 8-bit floats, and rows and columns of weights, that share a scale
 F8_BLOCK = 128
 
@@ -149,8 +150,28 @@ def _packer(cls):
 
 _pack_norm, _pack_dequantize, _pack_matmul = _packer(_RmsNorm), _packer(_Dequantize), _packer(_Matmul)
 _pack_write, _pack_read, _pack_attention = _packer(_Write), _packer(_Read), _packer(_Attention)
-_pack_rotate, _pack_rows_f8, _pack_dequantize_f8 = _packer(_Rotate), _packer(_RowsF8), _packer(_DequantizeF8)
-_pack_matmul_f8, _pack_experts, _pack_sort, _pack_combine = _packer(_MatmulF8), _packer(_MatmulF8Experts), _packer(_SortTokens), _packer(_Combine)
+
+
+#: the calls that take their tensors apart in native code (bindings/decoder_calls.cpp), once _bind() was called
+_calls = None
+
+
+def _bind():
+    """Loads that module and gives it the library's entry points."""
+    global _calls
+    from .build import CALLS
+
+    lib = load_library()
+    if not CALLS.exists():
+        raise RuntimeError(f"{CALLS} is not built; run `python -m spinnv2_amd.build`")
+    spec = importlib.util.spec_from_file_location("spinnv2_amd._decoder_calls", CALLS)
+    calls = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(calls)
+    calls.bind(_CODES, _code, struct.error, tuple(
+        ctypes.cast(getattr(lib, "spkv2_mi355x_" + name), _P).value
+        for name in ("rotate", "rows_f8", "dequantize_f8", "matmul_f8", "matmul_f8_experts", "sort_tokens", "combine")))
+    _calls = calls
+    return calls
 
 
 class DeviceArray:
@@ -403,6 +424,7 @@ class KvCache:
         self.buffers = (k, v, k_scale, v_scale)  # held as long as the cache is
         self._c = _Cache(*(t.data_ptr() for t in self.buffers), self.pages, self.kv_heads, self.page_size, self.head_dim, 0)
         self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int) -> "KvCache":
@@ -497,65 +519,10 @@ def rotate(q, k, positions, frequencies, q_out, k_out, *, axes=None, norm: bool 
     head_dim] are written into its slots (as KvCache.write takes them), and
     k_out may be None.
     """
-    x = k if q is None else q
-    if x is None:
-        _fail("q, k", "neither is there")
-    if len(x.shape) != 3:
-        _fail("q, k", "not [tokens, heads, head_dim]")
-    code, (tokens, _, dim) = _code(x), x.shape
-    if len(frequencies.shape) != 1:
-        _fail("frequencies", "not one-dimensional")
-    pairs = frequencies.shape[0]
-    heads = kv_heads = qp = qs = qo = qos = kp = ks = ko = kos = vp = vs = sp = qw = kw = w_code = 0
-    if q is not None:
-        shape = (tokens, q.shape[1], dim)
-        heads, qp, qs = shape[1], q.data_ptr(), _heads("q", q, _FLOATS, shape)
-        if q_out is None:
-            _fail("q_out", "queries without an output")
-        qo, qos = q_out.data_ptr(), _heads("q_out", q_out, (code,), shape)
-    if k is not None:
-        if len(k.shape) != 3:
-            _fail("k", "not [tokens, kv_heads, head_dim]")
-        shape = (tokens, k.shape[1], dim)
-        kv_heads, kp, ks = shape[1], k.data_ptr(), _heads("k", k, (code,) if q is not None else _FLOATS, shape)
-        if k_out is not None:
-            ko, kos = k_out.data_ptr(), _heads("k_out", k_out, (code,), shape)
-        elif cache is None:
-            _fail("k_out", "keys without an output or a cache")
-    if cache is not None:
-        if k is None or v is None or slots is None:
-            _fail("cache", "keys, values or slots are missing")
-        if (kv_heads, dim) != (cache.kv_heads, cache.head_dim):
-            _fail("k", f"{kv_heads} heads of {dim}, the cache has {cache.kv_heads} of {cache.head_dim}")
-        vp, vs, sp = v.data_ptr(), _heads("v", v, (code,), shape), _vector("slots", slots, _INT64S, tokens)
-    if norm:
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None:
-                at = _vector(name, w, (code, _FP32), dim)
-                if w_code and w_code != _CODES[w.dtype]:
-                    _fail(name, "the weights are of different types")
-                w_code = _CODES[w.dtype]
-                if name == "q_weight":
-                    qw = at
-                else:
-                    kw = at
-    if len(positions.shape) == 1:
-        count, stride, at = 1, 1, _vector("positions", positions, _INT32S, tokens)
-    else:
-        if len(positions.shape) != 2:
-            _fail("positions", "not [tokens] or [tokens, axes]")
-        count, at = positions.shape[1], positions.data_ptr()
-        stride = _rows("positions", positions, _INT32S, (tokens, count))
-    a = _pack_rotate(qp, qo, kp, ko, vp, qw, kw, at, _vector("frequencies", frequencies, _FP32S, pairs),
-                     0 if axes is None else _vector("axes", axes, _INT32S, pairs), sp, tokens, qs, qos, ks, kos, vs, stride, heads, kv_heads,
-                     dim, pairs, count, 1 if interleaved else 0, 1 if norm else 0, code, w_code, eps)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_rotate(None if cache is None else cache._ref, a, stream):
-        _check(lib, code, "rotate")
-
-
-def _blocks(n: int) -> int:
-    return -(-n // F8_BLOCK)
+    ref, *has = (None, 0, 0) if cache is None else (cache._at, cache.kv_heads, cache.head_dim)
+    if code := (_calls or _bind()).rotate(q, k, positions, frequencies, q_out, k_out, axes, norm, q_weight, k_weight, eps, interleaved,
+                                          ref, *has, v, slots, stream):
+        _check(load_library(), code, "rotate")
 
 
 def rmsnorm_f8(x, weight, q, scale, *, residual=None, residual_out=None, eps: float = 1e-6, stream: int = 0) -> None:
@@ -578,35 +545,14 @@ def gate_f8(x, q, scale, *, stream: int = 0) -> None:
 
 
 def _rows_f8(kind, x, weight, q, scale, residual, residual_out, eps, stream) -> None:
-    shape, code = q.shape, _code(x)
-    if len(shape) != 2:
-        _fail("q", "not two-dimensional")
-    rows, cols = shape
-    w = w_code = r = r_stride = h = h_stride = 0
-    if weight is not None:
-        w, w_code = _vector("weight", weight, (code, _FP32), cols), _CODES[weight.dtype]
-    if residual is not None:
-        r_stride, r = _rows("residual", residual, (code,), shape), residual.data_ptr()
-    if residual_out is not None:
-        h_stride, h = _rows("residual_out", residual_out, (code,), shape), residual_out.data_ptr()
-    a = _pack_rows_f8(x.data_ptr(), r, w, h, q.data_ptr(), scale.data_ptr(), rows, cols, _rows("x", x, _FLOATS, (rows, 2 * cols) if kind == 2 else shape),
-                      r_stride, h_stride, _rows("q", q, _F8S, shape), _rows("scale", scale, _FP32S, (rows, _blocks(cols))), kind, code, w_code, eps)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_rows_f8(a, stream):
-        _check(lib, code, "rows_f8")
+    if code := (_calls or _bind()).rows_f8(kind, x, weight, q, scale, residual, residual_out, eps, stream):
+        _check(load_library(), code, "rows_f8")
 
 
 def dequantize_f8(q, scale, out, *, stream: int = 0) -> None:
     """out = q * scale, each 128 columns by their scale; out float32, float16 or bfloat16."""
-    shape = q.shape
-    if len(shape) != 2:
-        _fail("q", "not two-dimensional")
-    rows, cols = shape
-    a = _pack_dequantize_f8(q.data_ptr(), scale.data_ptr(), out.data_ptr(), rows, cols, _rows("q", q, _F8S, shape),
-                            _rows("scale", scale, _FP32S, (rows, _blocks(cols))), _rows("out", out, _FLOATS, shape), _code(out), 0)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_dequantize_f8(a, stream):
-        _check(lib, code, "dequantize_f8")
+    if code := (_calls or _bind()).dequantize_f8(q, scale, out, stream):
+        _check(load_library(), code, "dequantize_f8")
 
 
 def matmul_f8(a, a_scale, b, b_scale, out, *, bias=None, stream: int = 0) -> None:
@@ -616,15 +562,8 @@ def matmul_f8(a, a_scale, b, b_scale, out, *, bias=None, stream: int = 0) -> Non
     [blocks of n, blocks of k] and bias [n] float32, out [m, n] float32,
     float16 or bfloat16.
     """
-    if len(a.shape) != 2 or len(b.shape) != 2:
-        _fail("a, b", "not two-dimensional")
-    (m, k), n = a.shape, b.shape[0]
-    g = _pack_matmul_f8(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), 0 if bias is None else _vector("bias", bias, _FP32S, n),
-                        out.data_ptr(), m, n, k, _rows("a", a, _F8S, (m, k)), _rows("b", b, _F8S, (n, k)), _rows("out", out, _FLOATS, (m, n)),
-                        _rows("a_scale", a_scale, _FP32S, (m, _blocks(k))), _rows("b_scale", b_scale, _FP32S, (_blocks(n), _blocks(k))), _code(out), 0)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_matmul_f8(g, stream):
-        _check(lib, code, "matmul_f8")
+    if code := (_calls or _bind()).matmul_f8(a, a_scale, b, b_scale, out, bias, stream):
+        _check(load_library(), code, "matmul_f8")
 
 
 def matmul_f8_experts(a, a_scale, b, b_scale, offsets, out, *, order=None, per_token: int = 1, bias=None, stream: int = 0) -> None:
@@ -635,36 +574,8 @@ def matmul_f8_experts(a, a_scale, b, b_scale, offsets, out, *, order=None, per_t
     with an order (int32 [rows of out], sort_tokens' own) row order[r] //
     per_token.  Rows behind offsets[experts] are left as they were.
     """
-    if len(a.shape) != 2 or len(b.shape) != 3 or len(out.shape) != 2:
-        _fail("a, b, out", "not of two, three and two axes")
-    (rows, k), (experts, n, _), m = a.shape, b.shape, out.shape[0]
-    shapes = []
-    for name, t, codes, shape in (("b", b, _F8S, (experts, n, k)), ("b_scale", b_scale, _FP32S, (experts, _blocks(n), _blocks(k)))):
-        if t.shape != shape or _CODES.get(t.dtype) not in codes or not t.is_cuda:
-            _refuse(name, t, codes, shape)
-        expert, row, step = t.stride()
-        if step != 1 and shape[2] > 1:
-            _fail(name, "its last axis is not contiguous")
-        shapes.append((expert, row))
-    if bias is not None:
-        stride = _rows("bias", bias, _FP32S, (experts, n))
-        if stride != n and experts > 1:
-            _fail("bias", "not contiguous")
-    g = _pack_experts(a.data_ptr(), b.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
-                      m, n, k, _rows("a", a, _F8S, (rows, k)), shapes[0][1], _rows("out", out, _FLOATS, (m, n)),
-                      _rows("a_scale", a_scale, _FP32S, (rows, _blocks(k))), shapes[1][1], _code(out), 0,
-                      _vector("offsets", offsets, _INT32S, experts + 1), 0 if order is None else _vector("order", order, _INT32S, m), rows,
-                      shapes[0][0], shapes[1][0], experts, per_token)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_matmul_f8_experts(g, stream):
-        _check(lib, code, "matmul_f8_experts")
-
-
-def _matrix(name: str, t, codes, shape) -> int:
-    """A contiguous matrix's address, its type and shape checked."""
-    if _rows(name, t, codes, shape) != shape[1] and shape[0] > 1:
-        _fail(name, "not contiguous")
-    return t.data_ptr()
+    if code := (_calls or _bind()).matmul_f8_experts(a, a_scale, b, b_scale, offsets, out, order, per_token, bias, stream):
+        _check(load_library(), code, "matmul_f8_experts")
 
 
 def sort_tokens(experts, offsets, order, place, *, stream: int = 0) -> None:
@@ -676,19 +587,8 @@ def sort_tokens(experts, offsets, order, place, *, stream: int = 0) -> None:
     one expert keep their order.  A choice below zero, or of an expert that is
     not there, has no row and the place -1.
     """
-    shape = experts.shape
-    if len(shape) != 2:
-        _fail("experts", "not two-dimensional")
-    if len(offsets.shape) != 1:
-        _fail("offsets", "not one-dimensional")
-    tokens, per_token = shape
-    count = offsets.shape[0] - 1
-    a = _pack_sort(_matrix("experts", experts, (_INT32, _INT64), shape), _vector("offsets", offsets, _INT32S, count + 1),
-                   _vector("order", order, _INT32S, tokens * per_token), _matrix("place", place, _INT32S, shape), tokens, per_token, count,
-                   1 if _CODES[experts.dtype] == _INT64 else 0, 0)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_sort_tokens(a, stream):
-        _check(lib, code, "sort_tokens")
+    if code := (_calls or _bind()).sort_tokens(experts, offsets, order, place, stream):
+        _check(load_library(), code, "sort_tokens")
 
 
 def combine(y, place, weights, out, *, residual=None, stream: int = 0) -> None:
@@ -698,18 +598,8 @@ def combine(y, place, weights, out, *, residual=None, stream: int = 0) -> None:
     one type; place int32 and weights float32 [tokens, per_token].  A place
     that y does not have adds nothing.
     """
-    if len(y.shape) != 2 or len(place.shape) != 2:
-        _fail("y, place", "not two-dimensional")
-    (rows, cols), shape, code = y.shape, place.shape, _code(y)
-    tokens, per_token = shape
-    r = r_stride = 0
-    if residual is not None:
-        r, r_stride = residual.data_ptr(), _rows("residual", residual, (code,), (tokens, cols))
-    a = _pack_combine(y.data_ptr(), _matrix("place", place, _INT32S, shape), _matrix("weights", weights, _FP32S, shape), r, out.data_ptr(), rows,
-                      tokens, cols, _rows("y", y, _FLOATS, (rows, cols)), r_stride, _rows("out", out, (code,), (tokens, cols)), per_token, code)
-    lib = load_library()
-    if code := lib.spkv2_mi355x_combine(a, stream):
-        _check(lib, code, "combine")
+    if code := (_calls or _bind()).combine(y, place, weights, out, residual, stream):
+        _check(load_library(), code, "combine")
 
 
 def _contiguous(t) -> bool:

@@ -297,3 +297,55 @@ def test_every_kernel_is_some_calls(dtype, by_expert):
     wanted = {"matmul_" + f for f in FORMS if not (dtype == "float32" and "256x256" in f)}
     missing = wanted - set(sizes_of_kernels(dtype, by_expert))
     assert not missing, missing
+
+
+# ------------------------------------------------------------ numbers and handles of a call
+
+def test_numbers_past_their_types_are_refused():
+    import struct
+
+    a, sa, b, sb = Fake((4, 300), F8), Fake((4, 3), "float32"), Fake((5, 200, 300), F8), Fake((5, 2, 3), "float32")
+    off, o = Fake((6,), "int32"), Fake((4, 200), "float16")
+    for n in (1 << 31, -(1 << 31) - 1, 1 << 63):
+        with pytest.raises(struct.error):
+            decoder.matmul_f8_experts(a, sa, b, sb, off, o, per_token=n)
+    with pytest.raises(struct.error):
+        decoder.sort_tokens(Fake((1, 1 << 31), "int32"), off, Fake((1 << 31,), "int32"), Fake((1, 1 << 31), "int32"))
+    with pytest.raises(struct.error):
+        decoder.quantize_f8(Fake((1, 8), "float32", strides=(1 << 63, 1)), Fake((1, 8), F8), Fake((1, 1), "float32"))
+    for per_token in (1.5, "1", None):
+        with pytest.raises(TypeError):
+            decoder.matmul_f8_experts(a, sa, b, sb, off, o, per_token=per_token)
+
+
+@pytest.mark.parametrize("stream", [0, None, np.int64(0), ctypes.c_void_p(None), ctypes.c_void_p(0)])
+def test_streams_as_numbers_or_handles(stream):
+    """No rows: nothing is launched, so no stream is touched."""
+    x, q, s = Fake((0, 300), "float32"), Fake((0, 300), F8), Fake((0, 3), "float32")
+    decoder.quantize_f8(x, q, s, stream=stream)
+    decoder.dequantize_f8(q, s, x, stream=stream)
+    for wrong in ("0", 1.0):
+        with pytest.raises((TypeError, AttributeError)):
+            decoder.quantize_f8(x, q, s, stream=wrong)
+
+
+def test_tensors_whose_axes_are_no_tuple():
+    """shape and stride() may be any sequence; what raises in them comes through."""
+    class Listed(Fake):
+        def stride(self):
+            return list(self._strides)
+
+    class Broken(Fake):
+        def data_ptr(self):
+            raise KeyError("no storage")
+
+    x, q, s = Listed((0, 300), "float32"), Listed((0, 300), F8), Listed((0, 3), "float32")
+    x.shape, q.shape = [0, 300], [0, 300]
+    decoder.quantize_f8(x, q, s)
+    with pytest.raises(KeyError):
+        decoder.quantize_f8(Broken((0, 300), "float32"), q, s)
+    with pytest.raises(ValueError):
+        decoder.quantize_f8(Fake((0, 300, 1, 1, 1), "float32"), q, s)  # more axes than any call takes
+    x._strides = (300,)
+    with pytest.raises(ValueError):
+        decoder.quantize_f8(x, q, s)
