@@ -243,8 +243,9 @@ int spkv2_mi355x_rotate(const Spkv2KvCacheI8 *cache, const Spkv2Rotate *args, vo
  * format): eight values to a power of two from 2^-6 to 448, multiples of 2^-9
  * below.  Each 128 columns of a row (the last block may be shorter) become
  * codes 448 v / max|v|, rounded to the nearest, ties to even, and one float
- * scale max|v| / 448.  The codes are those of exact arithmetic (of the gate:
- * of 64-bit).  A block of zeros has scale 0; one that holds a NaN or an
+ * scale max|v| / 448.  The codes are those of exact arithmetic; of the gate
+ * those of its value in 64 bits, of whose quotients those within 2^-49 of the
+ * border of two codes are ties.  A block of zeros has scale 0; one that holds a NaN or an
  * infinity has scale NaN and codes 0.  A scale below 2^-126 loses bits. */
 #define SPKV2_F8_BLOCK 128
 
@@ -327,7 +328,8 @@ int spkv2_mi355x_matmul_f8_experts_kernel_name(const Spkv2MatmulF8Experts *args,
  * expert by c: order[r] is the choice that is row r of the sorted rows, place
  * its inverse, offsets[e] expert e's first row.  A choice of no expert (below
  * zero, or experts and above) has no row: its place is -1, and order is left
- * as it was from offsets[experts] on. */
+ * as it was from offsets[experts] on.  The outputs share no memory with each
+ * other or with ids. */
 typedef struct {
     const void *ids;  /* [tokens, per_token] */
     int32_t *offsets; /* [experts + 1] */

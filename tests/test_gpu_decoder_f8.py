@@ -708,3 +708,167 @@ def test_streams_and_graphs(gpu):
     hip("hipGraphExecDestroy", run)
     hip("hipGraphDestroy", graph)
     hip("hipStreamDestroy", stream)
+
+
+# ------------------------------------------------------- rows far apart, calls at once
+
+class Far(Array):
+    """Rows of the last axis 2^27 bytes and a page apart in a buffer that arrays share, each from a place of its own in them."""
+
+    ROWS, STEP, AREA = 64, 2 ** 27 + 4096, 2 ** 16
+
+    def __init__(self, buffer, area, shape, dtype):
+        size = 2 if dtype in ("bfloat16", "float16") else 1 if dtype == F8 else 4
+        inner = shape[1:]
+        strides = (self.STEP // size, *(int(np.prod(inner[i + 1:])) for i in range(len(inner))))
+        assert shape[0] <= self.ROWS and np.prod(inner) * size <= self.AREA
+        super().__init__(shape, dtype, buffer=buffer, at=area * self.AREA // size, strides=strides)
+
+    def _each(self):
+        for i in range(self.shape[0]):
+            yield i, ctypes.c_void_p(self.data_ptr() + i * self.STEP), int(np.prod(self.shape[1:])) * self.itemsize
+
+    def upload(self, values):
+        values = np.broadcast_to(np.asarray(values), self.shape)
+        to = {"bfloat16": decoder.to_bfloat16, "float8_e4m3fn": to_float8}.get(self.dtype, lambda v: v.astype(self.dtype))
+        lib = self.buffer.lib
+        for i, p, n in self._each():
+            row = np.ascontiguousarray(to(values[i]))
+            assert row.nbytes == n and lib.spkv2_device_memcpy_h2d(p, row.ctypes.data, n) == 0
+        return self
+
+    def download(self):
+        kind, lib = self._kind(), self.buffer.lib
+        raw = np.empty(self.shape, kind)
+        for i, p, n in self._each():
+            assert lib.spkv2_device_memcpy_d2h(raw[i:].ctypes.data, p, n) == 0
+        if self.dtype == F8:
+            return _FLOAT8[raw]
+        return (raw.astype(np.uint32) << 16).view(np.float32) if self.dtype == "bfloat16" else raw
+
+
+@pytest.fixture(scope="module")
+def far(gpu):
+    """Far arrays of one buffer of 8 GiB: far(area, shape, dtype)."""
+    from spinnv2_amd.runtime import DeviceBuffer
+
+    buffer = DeviceBuffer(Far.ROWS * Far.STEP)
+    yield lambda area, shape, dtype: Far(buffer, area, shape, dtype)
+    buffer.free()
+
+
+@pytest.mark.parametrize("kind", ["values", "norm", "gate"])
+def test_rows_far_apart(far, kind):
+    """Rows past 2^32 bytes from the first, and back."""
+    rows, cols = 50, 1000
+    rng = np.random.default_rng(2)
+    x = rounded(rng.standard_normal((rows, 2 * cols if kind == "gate" else cols)), "bfloat16")
+    dx, q, s, back = far(0, x.shape, "bfloat16").upload(x), far(1, (rows, cols), F8), far(2, (rows, 8), "float32"), far(3, (rows, cols), "bfloat16")
+    want_q, want_s, want_back = Array((rows, cols), F8), Array((rows, 8), "float32"), Array((rows, cols), "bfloat16")
+    near = Array.of(x, "bfloat16")
+    w = Array.of(rounded(1 + 0.3 * rng.standard_normal(cols), "bfloat16"), "bfloat16")
+    for a, b, c, d, h in ((dx, q, s, back, far(4, (rows, cols), "bfloat16")), (near, want_q, want_s, want_back, Array((rows, cols), "bfloat16"))):
+        if kind == "norm":
+            decoder.rmsnorm_f8(a, w, b, c, residual=a, residual_out=h)
+            np.testing.assert_array_equal(h.download(), rounded(2 * x, "bfloat16"))
+        else:
+            (decoder.gate_f8 if kind == "gate" else decoder.quantize_f8)(a, b, c)
+        decoder.dequantize_f8(b, c, d)
+    for a, b in ((q, want_q), (s, want_s), (back, want_back)):
+        np.testing.assert_array_equal(a.download(), b.download())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("which", ["a", "b", "out"])
+def test_matmul_rows_far_apart(far, which, dtype):
+    m, n, k = (64, 60, 384) if which == "b" else (60, 300, 384)
+    rng = np.random.default_rng(3)
+    a, b, sa, sb = _whole(rng, (m, k)), _whole(rng, (n, k)), _twos(rng, (m, 3)), _twos(rng, (_blocks(n), 3))
+    put = lambda area, v, t, name: far(area, v.shape, t).upload(v) if which == name else Array.of(v, t)  # noqa: E731
+    out = far(4, (m, n), dtype) if which == "out" else Array((m, n), dtype)
+    decoder.matmul_f8(put(0, a, F8, "a"), put(1, sa, "float32", "a"), put(2, b, F8, "b"), put(3, sb, "float32", "b"), out)
+    with np.errstate(over="ignore"):
+        np.testing.assert_array_equal(out.download().astype(np.float64), rounded(_product(a, sa, b, sb), dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [4, 60, 900])
+def test_experts_far_apart(far, tokens, dtype):
+    """Experts' weights past 2^32 bytes from the first, and outputs where they are few."""
+    n, k, experts = 140, 256, 60
+    rng = np.random.default_rng(tokens)
+    ids = rng.integers(experts - 5, experts, (tokens, 1)).astype(np.int32)
+    offsets, order, _ = _order(ids, experts)
+    a, b, sa, sb = _whole(rng, (tokens, k)), _whole(rng, (experts, n, k)), _twos(rng, (tokens, 2)), _twos(rng, (experts, 2, 2))
+    out = far(4, (tokens, n), dtype) if tokens <= Far.ROWS else Array((tokens, n), dtype)
+    decoder.matmul_f8_experts(Array.of(a, F8), Array.of(sa, "float32"), far(0, b.shape, F8).upload(b), far(1, sb.shape, "float32").upload(sb),
+                              Array.of(offsets), out, order=Array.of(order))
+    want = np.zeros((tokens, n))
+    for e in range(experts):
+        row = order[offsets[e]:offsets[e + 1]]
+        want[offsets[e]:offsets[e + 1]] = _product(a[row], sa[row], b[e], sb[e])
+    with np.errstate(over="ignore"):
+        np.testing.assert_array_equal(out.download().astype(np.float64), rounded(want, dtype))
+
+
+def test_combine_and_rotate_far_apart(far):
+    rng = np.random.default_rng(6)
+    y, r = rounded(rng.standard_normal((60, 520)), "bfloat16"), rounded(rng.standard_normal((50, 520)), "bfloat16")
+    place, weights = Array.of(rng.integers(0, 60, (50, 3)).astype(np.int32)), Array.of(rng.standard_normal((50, 3)).astype(np.float32))
+    out, want = far(2, (50, 520), "bfloat16"), Array((50, 520), "bfloat16")
+    decoder.combine(far(0, y.shape, "bfloat16").upload(y), place, weights, out, residual=far(1, r.shape, "bfloat16").upload(r))
+    decoder.combine(Array.of(y, "bfloat16"), place, weights, want, residual=Array.of(r, "bfloat16"))
+    np.testing.assert_array_equal(out.download(), want.download())
+    heads = [rounded(rng.standard_normal((50, n, 64)), "bfloat16") for n in (4, 2, 2)]
+    positions, frequencies = rng.integers(0, 9999, (50, 2)).astype(np.int32), np.float32(1) / np.arange(1, 33, dtype=np.float32)
+    axes, slots = Array.of(rng.integers(0, 2, 32).astype(np.int32)), Array.of(rng.permutation(64)[:50].astype(np.int64))
+    results = []
+    for place_at in (lambda area, v, t: far(area, v.shape, t).upload(v), lambda area, v, t: Array.of(v, t)):
+        q, k, v = (place_at(i, x, "bfloat16") for i, x in enumerate(heads))
+        cache = KvCache.empty(4, 2, 16, 64)
+        for b in cache.buffers:
+            b.upload(np.zeros(b.shape))
+        decoder.rotate(q, k, place_at(3, positions, "int32"), Array.of(frequencies), q, k, axes=axes, norm=True, cache=cache, v=v, slots=slots)
+        results.append([x.download() for x in (q, k, *cache.buffers)])
+    for a, b in zip(*results):
+        np.testing.assert_array_equal(a, b)
+
+
+def test_calls_of_two_threads_at_once(gpu):
+    """Two threads, each with a layer and a stream of its own: nothing of a call is shared with another."""
+    import threading
+
+    hip = Hip()
+    layers = [_layer_arrays(np.random.default_rng(30 + i), 30 + 9 * i, 2, 5, 200, 150) for i in range(2)]
+    wanted = []
+    for s in layers:
+        _layer(s, 2)
+        wanted.append([s[k].download() for k in ("out", "order", "place", "offsets")])
+        s["out"].upload(0)
+    streams, failed = [hip.stream() for _ in layers], []
+
+    def work(s, stream):
+        try:
+            for _ in range(40):
+                _layer(s, 2, stream.value)
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(layers, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for stream in streams:
+        hip("hipStreamSynchronize", stream)
+        hip("hipStreamDestroy", stream)
+    assert not failed
+    for s, want in zip(layers, wanted):
+        for name, w in zip(("out", "order", "place", "offsets"), want):
+            np.testing.assert_array_equal(s[name].download(), w)
+
+
+@pytest.mark.parametrize("tokens", [1, 50, 3000])
+def test_as_many_experts_as_there_may_be(gpu, tokens):
+    rng = np.random.default_rng(tokens)
+    _experts_case(_ids(rng, tokens, 2, 4096, "any"), 4096, 9, 48, "float32", spare=3)
