@@ -31,7 +31,9 @@ struct MatmulArgs {
     // by expert
     const int32_t *offsets, *order;
     int64_t a_rows, b_expert, sb_expert;
-    int experts, per_token;
+    int experts;
+    unsigned token_mul;  // choice / per_token, by multiplication
+    int token_shift;
 };
 
 // 16 bytes at p, of which `left` are inside the row: zeros past them
@@ -100,54 +102,62 @@ __device__ __forceinline__ floatx4 product(const Operand<true> &x, const Operand
     return sum;
 }
 
+// Sums over a wave's lanes up to each, by lane moves: an LDS shuffle in their place waits for LDS six times
+__device__ __forceinline__ int sums_through(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // a row of 16 lanes, 1 lane on
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the last lane of rows 0 and 2 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 to rows 2 and 3
+    return v;
+}
+
 // Rows first .. end of one expert's that a workgroup of `height` rows takes
 struct Rows {
     int expert, first, end;
 };
+// 64 experts, one a lane: their rows, and workgroups of `height` of them, counted with those of the lanes before
+struct Experts {
+    int low, high, tiles, through;
+};
+__device__ __forceinline__ Experts experts_from(const MatmulArgs &a, int e0, int height) {
+    const int e = e0 + (threadIdx.x & 63);
+    Experts x{0, 0, 0, 0};
+    if (e < a.experts) {
+        x.low = min(max(a.offsets[e], 0), a.m);
+        x.high = min(max(a.offsets[e + 1], x.low), a.m);
+    }
+    x.tiles = (x.high - x.low + height - 1) / height;
+    x.through = sums_through(x.tiles);
+    return x;
+}
+__device__ __forceinline__ int tiles_of(const Experts &x) { return __builtin_amdgcn_readlane(x.through, 63); }
 // The workgroups of all experts' rows, one expert's after the other's: which of
-// them is number `at`; expert -1 where there are fewer.
-__device__ __forceinline__ Rows rows_of(const MatmulArgs &a, int at, int height) {
-    const int lane = threadIdx.x & 63;
-    for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int e = e0 + lane;
-        int low = 0, high = 0;
-        if (e < a.experts) {
-            low = min(max(a.offsets[e], 0), a.m);
-            high = min(max(a.offsets[e + 1], low), a.m);
-        }
-        const int tiles = (high - low + height - 1) / height;
-        int through = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int v = __shfl_up(through, d);
-            if (lane >= d) through += v;
-        }
-        const uint64_t past = __ballot(through > at);
+// them is number `at`, `x` the first 64 experts; expert -1 where there are fewer.
+__device__ __forceinline__ Rows rows_of(const MatmulArgs &a, Experts x, int at, int height) {
+    for (int e0 = 0;;) {
+        const uint64_t past = __ballot(x.through > at);
         if (past) {
             const int l = __builtin_ctzll(past);
             Rows r;
             r.expert = e0 + l;
-            const int before = __builtin_amdgcn_readlane(through, l) - __builtin_amdgcn_readlane(tiles, l);
-            r.first = __builtin_amdgcn_readlane(low, l) + (at - before) * height;
-            r.end = min(__builtin_amdgcn_readlane(high, l), r.first + height);
+            const int before = __builtin_amdgcn_readlane(x.through, l) - __builtin_amdgcn_readlane(x.tiles, l);
+            r.first = __builtin_amdgcn_readlane(x.low, l) + (at - before) * height;
+            r.end = min(__builtin_amdgcn_readlane(x.high, l), r.first + height);
             return r;
         }
-        at -= __builtin_amdgcn_readlane(through, 63);
+        at -= tiles_of(x);
+        e0 += 64;
+        if (e0 >= a.experts) return Rows{-1, 0, 0};
+        x = experts_from(a, e0, height);
     }
-    return Rows{-1, 0, 0};
 }
-
-// How many there are
-__device__ __forceinline__ int tiles_of(const MatmulArgs &a, int height) {
-    const int lane = threadIdx.x & 63;
-    int tiles = 0;
-    for (int e = lane; e < a.experts; e += 64) {
-        const int low = min(max(a.offsets[e], 0), a.m);
-        tiles += (min(max(a.offsets[e + 1], low), a.m) - low + height - 1) / height;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) tiles += __shfl_xor(tiles, d);
-    return __builtin_amdgcn_readfirstlane(tiles);
+// the row of a that output row r takes; negative: none, or one that a may not have
+__device__ __forceinline__ int row_of(const MatmulArgs &a, int r) {
+    if (!a.order) return r;
+    const int choice = a.order[r];
+    return choice < 0 ? -1 : static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(choice)) * a.token_mul) >> a.token_shift);
 }
 
 // 16 TM tokens x 16 TN channels a workgroup, whose waves deal k out among them,
@@ -167,7 +177,7 @@ __global__ void __launch_bounds__(512) matmul_rows(MatmulArgs a) {
     const int n0 = blockIdx.x * 16 * TN;
     int m0 = blockIdx.y * 16 * TM, end_m = a.m, expert = 0;
     if constexpr (EXPERTS) {
-        const Rows r = rows_of(a, blockIdx.y, 16 * TM);
+        const Rows r = rows_of(a, experts_from(a, 0, 16 * TM), blockIdx.y, 16 * TM);
         if (r.expert < 0) return;
         expert = r.expert;
         m0 = r.first;
@@ -178,7 +188,7 @@ __global__ void __launch_bounds__(512) matmul_rows(MatmulArgs a) {
     const auto input = [&](int r) -> int64_t {
         r = min(r, end_m - 1);
         if constexpr (!EXPERTS) return r;
-        const int64_t at = a.order ? static_cast<unsigned>(a.order[r]) / static_cast<unsigned>(a.per_token) : r;
+        const int at = row_of(a, r);
         return at < a.a_rows ? at : -1;
     };
     const int blocks = (a.k + 127) / 128, per = (blocks + WAVES - 1) / WAVES;
@@ -329,7 +339,12 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
     int m0, end_m = a.m, expert = 0, nt;
     {
         int m_tiles = (a.m + BM - 1) / BM;
-        if constexpr (EXPERTS) m_tiles = tiles_of(a, BM);
+        Experts x;
+        if constexpr (EXPERTS) {
+            x = experts_from(a, 0, BM);
+            m_tiles = tiles_of(x);
+            for (int e0 = 64; e0 < a.experts; e0 += 64) m_tiles += tiles_of(experts_from(a, e0, BM));
+        }
         const int tiles = m_tiles * a.n_tiles, per = tiles / 8, rest = tiles % 8;
         const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
         if (local >= per + (xcd < rest ? 1 : 0)) return;
@@ -340,7 +355,7 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         nt = in / height;
         m0 = mt * BM;
         if constexpr (EXPERTS) {
-            const Rows r = rows_of(a, mt, BM);
+            const Rows r = rows_of(a, x, mt, BM);
             if (r.expert < 0) return;
             expert = r.expert;
             m0 = r.first;
@@ -353,8 +368,8 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
     const auto input = [&](int r) -> unsigned {  // ~0: a row that is not there, for which the first is read
         r = min(r, end_m - 1);
         if constexpr (!EXPERTS) return r;
-        const unsigned at = a.order ? static_cast<unsigned>(a.order[r]) / static_cast<unsigned>(a.per_token) : r;
-        return at < a.a_rows ? at : 0xffffffffu;
+        const int at = row_of(a, r);
+        return at >= 0 && at < a.a_rows ? at : 0xffffffffu;
     };
 
     // A thread's pieces of a step: kA of a, then kB of b, kThreads / 8 rows apart.
@@ -639,7 +654,7 @@ int check(const Spkv2MatmulF8Experts *g, bool pointers) {
 
 MatmulArgs arguments(const Spkv2MatmulF8 &g) {
     MatmulArgs a{g.a, g.b, g.a_scale, g.b_scale, g.bias, g.out, g.a_stride, g.b_stride, g.out_stride, g.a_scale_stride, g.b_scale_stride,
-                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), 0, nullptr, nullptr, g.m, 0, 0, 1, 1};
+                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), 0, nullptr, nullptr, g.m, 0, 0, 1, 0, 0};
     if (g.m == 1) a.a_stride = 0, a.sa_stride = 0, a.out_stride = 0;
     if (g.n == 1) a.b_stride = 0;
     if (g.n <= 128) a.sb_stride = 0;
@@ -764,7 +779,7 @@ MatmulArgs arguments(const Spkv2MatmulF8Experts &g) {
     a.b_expert = g.experts > 1 ? g.b_expert_stride : 0;
     a.sb_expert = g.experts > 1 ? g.b_scale_expert_stride : 0;
     a.experts = g.experts;
-    a.per_token = g.per_token;
+    div_magic(static_cast<unsigned>(g.per_token), &a.token_mul, &a.token_shift);
     a.a_stride = g.product.a_stride, a.sa_stride = g.product.a_scale_stride;
     if (g.a_rows == 1) a.a_stride = 0, a.sa_stride = 0;
     return a;
