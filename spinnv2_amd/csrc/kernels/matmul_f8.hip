@@ -664,10 +664,11 @@ MatmulArgs arguments(const Spkv2MatmulF8 &g) {
 // A kernel's time: a launch's, then steps by every workgroup, of a block of k for
 // each of its groups of waves, which take `step` each where a CU's workgroups do
 // not fill it, or `work` for each of the CU's workgroups where they do, and the
-// workgroup's sums.  Fitted, in us, to 1300 products of log-uniform sizes (m 1 ..
+// workgroup's sums.  Fitted, in us, to 5450 products of log-uniform sizes (m 1 ..
 // 8192, n and k 64 .. 16384, up to 2^37 multiplications; half of them by expert):
-// the kernel of the least time by these is 2.0% slower than the fastest of them in
-// the mean, 28% in one of a hundred.
+// the kernel of the least time by these is 1.5% slower than the fastest of them in
+// the mean, 25% in one of a hundred.  Tiles of 128 x 256 are the fastest where they
+// fill the CUs once and larger ones half of them (2048 x 4096 x 4096 55 -> 41 us).
 struct Cost {
     float launch, step, work, sums;
 };
@@ -677,16 +678,17 @@ struct Form {
     Cost cost[4];  // 16-bit outputs with rows of whole runs of 16 bytes, and others; fp32 outputs likewise
 };
 constexpr Form kForms[] = {
-    {16, 16, 8, false, {{1.25f, 0.155f, 0.670f, 1.527f}, {1.62f, 0.194f, 0.868f, 1.268f}, {1.34f, 0.094f, 0.762f, 1.463f}, {1.38f, 1.038f, 0.948f, 1.380f}}},
-    {16, 32, 8, false, {{1.62f, 0.059f, 1.017f, 1.013f}, {1.97f, 1.164f, 1.304f, 0.741f}, {1.75f, 0.846f, 1.134f, 0.951f}, {1.88f, 0.818f, 1.449f, 0.760f}}},
-    {16, 64, 8, false, {{1.54f, 1.358f, 1.477f, 1.053f}, {1.93f, 1.262f, 2.150f, 0.464f}, {1.71f, 1.319f, 1.656f, 0.920f}, {1.76f, 2.152f, 2.447f, 0.357f}}},
-    {32, 64, 8, false, {{0.45f, 1.215f, 1.773f, 2.389f}, {1.02f, 2.192f, 2.541f, 1.621f}, {0.83f, 1.795f, 2.092f, 2.002f}, {0.88f, 2.868f, 2.883f, 1.528f}}},
-    {64, 64, 1, true, {{2.98f, 0.374f, 0.275f, 0.887f}, {2.96f, 0.792f, 0.433f, 0.838f}, {3.04f, 0.510f, 0.318f, 1.113f}, {2.78f, 0.980f, 0.507f, 1.003f}}},
-    {64, 64, 2, true, {{2.26f, 0.353f, 0.533f, 1.758f}, {2.25f, 1.141f, 0.854f, 1.516f}, {2.22f, 0.739f, 0.630f, 2.041f}, {2.08f, 1.403f, 1.029f, 1.644f}}},
-    {64, 64, 4, true, {{0.00f, 0.204f, 0.951f, 4.516f}, {0.39f, 0.832f, 1.875f, 3.531f}, {0.44f, 1.245f, 1.285f, 4.474f}, {0.39f, 2.212f, 2.228f, 3.669f}}},
-    {32, 128, 1, true, {{2.98f, 0.417f, 0.350f, 0.949f}, {2.99f, 0.907f, 0.568f, 0.789f}, {2.82f, 0.559f, 0.374f, 1.276f}, {2.54f, 1.102f, 0.636f, 1.094f}}},
-    {128, 128, 1, true, {{2.78f, 0.381f, 0.655f, 2.523f}, {2.57f, 1.406f, 0.998f, 2.355f}, {2.88f, 1.081f, 0.861f, 3.255f}, {2.36f, 2.117f, 1.439f, 2.945f}}},
-    {256, 256, 1, true, {{0.00f, 0.100f, 1.047f, 7.766f}, {0.00f, 2.080f, 2.113f, 7.675f}, {}, {}}},
+    {16, 16, 8, false, {{1.52f, 0.006f, 0.686f, 1.191f}, {1.54f, 0.878f, 0.906f, 1.109f}, {1.50f, 0.446f, 0.751f, 1.241f}, {1.69f, 0.337f, 0.989f, 1.009f}}},
+    {16, 32, 8, false, {{1.81f, 1.006f, 1.034f, 0.785f}, {1.89f, 1.298f, 1.340f, 0.630f}, {1.82f, 0.095f, 1.136f, 0.762f}, {2.04f, 1.059f, 1.445f, 0.500f}}},
+    {16, 64, 8, false, {{1.71f, 0.106f, 1.567f, 0.733f}, {1.78f, 2.246f, 2.251f, 0.262f}, {1.74f, 0.118f, 1.719f, 0.691f}, {2.01f, 2.253f, 2.328f, 0.183f}}},
+    {32, 64, 8, false, {{0.77f, 1.323f, 1.892f, 1.891f}, {0.85f, 0.993f, 2.681f, 1.388f}, {0.93f, 2.156f, 2.164f, 1.689f}, {1.18f, 2.480f, 2.851f, 1.187f}}},
+    {64, 64, 1, true, {{3.08f, 0.378f, 0.267f, 0.705f}, {2.77f, 0.809f, 0.443f, 0.731f}, {3.16f, 0.503f, 0.325f, 0.857f}, {2.93f, 0.939f, 0.510f, 0.865f}}},
+    {64, 64, 2, true, {{2.61f, 0.534f, 0.527f, 1.348f}, {2.19f, 1.187f, 0.885f, 1.271f}, {2.57f, 0.729f, 0.635f, 1.557f}, {2.45f, 1.351f, 1.033f, 1.308f}}},
+    {64, 64, 4, true, {{0.66f, 0.645f, 0.976f, 3.734f}, {0.69f, 0.900f, 1.959f, 2.926f}, {0.85f, 0.401f, 1.305f, 3.733f}, {0.97f, 1.046f, 2.220f, 2.994f}}},
+    {32, 128, 1, true, {{3.04f, 0.408f, 0.335f, 0.791f}, {2.67f, 0.929f, 0.556f, 0.804f}, {2.91f, 0.537f, 0.374f, 1.062f}, {2.66f, 1.063f, 0.626f, 0.978f}}},
+    {128, 128, 1, true, {{2.66f, 0.668f, 0.570f, 2.334f}, {1.94f, 1.439f, 0.992f, 2.511f}, {2.99f, 1.079f, 0.880f, 2.717f}, {2.39f, 2.080f, 1.425f, 2.711f}}},
+    {128, 256, 1, true, {{0.00f, 0.100f, 0.887f, 5.073f}, {0.00f, 0.100f, 1.655f, 4.976f}, {}, {}}},
+    {256, 256, 1, true, {{0.00f, 0.100f, 1.118f, 7.074f}, {0.00f, 1.863f, 2.145f, 6.893f}, {}, {}}},
 };
 constexpr int kFormCount = sizeof(kForms) / sizeof(kForms[0]);
 
@@ -720,7 +722,8 @@ int form(const MatmulArgs &a, bool experts, int dtype) {
         const int64_t across = (static_cast<int64_t>(a.n) + f.channels - 1) / f.channels, down = most_down(a, experts, f.tokens);
         // a launch has fewer than 2^32 threads along an axis, and as many workgroups along the second as 16 bits hold
         if (f.tiles ? !near || a.k < 16 || down * across >= 1 << 22 : down > 65535) continue;
-        if (f.tokens == 256 && dtype == SPKV2_DTYPE_FP32) continue;  // two registers' operands do not fit beside its sums
+        // outputs of 32 bits do not fit their LDS, nor two registers' operands beside sums of 256 x 256
+        if (f.channels == 256 && dtype == SPKV2_DTYPE_FP32) continue;
         const Cost &c = f.cost[kind];
         const double steps = (blocks + f.groups - 1) / f.groups, each = ceil(about_down(a, experts, f.tokens) * across / 256.0);
         const double time = c.launch + steps * std::max(static_cast<double>(c.step), each * c.work) + each * c.sums;
@@ -755,6 +758,7 @@ int run(const char *what, int dtype, MatmulArgs a, void *stream) {
             case 8: return tiles(matmul_tiles<T, EXPERTS, true, 2, 2, 1, 4, 4>, matmul_tiles<T, EXPERTS, false, 2, 2, 1, 4, 4>, 4);
             default:
                 if constexpr (sizeof(T) == 4) return -1;
+                else if (i == 9) return tiles(matmul_tiles<T, EXPERTS, true, 2, 4, 1, 4, 4>, matmul_tiles<T, EXPERTS, false, 2, 4, 1, 4, 4>, 8);
                 else return tiles(matmul_tiles<T, EXPERTS, true, 4, 2, 1, 4, 8>, matmul_tiles<T, EXPERTS, false, 4, 2, 1, 4, 8>, 8);
         }
     });

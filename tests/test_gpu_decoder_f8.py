@@ -369,7 +369,7 @@ def test_every_kernel_of_the_product(gpu, form, dtype):
     """Each kernel at the smallest sizes that take it, with rows apart, a bias, a row of NaN and codes behind the rows' ends."""
     sizes = sizes_of_kernels(dtype, False)
     if "matmul_" + form not in sizes:
-        assert dtype == "float32" and "256x256" in form
+        assert dtype == "float32" and "x256" in form
         return
     m, n, k, _ = sizes["matmul_" + form]
     _matmul_case(m, n, k, dtype)
@@ -551,7 +551,7 @@ def test_every_kernel_of_the_experts_product(gpu, form, dtype):
     """Each kernel at the smallest sizes that take it, the experts of ragged counts of rows."""
     sizes = sizes_of_kernels(dtype, True)
     if "matmul_" + form not in sizes:
-        assert dtype == "float32" and "256x256" in form
+        assert dtype == "float32" and "x256" in form
         return
     m, n, k, experts = sizes["matmul_" + form]
     rng = np.random.default_rng(m)
