@@ -8,8 +8,8 @@
 // turns by, and groups of 8, 16 or 32 lanes a head each, 8 elements a lane.
 //
 // Bound by HBM and by its arithmetic, each two thirds of the time: 8190 tokens of
-// 32 + 8 heads of 128 in bf16, values too, into the cache in 48 us (185 MB, 3.9
-// TB/s), without a cache in 38 (168 MB, 4.4 TB/s); fp32 without a cache at 5.2
+// 32 + 8 heads of 128 in bf16, values too, into the cache in 48 to 56 us (185 MB, 3.3
+// to 3.9 TB/s), without a cache in 38 (168 MB, 4.4 TB/s); fp32 without a cache at 5.2
 // TB/s.
 //
 // In 64 bits: angles of far positions need it (position 70001 times a frequency
