@@ -5,7 +5,7 @@
 // its numbers packed there too, costs 0.5 us, from here 0.3, which its five
 // attributes are themselves: a product's call without its launch took 2.7 us and
 // takes 1.5, 4 rows of 2048 normed and read back 14.3 us and 12.1, one token of
-// 4 sequences rotated into the cache and read back 17.9 us and 15.2.
+// 4 sequences rotated into the cache and read back 17.9 us and 14.0.
 //
 // A tensor is anything with data_ptr(), shape, stride(), dtype and is_cuda.
 // Nothing is kept between calls but the entry points' addresses.
@@ -44,6 +44,8 @@ struct Entries {
     int (*experts)(const Spkv2MatmulF8Experts *, void *);
     int (*sort)(const Spkv2SortTokens *, void *);
     int (*combine)(const Spkv2Combine *, void *);
+    int (*kv_write)(const Spkv2KvCacheI8 *, const Spkv2KvWrite *, void *);
+    int (*kv_read)(const Spkv2KvCacheI8 *, const Spkv2KvRead *, void *);
 } entries;
 
 struct Refused {};  // a Python exception is set
@@ -455,18 +457,59 @@ PyObject *combine(PyObject *, PyObject *const *a, Py_ssize_t count) {
     });
 }
 
+// (cache, kv_heads, head_dim, k, v, slots, stream): cache the address of its struct
+PyObject *kv_write(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded<7>(count, [&]() -> int {
+        Spkv2KvWrite g{};
+        const int64_t heads = number(a[1]), dim = number(a[2]);
+        Tensor k = first_look(a[3], "k", 3, "not [tokens, kv_heads, head_dim]");
+        g.tokens = k.shape[0], g.dtype = k.code;
+        g.k = heads_settled(k, kFloats, g.tokens, heads, dim).p, g.k_stride = k.stride[0];
+        const Tensor v = heads_of(a[4], "v", bit(k.code), g.tokens, heads, dim);
+        g.v = v.p, g.v_stride = v.stride[0];
+        g.slots = as<int64_t>(vector(a[5], "slots", bit(kInt64), g.tokens));
+        const auto *cache = static_cast<const Spkv2KvCacheI8 *>(address(a[0]));
+        void *stream = handle(a[6]);
+        return unlocked([&] { return entries.kv_write(cache, &g, stream); });
+    });
+}
+
+// (cache, kv_heads, head_dim, table, first, offsets, k, v, stream)
+PyObject *kv_read(PyObject *, PyObject *const *a, Py_ssize_t count) {
+    return guarded<9>(count, [&]() -> int {
+        Spkv2KvRead g{};
+        const int64_t heads = number(a[1]), dim = number(a[2]);
+        Tensor table = first_look(a[3], "table", 2, "not two-dimensional");
+        const int64_t sequences = table.shape[0];
+        rows_settled(table, bit(kInt32), sequences, table.shape[1]);
+        if (table.stride[0] != table.shape[1] && sequences > 1) refuse("table", "not contiguous");
+        g.table = as<int32_t>(table);
+        g.sequences = as_int32(sequences), g.table_width = as_int32(table.shape[1]);
+        if (given(a[4])) g.first = as<int32_t>(vector(a[4], "first", bit(kInt32), sequences));
+        g.offsets = as<int32_t>(vector(a[5], "offsets", bit(kInt32), sequences + 1));
+        Tensor k = first_look(a[6], "k", 3, "not [tokens, kv_heads, head_dim]");
+        g.tokens = k.shape[0], g.dtype = k.code;
+        g.k = heads_settled(k, kFloats, g.tokens, heads, dim).p, g.k_stride = k.stride[0];
+        const Tensor v = heads_of(a[7], "v", bit(k.code), g.tokens, heads, dim);
+        g.v = v.p, g.v_stride = v.stride[0];
+        const auto *cache = static_cast<const Spkv2KvCacheI8 *>(address(a[0]));
+        void *stream = handle(a[8]);
+        return unlocked([&] { return entries.kv_read(cache, &g, stream); });
+    });
+}
+
 // (codes, code_of, range_error, addresses): the dict of types, what looks one up that it lacks, struct.error, the entry
 // points' addresses in the order of Entries
 PyObject *bind(PyObject *, PyObject *args) {
     PyObject *d, *f, *r, *list;
     if (!PyArg_ParseTuple(args, "O!OOO!", &PyDict_Type, &d, &f, &r, &PyTuple_Type, &list)) return nullptr;
-    void *p[7];
+    void *p[9];
     static_assert(sizeof(p) == sizeof(entries), "an address for each entry");
-    if (PyTuple_GET_SIZE(list) != 7) {
-        PyErr_SetString(PyExc_TypeError, "expected seven addresses");
+    if (PyTuple_GET_SIZE(list) != 9) {
+        PyErr_SetString(PyExc_TypeError, "expected nine addresses");
         return nullptr;
     }
-    for (int i = 0; i < 7; i++) {
+    for (int i = 0; i < 9; i++) {
         p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(list, i));
         if (!p[i]) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "an address is 0");
@@ -491,6 +534,8 @@ PyMethodDef methods[] = {method<rotate>("rotate"),
                          method<matmul_f8_experts>("matmul_f8_experts"),
                          method<sort_tokens>("sort_tokens"),
                          method<combine>("combine"),
+                         method<kv_write>("kv_write"),
+                         method<kv_read>("kv_read"),
                          {"bind", bind, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -43,7 +43,7 @@ _FP32, _INT8, _FP16, _BF16, _INT32, _INT64, _F8 = 1, 2, 3, 4, 101, 102, 103
 _CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64,
           "float8_e4m3fn": _F8}
 _FLOATS = (_FP32, _FP16, _BF16)
-_FP32S, _INT8S, _INT32S, _INT64S = (_FP32,), (_INT8,), (_INT32,), (_INT64,)
+_FP32S, _INT8S, _INT32S = (_FP32,), (_INT8,), (_INT32,)
 #: columns of a row of 8-bit floats, and rows and columns of weights, that share a scale
 F8_BLOCK = 128
 
@@ -149,7 +149,7 @@ def _packer(cls):
 
 
 _pack_norm, _pack_dequantize, _pack_matmul = _packer(_RmsNorm), _packer(_Dequantize), _packer(_Matmul)
-_pack_write, _pack_read, _pack_attention = _packer(_Write), _packer(_Read), _packer(_Attention)
+_pack_attention = _packer(_Attention)
 
 
 #: the calls that take their tensors apart in native code (bindings/decoder_calls.cpp), once _bind() was called
@@ -169,7 +169,8 @@ def _bind():
     spec.loader.exec_module(calls)
     calls.bind(_CODES, _code, struct.error, tuple(
         ctypes.cast(getattr(lib, "spkv2_mi355x_" + name), _P).value
-        for name in ("rotate", "rows_f8", "dequantize_f8", "matmul_f8", "matmul_f8_experts", "sort_tokens", "combine")))
+        for name in ("rotate", "rows_f8", "dequantize_f8", "matmul_f8", "matmul_f8_experts", "sort_tokens", "combine",
+                     "kv_write_i8", "kv_read_i8")))
     _calls = calls
     return calls
 
@@ -436,27 +437,15 @@ class KvCache:
     def write(self, k, v, slots, *, stream: int = 0) -> None:
         """Quantises k and v [tokens, kv_heads, head_dim] into the slots (int64
         [tokens]; negative ones, and those past the cache, are not written)."""
-        shape = (k.shape[0], self.kv_heads, self.head_dim)
-        code = _code(k)
-        a = _pack_write(k.data_ptr(), v.data_ptr(), _vector("slots", slots, _INT64S, shape[0]), shape[0],
-                        _heads("k", k, _FLOATS, shape), _heads("v", v, (code,), shape), code, 0)
-        lib = load_library()
-        if code := lib.spkv2_mi355x_kv_write_i8(self._ref, a, stream):
-            _check(lib, code, "kv_write_i8")
+        if code := (_calls or _bind()).kv_write(self._at, self.kv_heads, self.head_dim, k, v, slots, stream):
+            _check(load_library(), code, "kv_write_i8")
 
     def read(self, table, first, offsets, k, v, *, stream: int = 0) -> None:
         """Reads tokens first[s] .. of each sequence s into rows offsets[s] ..
         offsets[s + 1] of k and v.  table int32 [sequences, width], first int32
         [sequences] or None, offsets int32 [sequences + 1]."""
-        shape = (k.shape[0], self.kv_heads, self.head_dim)
-        seqs, width = _table(table)
-        code = _code(k)
-        a = _pack_read(table.data_ptr(), 0 if first is None else _vector("first", first, _INT32S, seqs),
-                       _vector("offsets", offsets, _INT32S, seqs + 1), k.data_ptr(), v.data_ptr(), shape[0],
-                       _heads("k", k, _FLOATS, shape), _heads("v", v, (code,), shape), seqs, width, code, 0)
-        lib = load_library()
-        if code := lib.spkv2_mi355x_kv_read_i8(self._ref, a, stream):
-            _check(lib, code, "kv_read_i8")
+        if code := (_calls or _bind()).kv_read(self._at, self.kv_heads, self.head_dim, table, first, offsets, k, v, stream):
+            _check(load_library(), code, "kv_read_i8")
 
 
 def attention_workspace(sequences: int, queries: int, heads: int, cache: KvCache, *, max_queries: int, max_length: int) -> int:
