@@ -13,13 +13,13 @@
 // cores, whose operands hold 8-bit floats exactly, at half the rate.
 //
 // Many rows are bound by the matrix cores, at the clock that random operands leave
-// them: 8192 x 8192 x 8192 into bf16 441 to 468 us, 2.35 to 2.5 PFLOP/s, the cores at
+// them: 8192 x 8192 x 8192 into bf16 440 to 455 us, 2.4 to 2.5 PFLOP/s, the cores at
 // work in 60% of the cycles (a library's product, one scale for a whole matrix, 423).
 // Few rows are bound by the bytes of the weights: 1 x 4096 x 4096 4.6 to 5.8 us, a
 // launch's own time and 2.9 to 3.6 TB/s; 64 tokens of 8 experts of 64, 2048 x 2048,
 // 46 to 55 us, 4.8 to 5.8 TB/s.  Rows by expert leave part of each expert's last tile
 // empty and look their rows up ahead of the loop: 4001 tokens of 4 of 32, 4096 x
-// 2048, 176 to 187 us, where the products alone would take 103.
+// 2048, 165 to 178 us, where the products alone would take 103.
 #include <cmath>
 #include <cstdio>
 
@@ -162,10 +162,10 @@ __device__ __forceinline__ Rows rows_of(const MatmulArgs &a, Experts x, int at, 
         x = experts_from(a, e0, height);
     }
 }
-// the row of a that output row r takes; negative: none, or one that a may not have
-__device__ __forceinline__ int row_of(const MatmulArgs &a, int r) {
-    if (!a.order) return r;
-    const int choice = a.order[r];
+// the choice that output row r is, and the row of a that it takes (negative: none, or one that a may not have)
+__device__ __forceinline__ int choice_of(const MatmulArgs &a, int r) { return a.order ? a.order[r] : r; }
+__device__ __forceinline__ int row_of(const MatmulArgs &a, int choice) {
+    if (!a.order) return choice;
     return choice < 0 ? -1 : static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(choice)) * a.token_mul) >> a.token_shift);
 }
 
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(512) matmul_rows(MatmulArgs a) {
     const auto input = [&](int r) -> int64_t {
         r = min(r, end_m - 1);
         if constexpr (!EXPERTS) return r;
-        const int at = row_of(a, r);
+        const int at = row_of(a, choice_of(a, r));
         return at < a.a_rows ? at : -1;
     };
     const int blocks = (a.k + 127) / 128, per = (blocks + WAVES - 1) / WAVES;
@@ -320,6 +320,10 @@ __device__ __forceinline__ void wait_all() {
     asm volatile("" ::: "memory");
 }
 
+constexpr int kCus = 256;
+// whether tiles leave room for one workgroup on a CU, which then takes one after the other
+constexpr bool goes_on(bool direct, int channels) { return direct && channels == 256; }
+
 // WAVES_M x WAVES_N waves, each TJ x TI tiles of 16 x 16 (rows by channels), take
 // a block of k a step; where such tiles are few, WAVES_K groups of them take a
 // block each and join their sums in the end.
@@ -328,6 +332,11 @@ __device__ __forceinline__ void wait_all() {
 // buffers of LDS while the other is multiplied (a third and a fourth gained nothing:
 // what a CU can have under way is the limit).  Otherwise they wait in registers
 // for a step between memory and LDS, at 1.5 to 1.9 times the time of a step.
+//
+// Tiles so large that a CU holds one workgroup go on (kGoOn): the next tile's rows
+// are looked up ahead of a tile's loop, and its first block is under way while the
+// tile leaves, in two halves, through the buffer that the block does not take (4001
+// tokens of 4 of 32 experts, 4096 x 2048, 177 -> 167 us, 16384 x 8192 x 128 68 -> 56).
 template <typename T, bool EXPERTS, bool DIRECT, int WAVES_M, int WAVES_N, int WAVES_K, int TJ, int TI>
 __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ? 2 : sizeof(T) == 4 || WAVES_N == 4 ? 3 : 4)
     matmul_tiles(MatmulArgs a) {
@@ -339,83 +348,104 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
     constexpr int kScales = BM < 64 ? 64 : BM;
     __shared__ __align__(16) uint8_t lds[2 * kBuffer];
     __shared__ __align__(16) float row_scales[2][kScales][4];  // of four blocks of k
-    __shared__ bool row_there[EXPERTS ? kScales : 1];
+    constexpr bool kGoOn = goes_on(DIRECT, BN);
+    __shared__ bool row_there[kGoOn ? 2 : 1][EXPERTS ? kScales : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), tid = wave * 64 + lane;
     const int col = lane & 15, g = lane >> 4;
     // Workgroups go to the eight XCDs in turn; each XCD takes a run of tiles,
     // four tiles of rows by the channels one after the other, whose operands
     // its L2 then holds for several of them.
-    int m0, end_m = a.m, expert = 0, nt;
-    {
-        int m_tiles = (a.m + BM - 1) / BM;
-        Experts x;
-        if constexpr (EXPERTS) {
-            x = experts_from(a, 0, BM);
-            m_tiles = tiles_of(x);
-            for (int e0 = 64; e0 < a.experts; e0 += 64) m_tiles += tiles_of(experts_from(a, e0, BM));
-        }
-        const int tiles = m_tiles * a.n_tiles, per = tiles / 8, rest = tiles % 8;
-        const int xcd = blockIdx.x % 8, local = blockIdx.x / 8;
-        if (local >= per + (xcd < rest ? 1 : 0)) return;
+    int m_tiles = (a.m + BM - 1) / BM;
+    Experts x;
+    if constexpr (EXPERTS) {
+        x = experts_from(a, 0, BM);
+        m_tiles = tiles_of(x);
+        for (int e0 = 64; e0 < a.experts; e0 += 64) m_tiles += tiles_of(experts_from(a, e0, BM));
+    }
+    const int tiles = m_tiles * a.n_tiles, per = tiles / 8, rest = tiles % 8;
+    const int xcd = blockIdx.x % 8, count = per + (xcd < rest ? 1 : 0);
+    int local = blockIdx.x / 8;  // of the XCD's tiles
+    if (local >= count) return;
+    // A thread's pieces of a step: kA of a, then kB of b, kThreads / 8 rows apart.
+    // Row r's piece p lies at place p ^ (r / 2 % 8): any 16 rows' pieces of one
+    // column are then on different banks.
+    // Rows' scales, four blocks of a row a lane: a row at a time they are a request
+    // each, of 4 bytes as of 16.  The last four of a row may be some of those before.
+    constexpr int kRuns = kScales / 64;  // waves that load them
+    // the tile that is next: its place, and the choices that a thread's pieces of a and its scale are of
+    int next_m0, next_n0, next_end = a.m, next_expert = 0, choices[EXPERTS ? kA + 1 : 1];
+    const auto choose = [&]() {
         const int at = xcd * per + min(xcd, rest) + local;
         constexpr int kGroup = 4;
         const int grp = at / (kGroup * a.n_tiles), in = at - grp * kGroup * a.n_tiles, height = min(kGroup, m_tiles - grp * kGroup);
         const int mt = grp * kGroup + in % height;
-        nt = in / height;
-        m0 = mt * BM;
+        next_n0 = in / height * BN;
+        next_m0 = mt * BM;
         if constexpr (EXPERTS) {
             const Rows r = rows_of(a, x, mt, BM);
-            if (r.expert < 0) return;
-            expert = r.expert;
-            m0 = r.first;
-            end_m = r.end;
+            if (r.expert < 0) return false;
+            next_expert = r.expert, next_m0 = r.first, next_end = r.end;
+            int t = tid;
+            if constexpr (BN == 256) asm volatile("" : "+v"(t));
+#pragma unroll
+            for (int c = 0; c < kA; c++) choices[c] = choice_of(a, min(r.first + t / 8 + c * (kThreads / 8), r.end - 1));
+            choices[kA] = choice_of(a, min(r.first + (wave % kRuns * 64 + t % 64) % BM, r.end - 1));
         }
-    }
-    const int n0 = nt * BN;
+        return true;
+    };
+    if (!choose()) return;
     const int wm = wave / WAVES_N * (16 * TJ), wn = wave % WAVES_N * (16 * TI);
     const int blocks = (a.k + BK - 1) / BK, steps = (blocks + WAVES_K - 1) / WAVES_K;
-    const auto input = [&](int r) -> unsigned {  // ~0: a row that is not there, for which the first is read
-        r = min(r, end_m - 1);
-        if constexpr (!EXPERTS) return r;
-        const int at = row_of(a, r);
+    const auto input = [&](int choice) -> unsigned {  // ~0: a row that is not there, for which the first is read
+        const int at = row_of(a, choice);
         return at >= 0 && at < a.a_rows ? at : 0xffffffffu;
     };
 
-    // A thread's pieces of a step: kA of a, then kB of b, kThreads / 8 rows apart.
-    // Row r's piece p lies at place p ^ (r / 2 % 8): any 16 rows' pieces of one
-    // column are then on different banks.
+    int m0, n0, end_m, expert;
     const int place = tid & 7, piece = place ^ (tid / 16 & 7);
-    const uint8_t *pa = a.a, *pb = a.b + expert * a.b_expert + n0 * a.b_stride;
-    if constexpr (!EXPERTS) pa += m0 * a.a_stride;
+    const uint8_t *pa, *pb;
     unsigned offset[kPieces];
-#pragma unroll
-    for (int c = 0; c < kPieces; c++) {
-        const int r = tid / 8 + (c < kA ? c : c - kA) * (kThreads / 8);
-        if (c >= kA) offset[c] = static_cast<unsigned>(min(r, a.n - 1 - n0)) * static_cast<unsigned>(a.b_stride) + piece * 16;
-        else if (EXPERTS) offset[c] = (input(m0 + r) == 0xffffffffu ? 0 : input(m0 + r)) * static_cast<unsigned>(a.a_stride) + piece * 16;
-        else offset[c] = static_cast<unsigned>(min(r, a.m - 1 - m0)) * static_cast<unsigned>(a.a_stride) + piece * 16;
-    }
-    // Rows' scales, four blocks of a row a lane: a row at a time they are a request
-    // each, of 4 bytes as of 16.  The last four of a row may be some of those before.
-    constexpr int kRuns = kScales / 64;  // waves that load them
     const int scale_row = wave % kRuns * 64 + lane;
-    const float *sa = a.a_scale;
+    const float *sa;
     unsigned scale_at = 0;
-    if constexpr (EXPERTS) {
-        const unsigned row = input(m0 + scale_row % BM);
-        scale_at = (row == 0xffffffffu ? 0 : row) * static_cast<unsigned>(a.sa_stride) * 4;
-    } else {
-        sa += m0 * a.sa_stride;
-        scale_at = static_cast<unsigned>(min(scale_row % BM, a.m - 1 - m0)) * static_cast<unsigned>(a.sa_stride) * 4;
-    }
     const bool scaler = part == 0 && wave < kRuns;
-    if (EXPERTS && scaler) row_there[EXPERTS ? scale_row : 0] = input(m0 + scale_row % BM) != 0xffffffffu;
     const auto quad_from = [&](int q) { return max(min(4 * q, blocks - 4), 0); };
-    if (blocks < 4 && scaler) {
-        for (int t = 0; t < blocks; t++)
-            row_scales[0][scale_row][t] = *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(sa + t) + scale_at);
-    }
+    // The weights' scales of 64 blocks, one a lane: a scalar load in every step would have each of its reads of LDS
+    // wait for it, too.
+    const float *sb;
+    float sb_ahead = 0.0f;
+    // how many steps and runs of four scales the tiles before took, and tiles there were, as far as it says which buffer is next
+    int flip = 0, quads = 0, turn = 0;
+    const auto start = [&]() {
+        int tid = wave * 64 + lane;
+        if constexpr (BN == 256) asm volatile("" : "+v"(tid));
+        const int scale_row = wave % kRuns * 64 + tid % 64, place = tid & 7, piece = place ^ (tid / 16 & 7);
+        m0 = next_m0, n0 = next_n0, end_m = next_end, expert = next_expert;
+        pa = a.a, pb = a.b + expert * a.b_expert + n0 * a.b_stride, sa = a.a_scale;
+        if constexpr (!EXPERTS) pa += m0 * a.a_stride;
+#pragma unroll
+        for (int c = 0; c < kPieces; c++) {
+            const int r = tid / 8 + (c < kA ? c : c - kA) * (kThreads / 8);
+            if (c >= kA) offset[c] = static_cast<unsigned>(min(r, a.n - 1 - n0)) * static_cast<unsigned>(a.b_stride) + piece * 16;
+            else if (EXPERTS) offset[c] = (input(choices[EXPERTS ? c % kA : 0]) == 0xffffffffu ? 0 : input(choices[EXPERTS ? c % kA : 0])) * static_cast<unsigned>(a.a_stride) + piece * 16;
+            else offset[c] = static_cast<unsigned>(min(r, a.m - 1 - m0)) * static_cast<unsigned>(a.a_stride) + piece * 16;
+        }
+        if constexpr (EXPERTS) {
+            const unsigned row = input(choices[EXPERTS ? kA : 0]);
+            scale_at = (row == 0xffffffffu ? 0 : row) * static_cast<unsigned>(a.sa_stride) * 4;
+            if (scaler) row_there[turn][EXPERTS ? scale_row : 0] = row != 0xffffffffu;
+        } else {
+            sa += m0 * a.sa_stride;
+            scale_at = static_cast<unsigned>(min(scale_row % BM, a.m - 1 - m0)) * static_cast<unsigned>(a.sa_stride) * 4;
+        }
+        sb = a.b_scale + expert * a.sb_expert + min(n0 + wn, a.n - 1) / 128 * a.sb_stride;
+        if (blocks < 4 && scaler) {
+            for (int t = 0; t < blocks; t++)
+                row_scales[quads][scale_row][t] = *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(sa + t) + scale_at);
+        }
+    };
+    start();
     // DIRECT: a step's loads into its buffer
     const auto load = [&](int s) {
         const int t = s * WAVES_K + part;
@@ -423,9 +453,9 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         asm("" : "+v"(scale_at));
 #pragma unroll
         for (int c = 0; c < kPieces; c++) asm("" : "+v"(offset[c]));
-        if (t % 4 == 0 && blocks >= 4 && scaler) load_lds16(sa + quad_from(t / 4), scale_at, lds_address(&row_scales[t / 4 & 1][wave * 64]));
+        if (t % 4 == 0 && blocks >= 4 && scaler) load_lds16(sa + quad_from(t / 4), scale_at, lds_address(&row_scales[(t / 4 + quads) & 1][wave * 64]));
         const uint8_t *fa = pa + t * BK, *fb = pb + t * BK;
-        uint8_t *to = lds + (s & 1) * kBuffer + part * kPart + wave * 1024;
+        uint8_t *to = lds + ((s + flip) & 1) * kBuffer + part * kPart + wave * 1024;
         if (t * BK + BK <= a.k) {
 #pragma unroll
             for (int c = 0; c < kPieces; c++) load_lds16(c < kA ? fa : fb, offset[c], lds_address(to) + c * (kThreads * 16));
@@ -468,25 +498,16 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         // over those that were last read four blocks ago
         if (t % 4 == 0 && t < blocks && blocks >= 4 && scaler) *reinterpret_cast<floatx4 *>(row_scales[t / 4 & 1][scale_row]) = quad;
     };
-    // The weights' scales of 64 blocks, one a lane: a scalar load in every step would have each of its reads of LDS
-    // wait for it, too.
-    const float *sb = a.b_scale + expert * a.sb_expert + min(n0 + wn, a.n - 1) / 128 * a.sb_stride;
-    float sb_ahead = 0.0f;
-
     floatx4 acc[TI][TJ];
-#pragma unroll
-    for (int i = 0; i < TI; i++)
-#pragma unroll
-        for (int j = 0; j < TJ; j++) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const int at0 = col * BK + (g ^ (col / 2)) * 16, at1 = col * BK + ((4 + g) ^ (col / 2)) * 16;
     const auto read = [&](const uint8_t *rows, Operand<kWide> &x) {
         x.set(*reinterpret_cast<const intx4 *>(rows + at0), *reinterpret_cast<const intx4 *>(rows + at1));
     };
     // a wave whose rows or channels are all past the end leaves the matrix cores to the others
-    const bool active = m0 + wm < end_m && n0 + wn < a.n;
+    bool active;
     const auto step = [&](int s) {
         const int t = s * WAVES_K + part;
-        const uint8_t *now = lds + (s & 1) * kBuffer + part * kPart;
+        const uint8_t *now = lds + ((s + flip) & 1) * kBuffer + part * kPart;
         if (t % 64 < WAVES_K) {
             sb_ahead = sb[min(t / 64 * 64 + lane, blocks - 1)];
             asm volatile("" : "+v"(sb_ahead));  // waited for here, not in every step
@@ -499,7 +520,7 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
 #pragma unroll
             for (int j = 0; j < TJ; j++) read(now + (wm + 16 * j) * BK, fa[j]);
 #pragma unroll
-            for (int j = 0; j < TJ; j++) scale[j] = row_scales[t / 4 & 1][wm + 16 * j + col][t - quad_from(t / 4)];
+            for (int j = 0; j < TJ; j++) scale[j] = row_scales[(t / 4 + quads) & 1][wm + 16 * j + col][t - quad_from(t / 4)];
             if constexpr (!kWide) __builtin_amdgcn_sched_barrier(0);
             // a product, and the sums of the one two before it, which has ended
             floatx4 sum[3];
@@ -526,109 +547,152 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
     };
     if constexpr (DIRECT) {
         if (steps > 0) load(0);
-        for (int s = 0; s < steps; s++) {
-            // the barrier also ends the reads of the step before, whose buffer is loaded next
-            wait_all();
-            if (s + 1 < steps) load(s + 1);
-            step(s);
-        }
-    } else if (steps > 0) {
-        fetch(0);
-        store(0);
-        if (steps > 1) fetch(1);
-        for (int s = 0; s < steps; s++) {
-            __syncthreads();
-            if (s + 1 < steps) store(s + 1);
-            if (s + 2 < steps) fetch(s + 2);
-            step(s);
-        }
     }
-    __syncthreads();
-    if constexpr (WAVES_K > 1) {
-        // the groups' sums, joined in their order
-        floatx4 *sums = reinterpret_cast<floatx4 *>(lds);
-        static_assert((WAVES_K - 1) * BM * BN * 4 <= 2 * kBuffer, "LDS holds the groups' sums");
-        if (part > 0) {
+    while (true) {
+        bool more = false;
+        if constexpr (kGoOn) {
+            local += kCus / 8;
+            more = local < count && choose();
+        }
+        active = m0 + wm < end_m && n0 + wn < a.n;
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int j = 0; j < TJ; j++) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (DIRECT) {
+            for (int s = 0; s < steps; s++) {
+                // the barrier also ends the reads of the step before, whose buffer is loaded next
+                wait_all();
+                if (s + 1 < steps) load(s + 1);
+                step(s);
+            }
+        } else if (steps > 0) {
+            fetch(0);
+            store(0);
+            if (steps > 1) fetch(1);
+            for (int s = 0; s < steps; s++) {
+                __syncthreads();
+                if (s + 1 < steps) store(s + 1);
+                if (s + 2 < steps) fetch(s + 2);
+                step(s);
+            }
+        }
+        __syncthreads();
+        if constexpr (WAVES_K > 1) {
+            // the groups' sums, joined in their order
+            floatx4 *sums = reinterpret_cast<floatx4 *>(lds);
+            static_assert((WAVES_K - 1) * BM * BN * 4 <= 2 * kBuffer, "LDS holds the groups' sums");
+            if (part > 0) {
+#pragma unroll
+                for (int i = 0; i < TI; i++)
+#pragma unroll
+                    for (int j = 0; j < TJ; j++) sums[((part - 1) * TI * TJ + i * TJ + j) * kThreads + tid] = acc[i][j];
+            }
+            __syncthreads();
+            if (part > 0) return;
 #pragma unroll
             for (int i = 0; i < TI; i++)
 #pragma unroll
-                for (int j = 0; j < TJ; j++) sums[((part - 1) * TI * TJ + i * TJ + j) * kThreads + tid] = acc[i][j];
+                for (int j = 0; j < TJ; j++)
+#pragma unroll
+                    for (int w = 1; w < WAVES_K; w++) acc[i][j] += sums[((w - 1) * TI * TJ + i * TJ + j) * kThreads + tid];
+            // this group's waves write over others' sums
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         }
-        __syncthreads();
-        if (part > 0) return;
-#pragma unroll
-        for (int i = 0; i < TI; i++)
-#pragma unroll
-            for (int j = 0; j < TJ; j++)
-#pragma unroll
-                for (int w = 1; w < WAVES_K; w++) acc[i][j] += sums[((w - 1) * TI * TJ + i * TJ + j) * kThreads + tid];
-        // this group's waves write over others' sums
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    }
 
-    // Through this wave's own part of LDS (every wave is past its last read of the
-    // buffers), so that a row's channels leave as 16-byte pieces one after the other.
-    // A row's piece p lies at place p ^ (row / rows of 256 bytes): the accumulators'
-    // 8-byte writes and the rows' reads are then on different banks.  Sixteen rows at
-    // a time, each asked whether it is inside, this took a tile of 256 x 256 8 us.
-    constexpr int kPiece = 16 / static_cast<int>(sizeof(T)), kLanes = 16 * TI / kPiece;  // elements of a piece, pieces of a row
-    constexpr int kRows = 64 / kLanes, kReads = 16 * TJ / kRows, kPitch = kLanes * 16;
-    static_assert(16 * TJ * kPitch <= 2 * kBuffer / kWaves, "a wave's part of LDS holds its tile");
-    uint8_t *mine = lds + wave * (2 * kBuffer / kWaves);
-    const auto spot = [&](int row, int p) { return mine + row * kPitch + ((p ^ (row / (16 / kLanes > 0 ? 16 / kLanes : 1))) & (kLanes - 1)) * 16; };
-    const int left = a.n - n0 - wn, rows = end_m - m0 - wm;
-    floatx4 bias[TI];
-#pragma unroll
-    for (int i = 0; i < TI; i++) bias[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (a.bias) {
-        const float *from = a.bias + static_cast<int64_t>(expert) * a.n;
-#pragma unroll
-        for (int i = 0; i < TI; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) bias[i][e] = from[min(n0 + wn + 16 * i + 4 * g + e, a.n - 1)];
-    }
-#pragma unroll
-    for (int j = 0; j < TJ; j++) {
-        const bool there = !EXPERTS || row_there[EXPERTS ? wm + 16 * j + col : 0];
-#pragma unroll
-        for (int i = 0; i < TI; i++) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (there ? acc[i][j][e] : 0.0f) + bias[i][e];
-            const int at = 16 * i + 4 * g;
-            put_floats<4>(reinterpret_cast<T *>(spot(16 * j + col, at / kPiece)) + at % kPiece, v);
-        }
-    }
-    wait_lds();
-    const int c = lane % kLanes * kPiece, r0 = lane / kLanes;
-    T *out = static_cast<T *>(a.out) + (m0 + wm + r0) * a.out_stride + n0 + wn + c;
-    const auto piece_of = [&](int r) { return *reinterpret_cast<const Vec<T, kPiece> *>(spot(r + r0, lane % kLanes)); };
-    if (rows >= 16 * TJ && left >= 16 * TI) {
-        constexpr int kAhead = kReads < 8 ? kReads : 8;
-#pragma unroll
-        for (int q = 0; q < kReads; q += kAhead) {
-            Vec<T, kPiece> v[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) v[u] = piece_of((q + u) * kRows);
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) __builtin_memcpy(out + static_cast<int64_t>((q + u) * kRows) * a.out_stride, v[u].v, 16);
-        }
-    } else {
-#pragma unroll 1
-        for (int r = 0; r < min(rows, 16 * TJ); r += kRows) {
-            const Vec<T, kPiece> v = piece_of(r);
-            if (r + r0 >= rows) continue;
-            T *y = out + static_cast<int64_t>(r) * a.out_stride;
-            if (c + kPiece <= left) {
-                __builtin_memcpy(y, v.v, 16);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kPiece; e++)
-                    if (c + e < left) y[e] = v.v[e];
+        // This tile's place, and the buffer that its sums may take
+        const int n = n0 + wn, m = m0 + wm, left = a.n - n, rows = end_m - m, was = turn;
+        const float *bias_from = a.bias + static_cast<int64_t>(expert) * a.n;
+        uint8_t *room = lds;
+        if constexpr (kGoOn) {
+            room += (steps - 1 + flip & 1) * kBuffer;
+            if (more) {
+                flip = (flip + steps) & 1, quads = (quads + (steps - 1) / 4 + 1) & 1, turn ^= 1;
+                start();
+                load(0);
             }
         }
+
+        // Places that are the same for every tile are taken anew: kept, they would take registers that the loop needs.
+        int lane = threadIdx.x & 63;
+        if constexpr (BN == 256) asm volatile("" : "+v"(lane));
+        const int col = lane & 15, g = lane >> 4;
+
+        // Through this wave's own part of LDS (every wave is past its last read of the
+        // buffers), so that a row's channels leave as 16-byte pieces one after the other.
+        // A row's piece p lies at place p ^ (row / rows of 256 bytes): the accumulators'
+        // 8-byte writes and the rows' reads are then on different banks.  Sixteen rows at
+        // a time, each asked whether it is inside, this took a tile of 256 x 256 8 us.
+        constexpr int kHalves = kGoOn ? 2 : 1, kRoom = kGoOn ? kBuffer : 2 * kBuffer, kHigh = 16 * TJ / kHalves;  // rows at a time
+        constexpr int kPiece = 16 / static_cast<int>(sizeof(T)), kLanes = 16 * TI / kPiece;  // elements of a piece, pieces of a row
+        constexpr int kRows = 64 / kLanes, kReads = kHigh / kRows, kPitch = kLanes * 16;
+        static_assert(kHigh * kPitch <= kRoom / kWaves && TJ % kHalves == 0, "a wave's part of LDS holds its tile");
+        uint8_t *mine = room + wave * (kRoom / kWaves);
+        const auto spot = [&](int row, int p) { return mine + row * kPitch + ((p ^ (row / (16 / kLanes > 0 ? 16 / kLanes : 1))) & (kLanes - 1)) * 16; };
+        if constexpr (EXPERTS) {
+#pragma unroll
+            for (int j = 0; j < TJ; j++)
+                if (!row_there[was][wm + 16 * j + col]) {
+#pragma unroll
+                    for (int i = 0; i < TI; i++) acc[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < TI; i++) {
+                floatx4 bias;
+#pragma unroll
+                for (int e = 0; e < 4; e++) bias[e] = bias_from[min(n + 16 * i + 4 * g + e, a.n - 1)];
+#pragma unroll
+                for (int j = 0; j < TJ; j++) acc[i][j] += bias;
+            }
+        }
+        const int c = lane % kLanes * kPiece, r0 = lane / kLanes;
+        const auto piece_of = [&](int r) { return *reinterpret_cast<const Vec<T, kPiece> *>(spot(r + r0, lane % kLanes)); };
+#pragma unroll
+        for (int h = 0; h < kHalves; h++) {
+#pragma unroll
+            for (int j = h * TJ / kHalves; j < (h + 1) * TJ / kHalves; j++) {
+#pragma unroll
+                for (int i = 0; i < TI; i++) {
+                    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                    const int at = 16 * i + 4 * g;
+                    put_floats<4>(reinterpret_cast<T *>(spot(16 * j - h * kHigh + col, at / kPiece)) + at % kPiece, v);
+                }
+            }
+            wait_lds();
+            T *out = static_cast<T *>(a.out) + (m + h * kHigh + r0) * a.out_stride + n + c;
+            if (rows >= (h + 1) * kHigh && left >= 16 * TI) {
+                constexpr int kAhead = kReads < 8 ? kReads : 8;
+#pragma unroll
+                for (int q = 0; q < kReads; q += kAhead) {
+                    Vec<T, kPiece> v[kAhead];
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) v[u] = piece_of((q + u) * kRows);
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) __builtin_memcpy(out + static_cast<int64_t>((q + u) * kRows) * a.out_stride, v[u].v, 16);
+                }
+            } else {
+                const int high = min(rows - h * kHigh, kHigh);
+#pragma unroll 1
+                for (int r = 0; r < high; r += kRows) {
+                    const Vec<T, kPiece> v = piece_of(r);
+                    if (r + r0 >= high) continue;
+                    T *y = out + static_cast<int64_t>(r) * a.out_stride;
+                    if (c + kPiece <= left) {
+                        __builtin_memcpy(y, v.v, 16);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kPiece; e++)
+                            if (c + e < left) y[e] = v.v[e];
+                    }
+                }
+            }
+            wait_lds();
+        }
+        if (!more) return;
     }
 }
 
@@ -754,7 +818,8 @@ int run(const char *what, int dtype, MatmulArgs a, void *stream) {
         a.n_tiles = static_cast<int>(across);
         auto rows = [&](auto kernel) { return launch(what, kernel, dim3(across, down), dim3(64 * 8), stream, a); };
         auto tiles = [&](auto direct, auto staged, int waves) {
-            return launch(what, whole(a) ? direct : staged, dim3(across * down), dim3(64 * waves), stream, a);
+            const unsigned all = across * down;
+            return launch(what, whole(a) ? direct : staged, dim3(goes_on(whole(a), f.channels) ? std::min<unsigned>(all, kCus) : all), dim3(64 * waves), stream, a);
         };
         switch (i) {
             case 0: return rows(matmul_rows<T, EXPERTS, 1, 1>);
