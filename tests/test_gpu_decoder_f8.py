@@ -872,3 +872,18 @@ def test_calls_of_two_threads_at_once(gpu):
 def test_as_many_experts_as_there_may_be(gpu, tokens):
     rng = np.random.default_rng(tokens)
     _experts_case(_ids(rng, tokens, 2, 4096, "any"), 4096, 9, 48, "float32", spare=3)
+
+
+# tiles 256 channels wide of which a workgroup takes several: one to nine blocks of k, whole ones and not
+@pytest.mark.parametrize("m,n,k", [(4700, 4360, 16), (4700, 4360, 128), (4700, 4360, 400), (4700, 4360, 512), (4700, 4360, 1040), (8300, 4360, 272)])
+def test_workgroups_of_several_tiles(gpu, m, n, k):
+    assert kernel_of("bfloat16", m, n, k) == "matmul_tiles<256x256,groups=1,direct>"
+    _matmul_case(m, n, k, "bfloat16", bias=k > 300)
+
+
+@pytest.mark.parametrize("kind,kw", [("any", {}), ("holes", dict(bias=True)), ("any", dict(by_order=False, spare=5))])
+@pytest.mark.parametrize("k", [112, 384, 656])
+def test_workgroups_of_several_experts_tiles(gpu, k, kind, kw):
+    for tokens, experts, n in ((3300, 6, 4360), (9000, 70, 1540))[:2 if k == 112 else 1]:
+        assert "x256,groups=1,direct" in kernel_of("bfloat16", 2 * tokens, n, k, experts, tokens)
+        _experts_case(_ids(np.random.default_rng(k), tokens, 2, experts, kind), experts, n, k, "bfloat16", **kw)
