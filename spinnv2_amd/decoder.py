@@ -50,6 +50,8 @@ F8_BLOCK = 128
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
 
+# The header's structs: those of the calls below are laid out from here, or by the native module from the header itself;
+# all of them for programs that call the library's entry points through ctypes.
 class _RmsNorm(ctypes.Structure):
     _fields_ = [("x", _P), ("residual", _P), ("weight", _P), ("residual_out", _P), ("q", _P), ("scale", _P),
                 ("rows", _I64), ("cols", _I64), ("x_stride", _I64), ("residual_stride", _I64),
@@ -179,8 +181,8 @@ class DeviceArray:
     """A tensor in a `DeviceBuffer`, for callers without torch.
 
     ``dtype`` is one of float32, float16, bfloat16, float8_e4m3fn, int8, int32,
-    int64; bfloat16 and float8_e4m3fn values come and go as float32 arrays.  ``at`` elements from the
-    buffer's start; ``strides`` in elements, none below zero (default:
+    int64; bfloat16 and float8_e4m3fn values come and go as float32 arrays.
+    ``at`` elements from the buffer's start; ``strides`` in elements, none below zero (default:
     contiguous).
     """
 
