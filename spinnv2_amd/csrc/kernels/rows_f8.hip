@@ -348,7 +348,8 @@ extern "C" int spkv2_mi355x_rows_f8(const Spkv2RowsF8 *g, void *stream) {
             if (g->scale_stride < blocks) return bad("rows_f8: the scales' stride is below their count");
         }
         if (g->cols > (1 << 24) || g->rows > INT32_MAX) return unsupported("rows_f8: more than 2^24 columns or 2^31 rows");
-        if (!norm && g->rows * blocks >= (int64_t(1) << 28)) return unsupported("rows_f8: 2^28 blocks or more");
+        // 16 blocks a workgroup of 256; a launch has fewer than 2^32 threads along an axis
+        if (!norm && (g->rows * blocks + 15) / 16 >= 1 << 24) return unsupported("rows_f8: more than 2^28 - 16 blocks");
         RowsArgs a{g->x, g->residual, g->weight, g->residual_out, g->q, g->scale, g->rows, g->x_stride, g->residual_stride,
                    g->residual_out_stride, g->q_stride, g->scale_stride, static_cast<int>(g->cols), static_cast<int>(blocks), g->eps, 0, 0};
         div_magic(static_cast<unsigned>(blocks), &a.block_mul, &a.block_shift);
