@@ -123,9 +123,11 @@ __global__ void __launch_bounds__(256) quantise_blocks(RowsArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float t = v[j], up = g[j];
-            v[j] = silu(t) * up;
-            // where fp32's exponential or product leaves its range, 64 bits say what the value is
-            if (!(fabsf(v[j]) < 0x1p120f) || t < -80.0f) v[j] = __builtin_inff();
+            const float s = silu(t);
+            v[j] = s * up;
+            // where fp32's exponential, quotient (whose bits a large factor would show) or product leaves its range, 64 bits
+            // say what the value is
+            if (!(fabsf(v[j]) < 0x1p120f) || t < -80.0f || (fabsf(s) < 0x1p-125f && t != 0.0f && up != 0.0f)) v[j] = __builtin_inff();
         }
     }
     const auto wide = [&](int j) -> double {
