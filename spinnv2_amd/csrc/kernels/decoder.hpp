@@ -177,31 +177,29 @@ __device__ __forceinline__ unsigned four_f8(float a, float b, float c, float d) 
 }
 
 // Codes of 448 v / top of eight values, |v| <= top, both within 2^-(SLACK + 2) of
-// their values in 64 bits.  The quotient in fp32, of four roundings more, is then
-// within 2^-SLACK: where it and what lies that far on both sides have one code,
-// that is it.  Returns whether some have not, or all may not since top is so small
-// or large that quotients lose bits; beside_f8() says which.
+// their values in 64 bits.  The quotient in fp32, of a reciprocal within one step and
+// three roundings more, is then within 2^-SLACK: where what lies that far on both
+// sides has one code, that is it.  Returns whether some have not, or all may not
+// since top is so small or large that quotients lose bits; beside() says which.
 template <int SLACK>
 struct F8 {
-    static constexpr float kLess = 1.0f - 1.0f / (1 << SLACK), kMore = 1.0f + 1.0f / (1 << SLACK);
+    static constexpr float kLess = 448.0f * (1.0f - 1.0f / (1 << SLACK)), kMore = 448.0f * (1.0f + 1.0f / (1 << SLACK));
     static __device__ __forceinline__ bool plain(float top) { return top > 0x1p-90f && top < 0x1p120f; }
     static __device__ __forceinline__ bool quantise(const float (&v)[8], float top, unsigned (&q)[2]) {
-        const float inv = 448.0f / top;
+        const float inv = __builtin_amdgcn_rcpf(top), less = inv * kLess, more = inv * kMore;
         unsigned differ = 0;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float t[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) t[j] = v[4 * h + j] * inv;
-            q[h] = four_f8(t[0] * kLess, t[1] * kLess, t[2] * kLess, t[3] * kLess);
-            differ |= q[h] ^ four_f8(t[0] * kMore, t[1] * kMore, t[2] * kMore, t[3] * kMore);
+            const float *x = v + 4 * h;
+            q[h] = four_f8(x[0] * less, x[1] * less, x[2] * less, x[3] * less);
+            differ |= q[h] ^ four_f8(x[0] * more, x[1] * more, x[2] * more, x[3] * more);
         }
         return differ || !plain(top);
     }
     // whether a value's quotient lies beside the border of two codes
     static __device__ __forceinline__ bool beside(float v, float top) {
-        const float t = v * (448.0f / top);
-        const unsigned codes = four_f8(t * kLess, t * kMore, 0.0f, 0.0f);
+        const float inv = __builtin_amdgcn_rcpf(top);
+        const unsigned codes = four_f8(v * (inv * kLess), v * (inv * kMore), 0.0f, 0.0f);
         return !plain(top) || (codes & 0xffu) != (codes >> 8 & 0xffu);
     }
 };
@@ -217,6 +215,22 @@ __device__ __forceinline__ unsigned max_over(unsigned v) {
     if constexpr (LANES >= 16) v = max(v, static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 0xF, 0xF, true)));  // 16 mirrored
     if constexpr (LANES >= 32) v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), 16)));
     return v;
+}
+
+// A double from the lane that the DPP control names, by two 32-bit moves
+template <int CONTROL>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+    const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u), CONTROL, 0xF, 0xF, true));
+    const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u >> 32), CONTROL, 0xF, 0xF, true));
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+// and of doubles that are no NaN, over 16 lanes
+__device__ __forceinline__ double max_over16(double v) {
+    v = fmax(v, moved<0xB1>(v));
+    v = fmax(v, moved<0x4E>(v));
+    v = fmax(v, moved<0x141>(v));
+    return fmax(v, moved<0x140>(v));
 }
 
 // ---- host ------------------------------------------------------------------

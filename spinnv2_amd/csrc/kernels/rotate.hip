@@ -65,14 +65,6 @@ __device__ __forceinline__ void sine_cosine(double angle, double *s, double *c) 
     if (turn == 1.0 || turn == 2.0) *c = -*c;
 }
 
-// A double from the lane that the DPP control names, by two 32-bit moves
-template <int CONTROL>
-__device__ __forceinline__ double moved(double v) {
-    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
-    const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u), CONTROL, 0xF, 0xF, true));
-    const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u >> 32), CONTROL, 0xF, 0xF, true));
-    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
-}
 // The sum over groups of LANES neighbouring lanes, in each of them
 template <int LANES>
 __device__ __forceinline__ double sum_over(double v) {

@@ -8,10 +8,11 @@
 // moves.  The norm is one factor of the whole row and cancels out of q: codes
 // are those of h w.  fp32 quotients beside a border of two codes are taken again
 // in 64 bits, one in thirty thousand (of the gate, whose exponential is within
-// 2^-21 in fp32, one in eight thousand).  One pass, bound by HBM: 8190 x 8192 of
-// gates in bf16, 337 MB, in 74 to 84 us (4.0 to 4.6 TB/s; 107 with the math
-// library's exponential, an exact division and a flag for each code), back to
-// values, 203 MB, in 33 (the codes still cached).
+// 2^-21 in fp32, one in eight thousand), and so is the largest element of each
+// block, for its scale.  One pass, bound by HBM: 8190 x 8192 of gates in bf16, 337
+// MB, in 80 to 92 us (3.7 to 4.2 TB/s; its instructions take as long: 74 to 88 with
+// fp32 scales, off by a bit), back to values, 203 MB, in 33 (the codes
+// still cached).
 #include "decoder.hpp"
 
 namespace spk::dec {
@@ -38,9 +39,17 @@ __device__ __forceinline__ void run8(const T *row, int i, int cols, float (&f)[8
     if constexpr (TAIL == kShort) {
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] = i + j < cols ? static_cast<float>(row[i + j]) : 0.0f;
-    } else {
+    } else if constexpr (TAIL == kPart) {
         widen(load_vec<T, 8>(row + min(i, cols - 8)), f);
-        settle<8, TAIL == kPart>(i, cols, f);
+        settle<8, true>(i, cols, f);
+    } else {
+        unsigned words[2 * sizeof(T)];
+        Vec<T, 8> x = load_vec<T, 8>(row + min(i, cols - 8));
+        __builtin_memcpy(words, x.v, sizeof(words));
+#pragma unroll
+        for (unsigned &w : words) w = i < cols ? w : 0u;
+        __builtin_memcpy(x.v, words, sizeof(words));
+        widen(x, f);
     }
 }
 
@@ -59,42 +68,98 @@ __device__ __forceinline__ float silu(float g) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e * rest, 0.693147182f, e));
 }
 
-// The codes and the scale (times `norm`) of a block's 16 lanes with values v,
-// which wide(j) gives in 64 bits (alive(): some of them may not be 0 though all v
-// are).  All lanes of a wave come here together; `left` of the lane's elements are
-// there, `first` lanes write their block's scale.
-template <int SLACK, bool EXACT, typename Wide, typename Alive>
-__device__ __forceinline__ void put_block(const float (&v)[8], Wide &&wide, Alive &&alive, double norm, uint8_t *q, int left, float *scale, bool first) {
+// What fp32 holds of a value: itself, its nearest, or what is within 2^-21 of it
+enum Narrow { kSame, kNearest, kClose };
+
+// f(index, a's, b's) of those of eight elements that `mask` has, one after the other
+template <typename F>
+__device__ __forceinline__ void each_of(unsigned mask, const float (&a)[8], const float (&b)[8], F &&f) {
+    while (__any(mask != 0)) {
+        if (mask) {
+            const int at = __builtin_ctz(mask);
+            mask &= mask - 1;
+            float x = a[0], y = b[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) x = at == j ? a[j] : x, y = at == j ? b[j] : y;
+            f(at, x, y);
+        }
+    }
+}
+
+// The codes and the scale (times `norm`) of a block's 16 lanes with values v, which
+// wide(a[j], b[j]) gives in 64 bits (and which may not be 0 where v is, unless a or b
+// is).  The scale is the largest value's in 64 bits: the element that fp32 says is the
+// largest, and those so near it that fp32 may be wrong, are taken again, the first
+// such of each lane by all lanes at once.  All lanes of a wave come here together;
+// `left` of the lane's elements are there, `first` lanes write their block's scale.
+template <Narrow NARROW, typename Wide>
+__device__ __forceinline__ void put_block(const float (&v)[8], const float (&a)[8], const float (&b)[8], Wide &&wide, double norm, uint8_t *q, int left, float *scale,
+                                          bool first) {
+    using F = F8<NARROW == kClose ? 18 : 20>;
     unsigned top = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) top = max(top, abs_bits(v[j]));
     top = max_over<16>(top);
     unsigned code[2] = {0, 0};
-    bool near = false;
     const float amax = __uint_as_float(top);
-    if (top) near = F8<SLACK>::quantise(v, amax, code);
-    else near = alive();
-    double most = amax;
-    if (__any(near)) {
-        double f[8], m = 0.0;
+    const bool plain = F::plain(amax);
+    bool near = false;
+    if (top) {
+        near = F::quantise(v, amax, code);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) near |= a[j] != 0.0f && b[j] != 0.0f;
+    }
+    double most = NARROW == kSame ? amax : 0.0;  // of this lane
+    const auto raise = [&](int, float x, float y) {
+        const double f = fabs(wide(x, y));
+        most = f > most ? f : f == f ? most : __builtin_inf();
+    };
+    if constexpr (NARROW != kSame) {
+        // in fp32 the largest is within 2^-20, 16 steps at most, of what fp32 says is the largest
+        const float bound = __uint_as_float(NARROW == kClose ? top - 32 : top);
+        float x = 0.0f, y = 0.0f;
+        int count = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            f[j] = wide(j);
-            m = f[j] != f[j] ? __builtin_inf() : fmax(fabs(f[j]), m);
+            const bool is = fabsf(v[j]) >= bound;
+            x = is ? a[j] : x, y = is ? b[j] : y;
+            count += is;
         }
+        if (plain && count) raise(0, x, y);
+        if (__any(plain && count > 1)) {
+            unsigned mask = 0;
 #pragma unroll
-        for (int d = 1; d < 16; d *= 2) m = fmax(m, __shfl_xor(m, d));
-        most = m;
-        const bool finite = m < __builtin_inf();
+            for (int j = 0; j < 8; j++) mask |= plain && fabsf(v[j]) >= bound ? 1u << j : 0u;
+            each_of(mask, a, b, raise);
+        }
+    }
+    if (__any(!plain)) {
+        unsigned mask = 0;
+        if (!plain) {
+            most = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) mask |= v[j] != 0.0f || (a[j] != 0.0f && b[j] != 0.0f) ? 1u << j : 0u;
+        }
+        each_of(mask, a, b, raise);
+    }
+    if (__any(near)) {
+        const double all = max_over16(most);
+        unsigned mask = 0;
         if (near) {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (!top || F8<SLACK>::beside(v[j], amax)) {
-                    unsigned c = 0;
-                    if (finite && m > 0.0) c = exact_code_f8<EXACT>(fabs(f[j]), m) | (__builtin_signbit(f[j]) ? 0x80u : 0u);
-                    code[j / 4] = (code[j / 4] & ~(0xffu << (8 * (j % 4)))) | c << (8 * (j % 4));
-                }
+                if (F::beside(v[j], amax)) mask |= 1u << j;
         }
+        each_of(mask, a, b, [&](int at, float x, float y) {
+            const double f = wide(x, y);
+            unsigned c = 0;
+            if (all < __builtin_inf() && all > 0.0) c = exact_code_f8<NARROW != kClose>(fabs(f), all) | (__builtin_signbit(f) ? 0x80u : 0u);
+            const int shift = 8 * (at % 4);
+            const unsigned is = at < 4 ? code[0] : code[1], put = (is & ~(0xffu << shift)) | c << shift;
+            code[0] = at < 4 ? put : code[0];
+            code[1] = at < 4 ? code[1] : put;
+        });
     }
     if (left >= 8) {
         __builtin_memcpy(q, code, 8);
@@ -103,8 +168,10 @@ __device__ __forceinline__ void put_block(const float (&v)[8], Wide &&wide, Aliv
         for (int j = 0; j < 8; j++)
             if (j < left) q[j] = static_cast<uint8_t>(code[j / 4] >> (8 * (j % 4)));
     }
-    // 0 of a block of zeros, whose norm may be 0 / 0
-    if (first) *scale = !(most < __builtin_inf()) ? __builtin_nanf("") : most == 0.0 ? 0.0f : static_cast<float>(most * (norm * (1.0 / 448.0)));
+    // the largest of the lanes' scales, as bits: none is below 0, and NaN is above all; 0 of a block of zeros, whose norm may be 0 / 0
+    const float own = !(most < __builtin_inf()) ? __builtin_nanf("") : most == 0.0 ? 0.0f : static_cast<float>(most * (norm * (1.0 / 448.0)));
+    const unsigned bits = max_over<16>(abs_bits(own));
+    if (first) *scale = __uint_as_float(bits);
 }
 
 // Blocks of values or gates, 16 of them a workgroup, one row's after the other's
@@ -116,38 +183,36 @@ __global__ void __launch_bounds__(256) quantise_blocks(RowsArgs a) {
     const int64_t r = in ? row : a.rows - 1;
     const int block = in ? static_cast<int>(at - row * a.blocks) : 0, i = block * 128 + threadIdx.x % 16 * 8;
     const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
-    float v[8], g[8];
+    float v[8];
     run8<T, TAIL>(x, i, a.cols, v);
+    const auto put = [&](const float(&t)[8], const float(&up)[8], auto &&wide) {
+        put_block<GATE ? kClose : kSame>(v, t, up, wide, 1.0, a.q + r * a.q_stride + i, in ? a.cols - i : 0, a.scale + r * a.s_stride + block,
+                                         in && threadIdx.x % 16 == 0);
+    };
     if constexpr (GATE) {
-        run8<T, TAIL>(x + a.cols, i, a.cols, g);
+        float t[8], up[8], s[8], lowest = 0.0f;
+        unsigned most = 0, least = ~0u;
+        run8<T, TAIL>(x + a.cols, i, a.cols, up);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float t = v[j], up = g[j];
-            const float s = silu(t);
-            v[j] = s * up;
-            // where fp32's exponential, quotient (whose bits a large factor would show) or product leaves its range, 64 bits
-            // say what the value is
-            if (!(fabsf(v[j]) < 0x1p120f) || t < -80.0f || (fabsf(s) < 0x1p-125f && t != 0.0f && up != 0.0f)) v[j] = __builtin_inff();
+            t[j] = v[j];
+            s[j] = silu(t[j]);
+            v[j] = s[j] * up[j];
+            most = max(most, abs_bits(v[j]));
+            least = min(least, abs_bits(s[j]));
+            lowest = fminf(lowest, t[j]);
         }
-    }
-    const auto wide = [&](int j) -> double {
-        if constexpr (GATE) {
-            const int e = i + j;
-            if (e >= a.cols) return 0.0;
-            return silu(static_cast<double>(static_cast<float>(x[e]))) * static_cast<double>(g[j]);
-        } else {
-            return v[j];
-        }
-    };
-    const auto alive = [&]() {
-        bool some = false;
-        if constexpr (GATE) {
+        // where fp32's exponential, quotient (whose bits a large factor would show) or product leaves its range, 64 bits
+        // say what the value is
+        if (most >= __float_as_uint(0x1p120f) || least < __float_as_uint(0x1p-125f) || lowest < -80.0f) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) some |= g[j] != 0.0f;
+            for (int j = 0; j < 8; j++)
+                if (!(fabsf(v[j]) < 0x1p120f) || t[j] < -80.0f || (fabsf(s[j]) < 0x1p-125f && t[j] != 0.0f && up[j] != 0.0f)) v[j] = __builtin_inff();
         }
-        return some;
-    };
-    put_block<GATE ? 18 : 20, !GATE>(v, wide, alive, 1.0, a.q + r * a.q_stride + i, in ? a.cols - i : 0, a.scale + r * a.s_stride + block, in && threadIdx.x % 16 == 0);
+        put(t, up, [](float t, float up) { return silu(static_cast<double>(t)) * static_cast<double>(up); });
+    } else {
+        put(v, v, [](float x, float) { return static_cast<double>(x); });
+    }
 }
 
 // THREADS threads a row (a wave: several rows a workgroup), each with CHUNKS
@@ -216,14 +281,10 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) norm_blocks(Row
         if (w) run8<W, TAIL>(w, i, a.cols, g);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = f[j] * g[j];
-        const auto wide = [&](int j) { return static_cast<double>(f[j]) * static_cast<double>(g[j]); };
-        const auto alive = [&]() {
-            bool some = false;
-#pragma unroll
-            for (int j = 0; j < 8; j++) some |= f[j] != 0.0f && g[j] != 0.0f;
-            return some;
-        };
-        put_block<20, true>(v, wide, alive, norm, a.q + row * a.q_stride + i, a.cols - i, a.scale + row * a.s_stride + i / 128, tid % 16 == 0 && i < a.cols);
+        // products of two 16-bit values are exact in fp32
+        constexpr Narrow kNarrow = sizeof(T) == 2 && sizeof(W) == 2 ? kSame : kNearest;
+        put_block<kNarrow>(v, f, g, [](float x, float y) { return static_cast<double>(x) * static_cast<double>(y); }, norm, a.q + row * a.q_stride + i, a.cols - i,
+                           a.scale + row * a.s_stride + i / 128, tid % 16 == 0 && i < a.cols);
     };
     if constexpr (CHUNKS > 0) {
 #pragma unroll

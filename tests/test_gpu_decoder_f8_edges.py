@@ -44,3 +44,47 @@ def test_gates_below_fp32s_normal_values(gpu, factor, dtype, least):
     want, want_scale = coded(v)
     np.testing.assert_array_equal(got, want)
     np.testing.assert_allclose(scale, want_scale, rtol=2.0 ** -20.5, atol=2.0 ** -149)
+
+
+def _assert_nearest(got, want):
+    """Scales are the nearest fp32 values to `want`; either one where it lies within 2^-45 of the middle of two."""
+    with np.errstate(over="ignore", invalid="ignore"):
+        low, high = (np.asarray(want * (1 + d), np.float32) for d in (-2.0 ** -45, 2.0 ** -45))
+    assert (((got >= low) & (got <= high)) | (np.isnan(got) & np.isnan(low))).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("cols", [5, 128, 300, 1024])
+@pytest.mark.parametrize("kind", ["values", "norm", "gate"])
+def test_scales_are_those_of_the_largest_value_in_64_bits(gpu, kind, cols, dtype):
+    """A scale has one rounding, and no bit of what lies in other blocks."""
+    rng = np.random.default_rng(cols)
+    rows = 60
+    x = rounded(rng.standard_normal((rows, 2 * cols if kind == "gate" else cols)), dtype)
+    w = rounded(1 + 0.3 * rng.standard_normal(cols), "float32")
+
+    def call(x):
+        q, s = Array((len(x), cols), F8), Array((len(x), -(-cols // 128)), "float32")
+        if kind == "norm":
+            decoder.rmsnorm_f8(Array.of(x, dtype), Array.of(w, "float32"), q, s, eps=1e-6)
+        else:
+            (decoder.gate_f8 if kind == "gate" else decoder.quantize_f8)(Array.of(x, dtype), q, s)
+        return q.download(), s.download()
+
+    q, s = call(x)
+    v, norm = x, 1.0
+    if kind == "norm":
+        v, norm = x * w, 1 / np.sqrt((x * x).mean(1, keepdims=True) + 1e-6)
+    elif kind == "gate":
+        v = x[:, :cols] / (1 + np.exp(-x[:, :cols])) * x[:, cols:]
+    values, scale = coded(v)
+    np.testing.assert_array_equal(q, values)
+    _assert_nearest(s, scale * norm)
+    # every row by itself, and among others
+    other = np.roll(x, 7, 0)
+    other[::3] = x[::3]
+    for a, b in zip(call(other), (q, s)):
+        np.testing.assert_array_equal(a[::3], b[::3])
+    for r in (0, 17):
+        for a, b in zip(call(x[r:r + 1]), (q, s)):
+            np.testing.assert_array_equal(a[0], b[r])
