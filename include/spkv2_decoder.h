@@ -245,8 +245,11 @@ int spkv2_mi355x_rotate(const Spkv2KvCacheI8 *cache, const Spkv2Rotate *args, vo
  * codes 448 v / max|v|, rounded to the nearest, ties to even, and one float
  * scale max|v| / 448.  The codes are those of exact arithmetic; of the gate
  * those of its value in 64 bits, of whose quotients those within 2^-49 of the
- * border of two codes are ties.  A block of zeros has scale 0; one that holds a NaN or an
- * infinity has scale NaN and codes 0.  A scale below 2^-126 loses bits. */
+ * border of two codes are ties.  The scale is rounded once; below 2^-126 it loses bits, past
+ * 2^128 it is infinite.  A block of zeros has scale 0; one that holds a NaN or an
+ * infinity has scale NaN and codes 0.  The norm is one factor of the whole row: codes
+ * are those of h weight, and where another block of the row holds a NaN the scale is
+ * NaN, an infinity 0. */
 #define SPKV2_F8_BLOCK 128
 
 enum {

@@ -168,8 +168,9 @@ __device__ __forceinline__ void put_block(const float (&v)[8], const float (&a)[
         for (int j = 0; j < 8; j++)
             if (j < left) q[j] = static_cast<uint8_t>(code[j / 4] >> (8 * (j % 4)));
     }
-    // the largest of the lanes' scales, as bits: none is below 0, and NaN is above all; 0 of a block of zeros, whose norm may be 0 / 0
-    const float own = !(most < __builtin_inf()) ? __builtin_nanf("") : most == 0.0 ? 0.0f : static_cast<float>(most * (norm * (1.0 / 448.0)));
+    // The largest of the lanes' scales, as bits: none is below 0, and NaN is above all.  0 of a block of zeros, also where its
+    // norm is infinite, but not where its row holds a NaN and so has no norm.
+    const float own = !(most < __builtin_inf()) || norm != norm ? __builtin_nanf("") : most == 0.0 ? 0.0f : static_cast<float>(most * (norm * (1.0 / 448.0)));
     const unsigned bits = max_over<16>(abs_bits(own));
     if (first) *scale = __uint_as_float(bits);
 }

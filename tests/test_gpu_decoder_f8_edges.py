@@ -88,3 +88,21 @@ def test_scales_are_those_of_the_largest_value_in_64_bits(gpu, kind, cols, dtype
     for r in (0, 17):
         for a, b in zip(call(x[r:r + 1]), (q, s)):
             np.testing.assert_array_equal(a[0], b[r])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("cols", [300, 2000, 17000])
+def test_blocks_beside_ones_that_are_not_finite(gpu, cols, dtype):
+    """A row with a NaN has no norm: its scales are NaN in every block, one of zeros too; one with an infinity has norm 0."""
+    rng = np.random.default_rng(3)
+    x = rounded(rng.standard_normal((5, cols)), dtype)
+    x[:, 128:256] = 0.0
+    x[1, 3], x[2, 290], x[3, 7], x[4] = np.nan, np.nan, np.inf, 0.0
+    q, s = Array((5, cols), F8), Array((5, -(-cols // 128)), "float32")
+    decoder.rmsnorm_f8(Array.of(x, dtype), None, q, s, eps=0.0)
+    got, values = s.download(), Array((5, cols), "float32")
+    assert np.isnan(got[1:3]).all() and np.isnan(got[3, 0]) and (got[3, 1:] == 0).all() and (got[4] == 0).all()
+    assert (got[0, [0, 2]] > 0).all() and got[0, 1] == 0
+    decoder.dequantize_f8(q, s, values)
+    y = values.download()
+    assert np.isnan(y[1:3]).all() and (y[3, 128:] == 0).all() and (y[4] == 0).all()
