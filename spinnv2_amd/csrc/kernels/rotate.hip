@@ -111,10 +111,13 @@ __device__ __forceinline__ void rounded(const double (&v)[8], float (&y)[8]) {
     }
 }
 
-// What a lane's 8 elements are multiplied by, and their partners: y = norm (x own + partner other)
+// What a lane's 8 elements are multiplied by, and their partners: y = norm (x own + partner other); a bit for each that turns
 struct Turn {
     double own[8], other[8];
+    unsigned turns;
 };
+// in a cosine's place: the pair has no axis
+constexpr double kNoAxis = 2.0;
 
 // A lane's 8 elements of a head: four pairs, side by side (kBeside) or four of each
 // half (kApart: a multiple of 4 apart), or eight in a row whose partners other lanes
@@ -165,8 +168,10 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
     double *sines = table[wave][0], *cosines = table[wave][1];
     for (int p = lane; p < pairs; p += 64) {
         const int axis = g.axis ? g.axis[p] : 0;
-        const int position = static_cast<unsigned>(axis) < static_cast<unsigned>(g.axes) ? g.positions[token * g.position_stride + axis] : 0;
+        const bool there = static_cast<unsigned>(axis) < static_cast<unsigned>(g.axes);
+        const int position = there ? g.positions[token * g.position_stride + axis] : 0;
         sine_cosine(static_cast<double>(position) * static_cast<double>(g.frequencies[p]), &sines[p], &cosines[p]);
+        if (!there) cosines[p] = kNoAxis;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -179,6 +184,7 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
     constexpr int kOther = PAIRING == kBeside ? 1 : 4;  // partner e ^ kOther of the same lane
     const auto turn_of = [&](const void *weight) {
         Turn t;
+        t.turns = 0;
         float own[8], other[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) own[e] = other[e] = 1.0f;
@@ -191,9 +197,11 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int i = place(e);
-            const bool second = PAIRING == kBeside ? i & 1 : i >= pairs, turns = i < 2 * pairs;
-            const int p = !turns ? 0 : PAIRING == kBeside ? i / 2 : second ? i - pairs : i;
+            const bool second = PAIRING == kBeside ? i & 1 : i >= pairs;
+            const int p = i >= 2 * pairs ? 0 : PAIRING == kBeside ? i / 2 : second ? i - pairs : i;
             const double c = cosines[p], s = sines[p];
+            const bool turns = i < 2 * pairs && c != kNoAxis;
+            t.turns |= turns ? 1u << e : 0u;
             t.own[e] = (turns ? c : 1.0) * static_cast<double>(own[e]);
             t.other[e] = turns ? (second ? s : -s) * static_cast<double>(other[e]) : 0.0;
         }
@@ -226,8 +234,8 @@ __global__ void __launch_bounds__(256) rotate_heads(RotateArgs a) {
         double v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            // past the pairs nothing is added: 0 times what is not finite would be NaN
-            const float o = place(j) < 2 * pairs ? other[j] : 0.0f;
+            // to what does not turn nothing is added: 0 times what is not finite would be NaN
+            const float o = t.turns >> j & 1 ? other[j] : 0.0f;
             v[j] = __builtin_fma(static_cast<double>(o), t.other[j], static_cast<double>(x[j]) * t.own[j]) * factor;
         }
         rounded<T>(v, y);

@@ -15,6 +15,28 @@ from .test_gpu_decoder_f8 import F8, coded
 pytestmark = pytest.mark.gpu
 
 
+# ----------------------------------------------------------------- rotate
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("pairs,interleaved", [(32, False), (32, True), (29, False), (29, True)])
+def test_pairs_of_no_axis_are_not_turned(gpu, pairs, interleaved, dtype):
+    """... whatever their partners hold; and head norms of 0 / 0 are NaN, with eps zeros stay zeros."""
+    rng = np.random.default_rng(1)
+    x = rounded(rng.standard_normal((3, 2, 64)), dtype)
+    x[0, 0, :12], x[1, 1, 40:50] = np.inf, np.nan
+    dx, out = Array.of(x, dtype), Array(x.shape, dtype)
+    args = Array.of(np.array([[7, 8], [9, 10], [1, 2]], np.int32)), Array.of(np.ones(pairs, np.float32)), out, None
+    kw = dict(axes=Array.of(rng.choice([-1, 2, 2 ** 31 - 1], pairs).astype(np.int32)), interleaved=interleaved)
+    decoder.rotate(dx, None, *args, **kw)
+    np.testing.assert_array_equal(out.download(), x)
+    dx.upload(np.zeros(x.shape))
+    decoder.rotate(dx, None, *args, norm=True, eps=1e-6, **kw)
+    assert (out.download() == 0).all()
+    for axes in (kw["axes"], Array.of(np.zeros(pairs, np.int32))):
+        decoder.rotate(dx, None, *args, axes=axes, norm=True, eps=0.0, interleaved=interleaved)
+        assert np.isnan(out.download()).all()
+
+
 # ------------------------------------------------------------ 8-bit floats
 
 def _gate(x, dtype):
