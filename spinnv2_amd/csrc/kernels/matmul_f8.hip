@@ -311,7 +311,7 @@ __device__ __forceinline__ unsigned lds_address(const void *p) {
     return static_cast<unsigned>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
 }
 __device__ __forceinline__ void load_lds16(const void *base, unsigned offset, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 // A barrier ahead of which every wave's loads into LDS have arrived.
 __device__ __forceinline__ void wait_all() {
