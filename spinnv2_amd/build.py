@@ -84,17 +84,23 @@ def _compile(src: Path, force: bool, newest_header: float) -> tuple[Path, str]:
     return obj, warnings
 
 
-def build_calls(force: bool = False) -> Path:
-    """The module of the decoder layer's calls; host code only."""
+def build_calls(force: bool = False) -> Path | None:
+    """The module of the decoder layer's calls; host code only.  None, with a
+    note, where this interpreter's headers are missing: the library and
+    everything that needs it alone are whole without the module."""
+    include = Path(sysconfig.get_paths()["include"])
+    if not (include / "Python.h").exists():
+        CALLS.unlink(missing_ok=True)  # of another header's structs, perhaps
+        print(f"{include} has no Python.h: the decoder layer's native calls are not built", file=sys.stderr)
+        return None
     newest = max(BINDINGS.stat().st_mtime, max(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
     if not force and CALLS.exists() and CALLS.stat().st_mtime >= newest:
         return CALLS
-    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
-    if not cxx:
-        raise RuntimeError("no C++ compiler found (g++ or c++) for the decoder layer's calls")
+    # hipcc compiles host code as well
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++") or hipcc()
     tmp = CALLS.with_suffix(".so.tmp")
-    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-I{INCLUDE}",
-           f"-I{sysconfig.get_paths()['include']}", str(BINDINGS), "-o", str(tmp)]
+    cmd = [cxx, "-x", "c++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", f"-I{INCLUDE}",
+           f"-I{include}", str(BINDINGS), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"compile failed: {BINDINGS}\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")

@@ -43,15 +43,15 @@ _FP32, _INT8, _FP16, _BF16, _INT32, _INT64, _F8 = 1, 2, 3, 4, 101, 102, 103
 _CODES = {"float32": _FP32, "float16": _FP16, "bfloat16": _BF16, "int8": _INT8, "int32": _INT32, "int64": _INT64,
           "float8_e4m3fn": _F8}
 _FLOATS = (_FP32, _FP16, _BF16)
-_FP32S, _INT8S, _INT32S = (_FP32,), (_INT8,), (_INT32,)
+_FP32S, _INT8S, _INT32S, _INT64S = (_FP32,), (_INT8,), (_INT32,), (_INT64,)
 #: columns of a row of 8-bit floats, and rows and columns of weights, that share a scale
 F8_BLOCK = 128
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
 
-# The header's structs: those of the calls below are laid out from here, or by the native module from the header itself;
-# all of them for programs that call the library's entry points through ctypes.
+# The header's structs.  The calls of the int8 operators are laid out from here, the others by the native module from the
+# header itself, from _Rotate on; those are here for the tests of the C entry points, which ctypes calls.
 class _RmsNorm(ctypes.Structure):
     _fields_ = [("x", _P), ("residual", _P), ("weight", _P), ("residual_out", _P), ("q", _P), ("scale", _P),
                 ("rows", _I64), ("cols", _I64), ("x_stride", _I64), ("residual_stride", _I64),
@@ -151,22 +151,25 @@ def _packer(cls):
 
 
 _pack_norm, _pack_dequantize, _pack_matmul = _packer(_RmsNorm), _packer(_Dequantize), _packer(_Matmul)
-_pack_attention = _packer(_Attention)
+_pack_write, _pack_read, _pack_attention = _packer(_Write), _packer(_Read), _packer(_Attention)
 
 
 #: the calls that take their tensors apart in native code (bindings/decoder_calls.cpp), once _bind() was called
 _calls = None
 
 
-def _bind():
-    """Loads that module and gives it the library's entry points."""
+def _bind(needed: bool = True):
+    """Loads that module and gives it the library's entry points.  It is built
+    for one interpreter: where there is none for this one, None unless needed."""
     global _calls
-    from .build import CALLS
+    from . import build
 
     lib = load_library()
-    if not CALLS.exists():
-        raise RuntimeError(f"{CALLS} is not built; run `python -m spinnv2_amd.build`")
-    spec = importlib.util.spec_from_file_location("spinnv2_amd._decoder_calls", CALLS)
+    if not build.CALLS.exists():
+        if not needed:
+            return None
+        raise RuntimeError(f"{build.CALLS} is not built; run `python -m spinnv2_amd.build`")
+    spec = importlib.util.spec_from_file_location("spinnv2_amd._decoder_calls", build.CALLS)
     calls = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(calls)
     calls.bind(_CODES, _code, struct.error, tuple(
@@ -439,14 +442,30 @@ class KvCache:
     def write(self, k, v, slots, *, stream: int = 0) -> None:
         """Quantises k and v [tokens, kv_heads, head_dim] into the slots (int64
         [tokens]; negative ones, and those past the cache, are not written)."""
-        if code := (_calls or _bind()).kv_write(self._at, self.kv_heads, self.head_dim, k, v, slots, stream):
+        if calls := _calls or _bind(needed=False):
+            code = calls.kv_write(self._at, self.kv_heads, self.head_dim, k, v, slots, stream)
+        else:  # the same from here: these two calls need the library alone
+            shape, kind = (k.shape[0], self.kv_heads, self.head_dim), _code(k)
+            a = _pack_write(k.data_ptr(), v.data_ptr(), _vector("slots", slots, _INT64S, shape[0]), shape[0],
+                            _heads("k", k, _FLOATS, shape), _heads("v", v, (kind,), shape), kind, 0)
+            code = load_library().spkv2_mi355x_kv_write_i8(self._ref, a, stream)
+        if code:
             _check(load_library(), code, "kv_write_i8")
 
     def read(self, table, first, offsets, k, v, *, stream: int = 0) -> None:
         """Reads tokens first[s] .. of each sequence s into rows offsets[s] ..
         offsets[s + 1] of k and v.  table int32 [sequences, width], first int32
         [sequences] or None, offsets int32 [sequences + 1]."""
-        if code := (_calls or _bind()).kv_read(self._at, self.kv_heads, self.head_dim, table, first, offsets, k, v, stream):
+        if calls := _calls or _bind(needed=False):
+            code = calls.kv_read(self._at, self.kv_heads, self.head_dim, table, first, offsets, k, v, stream)
+        else:
+            shape, kind = (k.shape[0], self.kv_heads, self.head_dim), _code(k)
+            seqs, width = _table(table)
+            a = _pack_read(table.data_ptr(), 0 if first is None else _vector("first", first, _INT32S, seqs),
+                           _vector("offsets", offsets, _INT32S, seqs + 1), k.data_ptr(), v.data_ptr(), shape[0],
+                           _heads("k", k, _FLOATS, shape), _heads("v", v, (kind,), shape), seqs, width, kind, 0)
+            code = load_library().spkv2_mi355x_kv_read_i8(self._ref, a, stream)
+        if code:
             _check(load_library(), code, "kv_read_i8")
 
 

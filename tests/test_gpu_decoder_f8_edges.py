@@ -6,8 +6,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from spinnv2_amd import decoder
-from spinnv2_amd.decoder import DeviceArray as Array
+from spinnv2_amd import build, decoder
+from spinnv2_amd.decoder import DeviceArray as Array, KvCache
 
 from .test_gpu_decoder import rounded
 from .test_gpu_decoder_f8 import F8, coded
@@ -128,3 +128,29 @@ def test_blocks_beside_ones_that_are_not_finite(gpu, cols, dtype):
     decoder.dequantize_f8(q, s, values)
     y = values.download()
     assert np.isnan(y[1:3]).all() and (y[3, 128:] == 0).all() and (y[4] == 0).all()
+
+
+# ------------------------------------------------- the cache without the native calls
+
+def test_the_cache_writes_and_reads_the_same_without_the_native_calls(gpu, monkeypatch, tmp_path):
+    rng = np.random.default_rng(9)
+    k, v = (Array.of(rng.standard_normal((40, 2, 64)), "bfloat16") for _ in range(2))
+    slots = Array.of(rng.permutation(64)[:40].astype(np.int64))
+    table, first = Array.of(np.array([[2, 0], [1, 3]], np.int32)), Array.of(np.array([3, 0], np.int32))
+    offsets = Array.of(np.array([0, 20, 45], np.int32))
+
+    def results():
+        cache = KvCache.empty(4, 2, 16, 64)
+        for b in cache.buffers:
+            b.upload(np.zeros(b.shape))
+        cache.write(k, v, slots)
+        out = [Array((45, 2, 64), "bfloat16") for _ in range(4)]
+        cache.read(table, first, offsets, *out[:2])
+        cache.read(table, None, offsets, *out[2:])
+        return [x.download() for x in (*cache.buffers, *out)]
+
+    want = results()
+    monkeypatch.setattr(build, "CALLS", tmp_path / "calls.so")
+    monkeypatch.setattr(decoder, "_calls", None)
+    for a, b in zip(results(), want):
+        np.testing.assert_array_equal(a, b)
