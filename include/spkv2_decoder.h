@@ -315,7 +315,7 @@ int spkv2_mi355x_matmul_f8_kernel_name(const Spkv2MatmulF8 *args, char *buf, siz
  * a does not have counts as zeros. */
 typedef struct {
     Spkv2MatmulF8 product;  /* m: rows of out; b [experts, n, k], b_scale [experts, blocks of n, blocks of k], bias [experts, n] */
-    const int32_t *offsets; /* [experts + 1], from 0, not decreasing; what passes m is not computed */
+    const int32_t *offsets; /* [experts + 1], from 0, not decreasing (rows of several experts would be left, or any one's); what passes m is not computed */
     const int32_t *order;   /* [m], or NULL */
     int64_t a_rows;         /* rows of a and a_scale */
     int64_t b_expert_stride, b_scale_expert_stride; /* elements between experts */

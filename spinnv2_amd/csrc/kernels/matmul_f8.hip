@@ -40,7 +40,7 @@ struct MatmulArgs {
     // by expert
     const int32_t *offsets, *order;
     int64_t a_rows, b_expert, sb_expert;
-    int experts;
+    int experts, most_down;  // workgroups along the rows at most
     unsigned token_mul;  // choice / per_token, by multiplication
     int token_shift;
 };
@@ -362,6 +362,8 @@ __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ?
         x = experts_from(a, 0, BM);
         m_tiles = tiles_of(x);
         for (int e0 = 64; e0 < a.experts; e0 += 64) m_tiles += tiles_of(experts_from(a, e0, BM));
+        // offsets that fall name rows more than once: up to 2^27 tiles of rows, whose product with n_tiles passes 2^31
+        m_tiles = min(m_tiles, a.most_down);
     }
     const int tiles = m_tiles * a.n_tiles, per = tiles / 8, rest = tiles % 8;
     const int xcd = blockIdx.x % 8, count = per + (xcd < rest ? 1 : 0);
@@ -728,7 +730,7 @@ int check(const Spkv2MatmulF8Experts *g, bool pointers) {
 
 MatmulArgs arguments(const Spkv2MatmulF8 &g) {
     MatmulArgs a{g.a, g.b, g.a_scale, g.b_scale, g.bias, g.out, g.a_stride, g.b_stride, g.out_stride, g.a_scale_stride, g.b_scale_stride,
-                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), 0, nullptr, nullptr, g.m, 0, 0, 1, 0, 0};
+                 static_cast<int>(g.m), static_cast<int>(g.n), static_cast<int>(g.k), 0, nullptr, nullptr, g.m, 0, 0, 1, 0, 0, 0};
     if (g.m == 1) a.a_stride = 0, a.sa_stride = 0, a.out_stride = 0;
     if (g.n == 1) a.b_stride = 0;
     if (g.n <= 128) a.sb_stride = 0;
@@ -816,6 +818,7 @@ int run(const char *what, int dtype, MatmulArgs a, void *stream) {
         const unsigned across = static_cast<unsigned>((static_cast<int64_t>(a.n) + f.channels - 1) / f.channels);
         const unsigned down = static_cast<unsigned>(most_down(a, EXPERTS, f.tokens));
         a.n_tiles = static_cast<int>(across);
+        a.most_down = static_cast<int>(down);
         auto rows = [&](auto kernel) { return launch(what, kernel, dim3(across, down), dim3(64 * 8), stream, a); };
         auto tiles = [&](auto direct, auto staged, int waves) {
             const unsigned all = across * down;

@@ -3,6 +3,7 @@ GPU: what is refused at the last size that a launch cannot take."""
 
 from __future__ import annotations
 
+import functools
 import re
 from pathlib import Path
 
@@ -12,7 +13,7 @@ from spinnv2_amd import build, decoder
 
 from .test_decoder import UNSUPPORTED, Fake, _cache, _refused
 from .test_decoder import test_cache_refuses_what_does_not_fit as cache_refusals
-from .test_decoder_f8 import F8, _rows
+from .test_decoder_f8 import F8, FORMS, _rows, kernel_of
 from .test_decoder_f8 import Fake as FakeF8
 
 
@@ -64,3 +65,41 @@ def test_builds_without_the_interpreters_headers(no_calls, monkeypatch, tmp_path
     build.CALLS.write_bytes(b"of another header")
     assert build.build_calls() is None and not build.CALLS.exists()
     assert "Python.h" in capsys.readouterr().err
+
+
+# ------------------------------------------------ sizes that take a kernel over several steps of k
+
+#: blocks of k -> k of whole runs of 16 bytes, k of none; the last block is never whole
+STEPS = {5: (528, 517), 9: (1040, 1030), 22: (2704, 2701), 70: (8848, 8837)}
+
+
+@functools.lru_cache(maxsize=None)
+def sizes_of_steps(dtype, by_expert):
+    """(kernel, blocks of k) -> (m, n, k, experts): the smallest sizes found, none of them a multiple of a tile."""
+    found = {}
+    for blocks, ks in STEPS.items():
+        for k in ks:
+            for m in (1, 3, 9, 18, 33, 70, 100, 130, 200, 400, 520, 700, 1030, 1500, 2100, 3000, 4100):
+                for n in (17, 33, 65, 100, 130, 190, 260, 390, 515, 770, 1029, 1540, 2050, 3000, 4100, 6200):
+                    for experts in ((1, 3, 7, 40) if by_expert else (0,)):
+                        if m * n * k > 1.2e10 or max(1, experts) * n * k > 4e7:
+                            continue
+                        key, size = (kernel_of(dtype, m, n, k, experts, m), blocks), m * n * k + experts * n * k * 20
+                        if key not in found or size < found[key][0]:
+                            found[key] = (size, m, n, k, experts)
+    return {key: v[1:] for key, v in found.items()}
+
+
+def _groups(form):
+    return int(re.search(r"groups=(\d)", form).group(1)) if "groups" in form else 8
+
+
+@pytest.mark.parametrize("by_expert", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_sizes_take_every_kernel_over_several_steps(dtype, by_expert):
+    sizes = sizes_of_steps(dtype, by_expert)
+    for form in FORMS:
+        if not (dtype == "float32" and "x256" in form):
+            steps = {-(-blocks // _groups(form)) for kernel, blocks in sizes if kernel == "matmul_" + form}
+            assert max(steps) >= 3, (form, steps)
+    assert any(blocks == 70 for _, blocks in sizes)

@@ -7,9 +7,11 @@ import numpy as np
 import pytest
 
 from spinnv2_amd import build, decoder
-from spinnv2_amd.decoder import DeviceArray as Array, KvCache
+from spinnv2_amd.decoder import DeviceArray as Array, KvCache, _FLOAT8, to_float8
 
-from .test_gpu_decoder import rounded
+from .test_decoder_f8 import FORMS, kernel_of
+from .test_decoder_f8_edges import sizes_of_steps
+from .test_gpu_decoder import gaps, rounded, strided
 from .test_gpu_decoder_f8 import F8, coded
 
 pytestmark = pytest.mark.gpu
@@ -154,3 +156,100 @@ def test_the_cache_writes_and_reads_the_same_without_the_native_calls(gpu, monke
     monkeypatch.setattr(decoder, "_calls", None)
     for a, b in zip(results(), want):
         np.testing.assert_array_equal(a, b)
+
+
+# ---------------------------------------------------------------- products
+
+_CODE_OF = to_float8(np.arange(-8, 9))  # of whole numbers up to 8
+
+
+def _codes(codes, pad):
+    """An array of these 8-bit codes [.., rows, k], whose rows lie `pad` codes of NaN apart."""
+    *outer, k = codes.shape
+    raw = np.full((*outer, k + pad), 0x7F, np.uint8)
+    raw[..., :k] = codes
+    whole = Array(raw.shape, "int8")
+    whole.upload(raw.view(np.int8))
+    return Array(codes.shape, F8, buffer=whole.buffer, strides=whole.strides)
+
+
+class Product:
+    """A product of rows with weights, by expert where there are some: its arrays, the call, and its values in 64 bits."""
+
+    def __init__(self, m, n, k, experts, dtype, *, seed, any_codes=False, a_rows=None, order=False, bias=False):
+        rng = np.random.default_rng(seed)
+        self.m, self.n, self.k, self.experts, self.dtype = m, n, k, experts, dtype
+        self.blocks, pad = -(-k // 128), 0 if k % 16 else 16
+        a_rows, e = m if a_rows is None else a_rows, max(experts, 1)
+        if any_codes:
+            ca, cb = (to_float8(np.clip(rng.standard_normal(4096) * 160, -448, 448))[rng.integers(0, 4096, s)] for s in ((a_rows, k), (e, n, k)))
+            self.a_scale, self.b_scale = (rounded(0.01 * rng.random(s) + 0.001, "float32") for s in ((a_rows, self.blocks), (e, -(-n // 128), self.blocks)))
+        else:  # whole numbers and powers of two: their sums have no rounding in any order
+            ca, cb = (_CODE_OF[rng.integers(0, 17, s, np.int8)] for s in ((a_rows, k), (e, n, k)))
+            self.a_scale, self.b_scale = (2.0 ** rng.integers(-1, 2, s) for s in ((a_rows, self.blocks), (e, -(-n // 128), self.blocks)))
+        self.ca, self.cb, self.pad = ca, cb, pad
+        self.bias = rng.integers(-99, 99, (e, n)).astype(np.float64) if bias else None
+        if experts:
+            counts = np.bincount(np.minimum(rng.integers(0, experts, m), rng.integers(0, experts, m)), minlength=experts)
+            self.offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        else:
+            self.offsets = np.array([0, m], np.int32)
+        self.order = rng.permutation(max(a_rows, m))[:m].astype(np.int32) if order else None
+
+    def inputs(self):
+        """Each output row's input; -1: none."""
+        row = np.arange(self.m) if self.order is None else self.order.astype(np.int64)
+        return np.where((row >= 0) & (row < len(self.ca)), row, -1)
+
+    def __call__(self):
+        out = strided(np.zeros((self.m, self.n)), self.dtype, 8)
+        sa, sb = Array.of(self.a_scale, "float32"), Array.of(self.b_scale if self.experts else self.b_scale[0], "float32")
+        a, b = _codes(self.ca, self.pad), _codes(self.cb if self.experts else self.cb[0], self.pad)
+        if self.experts:
+            decoder.matmul_f8_experts(a, sa, b, sb, Array.of(self.offsets), out, order=None if self.order is None else Array.of(self.order),
+                                      bias=None if self.bias is None else Array.of(self.bias, "float32"))
+        else:
+            decoder.matmul_f8(a, sa, b, sb, out, bias=None if self.bias is None else Array.of(self.bias[0], "float32"))
+        got = out.download().astype(np.float64)
+        assert (gaps(out) == 77).all()
+        return got
+
+    def rows(self, rows):
+        """Those input rows' values."""
+        a = _FLOAT8[self.ca[rows]].astype(np.float64) * np.repeat(self.a_scale[rows], 128, 1)[:, :self.k]
+        a[np.asarray(rows) < 0] = 0.0
+        return a
+
+    def weights(self, e, cols=slice(None)):
+        scale = np.repeat(np.repeat(self.b_scale[e], 128, 0)[:self.n], 128, 1)[:, :self.k]
+        return _FLOAT8[self.cb[e, cols]].astype(np.float64) * scale[cols]
+
+    def values(self):
+        want, rows = np.zeros((self.m, self.n)), self.inputs()
+        for e in range(max(self.experts, 1)):
+            low, high = self.offsets[e], self.offsets[e + 1]
+            if high > low:
+                want[low:high] = self.rows(rows[low:high]) @ self.weights(e).T
+                if self.bias is not None:
+                    want[low:high] += self.bias[e]
+        return want
+
+    def kernel(self):
+        return kernel_of(self.dtype, self.m, self.n, self.k, self.experts, len(self.ca), self.pad)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_experts_whose_offsets_fall(gpu, form, dtype):
+    """Values of rows that several experts have are one's of them, in any mixture; nothing else is written, and no more tiles
+    are taken than the rows have."""
+    size = sizes_of_steps(dtype, True).get(("matmul_" + form, 5))
+    if size is None:
+        return
+    m, n, k, _ = size
+    p = Product(m, n, k, 4, dtype, seed=5)
+    p.offsets = np.array([0, m, 3, m, 0], np.int32)
+    got, a = p(), p.rows(np.arange(m))
+    each = [rounded(a @ p.weights(e).T, dtype) for e in range(4)]
+    known = np.logical_or.reduce([got == y for y in (*each, np.zeros((m, n)))])
+    assert known.all()
