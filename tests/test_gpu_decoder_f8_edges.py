@@ -12,7 +12,7 @@ from spinnv2_amd.decoder import DeviceArray as Array, KvCache, _FLOAT8, to_float
 from .test_decoder_f8 import FORMS, kernel_of
 from .test_decoder_f8_edges import sizes_of_steps
 from .test_gpu_decoder import gaps, rounded, strided
-from .test_gpu_decoder_f8 import F8, coded
+from .test_gpu_decoder_f8 import F8, _limit, coded
 
 pytestmark = pytest.mark.gpu
 
@@ -179,7 +179,7 @@ class Product:
     def __init__(self, m, n, k, experts, dtype, *, seed, any_codes=False, a_rows=None, order=False, bias=False):
         rng = np.random.default_rng(seed)
         self.m, self.n, self.k, self.experts, self.dtype = m, n, k, experts, dtype
-        self.blocks, pad = -(-k // 128), 0 if k % 16 else 16
+        self.blocks, pad = -(-k // 128), 16
         a_rows, e = m if a_rows is None else a_rows, max(experts, 1)
         if any_codes:
             ca, cb = (to_float8(np.clip(rng.standard_normal(4096) * 160, -448, 448))[rng.integers(0, 4096, s)] for s in ((a_rows, k), (e, n, k)))
@@ -253,3 +253,92 @@ def test_experts_whose_offsets_fall(gpu, form, dtype):
     each = [rounded(a @ p.weights(e).T, dtype) for e in range(4)]
     known = np.logical_or.reduce([got == y for y in (*each, np.zeros((m, n)))])
     assert known.all()
+
+
+def _steps_cases():
+    """(form, type, blocks of k, by expert): every kernel over several steps of k."""
+    for dtype in ("float32", "float16", "bfloat16"):
+        for by_expert in (False, True):
+            for kernel, blocks in sorted(sizes_of_steps(dtype, by_expert)):
+                if blocks < 70 or dtype != "float16":
+                    yield kernel, dtype, blocks, by_expert
+
+
+@pytest.mark.parametrize("kernel,dtype,blocks,by_expert", _steps_cases())
+def test_every_kernel_over_several_steps(gpu, kernel, dtype, blocks, by_expert):
+    """k of 5 to 70 blocks, the last one not whole, codes of NaN behind rows' ends, a bias; by expert through an order of which
+    a tenth names rows that are not there: below zero, past a's rows, far past them."""
+    m, n, k, experts = sizes_of_steps(dtype, by_expert)[kernel, blocks]
+    p = Product(m, n, k, experts, dtype, seed=blocks, order=by_expert, bias=blocks != 9)
+    if by_expert:
+        rng = np.random.default_rng(2)
+        absent = rng.random(m) < 0.1
+        p.order[absent] = rng.choice([-1, -2 ** 31, m, m + 1, 2 ** 31 - 1], m).astype(np.int32)[absent]
+    if p.kernel() != kernel:  # rows that lie apart may take another: then side by side
+        p.pad = 0
+    assert p.kernel() == kernel
+    with np.errstate(over="ignore"):
+        want = rounded(p.values(), dtype)
+    np.testing.assert_array_equal(p(), want)
+
+
+@pytest.mark.parametrize("by_expert", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_every_kernel_with_any_codes(gpu, form, dtype, by_expert):
+    """Codes of all sizes and scales that are no powers of two; a NaN code of a row, one of a channel, a scale of infinity and one
+    of NaN change their rows and channels and no other; by expert without an order, more rows than a has."""
+    sizes = sizes_of_steps(dtype, by_expert)
+    size = next((sizes["matmul_" + form, b] for b in (9, 5, 22, 70) if ("matmul_" + form, b) in sizes), None)
+    if size is None:
+        assert dtype == "float32" and "x256" in form
+        return
+    m, n, k, experts = size
+    p = Product(m, n, k, experts, dtype, seed=7, any_codes=True, a_rows=max(1, m - m // 9) if by_expert else None)
+    rng = np.random.default_rng(8)
+    rows, channel, e = rng.permutation(len(p.ca))[:3], int(rng.integers(n)), int(np.searchsorted(p.offsets, m // 2, side="right")) - 1
+    odd = np.zeros((m, n), bool)
+    if len(rows) == 3:
+        p.ca[rows[0], k - 1], p.a_scale[rows[1], 1], p.a_scale[rows[2], p.blocks - 1] = 0x7F, np.inf, np.nan
+        odd[rows] = True
+        p.cb[e, channel, k // 2] = 0xFF
+        odd[p.offsets[e]:p.offsets[e + 1], channel] = True
+        odd[p.inputs() < 0] = False
+    got = p()
+    assert (np.isfinite(got) == ~odd).all()
+    assert np.isnan(got[rows[[0, 2]]]).all() if len(rows) == 3 else True
+    assert (got[p.inputs() < 0] == 0).all()
+    # some rows and channels, those of the tiles' ends among them
+    some = np.unique(np.concatenate([rng.integers(0, m, 30), [0, m - 1], p.offsets[1:-1]]))
+    some = some[some < m]
+    some = some[~odd[some].all(1)]
+    cols = np.unique(np.concatenate([rng.integers(0, n, 40), [0, n - 1]]))
+    for e in range(max(experts, 1)):
+        mine = some[(some >= p.offsets[e]) & (some < p.offsets[e + 1])]
+        if not len(mine):
+            continue
+        a, b = p.rows(p.inputs()[mine]), p.weights(e, cols)
+        keep = ~odd[np.ix_(mine, cols)]
+        b = np.nan_to_num(b, nan=0.0)
+        want = a @ b.T
+        ones = np.ones((len(a), p.blocks)), np.ones((-(-len(b) // 128), p.blocks))
+        limit = _limit(a, ones[0], b, ones[1], dtype, want)
+        assert (np.abs(got[np.ix_(mine, cols)] - want) <= limit)[keep].all()
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,n,k,experts", [(6600, 4360, 112, 6), (6600, 4360, 656, 6), (18000, 1540, 112, 70), (9000, 4360, 1040, 3), (5000, 3000, 272, 5)])
+def test_rows_that_are_not_there_in_workgroups_of_several_tiles(gpu, m, n, k, experts, dtype, bias):
+    """Through an order and without one; which rows are there differs from tile to tile."""
+    rng = np.random.default_rng(k)
+    for order in (True, False):
+        p = Product(m, n, k, experts, dtype, seed=m + order, order=order, bias=bias, a_rows=m if order else m - m // 5)
+        if order:
+            absent = rng.random(m) < np.repeat(rng.choice([0.0, 0.02, 0.5, 1.0], -(-m // 100)), 100)[:m]
+            p.order[absent] = rng.choice([-1, -2 ** 31, m, 2 ** 31 - 1], m).astype(np.int32)[absent]
+        p.pad = 0
+        assert "x256,groups=1,direct" in p.kernel()
+        with np.errstate(over="ignore"):
+            want = rounded(p.values(), dtype)
+        np.testing.assert_array_equal(p(), want)
