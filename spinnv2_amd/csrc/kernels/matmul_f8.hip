@@ -7,19 +7,23 @@
 // them starts from zero and its sums are scaled and added in fp32.
 //
 // The 8-bit float matrix cores add eight products at a time and keep 13 bits
-// below the largest of them: results are within 4e-5 of a sum's size, which 16-bit
-// outputs, with 2^-9 and 2^-12 of their own, do not show.  fp32 outputs would
-// (1.1e-5 relative where fp32 sums leave 3e-7), so theirs are computed on the fp16
-// cores, whose operands hold 8-bit floats exactly, at half the rate.
+// below the largest of them: a sum may be off by 2^-10 of the largest product of
+// every eight, at random by 4e-5 of its size, which 16-bit outputs, with 2^-9 and
+// 2^-12 of their own, hardly show.  fp32 outputs would (1.1e-5 relative where fp32
+// sums leave 3e-7), so theirs are computed on the fp16 cores, whose operands hold
+// 8-bit floats exactly, at half the rate: a caller chooses by the output's type.
 //
 // Many rows are bound by the matrix cores, at the clock that random operands leave
-// them: 8192 x 8192 x 8192 into bf16 440 to 455 us, 2.4 to 2.5 PFLOP/s, the cores at
-// work in 60% of the cycles (a library's product, one scale for a whole matrix, 423).
+// them: 8192 x 8192 x 8192 into bf16 408 to 460 us, 2.4 to 2.7 PFLOP/s, the cores at
+// work in 61% of the cycles (a library's product, one scale for a whole matrix, 423),
+// into fp32 908, 1.2 PFLOP/s.
 // Few rows are bound by the bytes of the weights: 1 x 4096 x 4096 4.6 to 5.8 us, a
 // launch's own time and 2.9 to 3.6 TB/s; 64 tokens of 8 experts of 64, 2048 x 2048,
-// 46 to 55 us, 4.8 to 5.8 TB/s.  Rows by expert leave part of each expert's last tile
-// empty and look their rows up ahead of the loop: 4001 tokens of 4 of 32, 4096 x
-// 2048, 165 to 178 us, where the products alone would take 103.
+// 46 to 55 us, 4.8 to 5.9 TB/s.  32 to 300 rows are bound by a workgroup's walk along k
+// and by weights read once for each 16 to 64 rows: 64 x 4096 x 4096 7.9 us, 256 x 4096 x
+// 14336 33.  Rows by expert leave part of each expert's last tile empty and look their
+// rows up ahead of the loop: 4001 tokens of 4 of 32, 4096 x 2048, 172 to 177 us, where
+// the products alone would take 103.
 #include <cmath>
 #include <cstdio>
 
@@ -336,7 +340,7 @@ constexpr bool goes_on(bool direct, int channels) { return direct && channels ==
 // Tiles so large that a CU holds one workgroup go on (kGoOn): the next tile's rows
 // are looked up ahead of a tile's loop, and its first block is under way while the
 // tile leaves, in two halves, through the buffer that the block does not take (4001
-// tokens of 4 of 32 experts, 4096 x 2048, 177 -> 167 us, 16384 x 8192 x 128 68 -> 56).
+// tokens of 4 of 32 experts, 4096 x 2048, 187 -> 175 us, 16384 x 8192 x 128 68 -> 56).
 template <typename T, bool EXPERTS, bool DIRECT, int WAVES_M, int WAVES_N, int WAVES_K, int TJ, int TI>
 __global__ void __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K, TJ *TI >= 16 ? 2 : sizeof(T) == 4 || WAVES_N == 4 ? 3 : 4)
     matmul_tiles(MatmulArgs a) {

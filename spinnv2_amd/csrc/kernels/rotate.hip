@@ -8,9 +8,10 @@
 // turns by, and groups of 8, 16 or 32 lanes a head each, 8 elements a lane.
 //
 // Bound by HBM and by its arithmetic, each two thirds of the time: 8190 tokens of
-// 32 + 8 heads of 128 in bf16, values too, into the cache in 48 to 56 us (185 MB, 3.3
-// to 3.9 TB/s), without a cache in 38 (168 MB, 4.4 TB/s); fp32 without a cache at 5.2
-// TB/s.
+// 32 + 8 heads of 128 in bf16, values too, into the cache in 48 to 57 us (185 MB, 3.3
+// to 3.9 TB/s), without a cache in 40 (168 MB, 4.2 TB/s); fp32 without a cache at 5.0
+// TB/s.  Lanes read the pairs' doubles 32 bytes apart, which loses 44% of the LDS
+// cycles to conflicts.
 //
 // In 64 bits: angles of far positions need it (position 70001 times a frequency
 // near 1 keeps 7 bits behind the point in fp32), and a key beside the border of

@@ -4,11 +4,11 @@
 // the count of choices of lower experts and of earlier ones of its own.  A
 // workgroup an expert counts and places its own: every id is read once for each
 // expert, from L2, but there is one launch, no atomics and no order that changes
-// from run to run (65520 choices of 128 experts 14 us, 17 where ids come from
-// memory: bound by the instructions for each 64 of them; 512 of 64 3.3 to 4.0 us).
+// from run to run (65520 choices of 128 experts 14 us, 17.5 where ids come from
+// memory: bound by the instructions for each 64 of them; 512 of 64 3.7 to 4.0 us).
 //
 // combine: bound by the bytes of the rows picked (8190 tokens of 8 rows of 2048,
-// 302 MB: 64 us, 4.7 TB/s).
+// 302 MB: 65 us, 4.7 TB/s).
 #include "decoder.hpp"
 
 namespace spk::dec {

@@ -8,11 +8,13 @@
 // moves.  The norm is one factor of the whole row and cancels out of q: codes
 // are those of h w.  fp32 quotients beside a border of two codes are taken again
 // in 64 bits, one in thirty thousand (of the gate, whose exponential is within
-// 2^-21 in fp32, one in eight thousand), and so is the largest element of each
-// block, for its scale.  One pass, bound by HBM: 8190 x 8192 of gates in bf16, 337
-// MB, in 80 to 92 us (3.7 to 4.2 TB/s; its instructions take as long: 74 to 88 with
-// fp32 scales, off by a bit), back to values, 203 MB, in 33 (the codes
-// still cached).
+// 2^-21 in fp32, one in eight thousand), and so is the largest element of a block,
+// for its scale, where fp32 does not hold values exactly.  One pass, bound by HBM and, of 16-bit rows, by their
+// instructions: 8190 x 8192 of gates in bf16, 337 MB, in 75 to 79 us (4.3 to 4.5
+// TB/s; 92 at the clocks that calls one behind the other leave, 88 with fp32 scales,
+// off by a bit), of a norm with a residual, 470 MB, in 97 (4.9 TB/s), of values, 203
+// MB, in 55, and back to values in 33 (the codes still cached); fp32 rows at 5.5 to
+// 5.7 TB/s.
 #include "decoder.hpp"
 
 namespace spk::dec {
